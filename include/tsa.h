@@ -254,6 +254,100 @@ int tsa_ggml_gated_delta_net(const tsa_tensor* q, const tsa_tensor* k, const tsa
                              const tsa_tensor* state_out, float scale, void* ws,
                              size_t ws_bytes, void* stream);
 
+/* ---- The 8-bit K/V cache of the attention layers, and the attention that reads it.  The
+ * reference has no cache (its lab runs whole prompts); a server of its target model keeps one per
+ * attention layer, next to the GDN layers' state.
+ *
+ * A sequence is cut into blocks of 64 tokens.  A full block's keys (values) of one K/V head are
+ * 64 x D codes of 8 bits with one fp32 scale: with a = max|x| over the block (at least 2^-24),
+ * scale = a / 127 and code = rint(127 x / a), ties to even; the cache stands for code * scale.
+ * A block with an infinity or NaN has the scale NaN and reads as NaN.  The tokens behind the last
+ * full block stay fp16, so what a block holds does not depend on how its tokens came.  Blocks lie
+ * in pages named by a table: block i of sequence b is page table[b * max_blocks + i].  A page
+ * number outside 0 .. n_pages - 1 names no page: what would be written there is dropped, and its
+ * keys are seen by no query.  Sequences may share pages of full blocks.
+ *
+ * All buffers are the caller's, on the device, 16-byte aligned, sizes in bytes:
+ *   k, v                  n_pages * Hkv * 64 * D     codes, in an order of this library's own
+ *   k_scale, v_scale      n_pages * Hkv * 4
+ *   k_sum, k_sum_scale    n_pages * Hkv * D, n_pages * Hkv * 4   a block's keys summed: 8-bit
+ *                         codes c with rint(127 c / max|c|), their scale k_scale * max|c| / (64 * 127)
+ *   k_open, v_open        B * 2 * Hkv * 64 * D * 2   fp16 rows of the last two blocks
+ *   table                 B * max_blocks int32
+ * len (int32 [B], on the device) counts each sequence's tokens, the call's new ones among them;
+ * n_new (int32 [B], or NULL for T each) says how many of the call's T rows are new tokens, the
+ * rows behind them being padding that is neither read nor written.  New token t of a sequence is
+ * at position len - n_new + t.  len is taken as at most 64 * max_blocks and at least 0, n_new as
+ * at most T and at least 0; new tokens in front of position 0 (n_new > len) are not written and
+ * see no key.  After a write, a sequence may be cut back (a smaller len) by up to 64 tokens.
+ * Calls on one cache must be ordered on one stream (or by the caller's events). ---- */
+typedef struct tsa_kv8 {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    void* k_sum;
+    float* k_sum_scale;
+    void* k_open;
+    void* v_open;
+    const int32_t* table;
+    int B, Hkv, D, n_pages, max_blocks;
+} tsa_kv8;
+
+/* Rows of D consecutive fp16 elements, 16-byte aligned: row (b, h, t) starts at element
+ * b * stride_b + h * stride_h + t * stride_t (multiples of 8, at least 0; of an output, above 0
+ * where its dimension is longer than 1). */
+typedef struct tsa_rows {
+    void* data;
+    int64_t stride_b, stride_h, stride_t;
+} tsa_rows;
+
+/* Writes T rows of keys and values (k, v [B][Hkv][T][D]) at the end of each sequence. */
+int tsa_kv8_write(const tsa_kv8* cache, const tsa_rows* k, const tsa_rows* v, const int32_t* len,
+                  const int32_t* n_new, int T, void* stream);
+
+/* Reads positions start .. start + S - 1 of each sequence back as fp16 (start: int32 [B] on the
+ * device, NULL for 0; k, v [B][Hkv][S][D], either may be NULL).  Rows of positions behind the
+ * sequence or without a page are left as they were. */
+int tsa_kv8_read(const tsa_kv8* cache, const int32_t* len, const int32_t* start, int S, const tsa_rows* k,
+                 const tsa_rows* v, void* stream);
+
+/* Workspace bytes of the calls below for T rows of Hq query heads; max_len: no sequence is longer
+ * (at most 64 * max_blocks).  top = 0: tsa_attn_kv8_fwd; top > 0: tsa_kv8_select and
+ * tsa_attn_kv8_blocks_fwd, which may share one workspace.  0 for invalid arguments, and where no
+ * workspace is needed.  Calls that share a workspace must be ordered on one stream. */
+size_t tsa_kv8_workspace_bytes(const tsa_kv8* cache, int T, int Hq, int max_len, int top);
+
+/* Attention of T new tokens per sequence over the cache that holds them already (write first):
+ * O = softmax(scale * q K^T) V over the keys j <= the query's position (causal = 1) or j < len,
+ * times sigmoid(gate) when gate is not NULL.  q, gate, o [B][Hq][T][D], Hq % Hkv == 0, query head
+ * h reads K/V head h / (Hq / Hkv); D in {64, 128, 256}.  A query that sees no key gets 0.  o may
+ * be q.  max_len: no sequence is longer; it decides only how the keys are split over workgroups
+ * (results for longer ones are right as well). */
+int tsa_attn_kv8_fwd(const tsa_kv8* cache, const tsa_rows* q, const tsa_rows* gate, const tsa_rows* o,
+                     const int32_t* len, const int32_t* n_new, int T, int Hq, int max_len, float scale, int causal,
+                     void* ws, size_t ws_bytes, void* stream);
+
+/* The blocks that each query attends to, by a cheap score.  With A = max|q| over the heads of a
+ * group (Hq / Hkv of them), qc = rint(127 q / A): score(block) = max over the heads of
+ * sum_d qc[d] k_sum[d], a whole number, times k_sum_scale (one fp32 product).  A query at position
+ * p keeps, of the blocks 0 .. p / 64: the first `first`, its own and the `recent` before it, and
+ * then the best scores, the lowest index first among equals, up to `top` in all
+ * (top >= first + recent + 1).  A full block that holds an infinity or NaN, or has no page, scores
+ * below every other; a group with an infinity or NaN scores every block 0.
+ * blocks: int32 [B][Hkv][T][top], ascending, -1 behind the last; rows of padding are left as they
+ * were.  Blocks behind max_len have no score. */
+int tsa_kv8_select(const tsa_kv8* cache, const tsa_rows* q, const int32_t* len, const int32_t* n_new, int T, int Hq,
+                   int top, int first, int recent, int32_t* blocks, int max_len, void* ws, size_t ws_bytes,
+                   void* stream);
+
+/* tsa_attn_kv8_fwd (causal) over listed blocks only: query (b, t) of K/V head h's group attends to
+ * the blocks blocks[b][h][t][0 .. top - 1].  Entries that are no block of the sequence up to the
+ * query's own are passed over; a block listed twice counts twice. */
+int tsa_attn_kv8_blocks_fwd(const tsa_kv8* cache, const tsa_rows* q, const tsa_rows* gate, const tsa_rows* o,
+                            const int32_t* len, const int32_t* n_new, int T, int Hq, const int32_t* blocks, int top,
+                            float scale, void* ws, size_t ws_bytes, void* stream);
+
 /* The lab's naive GDN check on the device: one thread per state column, fp32, state read
  * and written in global memory, the order of gdn_cpu (src/gdn_sm75.cu:1078-1106) and
  * gdn_serial_kernel (:57-92).  Used by the gdn driver's error check.  Any dk, dv >= 1. */

@@ -881,3 +881,7 @@ hipError_t attn_naive(const void* q, const void* k, const void* v, const void* g
 }
 
 }  // namespace tsa
+
+// Attention over the 8-bit K/V cache: every block, and blocks that a cheap score selects.
+#include "kv8_attn.h"
+#include "kv8_select.h"

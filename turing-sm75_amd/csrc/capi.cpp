@@ -4,6 +4,7 @@
 // way on machines without a GPU.  The launch functions in kernels.h assume valid input.
 #include <climits>
 #include <cmath>
+#include <cstdint>
 
 #include "../../include/tsa.h"
 #include "kernels.h"
@@ -64,7 +65,7 @@ extern "C" const char* tsa_strerror(int code) {
         case TSA_ERR_UNSUPPORTED: return "shape not supported by this library (attention: D in {64,128,256}; GDN: dk = dv = 128, chunk = 64)";
         case TSA_ERR_WORKSPACE: return "workspace is NULL or smaller than the required size";
         case TSA_ERR_LAUNCH: return "the HIP runtime rejected a kernel launch";
-        case TSA_ERR_ARG: return "invalid argument (causal not 0/1, scale not finite / not > 0, or eps not finite / not > 0)";
+        case TSA_ERR_ARG: return "invalid argument (causal not 0/1, scale not finite / not > 0, eps not finite / not > 0, 8-bit cache: misaligned rows, or top < first + recent + 1)";
         case TSA_ERR_SCRATCH: return "the shapes need more than the 64 MiB device scratch of tsa_gdn_chunked_fwd_noalloc (use tsa_gdn_chunked_fwd with a workspace)";
         default: return "unknown tsa error code";
     }
@@ -322,4 +323,145 @@ extern "C" int tsa_gdn_gated_rmsnorm(const void* x, const void* z, const float* 
     if (!(eps > 0.f) || !std::isfinite(eps)) return TSA_ERR_ARG;
     if (!fits_int(B, T, Hv)) return TSA_ERR_SHAPE;
     return from_hip(tsa::gdn_gated_rmsnorm(x, z, w, y, B, T, Hv, eps, as_stream(stream)));
+}
+
+// ---- the 8-bit K/V cache ----
+namespace {
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int check_kv8(const tsa_kv8* c) {
+    if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale || !c->k_sum || !c->k_sum_scale || !c->k_open || !c->v_open || !c->table)
+        return TSA_ERR_NULL;
+    if (c->B < 1 || c->Hkv < 1 || c->D < 1 || c->n_pages < 1 || c->max_blocks < 1) return TSA_ERR_SHAPE;
+    if (c->D != 64 && c->D != 128 && c->D != 256) return TSA_ERR_UNSUPPORTED;
+    // positions are ints, a workgroup per (sequence, K or V, head) at least
+    if (c->max_blocks > INT_MAX / 64 - 1 || !fits_int(c->B, c->Hkv) || c->B > 65535 || c->Hkv > 32767 ||
+        (long long)c->B * c->Hkv > 65535)
+        return TSA_ERR_SHAPE;
+    if (!aligned16(c->k) || !aligned16(c->v) || !aligned16(c->k_sum) || !aligned16(c->k_open) || !aligned16(c->v_open))
+        return TSA_ERR_ARG;
+    return TSA_OK;
+}
+
+int check_rows(const tsa_rows* r, int B, int H, int T, bool out) {
+    if (!r || !r->data) return TSA_ERR_NULL;
+    if (!aligned16(r->data)) return TSA_ERR_ARG;
+    const int64_t stride[3] = {r->stride_b, r->stride_h, r->stride_t};
+    const int size[3] = {B, H, T};
+    for (int i = 0; i < 3; ++i)
+        if (size[i] > 1 && (stride[i] < (out ? 1 : 0) || stride[i] % 8 != 0)) return TSA_ERR_ARG;
+    return TSA_OK;
+}
+
+tsa::Kv8 as_kv8(const tsa_kv8* c) {
+    return {static_cast<unsigned char*>(c->k), static_cast<unsigned char*>(c->v), c->k_scale, c->v_scale,
+            static_cast<signed char*>(c->k_sum), c->k_sum_scale, static_cast<_Float16*>(c->k_open),
+            static_cast<_Float16*>(c->v_open), c->table, c->B, c->Hkv, c->D, c->n_pages, c->max_blocks};
+}
+
+// Strides of dimensions of one row are not looked at by the caller: 0 here, so that none is used.
+tsa::Rows16 as_rows(const tsa_rows* r, int B, int H, int T) {
+    if (!r || !r->data) return {nullptr, 0, 0, 0};
+    return {static_cast<_Float16*>(r->data), B > 1 ? r->stride_b : 0, H > 1 ? r->stride_h : 0, T > 1 ? r->stride_t : 0};
+}
+
+// Queries: rows per K/V head and workgroups must fit an int.
+int check_kv8_queries(const tsa_kv8* c, int T, int Hq) {
+    if (T < 1 || Hq < 1 || Hq % c->Hkv != 0) return TSA_ERR_SHAPE;
+    if (!fits_int(c->B, Hq, T) || !fits_int(T, c->max_blocks)) return TSA_ERR_SHAPE;
+    return TSA_OK;
+}
+
+int kv8_nb(const tsa_kv8* c, int max_len) {
+    const int nb = (int)((max_len + 63LL) / 64);
+    return nb < c->max_blocks ? nb : c->max_blocks;
+}
+
+int check_kv8_attn(const tsa_kv8* c, const tsa_rows* q, const tsa_rows* gate, const tsa_rows* o, const int32_t* len,
+                   int T, int Hq, float scale) {
+    int rc = check_kv8(c);
+    if (rc) return rc;
+    if (!len) return TSA_ERR_NULL;
+    if ((rc = check_kv8_queries(c, T, Hq))) return rc;
+    if ((rc = check_rows(q, c->B, Hq, T, false)) || (rc = check_rows(o, c->B, Hq, T, true))) return rc;
+    if (gate && (rc = check_rows(gate, c->B, Hq, T, false))) return rc;
+    if (!(scale > 0.f) || !std::isfinite(scale)) return TSA_ERR_ARG;
+    return TSA_OK;
+}
+
+}  // namespace
+
+extern "C" int tsa_kv8_write(const tsa_kv8* cache, const tsa_rows* k, const tsa_rows* v, const int32_t* len,
+                             const int32_t* n_new, int T, void* stream) {
+    int rc = check_kv8(cache);
+    if (rc) return rc;
+    if (!len) return TSA_ERR_NULL;
+    if (T < 1 || T > INT_MAX - 64) return TSA_ERR_SHAPE;
+    if ((rc = check_rows(k, cache->B, cache->Hkv, T, false)) || (rc = check_rows(v, cache->B, cache->Hkv, T, false))) return rc;
+    return from_hip(tsa::kv8_write(as_kv8(cache), as_rows(k, cache->B, cache->Hkv, T), as_rows(v, cache->B, cache->Hkv, T),
+                                   len, n_new, T, as_stream(stream)));
+}
+
+extern "C" int tsa_kv8_read(const tsa_kv8* cache, const int32_t* len, const int32_t* start, int S, const tsa_rows* k,
+                            const tsa_rows* v, void* stream) {
+    int rc = check_kv8(cache);
+    if (rc) return rc;
+    if (!len || (!k && !v)) return TSA_ERR_NULL;
+    if (S < 1 || S > INT_MAX - 64) return TSA_ERR_SHAPE;
+    if (k && (rc = check_rows(k, cache->B, cache->Hkv, S, true))) return rc;
+    if (v && (rc = check_rows(v, cache->B, cache->Hkv, S, true))) return rc;
+    return from_hip(tsa::kv8_read(as_kv8(cache), len, start, S, as_rows(k, cache->B, cache->Hkv, S),
+                                  as_rows(v, cache->B, cache->Hkv, S), as_stream(stream)));
+}
+
+extern "C" size_t tsa_kv8_workspace_bytes(const tsa_kv8* cache, int T, int Hq, int max_len, int top) {
+    if (check_kv8(cache) || check_kv8_queries(cache, T, Hq) || max_len < 1 || top < 0) return 0;
+    return tsa::kv8_ws_bytes(cache->B, T, Hq, cache->Hkv, cache->D, kv8_nb(cache, max_len), top);
+}
+
+extern "C" int tsa_attn_kv8_fwd(const tsa_kv8* cache, const tsa_rows* q, const tsa_rows* gate, const tsa_rows* o,
+                                const int32_t* len, const int32_t* n_new, int T, int Hq, int max_len, float scale,
+                                int causal, void* ws, size_t ws_bytes, void* stream) {
+    const int rc = check_kv8_attn(cache, q, gate, o, len, T, Hq, scale);
+    if (rc) return rc;
+    if (max_len < 1) return TSA_ERR_SHAPE;
+    if (causal != 0 && causal != 1) return TSA_ERR_ARG;
+    const int B = cache->B, nb = kv8_nb(cache, max_len);
+    const size_t need = tsa::kv8_ws_bytes(B, T, Hq, cache->Hkv, cache->D, nb, 0);
+    if (need && (!ws || ws_bytes < need)) return TSA_ERR_WORKSPACE;
+    return from_hip(tsa::kv8_attn(as_kv8(cache), as_rows(q, B, Hq, T), as_rows(gate, B, Hq, T), as_rows(o, B, Hq, T), len,
+                                  n_new, T, Hq, nb, scale, causal, ws, as_stream(stream)));
+}
+
+extern "C" int tsa_kv8_select(const tsa_kv8* cache, const tsa_rows* q, const int32_t* len, const int32_t* n_new, int T,
+                              int Hq, int top, int first, int recent, int32_t* blocks, int max_len, void* ws,
+                              size_t ws_bytes, void* stream) {
+    int rc = check_kv8(cache);
+    if (rc) return rc;
+    if (!len || !blocks) return TSA_ERR_NULL;
+    if ((rc = check_kv8_queries(cache, T, Hq))) return rc;
+    if (max_len < 1 || top < 1 || first < 0 || recent < 0) return TSA_ERR_SHAPE;
+    if ((long long)first + recent + 1 > top) return TSA_ERR_ARG;
+    if ((long long)Hq / cache->Hkv > 256) return TSA_ERR_UNSUPPORTED;
+    const int B = cache->B, nb = kv8_nb(cache, max_len);
+    if ((rc = check_rows(q, B, Hq, T, false))) return rc;
+    const size_t need = tsa::kv8_ws_bytes(B, T, Hq, cache->Hkv, cache->D, nb, top);
+    if (need && (!ws || ws_bytes < need)) return TSA_ERR_WORKSPACE;
+    return from_hip(tsa::kv8_select(as_kv8(cache), as_rows(q, B, Hq, T), len, n_new, T, Hq, top, first, recent, blocks, nb,
+                                    ws, as_stream(stream)));
+}
+
+extern "C" int tsa_attn_kv8_blocks_fwd(const tsa_kv8* cache, const tsa_rows* q, const tsa_rows* gate, const tsa_rows* o,
+                                       const int32_t* len, const int32_t* n_new, int T, int Hq, const int32_t* blocks,
+                                       int top, float scale, void* ws, size_t ws_bytes, void* stream) {
+    const int rc = check_kv8_attn(cache, q, gate, o, len, T, Hq, scale);
+    if (rc) return rc;
+    if (!blocks) return TSA_ERR_NULL;
+    if (top < 1) return TSA_ERR_SHAPE;
+    const int B = cache->B;
+    const size_t need = tsa::kv8_ws_bytes(B, T, Hq, cache->Hkv, cache->D, 1, top);
+    if (need && (!ws || ws_bytes < need)) return TSA_ERR_WORKSPACE;
+    return from_hip(tsa::kv8_attn_blocks(as_kv8(cache), as_rows(q, B, Hq, T), as_rows(gate, B, Hq, T), as_rows(o, B, Hq, T),
+                                         len, n_new, T, Hq, blocks, top, scale, ws, as_stream(stream)));
 }

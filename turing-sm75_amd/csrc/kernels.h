@@ -99,4 +99,36 @@ hipError_t gdn_naive(const void* q, const void* k, const void* v, const float* g
                      const float* beta, float* state, void* out, int B, int T, int Hq, int Hv,
                      int dk, int dv, float scale, bool f32, hipStream_t stream);
 
+// The 8-bit K/V cache (tsa_kv8 of include/tsa.h, with typed pointers) and fp16 rows of D
+// elements that lie anywhere (tsa_rows).  len, n_new: device arrays [B]; n_new may be null.
+struct Kv8 {
+    unsigned char *k, *v;
+    float *k_scale, *v_scale;
+    signed char* k_sum;
+    float* k_sum_scale;
+    _Float16 *k_open, *v_open;
+    const int* table;
+    int B, Hkv, D, n_pages, max_blocks;
+};
+struct Rows16 {
+    _Float16* data;
+    long long b, h, t;
+};
+hipError_t kv8_write(const Kv8& c, const Rows16& k, const Rows16& v, const int* len, const int* n_new, int T,
+                     hipStream_t stream);
+hipError_t kv8_read(const Kv8& c, const int* len, const int* start, int S, const Rows16& k, const Rows16& v,
+                    hipStream_t stream);
+// Workspace of an attention call (blocks of its keys: nb) or, with top > 0, of a selection and
+// the attention over it.
+size_t kv8_ws_bytes(int B, int T, int Hq, int Hkv, int D, int nb, int top);
+// nb_hint: the longest sequence's blocks as the caller knows it; any length is right.
+hipError_t kv8_attn(const Kv8& c, const Rows16& q, const Rows16& gate, const Rows16& o, const int* len,
+                    const int* n_new, int T, int Hq, int nb_hint, float scale, int causal, void* ws,
+                    hipStream_t stream);
+hipError_t kv8_select(const Kv8& c, const Rows16& q, const int* len, const int* n_new, int T, int Hq, int top,
+                      int first, int recent, int* blocks, int nb_hint, void* ws, hipStream_t stream);
+hipError_t kv8_attn_blocks(const Kv8& c, const Rows16& q, const Rows16& gate, const Rows16& o, const int* len,
+                           const int* n_new, int T, int Hq, const int* blocks, int top, float scale, void* ws,
+                           hipStream_t stream);
+
 }  // namespace tsa

@@ -1,0 +1,73 @@
+// kv8.h -- the 8-bit K/V cache: where its elements lie, shared by the kernels that write it
+// (kv8_cache.h), attend to it (kv8_attn.h) and select blocks of it (kv8_select.h).
+//
+// A block is 64 tokens of one sequence.  A full block of one K/V head is 64 x D codes, a byte
+// each (code + 128, code = rint(127 x / max|x|) in -127 .. 127), with one fp32 scale max|x| / 127.
+// The tokens behind the last full block are fp16 rows in a ring of two blocks per sequence, so a
+// sequence may be cut back by up to a block.
+//
+// Both are laid out as the operands of v_mfma_f32_16x16x32_f16 (lane l holds row l % 16 and 8
+// consecutive k at 8 * (l / 16)), so that a wave reads 1 KiB of consecutive codes per load, 16
+// bytes a lane, and no transpose is left for the attention:
+//   K, operand A of S^T = K Q^T: the 16 bytes of lane l in tile (a, i) are key 16 a + l % 16,
+//      d = 64 i + 16 (l / 16) + 0 .. 15: the first 8 are one k-step, the last 8 another (k is
+//      any order of d that Q follows too);
+//   V, operand A of O^T = V^T P^T: the 16 bytes of lane l in tile dt are d = 16 dt + l % 16, keys
+//      16 i + 4 (l / 16) + e for byte 4 i + e: the keys whose P the lane holds after S^T, so P
+//      needs no exchange.  Bytes 0 .. 7 (keys below 32) are one k-step, the others the second.
+// The ring holds its fp16 elements in the same order.
+#pragma once
+#include <stdint.h>
+
+#include "common.h"
+#include "kernels.h"
+
+namespace tsa {
+namespace {
+
+constexpr int kKvBlock = 64;
+
+// Element offset of (key r, d) within a block of one head.
+template <int D>
+__device__ __forceinline__ int kv8_k_at(int r, int d) {
+    return ((((r >> 4) * (D / 64) + (d >> 6)) * 4 + ((d >> 4) & 3)) * 16 + (r & 15)) * 16 + (d & 15);
+}
+template <int D>
+__device__ __forceinline__ int kv8_v_at(int r, int d) {
+    return (((d >> 4) * 4 + ((r >> 2) & 3)) * 16 + (d & 15)) * 16 + (r >> 4) * 4 + (r & 3);
+}
+template <int D>
+__device__ __forceinline__ int kv8_at(bool isv, int r, int d) {
+    return isv ? kv8_v_at<D>(r, d) : kv8_k_at<D>(r, d);
+}
+
+// A sequence's tokens: `len` of them, the last `n` new; rows of a call's T start at new row `t0`
+// (rows before it would lie in front of the sequence).  Every count is clamped to what the cache
+// and the call hold, so that no value of the device arrays leads out of bounds.
+struct Kv8Seq {
+    int len, n, t0;
+};
+__device__ __forceinline__ Kv8Seq kv8_seq(const Kv8& c, const int* __restrict__ len, const int* __restrict__ n_new,
+                                          int b, int T) {
+    Kv8Seq s;
+    s.len = min(max(len[b], 0), c.max_blocks * kKvBlock);
+    const int n = n_new ? min(max(n_new[b], 0), T) : T;
+    s.n = min(n, s.len);
+    s.t0 = n - s.n;
+    return s;
+}
+
+// The page of block `blk` of sequence b, -1 where the table names none.
+__device__ __forceinline__ int kv8_page(const Kv8& c, int b, int blk) {
+    const int p = c.table[(size_t)b * c.max_blocks + blk];
+    return p >= 0 && p < c.n_pages ? p : -1;
+}
+
+// The ring's fp16 block of (sequence, head) that block blk uses, as an element offset.
+template <int D>
+__device__ __forceinline__ size_t kv8_open_at(const Kv8& c, int b, int h, int blk) {
+    return ((size_t)(b * 2 + (blk & 1)) * c.Hkv + h) * (kKvBlock * D);
+}
+
+}  // namespace
+}  // namespace tsa

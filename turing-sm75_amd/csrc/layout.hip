@@ -48,3 +48,6 @@ hipError_t copy4d(const void* src, int src_f16, const View4& s, void* dst, int d
 }
 
 }  // namespace tsa
+
+// The 8-bit K/V cache keeps its blocks in the order of the matrix instructions' operands.
+#include "kv8_cache.h"

@@ -43,6 +43,19 @@ class TsaTensor(ctypes.Structure):
                 ("ne", ctypes.c_int64 * 4), ("nb", ctypes.c_size_t * 4)]
 
 
+class TsaKv8(ctypes.Structure):
+    """The tsa_kv8 cache of include/tsa.h."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "k_sum", "k_sum_scale", "k_open",
+                                               "v_open", "table")] + \
+               [(n, ctypes.c_int) for n in ("B", "Hkv", "D", "n_pages", "max_blocks")]
+
+
+class TsaRows(ctypes.Structure):
+    """The tsa_rows view of include/tsa.h."""
+    _fields_ = [("data", ctypes.c_void_p), ("stride_b", ctypes.c_int64), ("stride_h", ctypes.c_int64),
+                ("stride_t", ctypes.c_int64)]
+
+
 _tp = ctypes.POINTER(TsaTensor)
 
 
@@ -75,6 +88,12 @@ _SIGNATURES = {
     "tsa_gdn_gated_rmsnorm": (_i, [_vp] * 4 + [_i] * 4 + [_f, _vp]),
     "tsa_ggml_gdn_workspace_bytes": (_sz, [_tp, _tp]),
     "tsa_ggml_gated_delta_net": (_i, [_tp] * 8 + [_f, _vp, _sz, _vp]),
+    "tsa_kv8_write": (_i, [_vp] * 5 + [_i, _vp]),
+    "tsa_kv8_read": (_i, [_vp] * 3 + [_i] + [_vp] * 3),
+    "tsa_kv8_workspace_bytes": (_sz, [_vp] + [_i] * 4),
+    "tsa_attn_kv8_fwd": (_i, [_vp] * 6 + [_i] * 3 + [_f, _i, _vp, _sz, _vp]),
+    "tsa_kv8_select": (_i, [_vp] * 4 + [_i] * 5 + [_vp, _i, _vp, _sz, _vp]),
+    "tsa_attn_kv8_blocks_fwd": (_i, [_vp] * 6 + [_i] * 2 + [_vp, _i, _f, _vp, _sz, _vp]),
 }
 
 
@@ -486,4 +505,222 @@ def ggml_gated_delta_net(q, k, v, g_log, beta, state, out, state_out=None, scale
         [_pack_view(x) for x in (q, k, v, g_log, beta, state, out, state_out)])))
     _check(load().tsa_ggml_gated_delta_net(*views, float(scale), _ptr(ws), ws.numel() * ws.element_size(),
                                            _stream(stream)))
+    return out
+
+
+# ---------------------------------------------------------------------------------------
+# the 8-bit K/V cache and the attention that reads it
+# ---------------------------------------------------------------------------------------
+KV8_BLOCK = 64
+
+
+class Kv8Cache:
+    """The 8-bit K/V cache of one attention layer for B sequences of at most max_len tokens: codes
+    and scales of full blocks of 64 tokens in n_pages pages, the open blocks' rows in fp16
+    (include/tsa.h, tsa_kv8).  Without n_pages every sequence has pages of its own for max_len
+    tokens; with it, `table` ([B, blocks] int32, -1: no page) is the caller's to fill, in place,
+    before a block is written or read."""
+
+    def __init__(self, B, Hkv, D, max_len, n_pages=None, device="cuda"):
+        torch = _torch or _t()
+        if torch.device(device).type != "cuda":
+            raise ValueError(f"a cache lies on a GPU, not on {device}")
+        for name, x in (("B", B), ("Hkv", Hkv), ("max_len", max_len)):
+            if x < 1:
+                raise ValueError(f"{name} must be at least 1, got {x}")
+        if D not in (64, 128, 256):
+            raise ValueError(f"D must be 64, 128 or 256, got {D}")
+        blocks = -(-max_len // KV8_BLOCK)
+        own = n_pages is None
+        if own:
+            n_pages = B * blocks
+        if n_pages < 1:
+            raise ValueError(f"n_pages must be at least 1, got {n_pages}")
+        z = lambda dtype, *shape: torch.zeros(*shape, dtype=dtype, device=device)  # noqa: E731
+        self.k, self.v = (z(torch.uint8, n_pages, Hkv, KV8_BLOCK * D) for _ in range(2))
+        self.k_scale, self.v_scale, self.k_sum_scale = (z(torch.float32, n_pages, Hkv) for _ in range(3))
+        self.k_sum = z(torch.int8, n_pages, Hkv, D)
+        self.k_open, self.v_open = (z(torch.float16, B, 2, Hkv, KV8_BLOCK * D) for _ in range(2))
+        self.table = torch.arange(n_pages, dtype=torch.int32, device=device).view(B, blocks) if own else \
+            torch.full((B, blocks), -1, dtype=torch.int32, device=device)
+        self.B, self.Hkv, self.D, self.n_pages, self.max_blocks = B, Hkv, D, n_pages, blocks
+        self.max_len = blocks * KV8_BLOCK
+        self.device = self.k.device
+        self.view = TsaKv8(*(_ptr(getattr(self, n)) for n, _ in TsaKv8._fields_[:9]), B, Hkv, D, n_pages, blocks)
+        self._ref = ctypes.byref(self.view)
+
+
+# a tsa_rows as bytes: data, strides of b, h and t
+_ROWS = struct.Struct("@P3q")
+assert _ROWS.size == ctypes.sizeof(TsaRows)
+
+
+def _rows(t, shape, name, cache):
+    """A [B, H, T, D] fp16 tensor on the cache's device as a tsa_rows: rows of consecutive elements,
+    any other strides."""
+    torch = _torch or _t()
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype is not torch.float16 or t.device != cache.device or t.shape != shape or t.stride(3) != 1:
+        raise ValueError(f"{name}: expected fp16 {tuple(shape)} on {cache.device} with consecutive row elements, got "
+                         f"{tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}")
+    return _ROWS.pack(t.data_ptr(), *t.stride()[:3])
+
+
+def _counts(t, name, cache):
+    torch = _torch or _t()
+    if t is None:
+        return None
+    if t.dtype is not torch.int32 or t.device != cache.device or t.shape != (cache.B,) or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous int32 tensor of {cache.B} on {cache.device}, got "
+                         f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
+class _on:
+    """The cache's device as the current one for the length of a call, where it is another."""
+
+    def __init__(self, device):
+        torch = _torch or _t()
+        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *a):
+        if self.guard is not None:
+            self.guard.__exit__(*a)
+
+
+def _len(t, cache):
+    if t is None:
+        raise TypeError("len must be a torch.Tensor")
+    return _counts(t, "len", cache)
+
+
+def kv8_write(cache, k, v, len, n_new=None, stream=None):
+    """Writes k, v [B, Hkv, T, D] fp16 (rows of consecutive elements, any other strides) at the end of
+    each sequence: len [B] int32 counts its tokens, these among them; n_new [B] int32 (default T each)
+    says how many of the T rows are tokens, the rest is padding."""
+    T = k.shape[2]
+    shape = (cache.B, cache.Hkv, T, cache.D)
+    r = (TsaRows * 2).from_buffer(bytearray(_rows(k, shape, "k", cache) + _rows(v, shape, "v", cache)))
+    with _on(cache.device):
+        _check(load().tsa_kv8_write(cache._ref, ctypes.byref(r), ctypes.byref(r, 32), _len(len, cache),
+                                    _counts(n_new, "n_new", cache), T, _stream(stream)))
+
+
+def kv8_read(cache, len, S=None, start=None, k_out=None, v_out=None, stream=None):
+    """Positions start .. start + S - 1 of each sequence (start [B] int32, default 0) as fp16 k, v
+    [B, Hkv, S, D]; rows of positions behind the sequence or without a page are left as they were
+    (0 in outputs made here)."""
+    torch = _torch or _t()
+    if S is None:
+        S = k_out.shape[2] if k_out is not None else v_out.shape[2] if v_out is not None else cache.max_len
+    shape = (cache.B, cache.Hkv, S, cache.D)
+    if k_out is None and v_out is None:
+        k_out, v_out = (torch.zeros(shape, dtype=torch.float16, device=cache.device) for _ in range(2))
+    packs = [None if t is None else _rows(t, shape, n, cache) for t, n in ((k_out, "k_out"), (v_out, "v_out"))]
+    r = (TsaRows * 2).from_buffer(bytearray(b"".join(p or bytes(32) for p in packs)))
+    with _on(cache.device):
+        _check(load().tsa_kv8_read(cache._ref, _len(len, cache), _counts(start, "start", cache), S,
+                                   ctypes.byref(r) if packs[0] else None, ctypes.byref(r, 32) if packs[1] else None,
+                                   _stream(stream)))
+    return k_out, v_out
+
+
+def kv8_workspace_bytes(cache, T, Hq, max_len=None, top=0) -> int:
+    """Workspace bytes of attn_kv8_fwd (top = 0), or of kv8_select and attn_kv8_blocks_fwd, which may
+    share one (top > 0)."""
+    return int(load().tsa_kv8_workspace_bytes(cache._ref, T, Hq, cache.max_len if max_len is None else max_len, top))
+
+
+def _queries(q, cache, gate, out, extra):
+    """Views of q, gate and out, the output, and Hq, T; made before anything is launched."""
+    torch = _torch or _t()
+    if q.dim() != 4:
+        raise ValueError(f"q: expected [B, Hq, T, D], got {tuple(q.shape)}")
+    shape = (cache.B, q.shape[1], q.shape[2], cache.D)
+    packed = _rows(q, shape, "q", cache)
+    if gate is not None:
+        packed += _rows(gate, shape, "gate", cache)
+    else:
+        packed += bytes(32)
+    if out is None:
+        out = torch.zeros(shape, dtype=torch.float16, device=cache.device) if extra else \
+            torch.empty(shape, dtype=torch.float16, device=cache.device)
+    r = (TsaRows * 3).from_buffer(bytearray(packed + _rows(out, shape, "out", cache)))
+    return r, ctypes.byref(r, 32) if gate is not None else None, out, shape[1], shape[2]
+
+
+def _ws(ws, cache, T, Hq, max_len, top, stream):
+    if ws is None:
+        ws = _scratch(kv8_workspace_bytes(cache, T, Hq, max_len, top), cache.device, stream)
+    elif ws.device != cache.device or not ws.is_contiguous():
+        raise ValueError(f"ws: expected a contiguous tensor on {cache.device}, got one on {ws.device}")
+    return ws
+
+
+def attn_kv8_fwd(q, cache, len, n_new=None, gate=None, out=None, scale=None, causal=True, max_len=None, ws=None,
+                 stream=None):
+    """Attention of q [B, Hq, T, D], the last n_new tokens of each sequence (default T each), over the
+    cache that holds them already: softmax(scale q K^T) V over the keys up to each query's own
+    (causal) or all len of them, times sigmoid(gate) if given.  Hq % Hkv == 0.  Rows of padding (t >= n_new) are left
+    as they were (0 in an output made here).  max_len: no sequence is longer (a tighter split of the
+    keys; results do not depend on it)."""
+    r, gp, out, Hq, T = _queries(q, cache, gate, out, n_new is not None)
+    if max_len is None:
+        max_len = cache.max_len
+    with _on(cache.device):
+        ws = _ws(ws, cache, T, Hq, max_len, 0, stream)
+        _check(load().tsa_attn_kv8_fwd(
+            cache._ref, ctypes.byref(r), gp, ctypes.byref(r, 64), _len(len, cache), _counts(n_new, "n_new", cache), T, Hq,
+            max_len, 1.0 / math.sqrt(cache.D) if scale is None else float(scale), int(bool(causal)), _ptr(ws),
+            ws.numel() * ws.element_size(), _stream(stream)))
+    return out
+
+
+def _blocks(blocks, cache, T, top):
+    torch = _torch or _t()
+    if blocks.dtype is not torch.int32 or blocks.device != cache.device or not blocks.is_contiguous() or \
+            blocks.shape != (cache.B, cache.Hkv, T, top):
+        raise ValueError(f"blocks: expected contiguous int32 {(cache.B, cache.Hkv, T, top)} on {cache.device}, got "
+                         f"{tuple(blocks.shape)} {blocks.dtype} on {blocks.device}")
+    return blocks.data_ptr()
+
+
+def kv8_select(q, cache, len, top, n_new=None, first=1, recent=1, out=None, max_len=None, ws=None, stream=None):
+    """The blocks [B, Hkv, T, top] int32 that each query of q [B, Hq, T, D] attends to: the first
+    `first`, its own and the `recent` before it, and the best by score, ascending, -1 behind the last.
+    max_len: no sequence is longer (blocks behind it have no score)."""
+    torch = _torch or _t()
+    if q.dim() != 4:
+        raise ValueError(f"q: expected [B, Hq, T, D], got {tuple(q.shape)}")
+    _, Hq, T, _ = q.shape
+    r = TsaRows.from_buffer(bytearray(_rows(q, (cache.B, Hq, T, cache.D), "q", cache)))
+    if out is None:
+        out = torch.full((cache.B, cache.Hkv, T, top), -1, dtype=torch.int32, device=cache.device)
+    if max_len is None:
+        max_len = cache.max_len
+    with _on(cache.device):
+        ws = _ws(ws, cache, T, Hq, max_len, top, stream)
+        _check(load().tsa_kv8_select(
+            cache._ref, ctypes.byref(r), _len(len, cache), _counts(n_new, "n_new", cache), T, Hq, top, first, recent,
+            _blocks(out, cache, T, top), max_len, _ptr(ws), ws.numel() * ws.element_size(), _stream(stream)))
+    return out
+
+
+def attn_kv8_blocks_fwd(q, cache, len, blocks, n_new=None, gate=None, out=None, scale=None, ws=None, stream=None):
+    """attn_kv8_fwd (causal) over the listed blocks [B, Hkv, T, top] only (of kv8_select, or the
+    caller's own: entries that are no block up to the query's own are passed over, a block listed
+    twice counts twice)."""
+    r, gp, out, Hq, T = _queries(q, cache, gate, out, n_new is not None)
+    top = blocks.shape[-1]
+    with _on(cache.device):
+        ws = _ws(ws, cache, T, Hq, 1, top, stream)
+        _check(load().tsa_attn_kv8_blocks_fwd(
+            cache._ref, ctypes.byref(r), gp, ctypes.byref(r, 64), _len(len, cache), _counts(n_new, "n_new", cache), T, Hq,
+            _blocks(blocks, cache, T, top), top, 1.0 / math.sqrt(cache.D) if scale is None else float(scale), _ptr(ws),
+            ws.numel() * ws.element_size(), _stream(stream)))
     return out
