@@ -81,6 +81,25 @@ __device__ __forceinline__ float sum_xor32(float x) {
     return a + b;
 }
 
+// The same for lanes l and l ^ 16 (v_permlane16_swap: rows 1 and 3 of the first operand change
+// places with rows 0 and 2 of the second).
+__device__ __forceinline__ void rows16(float x, float& lo, float& hi) {
+    unsigned a = __builtin_bit_cast(unsigned, x), b = a;
+    asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+    lo = __builtin_bit_cast(float, a);
+    hi = __builtin_bit_cast(float, b);
+}
+__device__ __forceinline__ float max_xor16(float x) {
+    float a, b;
+    rows16(x, a, b);
+    return fmaxf(a, b);
+}
+__device__ __forceinline__ float sum_xor16(float x) {
+    float a, b;
+    rows16(x, a, b);
+    return a + b;
+}
+
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // The gates of the target model's Gated DeltaNet layer: softplus(x) = log(1 + e^x), with x

@@ -12,10 +12,12 @@
 //   K, operand A of S^T = K Q^T: the 16 bytes of lane l in tile (a, i) are key 16 a + l % 16,
 //      d = 64 i + 16 (l / 16) + 0 .. 15: the first 8 are one k-step, the last 8 another (k is
 //      any order of d that Q follows too);
-//   V, operand A of O^T = V^T P^T: the 16 bytes of lane l in tile dt are d = 16 dt + l % 16, keys
-//      16 i + 4 (l / 16) + e for byte 4 i + e: the keys whose P the lane holds after S^T, so P
-//      needs no exchange.  Bytes 0 .. 7 (keys below 32) are one k-step, the others the second.
-// The ring holds its fp16 elements in the same order.
+//   V, operand A of O^T = V^T P^T: the 16 bytes of lane l in tile (s, m) are keys 32 s + 16 i +
+//      4 (l / 16) + e of d = 32 m + 16 o + l % 16 for byte 8 o + 4 i + e: the keys whose P the lane
+//      holds after S^T, so P needs no exchange.  The first 8 bytes are tile 2 m of O^T, the others
+//      2 m + 1.
+// Both halves of a block (32 keys) are consecutive.  The ring holds its fp16 elements in the same
+// order.
 #pragma once
 #include <stdint.h>
 
@@ -34,7 +36,8 @@ __device__ __forceinline__ int kv8_k_at(int r, int d) {
 }
 template <int D>
 __device__ __forceinline__ int kv8_v_at(int r, int d) {
-    return (((d >> 4) * 4 + ((r >> 2) & 3)) * 16 + (d & 15)) * 16 + (r >> 4) * 4 + (r & 3);
+    return ((((r >> 5) * (D / 32) + (d >> 5)) * 4 + ((r >> 2) & 3)) * 16 + (d & 15)) * 16 + ((d >> 4) & 1) * 8 +
+           ((r >> 4) & 1) * 4 + (r & 3);
 }
 template <int D>
 __device__ __forceinline__ int kv8_at(bool isv, int r, int d) {

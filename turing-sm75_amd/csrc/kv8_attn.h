@@ -4,12 +4,16 @@
 // o = softmax(scale q K^T) V per query row, one pass over the keys with a running maximum.  With
 // codes k', v' and block scales sk, sv:
 //   score  u_j = scale log2(e) sk (q . k'_j) + log2(sv)      (fp32, k' exact in fp16)
-//   weight w_j = 2^(u_j - m + 12), m the running max of u    (fp16 operand of P V)
+//   weight w_j = 2^(u_j - m + 12), m a running max of u      (fp16 operand of P V)
 //   o = sum_j w_j v'_j / sum_j w_j / sv
 // The value scale goes into the exponent, so the matrix instructions see whole numbers only and a
-// weight is rounded once, whatever the blocks' scales are; 2^12 keeps weights down to 2^-36 of the
-// largest in fp16's range.
+// weight is rounded once, whatever the blocks' scales are.  m is raised only when a score passes it
+// by more than 3, so most blocks rescale nothing; weights reach up to 2^15 and keep fp16's whole
+// range below (2^-24 is 2^-36 of the largest's at least: with m raised past 8 and weights of 2^7
+// at m, small values next to a dominant key lost their last bits).
 #pragma once
+#include <climits>
+
 #include "kv8.h"
 
 namespace tsa {
@@ -24,7 +28,8 @@ struct Kv8AttnArgs {
     float c2;  // scale log2(e)
 };
 
-constexpr float kKvBias = 12.f;
+constexpr float kKvBias = 12.f;  // a weight at the running maximum is 2^12,
+constexpr float kKvSlack = 3.f;  // and up to 2^15 before the maximum is raised
 
 // 8 codes (two words) as fp16: the byte under 0x64 is 1024 + code + 128.
 __device__ __forceinline__ half8_t kv8_halves(unsigned w0, unsigned w1) {
@@ -37,15 +42,8 @@ __device__ __forceinline__ half8_t kv8_halves(unsigned w0, unsigned w1) {
     r.h[3] = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(hi, w1, 0x04030402u)) - off;
     return r.v;
 }
-
-// max / sum over the four lanes that hold a row's keys (l, l ^ 16, l ^ 32, l ^ 48).
-__device__ __forceinline__ float kv8_max4(float x) {
-    x = fmaxf(x, __shfl_xor(x, 16));
-    return max_xor32(x);
-}
-__device__ __forceinline__ float kv8_sum4(float x) {
-    x += __shfl_xor(x, 16);
-    return sum_xor32(x);
+__device__ __forceinline__ bool kv8_bad(half_t x) {
+    return (__builtin_bit_cast(unsigned short, x) & 0x7c00) == 0x7c00;
 }
 
 // A wave's state for NT tiles of 16 query rows: lane l owns row l % 16 of each.
@@ -57,177 +55,206 @@ struct Kv8State {
     int limit[NT];          // last key the row sees, -1: none
 };
 
-// One block's keys: kload(a, i, s) and vload(dt, s) give the operands, f the score factor, lsv
-// and isv the value scale's log2 and reciprocal, p0 the block's first key; w returns the weights.
-template <int D, int NT, class KLoad, class VLoad>
-__device__ __forceinline__ void kv8_block(Kv8State<D, NT>& st, int p0, float f, float lsv, float isv, KLoad kload,
-                                          VLoad vload, float4_t (&w)[NT][4]) {
-    const int lane = threadIdx.x & 63, g4 = lane >> 4;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int a = 0; a < 4; ++a) w[nt][a] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int a = 0; a < 4; ++a)
-#pragma unroll
-        for (int i = 0; i < D / 64; ++i)
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const half8_t kf = kload(a, i, s);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) w[nt][a] = mfma16(kf, st.q[nt][2 * i + s], w[nt][a]);
-            }
-    half8_t p[NT][2];
+// Scales of a block as the softmax takes them: the score's factor (scale log2(e) sk), log2(sv) and
+// 1 / sv.
+struct Kv8Scale {
+    float f, lsv, isv;
+};
+__device__ __forceinline__ Kv8Scale kv8_scale(const Kv8& c, int page, int h, float c2) {
+    const size_t head = (size_t)page * c.Hkv + h;
+    const float sv = c.v_scale[head];
+    return {c2 * c.k_scale[head], __builtin_amdgcn_logf(sv), __builtin_amdgcn_rcpf(sv)};
+}
+
+// Scores (w: raw q . k') to weights for 16 KA keys from p0 on: raises the running maximum where a
+// score passes it by more than the slack, rescaling what there is, and adds to the row sums.
+// `masked` (the same on all lanes): some row may not see all of the keys.
+template <int D, int NT, int KA>
+__device__ __forceinline__ void kv8_softmax(Kv8State<D, NT>& st, float4_t (&w)[NT][KA], int p0, const Kv8Scale& sc,
+                                            bool masked) {
+    const int k0 = p0 + 4 * ((threadIdx.x & 63) >> 4);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+        if (masked) {
+#pragma unroll
+            for (int a = 0; a < KA; ++a)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) w[nt][a][r] = k0 + 16 * a + r <= st.limit[nt] ? w[nt][a][r] : -INFINITY;
+        }
         float big = -INFINITY;
 #pragma unroll
-        for (int a = 0; a < 4; ++a)
+        for (int a = 0; a < KA; ++a)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float u = w[nt][a][r] * f + lsv;
-                w[nt][a][r] = p0 + 16 * a + 4 * g4 + r <= st.limit[nt] ? u : -INFINITY;
-                big = fmaxf(big, w[nt][a][r]);
-            }
-        big = kv8_max4(big);
-        const float m_new = fmaxf(st.m[nt], big);
-        if (__any(m_new != st.m[nt])) {
+            for (int r = 0; r < 4; ++r) big = fmaxf(big, w[nt][a][r]);
+        big = max_xor32(max_xor16(big));
+        big = __builtin_fmaf(big, sc.f, sc.lsv);
+        if (__any(big > st.m[nt] + kKvSlack)) {
+            const float m_new = fmaxf(st.m[nt], big);
             const float alpha = m_new == st.m[nt] ? 1.f : fast_exp2(st.m[nt] - m_new);
             st.m[nt] = m_new;
             st.l[nt] *= alpha;
 #pragma unroll
             for (int dt = 0; dt < D / 16; ++dt) st.o[nt][dt] *= alpha;
         }
-        const float ref = m_new == -INFINITY ? 0.f : m_new - kKvBias;
+        const float c = sc.lsv - (st.m[nt] == -INFINITY ? 0.f : st.m[nt] - kKvBias);
         float sum = 0.f;
 #pragma unroll
-        for (int a = 0; a < 4; ++a)
+        for (int a = 0; a < KA; ++a)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                w[nt][a][r] = fast_exp2(w[nt][a][r] - ref);
-                sum += w[nt][a][r];
-                p[nt][a >> 1][4 * (a & 1) + r] = (half_t)w[nt][a][r];
-            }
-        // a block of scale NaN adds nothing where every key is masked
-        st.l[nt] += sum == 0.f ? 0.f : sum * isv;
-    }
+            for (int r = 0; r < 4; ++r) w[nt][a][r] = fast_exp2(__builtin_fmaf(w[nt][a][r], sc.f, c));
+        if (masked) {  // again: of a block of scale NaN, a key that is not seen weighs 0
 #pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt)
+            for (int a = 0; a < KA; ++a)
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const half8_t vf = vload(dt, s);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) st.o[nt][dt] = mfma16(vf, p[nt][s], st.o[nt][dt]);
+                for (int r = 0; r < 4; ++r) w[nt][a][r] = k0 + 16 * a + r <= st.limit[nt] ? w[nt][a][r] : 0.f;
         }
+#pragma unroll
+        for (int a = 0; a < KA; ++a)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sum += w[nt][a][r];
+        st.l[nt] += sum == 0.f ? 0.f : sum * sc.isv;
+    }
+}
+// Weights of key tiles 2 s and 2 s + 1 as operand B.
+template <int KA>
+__device__ __forceinline__ half8_t kv8_weights(const float4_t (&w)[KA], int s) {
+    return half8_t{(half_t)w[2 * s][0],     (half_t)w[2 * s][1],     (half_t)w[2 * s][2],     (half_t)w[2 * s][3],
+                   (half_t)w[2 * s + 1][0], (half_t)w[2 * s + 1][1], (half_t)w[2 * s + 1][2], (half_t)w[2 * s + 1][3]};
 }
 
-__device__ __forceinline__ bool kv8_bad(half_t x) {
-    return (__builtin_bit_cast(unsigned short, x) & 0x7c00) == 0x7c00;
-}
-
-// A full block from its page.
-template <int D, int NT>
-__device__ __forceinline__ void kv8_page_block(Kv8State<D, NT>& st, const Kv8& c, int page, int h, int blk, float c2) {
-    const int lane = threadIdx.x & 63;
-    const size_t head = (size_t)page * c.Hkv + h;
-    const uint4* kp = reinterpret_cast<const uint4*>(c.k + head * (kKvBlock * D)) + lane;
-    const uint4* vp = reinterpret_cast<const uint4*>(c.v + head * (kKvBlock * D)) + lane;
-    const float sk = c.k_scale[head], sv = c.v_scale[head];
-    uint4 kr[4][D / 64], vr[D / 16];
-#pragma unroll
-    for (int a = 0; a < 4; ++a)
-#pragma unroll
-        for (int i = 0; i < D / 64; ++i) kr[a][i] = kp[(a * (D / 64) + i) * 64];
-#pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt) vr[dt] = vp[dt * 64];
-    float4_t w[NT][4];
-    kv8_block<D, NT>(
-        st, blk * kKvBlock, c2 * sk, __builtin_amdgcn_logf(sv), 1.f / sv,
-        [&](int a, int i, int s) { return s ? kv8_halves(kr[a][i].z, kr[a][i].w) : kv8_halves(kr[a][i].x, kr[a][i].y); },
-        [&](int dt, int s) { return s ? kv8_halves(vr[dt].z, vr[dt].w) : kv8_halves(vr[dt].x, vr[dt].y); }, w);
-}
-
-// The open block from the ring.  Values that are not finite are left out of the matrix products,
-// where a masked key's weight 0 would turn them into NaN for every query, and added for the
-// queries that see them.  Elements of rows behind the sequence are whatever the ring held.
-template <int D, int NT>
-__device__ __forceinline__ void kv8_open_block(Kv8State<D, NT>& st, const Kv8& c, int b, int h, int blk, int len, float c2) {
-    const int lane = threadIdx.x & 63, g4 = lane >> 4;
-    const size_t at = kv8_open_at<D>(c, b, h, blk);
-    const half_t* kp = c.k_open + at + lane * 16;
-    const half_t* vp = c.v_open + at + lane * 16;
-    const int p0 = blk * kKvBlock;
-    bool bad = false;
-    float4_t w[NT][4];
-    kv8_block<D, NT>(
-        st, p0, c2, 0.f, 1.f,
-        [&](int a, int i, int s) { return *reinterpret_cast<const half8_t*>(kp + (a * (D / 64) + i) * 1024 + 8 * s); },
-        [&](int dt, int s) {
-            half8_t v = *reinterpret_cast<const half8_t*>(vp + dt * 1024 + 8 * s);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int key = p0 + 32 * s + 16 * (j >> 2) + 4 * g4 + (j & 3);
-                const bool x = kv8_bad(v[j]);
-                bad |= x && key < len;
-                if (x || key >= len) v[j] = (half_t)0.f;
-            }
-            return v;
-        },
-        w);
-    if (!__any(bad)) return;
-    const half_t* vo = c.v_open + at;
+// 16 KA keys: kload(a, i, s) and vload(s, m, o) give the operands; between() is called where the
+// keys' operands are done with.
+template <int D, int NT, int KA, class KLoad, class VLoad, class Between>
+__device__ __forceinline__ void kv8_keys(Kv8State<D, NT>& st, int p0, const Kv8Scale& sc, bool masked, KLoad kload,
+                                         VLoad vload, Between between) {
+    float4_t w[NT][KA];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int a = 0; a < KA; ++a) w[nt][a] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int a = 0; a < KA; ++a) {
+                const half8_t kf = kload(a, i, s);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) w[nt][a] = mfma16(kf, st.q[nt][2 * i + s], w[nt][a]);
+            }
+    between();
+    kv8_softmax<D, NT, KA>(st, w, p0, sc, masked);
+#pragma unroll
+    for (int s = 0; s < KA / 2; ++s) {
+        half8_t p[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) p[nt] = kv8_weights<KA>(w[nt], s);
+#pragma unroll
+        for (int m = 0; m < D / 32; ++m)
+#pragma unroll
+            for (int o = 0; o < 2; ++o) {
+                const half8_t vf = vload(s, m, o);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) st.o[nt][2 * m + o] = mfma16(vf, p[nt], st.o[nt][2 * m + o]);
+            }
+    }
+}
+
+// The open block from the ring: n of its rows are the sequence's, those behind are whatever the
+// ring held.  Values that are not finite are left out of the matrix products, where a masked key's
+// weight 0 would turn them into NaN for every query, and added for the queries that see them.
+template <int D, int NT>
+__device__ __forceinline__ void kv8_open_block(Kv8State<D, NT>& st, const Kv8& c, int b, int h, int blk, int n, float c2) {
+    typedef unsigned uint4_v __attribute__((ext_vector_type(4)));
+    typedef unsigned short ushort8_t __attribute__((ext_vector_type(8)));
+    const int lane = threadIdx.x & 63, g4 = lane >> 4;
+    const size_t at = kv8_open_at<D>(c, b, h, blk);
+    const half8_t* kp = reinterpret_cast<const half8_t*>(c.k_open + at) + 2 * lane;
+    const half8_t* vp = reinterpret_cast<const half8_t*>(c.v_open + at) + 2 * lane;
 #pragma unroll 1
-        for (int x = 0; x < kKvBlock; ++x) {
-            const int j = x >> 2, g = x & 3, key = 16 * (j >> 2) + 4 * g + (j & 3);
-            float wj = 0.f;
+    for (int s = 0; 32 * s < n; ++s) {  // half a block at a time
+        const int p0 = blk * kKvBlock + 32 * s;
+        float4_t w[NT][2];
 #pragma unroll
-            for (int a = 0; a < 4; ++a)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) wj = j == 4 * a + r ? w[nt][a][r] : wj;
-            wj = __shfl(wj, 16 * g + (lane & 15));
-            if (p0 + key > st.limit[nt]) continue;
+            for (int a = 0; a < 2; ++a) w[nt][a] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    const half8_t kf = kp[((2 * s + a) * (D / 64) + i) * 128 + x];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) w[nt][a] = mfma16(kf, st.q[nt][2 * i + x], w[nt][a]);
+                }
+        half8_t v[D / 16];
+#pragma unroll
+        for (int m = 0; m < D / 32; ++m)
+#pragma unroll
+            for (int o = 0; o < 2; ++o) v[2 * m + o] = vp[(s * (D / 32) + m) * 128 + o];
+        uint4_v keep;  // elements of rows that there are
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int key = 32 * s + 16 * (j >> 1) + 4 * g4 + 2 * (j & 1);
+            keep[j] = (key < n ? 0xffffu : 0u) | (key + 1 < n ? 0xffff0000u : 0u);
+        }
+        ushort8_t big = {};
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) {
+            v[dt] = __builtin_bit_cast(half8_t, __builtin_bit_cast(uint4_v, v[dt]) & keep);
+            big = __builtin_elementwise_max(big, __builtin_bit_cast(ushort8_t, v[dt]) & (unsigned short)0x7fff);
+        }
+        int most = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = max(most, (int)big[j]);
+        const bool bad = __any(most >= 0x7c00);
+        if (bad) {
 #pragma unroll
             for (int dt = 0; dt < D / 16; ++dt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const half_t y = vo[kv8_v_at<D>(key, 16 * dt + 4 * g4 + e)];
-                    if (kv8_bad(y)) st.o[nt][dt][e] += wj * (float)y;
-                }
+                for (int j = 0; j < 8; ++j) v[dt][j] = kv8_bad(v[dt][j]) ? (half_t)0.f : v[dt][j];
         }
+        kv8_softmax<D, NT, 2>(st, w, p0, {c2, 0.f, 1.f}, true);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const half8_t p = kv8_weights<2>(w[nt], 0);
+#pragma unroll
+            for (int dt = 0; dt < D / 16; ++dt) st.o[nt][dt] = mfma16(v[dt], p, st.o[nt][dt]);
+        }
+        if (!bad) continue;
+        const half_t* vo = c.v_open + at;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll 1
+            for (int x = 0; x < 32; ++x) {
+                const int j = x >> 2, g = x & 3, key = 16 * (j >> 2) + 4 * g + (j & 3);
+                float wj = 0.f;
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) wj = j == 4 * a + r ? w[nt][a][r] : wj;
+                wj = __shfl(wj, 16 * g + (lane & 15));
+                if (p0 + key > st.limit[nt]) continue;
+#pragma unroll
+                for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const half_t y = vo[kv8_v_at<D>(32 * s + key, 16 * dt + 4 * g4 + e)];
+                        if (kv8_bad(y)) st.o[nt][dt][e] += wj * (float)y;
+                    }
+            }
+    }
 }
 
-// Workgroup (tile, b Hkv + h, split): 16 NT query rows of one K/V head's group over the split's
-// share of their blocks, the blocks dealt to the four waves in turn.
-// kList: a tile is one query's heads (16 NT at a time) over its listed blocks; otherwise rows are
-// t G + g over all the sequence's blocks.
-template <int D, int NT, bool kList>
-__global__ void __launch_bounds__(256)
-kv8_attn_kernel(Kv8AttnArgs p) {
-    constexpr int kRows = 16 * NT;
-    __shared__ float acc[kRows][D + 4];
-    __shared__ float ml[4][2][kRows];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int g4 = lane >> 4, n = lane & 15;
-    const Kv8& c = p.c;
-    const int b = blockIdx.y / c.Hkv, h = blockIdx.y % c.Hkv, split = blockIdx.z;
-    const Kv8Seq sq = kv8_seq(c, p.len, p.n_new, b, p.T);
-    int row0, row_end;
-    if constexpr (kList) {
-        const int per = (p.G + kRows - 1) / kRows;
-        const int t = blockIdx.x / per;
-        row0 = t * p.G + blockIdx.x % per * kRows;
-        row_end = (t + 1) * p.G;
-    } else {
-        row0 = blockIdx.x * kRows;
-        row_end = p.T * p.G;
-    }
-    row_end = min(row_end, (sq.n + sq.t0) * p.G);
-    if (row0 >= row_end) return;
-
-    Kv8State<D, NT> st;
-    int see = -1;  // the last key that any row sees
+// The rows of a tile: row0 + 0 .. of the T G rows t G + g of a K/V head's group.  Loads the queries
+// of NT tiles of 16 from row0 on and clears the state; returns the last key that any row sees.
+template <int D, int NT>
+__device__ __forceinline__ int kv8_begin(Kv8State<D, NT>& st, const Kv8AttnArgs& p, const Kv8Seq& sq, int b, int h, int row0,
+                                         int row_end) {
+    const int lane = threadIdx.x & 63, g4 = lane >> 4, n = lane & 15;
+    int see = -1;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int row = row0 + 16 * nt + n;
@@ -249,105 +276,250 @@ kv8_attn_kernel(Kv8AttnArgs p) {
     }
 #pragma unroll
     for (int x = 1; x < 16; x <<= 1) see = max(see, __shfl_xor(see, x));
-    see = __builtin_amdgcn_readfirstlane(see);
+    return __builtin_amdgcn_readfirstlane(see);
+}
 
+// The last key that every row of the tile sees.
+template <int D, int NT>
+__device__ __forceinline__ int kv8_least(const Kv8State<D, NT>& st, int row0, int row_end) {
+    int least = INT_MAX;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+        if (row0 + 16 * nt + (int)(threadIdx.x & 15) < row_end) least = min(least, st.limit[nt]);
+#pragma unroll
+    for (int x = 1; x < 16; x <<= 1) least = min(least, __shfl_xor(least, x));
+    return __builtin_amdgcn_readfirstlane(least);
+}
+
+// Where a split's sums of a row lie: [row][split][D] sums, behind all of them (m, l) pairs.
+template <int D>
+__device__ __forceinline__ float* kv8_part(const Kv8AttnArgs& p, size_t bh, int row, int split) {
+    return p.part + ((bh * p.T * p.G + row) * p.nsplit + split) * D;
+}
+template <int D>
+__device__ __forceinline__ float* kv8_pair(const Kv8AttnArgs& p, size_t bh, int row, int split) {
+    const size_t rows = (size_t)p.c.B * p.c.Hkv * p.T * p.G;
+    return p.part + rows * p.nsplit * D + ((bh * p.T * p.G + row) * p.nsplit + split) * 2;
+}
+
+// 4 consecutive d of a finished row, times the gate.
+__device__ __forceinline__ void kv8_store4(const Kv8AttnArgs& p, int b, int h, int row, int d, float4_t y, float l) {
+    const int t = row / p.G, hq = h * p.G + row % p.G;
+    const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that saw no key is 0
+    half4_t out;
+    float g[4] = {inv, inv, inv, inv};
+    if (p.gate.data) {
+        const half4_t x = *reinterpret_cast<const half4_t*>(p.gate.data + b * p.gate.b + hq * p.gate.h + t * p.gate.t + d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) g[e] = inv * __builtin_amdgcn_rcpf(1.f + __expf(-(float)x[e]));
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = (half_t)(y[e] * g[e]);
+    *reinterpret_cast<half4_t*>(p.o.data + b * p.o.b + hq * p.o.h + t * p.o.t + d) = out;
+}
+
+// Keys that a wave of the row kernel takes at a time, and their codes in registers.
+template <int D>
+struct Kv8Regs {
+    static constexpr int kKeys = D == 256 ? 32 : 64, kN = kKeys * D / 1024;
+    uint4 k[kN], v[kN];
+    float sk, sv;
+
+    __device__ __forceinline__ void load_k(const Kv8& c, int page, int h, int part) {
+        const size_t head = (size_t)page * c.Hkv + h;
+        const uint4* kp = reinterpret_cast<const uint4*>(c.k + head * (kKvBlock * D)) + part * (kN * 64) + (threadIdx.x & 63);
+#pragma unroll
+        for (int i = 0; i < kN; ++i) k[i] = kp[i * 64];
+        sk = c.k_scale[head];
+        sv = c.v_scale[head];
+    }
+    __device__ __forceinline__ void load_v(const Kv8& c, int page, int h, int part) {
+        const size_t head = (size_t)page * c.Hkv + h;
+        const uint4* vp = reinterpret_cast<const uint4*>(c.v + head * (kKvBlock * D)) + part * (kN * 64) + (threadIdx.x & 63);
+#pragma unroll
+        for (int i = 0; i < kN; ++i) v[i] = vp[i * 64];
+    }
+};
+
+// Few rows: workgroup (tile, b Hkv + h, split), one tile of 16 query rows of a K/V head's group over
+// the split's share of their blocks, the blocks dealt to the four waves in turn.  A wave's
+// next keys are on their way to registers as soon as its last ones have been multiplied, its next
+// values likewise.
+// kList: a tile is one query's heads (16 at a time) over its listed blocks; otherwise rows are
+// t G + g over all the sequence's blocks.
+template <int D, bool kList>
+__global__ void __launch_bounds__(256, 2)
+kv8_row_kernel(Kv8AttnArgs p) {
+    constexpr int kParts = kKvBlock / Kv8Regs<D>::kKeys, kRow = D + 4;
+    __shared__ __align__(16) float acc[2][16][kRow];
+    __shared__ float ml[4][2][16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g4 = lane >> 4, n = lane & 15;
+    const Kv8& c = p.c;
+    const int b = blockIdx.y / c.Hkv, h = blockIdx.y % c.Hkv, split = blockIdx.z;
+    const Kv8Seq sq = kv8_seq(c, p.len, p.n_new, b, p.T);
+    int row0, row_end;
+    if constexpr (kList) {
+        const int per = (p.G + 15) / 16, t = blockIdx.x / per;
+        row0 = t * p.G + blockIdx.x % per * 16;
+        row_end = (t + 1) * p.G;
+    } else {
+        row0 = blockIdx.x * 16;
+        row_end = p.T * p.G;
+    }
+    row_end = min(row_end, (sq.n + sq.t0) * p.G);
+    if (row0 >= row_end) return;
+
+    Kv8State<D, 1> st;
+    const int see = kv8_begin<D, 1>(st, p, sq, b, h, row0, row_end);
     const int nb = see / kKvBlock + (see >= 0 ? 1 : 0);  // blocks that any row sees
+    const int n_full = min(sq.len / kKvBlock, nb);
     const int items = kList ? p.top : nb;
     const int per = (items + p.nsplit - 1) / p.nsplit;
     const int end = min(items, (split + 1) * per);
     const int* list = kList ? p.blocks + (((size_t)b * c.Hkv + h) * p.T + row0 / p.G) * p.top : nullptr;
-    const int n_full = sq.len / kKvBlock;
     int open = 0;  // how often the open block is among this wave's
-    for (int i = split * per + wave; i < end; i += 4) {
-        const int blk = kList ? list[i] : i;
-        if (blk < 0 || blk >= nb) continue;
-        if (blk >= n_full) {
-            ++open;
-            continue;
+    int i = split * per + wave, blk = 0, page = -1;
+    // the next of this wave's full blocks that has a page; i is behind it
+    auto next = [&]() {
+        for (page = -1; page < 0 && i < end; i += 4) {
+            blk = kList ? list[i] : i;
+            if (blk < 0 || blk >= nb) continue;
+            if (blk >= n_full)
+                ++open;
+            else
+                page = kv8_page(c, b, blk);
         }
-        const int page = kv8_page(c, b, blk);
-        if (page >= 0) kv8_page_block<D, NT>(st, c, page, h, blk, p.c2);
+    };
+    // rows of one query see whole blocks but the last; several queries' last one or two are masked
+    const int least = kv8_least<D, 1>(st, row0, row_end);
+    auto masked = [&](int k) { return (k + 1) * kKvBlock - 1 > least; };
+    next();
+    if (page >= 0) {
+        Kv8Regs<D> x;
+        x.load_k(c, page, h, 0);
+        x.load_v(c, page, h, 0);
+        while (page >= 0) {
+            const int now = blk, here = page;
+            const Kv8Scale sc = {p.c2 * x.sk, __builtin_amdgcn_logf(x.sv), __builtin_amdgcn_rcpf(x.sv)};
+#pragma unroll
+            for (int part = 0; part < kParts; ++part) {
+                const bool last = part == kParts - 1;
+                if (last) next();
+                const int to = last ? page : here;
+                kv8_keys<D, 1, Kv8Regs<D>::kKeys / 16>(
+                    st, now * kKvBlock + part * Kv8Regs<D>::kKeys, sc, masked(now),
+                    [&](int a, int i, int s) {
+                        const uint4& k = x.k[a * (D / 64) + i];
+                        return s ? kv8_halves(k.z, k.w) : kv8_halves(k.x, k.y);
+                    },
+                    [&](int s, int m, int o) {
+                        const uint4& v = x.v[s * (D / 32) + m];
+                        return o ? kv8_halves(v.z, v.w) : kv8_halves(v.x, v.y);
+                    },
+                    [&]() {
+                        if (to >= 0) x.load_k(c, to, h, last ? 0 : part + 1);
+                    });
+                if (to >= 0) x.load_v(c, to, h, last ? 0 : part + 1);
+            }
+        }
     }
-    for (; open > 0; --open) kv8_open_block<D, NT>(st, c, b, h, n_full, sq.len, p.c2);
+    for (; open > 0; --open) kv8_open_block<D, 1>(st, c, b, h, n_full, sq.len - n_full * kKvBlock, p.c2);
 
     // the four waves' sums, relative to their common maximum
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        st.l[nt] = kv8_sum4(st.l[nt]);
-        if (g4 == 0) {
-            ml[wave][0][16 * nt + n] = st.m[nt];
-            ml[wave][1][16 * nt + n] = st.l[nt];
-        }
+    st.l[0] = sum_xor32(sum_xor16(st.l[0]));
+    if (g4 == 0) {
+        ml[wave][0][n] = st.m[0];
+        ml[wave][1][n] = st.l[0];
     }
-    for (int w = 0; w < 4; ++w) {
-        __syncthreads();
-        if (wave != w) continue;
+    __syncthreads();
+    {
+        const float m = fmaxf(fmaxf(ml[0][0][n], ml[1][0][n]), fmaxf(ml[2][0][n], ml[3][0][n]));
+        const float f = st.m[0] == m ? 1.f : fast_exp2(st.m[0] - m);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int r = 16 * nt + n;
-            const float m = fmaxf(fmaxf(ml[0][0][r], ml[1][0][r]), fmaxf(ml[2][0][r], ml[3][0][r]));
-            const float f = st.m[nt] == m ? 1.f : fast_exp2(st.m[nt] - m);
+        for (int dt = 0; dt < D / 16; ++dt) st.o[0][dt] *= f;
+    }
+    if (wave >= 2) {
 #pragma unroll
-            for (int dt = 0; dt < D / 16; ++dt) {
-                float4_t* at = reinterpret_cast<float4_t*>(&acc[r][16 * dt + 4 * g4]);
-                *at = w ? *at + st.o[nt][dt] * f : st.o[nt][dt] * f;
-            }
+        for (int dt = 0; dt < D / 16; ++dt) *reinterpret_cast<float4_t*>(&acc[wave & 1][n][16 * dt + 4 * g4]) = st.o[0][dt];
+    }
+    __syncthreads();
+    if (wave < 2) {
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) {
+            float4_t* at = reinterpret_cast<float4_t*>(&acc[wave][n][16 * dt + 4 * g4]);
+            *at += st.o[0][dt];
         }
     }
     __syncthreads();
-    const size_t rows_all = (size_t)p.T * p.G;
-    for (int i = threadIdx.x; i < min(kRows, row_end - row0) * D; i += 256) {
-        const int r = i / D, d = i % D, row = row0 + r;
+    for (int i = threadIdx.x; i < min(16, row_end - row0) * (D / 4); i += 256) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
         float m = -INFINITY, l = 0.f;
+#pragma unroll
         for (int w = 0; w < 4; ++w) m = fmaxf(m, ml[w][0][r]);
+#pragma unroll
         for (int w = 0; w < 4; ++w) l += ml[w][0][r] == m ? ml[w][1][r] : ml[w][1][r] * fast_exp2(ml[w][0][r] - m);
+        const float4_t y = *reinterpret_cast<const float4_t*>(&acc[0][r][d]) + *reinterpret_cast<const float4_t*>(&acc[1][r][d]);
         if (p.nsplit > 1) {
-            const size_t at = ((size_t)blockIdx.y * rows_all + row) * p.nsplit + split;
-            p.part[at * D + d] = acc[r][d];
-            if (d == 0) {
-                float* pair = p.part + (size_t)gridDim.y * rows_all * p.nsplit * D + 2 * at;
-                pair[0] = m;
-                pair[1] = l;
-            }
+            if (l != 0.f) *reinterpret_cast<float4_t*>(kv8_part<D>(p, blockIdx.y, row0 + r, split) + d) = y;
+            if (d == 0) *reinterpret_cast<float2*>(kv8_pair<D>(p, blockIdx.y, row0 + r, split)) = float2{m, l};
         } else {
-            const int t = row / p.G, hq = h * p.G + row % p.G;
-            float y = l == 0.f ? 0.f : acc[r][d] / l;
-            if (p.gate.data) y /= 1.f + __expf(-(float)p.gate.data[b * p.gate.b + hq * p.gate.h + t * p.gate.t + d]);
-            p.o.data[b * p.o.b + hq * p.o.h + t * p.o.t + d] = (half_t)y;
+            kv8_store4(p, b, h, row0 + r, d, y, l);
         }
     }
 }
 
-// Joins the splits of one row: workgroup (row, b Hkv + h), thread d.
+constexpr int kKvMaxSplits = 128;
+
+// Joins the splits of 1024 / D rows: workgroup (rows, b Hkv + h), D / 4 lanes a row.
 template <int D>
-__global__ void __launch_bounds__(D)
+__global__ void __launch_bounds__(256)
 kv8_join_kernel(Kv8AttnArgs p) {
+    constexpr int kLanes = D / 4, kRows = 256 / kLanes;
+    __shared__ float fs[kRows][kKvMaxSplits];
     const Kv8& c = p.c;
-    const int b = blockIdx.y / c.Hkv, h = blockIdx.y % c.Hkv, row = blockIdx.x, d = threadIdx.x;
+    const int b = blockIdx.y / c.Hkv, h = blockIdx.y % c.Hkv;
+    const int r = threadIdx.x / kLanes, x = threadIdx.x % kLanes, row = blockIdx.x * kRows + r;
     const Kv8Seq sq = kv8_seq(c, p.len, p.n_new, b, p.T);
-    const int t = row / p.G, hq = h * p.G + row % p.G;
-    if (t >= sq.n + sq.t0) return;
-    const size_t rows_all = (size_t)p.T * p.G;
-    const size_t at = ((size_t)blockIdx.y * rows_all + row) * p.nsplit;
-    const float* pair = p.part + (size_t)gridDim.y * rows_all * p.nsplit * D + 2 * at;
-    float m = -INFINITY, l = 0.f, y = 0.f;
-    for (int s = 0; s < p.nsplit; ++s) m = fmaxf(m, pair[2 * s]);
-    for (int s = 0; s < p.nsplit; ++s) {
-        if (pair[2 * s + 1] == 0.f) continue;
-        const float f = pair[2 * s] == m ? 1.f : fast_exp2(pair[2 * s] - m);
-        l += f * pair[2 * s + 1];
-        y += f * p.part[(at + s) * D + d];
+    const bool is = row < (sq.n + sq.t0) * p.G;  // rows of padding have no sums
+    const float2* pair = reinterpret_cast<const float2*>(kv8_pair<D>(p, blockIdx.y, is ? row : 0, 0));
+    float m = -INFINITY, l = 0.f;
+    float2 ml[kKvMaxSplits / kLanes];
+#pragma unroll
+    for (int i = 0; i < kKvMaxSplits / kLanes; ++i) {
+        ml[i] = is && x + i * kLanes < p.nsplit ? pair[x + i * kLanes] : float2{-INFINITY, 0.f};
+        m = fmaxf(m, ml[i].x);
     }
-    y = l == 0.f ? 0.f : y / l;
-    if (p.gate.data) y /= 1.f + __expf(-(float)p.gate.data[b * p.gate.b + hq * p.gate.h + t * p.gate.t + d]);
-    p.o.data[b * p.o.b + hq * p.o.h + t * p.o.t + d] = (half_t)y;
+#pragma unroll
+    for (int o = 1; o < kLanes; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+#pragma unroll
+    for (int i = 0; i < kKvMaxSplits / kLanes; ++i) {
+        float f = ml[i].y == 0.f ? 0.f : ml[i].x == m ? 1.f : fast_exp2(ml[i].x - m);
+        if (ml[i].y != ml[i].y) f = ml[i].y;  // a row of NaN, whatever its maximum
+        l += ml[i].y == 0.f ? 0.f : f * ml[i].y;
+        if (x + i * kLanes < p.nsplit) fs[r][x + i * kLanes] = f;
+    }
+#pragma unroll
+    for (int o = 1; o < kLanes; o <<= 1) l += __shfl_xor(l, o);
+    __syncthreads();
+    if (!is) return;
+    const float* at = kv8_part<D>(p, blockIdx.y, row, 0) + 4 * x;
+    float4_t y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int s = 0; s < p.nsplit; ++s) {
+        const float f = fs[r][s];
+        // sums that no key went into were not written
+        if (f != 0.f) y += *reinterpret_cast<const float4_t*>(at + (size_t)s * D) * f;
+    }
+    kv8_store4(p, b, h, row, 4 * x, y, l);
 }
 
 // Key splits of one tile: as many workgroups as the chip takes twice, not fewer than 4 blocks each.
 inline int kv8_splits(long long tiles, int items) {
     const long long want = (1024 + tiles - 1) / tiles;
     const long long most = (items + 3) / 4;
-    return (int)(want < most ? want : most);
+    const long long n = want < most ? want : most;
+    return (int)(n < kKvMaxSplits ? n : kKvMaxSplits);
 }
 inline long long kv8_tiles(int B, int T, int Hq, int Hkv, bool list) {
     const long long G = Hq / Hkv;
@@ -361,11 +533,12 @@ template <int D, bool kList>
 hipError_t kv8_attn_d(Kv8AttnArgs p, hipStream_t stream) {
     const long long tiles = kv8_tiles(1, p.T, p.G, 1, kList);
     const dim3 grid((unsigned)tiles, (unsigned)(p.c.B * p.c.Hkv), (unsigned)p.nsplit);
-    hipLaunchKernelGGL((kv8_attn_kernel<D, 1, kList>), grid, dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((kv8_row_kernel<D, kList>), grid, dim3(256), 0, stream, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.nsplit == 1) return e;
-    const dim3 rows((unsigned)(p.T * p.G), (unsigned)(p.c.B * p.c.Hkv));
-    hipLaunchKernelGGL(kv8_join_kernel<D>, rows, dim3(D), 0, stream, p);
+    constexpr int kRows = 1024 / D;
+    const dim3 rows((unsigned)((p.T * p.G + kRows - 1) / kRows), (unsigned)(p.c.B * p.c.Hkv));
+    hipLaunchKernelGGL(kv8_join_kernel<D>, rows, dim3(256), 0, stream, p);
     return hipGetLastError();
 }
 template <bool kList>

@@ -242,9 +242,10 @@ kv8_read_kernel(Kv8 c, const int* __restrict__ len, const int* __restrict__ star
     for (int i = 0; i < kN; ++i) {
         const int u = tid + i * kThreads;
         if (isv) {
-            const int d = (u >> 6) * 16 + (u & 15), r = ((u >> 4) & 3) * 4;
+            const int t = u >> 6, d = t % (D / 32) * 32 + (u & 15), r = t / (D / 32) * 32 + ((u >> 4) & 3) * 4;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) tile[((j >> 2) * 16 + r + (j & 3)) * kRow + d] = y[i][j >> 3][j & 7];
+            for (int j = 0; j < 16; ++j)
+                tile[(r + ((j >> 2) & 1) * 16 + (j & 3)) * kRow + d + (j >> 3) * 16] = y[i][j >> 3][j & 7];
         } else {
             const int t = u >> 6, r = t / (D / 64) * 16 + (u & 15), d = t % (D / 64) * 64 + ((u >> 4) & 3) * 16;
 #pragma unroll
