@@ -452,7 +452,8 @@ def as_lists(blocks):
 
 
 @pytest.mark.parametrize("D,G,T,top,first,recent", [(64, 1, 1, 4, 1, 1), (128, 6, 1, 7, 1, 2), (256, 6, 3, 16, 0, 0), (64, 20, 2, 3, 2, 0),
-                                                    (128, 2, 40, 5, 1, 1), (256, 3, 1, 64, 1, 1), (64, 2, 70, 1, 0, 0)])
+                                                    (128, 2, 40, 5, 1, 1), (256, 3, 1, 64, 1, 1), (64, 2, 70, 1, 0, 0),
+                                                    (64, 100, 1, 6, 1, 1), (128, 48, 3, 5, 0, 1), (64, 16, 5, 9, 1, 1)])
 def test_select_and_attend(dev, D, G, T, top, first, recent):
     gen = torch.Generator().manual_seed(D + 7 * G + T + top)
     H = 2
@@ -513,10 +514,12 @@ def test_listed_blocks_of_the_callers(dev):
     assert not bool(o[0, :, 3].any())
 
 
-def test_select_many_blocks(dev):
-    """More blocks than one workgroup scores at once, against the definition in whole numbers."""
+@pytest.mark.parametrize("nb,top", [(500, 40), (1999, 300), (3001, 40), (9000, 1), (9000, 8500)])
+def test_select_many_blocks(dev, nb, top):
+    """More blocks than one workgroup scores at once or holds in registers, against the definition in
+    whole numbers."""
     gen = torch.Generator().manual_seed(33)
-    D, G, nb, top = 64, 4, 3001, 40
+    D, G = 64, 4
     L = 64 * nb + 9
     c = tsa.Kv8Cache(1, 1, D, L, device=dev)
     c.k_sum.copy_(torch.randint(-127, 128, c.k_sum.shape, generator=gen, dtype=torch.int8))
@@ -524,13 +527,14 @@ def test_select_many_blocks(dev):
     c.k_sum[100:1500:7] = c.k_sum[99]  # many equals
     c.k_sum_scale[100:1500:7] = c.k_sum_scale[99]
     q = rand(gen, 1, G, 2, D)
-    got = tsa.kv8_select(q.to(dev), c, ints([L], dev), top, first=2, recent=3).cpu()
+    first, recent = (2, 3) if top > 5 else (0, 0)
+    got = tsa.kv8_select(q.to(dev), c, ints([L], dev), top, first=first, recent=recent).cpu()
     m, s = c.k_sum.cpu().double()[:, 0], c.k_sum_scale.cpu().numpy()[:, 0]
     for t in range(2):
         x = q[0, :, t].double()
         score = (torch.round(127 * x / x.abs().max()) @ m.T).amax(0).numpy().astype(np.float32) * s
         own = nb
-        rank = [(np.inf if i < 2 or i >= own - 3 else score[i], -i) for i in range(own + 1)]
+        rank = [(np.inf if i < first or i >= own - recent else score[i], -i) for i in range(own + 1)]
         assert got[0, 0, t].tolist() == sorted(-r[1] for r in sorted(rank, reverse=True)[:top])
 
 

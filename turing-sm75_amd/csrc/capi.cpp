@@ -443,7 +443,6 @@ extern "C" int tsa_kv8_select(const tsa_kv8* cache, const tsa_rows* q, const int
     if ((rc = check_kv8_queries(cache, T, Hq))) return rc;
     if (max_len < 1 || top < 1 || first < 0 || recent < 0) return TSA_ERR_SHAPE;
     if ((long long)first + recent + 1 > top) return TSA_ERR_ARG;
-    if ((long long)Hq / cache->Hkv > 256) return TSA_ERR_UNSUPPORTED;
     const int B = cache->B, nb = kv8_nb(cache, max_len);
     if ((rc = check_rows(q, B, Hq, T, false))) return rc;
     const size_t need = tsa::kv8_ws_bytes(B, T, Hq, cache->Hkv, cache->D, nb, top);

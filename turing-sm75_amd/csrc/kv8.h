@@ -44,6 +44,19 @@ __device__ __forceinline__ int kv8_at(bool isv, int r, int d) {
     return isv ? kv8_v_at<D>(r, d) : kv8_k_at<D>(r, d);
 }
 
+// 127 x / a as a division would round it (with r = 1 / a rounded, one correction of y r by its exact
+// remainder gives the correctly rounded quotient), then to a whole number, ties to even: the sum
+// with 1.5 2^23 + 128 leaves rint(127 x / a) + 128 in its low byte.
+constexpr float kKvMagic = 12582912.f + 128.f;
+__device__ __forceinline__ unsigned kv8_code(float x, float a, float r) {
+    const float y = 127.f * x, q = y * r;
+    return __builtin_bit_cast(unsigned, __builtin_fmaf(__builtin_fmaf(-q, a, y), r, q) + kKvMagic);
+}
+// The low bytes of four words.
+__device__ __forceinline__ unsigned kv8_pack(unsigned b0, unsigned b1, unsigned b2, unsigned b3) {
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(b3, b2, 0x0c0c0400u), __builtin_amdgcn_perm(b1, b0, 0x0c0c0400u), 0x05040100u);
+}
+
 // A sequence's tokens: `len` of them, the last `n` new; rows of a call's T start at new row `t0`
 // (rows before it would lie in front of the sequence).  Every count is clamped to what the cache
 // and the call hold, so that no value of the device arrays leads out of bounds.

@@ -303,19 +303,21 @@ __device__ __forceinline__ float* kv8_pair(const Kv8AttnArgs& p, size_t bh, int 
 }
 
 // 4 consecutive d of a finished row, times the gate.
-__device__ __forceinline__ void kv8_store4(const Kv8AttnArgs& p, int b, int h, int row, int d, float4_t y, float l) {
-    const int t = row / p.G, hq = h * p.G + row % p.G;
+__device__ __forceinline__ void kv8_store4(const Kv8AttnArgs& p, int b, int hq, int t, int d, float4_t y, float l, half4_t gate) {
     const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that saw no key is 0
     half4_t out;
     float g[4] = {inv, inv, inv, inv};
     if (p.gate.data) {
-        const half4_t x = *reinterpret_cast<const half4_t*>(p.gate.data + b * p.gate.b + hq * p.gate.h + t * p.gate.t + d);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) g[e] = inv * __builtin_amdgcn_rcpf(1.f + __expf(-(float)x[e]));
+        for (int e = 0; e < 4; ++e) g[e] = inv * __builtin_amdgcn_rcpf(1.f + __expf(-(float)gate[e]));
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) out[e] = (half_t)(y[e] * g[e]);
     *reinterpret_cast<half4_t*>(p.o.data + b * p.o.b + hq * p.o.h + t * p.o.t + d) = out;
+}
+__device__ __forceinline__ half4_t kv8_gate4(const Kv8AttnArgs& p, int b, int hq, int t, int d) {
+    if (!p.gate.data) return half4_t{};
+    return *reinterpret_cast<const half4_t*>(p.gate.data + b * p.gate.b + hq * p.gate.h + t * p.gate.t + d);
 }
 
 // Keys that a wave of the row kernel takes at a time, and their codes in registers.
@@ -464,30 +466,42 @@ kv8_row_kernel(Kv8AttnArgs p) {
             if (l != 0.f) *reinterpret_cast<float4_t*>(kv8_part<D>(p, blockIdx.y, row0 + r, split) + d) = y;
             if (d == 0) *reinterpret_cast<float2*>(kv8_pair<D>(p, blockIdx.y, row0 + r, split)) = float2{m, l};
         } else {
-            kv8_store4(p, b, h, row0 + r, d, y, l);
+            const int t = (row0 + r) / p.G, hq = h * p.G + (row0 + r) % p.G;
+            kv8_store4(p, b, hq, t, d, y, l, kv8_gate4(p, b, hq, t, d));
         }
     }
 }
 
 constexpr int kKvMaxSplits = 128;
 
-// Joins the splits of 1024 / D rows: workgroup (rows, b Hkv + h), D / 4 lanes a row.
+// Joins the splits of 1024 / D rows: workgroup (rows, b Hkv + h), D / 4 lanes a row.  Every address
+// is known at once, so that the loads wait for memory together and not for each other: a row's
+// maxima and sums, its first splits' sums (unread where they were not written), its gate.
 template <int D>
 __global__ void __launch_bounds__(256)
 kv8_join_kernel(Kv8AttnArgs p) {
-    constexpr int kLanes = D / 4, kRows = 256 / kLanes;
+    constexpr int kLanes = D / 4, kRows = 256 / kLanes, kAhead = 16;
     __shared__ float fs[kRows][kKvMaxSplits];
     const Kv8& c = p.c;
     const int b = blockIdx.y / c.Hkv, h = blockIdx.y % c.Hkv;
-    const int r = threadIdx.x / kLanes, x = threadIdx.x % kLanes, row = blockIdx.x * kRows + r;
-    const Kv8Seq sq = kv8_seq(c, p.len, p.n_new, b, p.T);
-    const bool is = row < (sq.n + sq.t0) * p.G;  // rows of padding have no sums
-    const float2* pair = reinterpret_cast<const float2*>(kv8_pair<D>(p, blockIdx.y, is ? row : 0, 0));
-    float m = -INFINITY, l = 0.f;
+    const int r = threadIdx.x / kLanes, x = threadIdx.x % kLanes, n_rows = p.T * p.G;
+    const int row = min((int)blockIdx.x * kRows + r, n_rows - 1);
+    const float2* pair = reinterpret_cast<const float2*>(kv8_pair<D>(p, blockIdx.y, row, 0));
+    const float4_t* at = reinterpret_cast<const float4_t*>(kv8_part<D>(p, blockIdx.y, row, 0)) + x;
     float2 ml[kKvMaxSplits / kLanes];
 #pragma unroll
+    for (int i = 0; i < kKvMaxSplits / kLanes; ++i) ml[i] = pair[min(x + i * kLanes, p.nsplit - 1)];
+    float4_t part[kAhead];
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) part[s] = at[(size_t)min(s, p.nsplit - 1) * (D / 4)];
+    const int t = row / p.G, hq = h * p.G + row % p.G;
+    const half4_t gate = kv8_gate4(p, b, hq, t, 4 * x);
+    const Kv8Seq sq = kv8_seq(c, p.len, p.n_new, b, p.T);
+    const bool is = (int)blockIdx.x * kRows + r < n_rows && t < sq.n + sq.t0;  // rows of padding have no sums
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
     for (int i = 0; i < kKvMaxSplits / kLanes; ++i) {
-        ml[i] = is && x + i * kLanes < p.nsplit ? pair[x + i * kLanes] : float2{-INFINITY, 0.f};
+        if (x + i * kLanes >= p.nsplit) ml[i] = float2{-INFINITY, 0.f};
         m = fmaxf(m, ml[i].x);
     }
 #pragma unroll
@@ -503,15 +517,21 @@ kv8_join_kernel(Kv8AttnArgs p) {
     for (int o = 1; o < kLanes; o <<= 1) l += __shfl_xor(l, o);
     __syncthreads();
     if (!is) return;
-    const float* at = kv8_part<D>(p, blockIdx.y, row, 0) + 4 * x;
     float4_t y = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-    for (int s = 0; s < p.nsplit; ++s) {
-        const float f = fs[r][s];
-        // sums that no key went into were not written
-        if (f != 0.f) y += *reinterpret_cast<const float4_t*>(at + (size_t)s * D) * f;
+    auto add = [&](const float4_t& v, float f) {
+        if (f != 0.f) y += v * f;  // sums that no key went into were not written
+    };
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s)
+        if (s < p.nsplit) add(part[s], fs[r][s]);
+    for (int s0 = kAhead; s0 < p.nsplit; s0 += kAhead) {
+#pragma unroll
+        for (int s = 0; s < kAhead; ++s) part[s] = at[(size_t)min(s0 + s, p.nsplit - 1) * (D / 4)];
+#pragma unroll
+        for (int s = 0; s < kAhead; ++s)
+            if (s0 + s < p.nsplit) add(part[s], fs[r][s0 + s]);
     }
-    kv8_store4(p, b, h, row, 4 * x, y, l);
+    kv8_store4(p, b, hq, t, 4 * x, y, l, gate);
 }
 
 // Key splits of one tile: as many workgroups as the chip takes twice, not fewer than 4 blocks each.

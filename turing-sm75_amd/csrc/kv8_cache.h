@@ -111,11 +111,7 @@ __device__ __forceinline__ void kv8_write_block(const Kv8& c, const half_t* __re
     const bool finite = most < 0x7c00;
     const float a = finite ? (float)__builtin_bit_cast(half_t, (unsigned short)max(most, 1)) : 1.f;
     const float scale = finite ? a / 127.f : __builtin_nanf("");
-    // 127 x / a, rounded as a division would: with r the rounded reciprocal, one correction of
-    // q = y r by its exact remainder gives the correctly rounded quotient.  The sum with 1.5 2^23
-    // + 128 rounds it to a whole number, ties to even, and leaves code + 128 in the low byte.
     const float r = 1.f / a;
-    constexpr float kMagic = 12582912.f + 128.f;
     const size_t head = (size_t)page * c.Hkv + h;
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
@@ -124,30 +120,23 @@ __device__ __forceinline__ void kv8_write_block(const Kv8& c, const half_t* __re
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float y = finite ? 127.f * (float)x[n][e][j] : 0.f;
-                const float q0 = y * r;
-                q[e][j] = __builtin_bit_cast(unsigned, __builtin_fmaf(__builtin_fmaf(-q0, a, y), r, q0) + kMagic);
-            }
-        auto pack = [](unsigned b0, unsigned b1, unsigned b2, unsigned b3) {
-            return __builtin_amdgcn_perm(__builtin_amdgcn_perm(b3, b2, 0x0c0c0400u), __builtin_amdgcn_perm(b1, b0, 0x0c0c0400u), 0x05040100u);
-        };
+            for (int j = 0; j < 8; ++j) q[e][j] = kv8_code(finite ? (float)x[n][e][j] : 0.f, a, r);
         if (kV) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int at = kv8_v_at<D>(row, d + j);
-                reinterpret_cast<unsigned*>(&lds.units[kv8_swz(true, at >> 4)])[(at & 15) >> 2] = pack(q[0][j], q[1][j], q[2][j], q[3][j]);
+                reinterpret_cast<unsigned*>(&lds.units[kv8_swz(true, at >> 4)])[(at & 15) >> 2] = kv8_pack(q[0][j], q[1][j], q[2][j], q[3][j]);
             }
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int at = kv8_k_at<D>(row + e, d);
                 reinterpret_cast<uint2*>(&lds.units[kv8_swz(false, at >> 4)])[(at & 15) >> 3] =
-                    uint2{pack(q[e][0], q[e][1], q[e][2], q[e][3]), pack(q[e][4], q[e][5], q[e][6], q[e][7])};
+                    uint2{kv8_pack(q[e][0], q[e][1], q[e][2], q[e][3]), kv8_pack(q[e][4], q[e][5], q[e][6], q[e][7])};
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                atomicAdd(&lds.sum[d + j], (int)(q[0][j] + q[1][j] + q[2][j] + q[3][j] - 4u * __builtin_bit_cast(unsigned, kMagic)));
+                atomicAdd(&lds.sum[d + j], (int)(q[0][j] + q[1][j] + q[2][j] + q[3][j] - 4u * __builtin_bit_cast(unsigned, kKvMagic)));
         }
     }
     __syncthreads();

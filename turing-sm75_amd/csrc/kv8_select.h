@@ -16,69 +16,114 @@ struct Kv8SelectArgs {
     Kv8 c;
     Rows16 q;
     const int *len, *n_new;
-    signed char* qc;   // [B][Hkv][T][G][D]
     float* score;      // [B][Hkv][T][nb]
     int* blocks;       // [B][Hkv][T][top]
     int T, Hq, G, top, first, recent, nb;
+    int tq;            // queries of a score workgroup
 };
 
-// Workgroup (t, b Hkv + h): the group's query codes.
-template <int D>
-__global__ void __launch_bounds__(256)
-kv8_qcode_kernel(Kv8SelectArgs p) {
-    __shared__ int red;
-    const int b = blockIdx.y / p.c.Hkv, h = blockIdx.y % p.c.Hkv, t = blockIdx.x;
-    const Kv8Seq sq = kv8_seq(p.c, p.len, p.n_new, b, p.T);
-    if (t >= sq.n + sq.t0) return;
-    const half_t* q = p.q.data + b * p.q.b + (long long)h * p.G * p.q.h + t * p.q.t;
-    if (threadIdx.x == 0) red = 1;
-    __syncthreads();
-    int most = 0;
-    for (int i = threadIdx.x; i < p.G * D; i += 256)
-        most = max(most, (int)(__builtin_bit_cast(unsigned short, q[i / D * p.q.h + i % D]) & 0x7fff));
-    atomicMax(&red, most);
-    __syncthreads();
-    most = red;
-    const float a = (float)__builtin_bit_cast(half_t, (unsigned short)most);
-    signed char* qc = p.qc + ((size_t)blockIdx.y * p.T + t) * p.G * D;
-    // a group with an infinity or NaN has no order: all its codes are 0
-    for (int i = threadIdx.x; i < p.G * D; i += 256)
-        qc[i] = most < 0x7c00 ? (signed char)(int)rintf(127.f * (float)q[i / D * p.q.h + i % D] / a) : (signed char)0;
-}
+constexpr int kKvScoreCols = 48;    // query rows (t, g) of a score workgroup at the most, or one query's heads
+constexpr int kKvScoreBlocks = 128; // blocks of one
 
-// Workgroup (t and 256 blocks, b Hkv + h): a block a thread.
+// Workgroup (queries and blocks, b Hkv + h): scores of 128 blocks, 32 a wave, for `tq` queries whose
+// codes lie in LDS, by v_mfma_i32_16x16x64_i8 with the summaries as operand A straight from memory
+// (lane l: block l % 16, d = 64 k + 16 (l / 16) + 0 .. 15) and 16 query rows as operand B.  Lane l
+// then has 4 blocks' scores of row l % 16; the maximum over a query's heads goes through LDS.  With
+// more than 48 heads a group, the rows of one query are taken 48 at a time.
 template <int D>
 __global__ void __launch_bounds__(256)
 kv8_score_kernel(Kv8SelectArgs p) {
-    extern __shared__ int qs[];
-    const int parts = (p.nb + 255) / 256, i0 = (int)(blockIdx.x % parts) * 256;
-    const int b = blockIdx.y / p.c.Hkv, h = blockIdx.y % p.c.Hkv, t = blockIdx.x / parts;
-    const Kv8Seq sq = kv8_seq(p.c, p.len, p.n_new, b, p.T);
-    const int pos = sq.len - (sq.n + sq.t0) + t;
-    if (t >= sq.n + sq.t0 || pos < 0) return;
-    const int own = min(pos / kKvBlock, p.nb);
-    if (i0 >= own) return;  // the own block has no score
-    const size_t row = (size_t)blockIdx.y * p.T + t;
-    const int* qc = reinterpret_cast<const int*>(p.qc + row * p.G * D);
-    for (int i = threadIdx.x; i < p.G * D / 4; i += 256) qs[i] = qc[i];
-    __syncthreads();
-    const int blk = i0 + threadIdx.x;
-    if (blk >= own) return;
-    const int page = kv8_page(p.c, b, blk);
-    float score = -INFINITY;
-    if (page >= 0) {
-        const size_t head = (size_t)page * p.c.Hkv + h;
-        const int* m = reinterpret_cast<const int*>(p.c.k_sum + head * D);
-        int best = INT_MIN;
-        for (int g = 0; g < p.G; ++g) {
-            int s = 0;
-            for (int i = 0; i < D / 4; ++i) s = __builtin_amdgcn_sdot4(m[i], qs[g * (D / 4) + i], s, false);
-            best = max(best, s);
-        }
-        const float x = (float)best * p.c.k_sum_scale[head];
-        score = x == x ? x : -INFINITY;  // a block that holds an infinity or NaN
+    typedef int int4_v __attribute__((ext_vector_type(4)));
+    constexpr int kRow = D + 16, kWaveTiles = kKvScoreBlocks / 64;
+    __shared__ __align__(16) signed char qs[kKvScoreCols * kRow];
+    __shared__ int sc[kKvScoreCols][kKvScoreBlocks + 4];
+    __shared__ int most[kKvScoreCols];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g4 = lane >> 4, n = lane & 15;
+    const int parts = (p.nb + kKvScoreBlocks - 1) / kKvScoreBlocks, blk0 = (int)(blockIdx.x % parts) * kKvScoreBlocks;
+    const int b = blockIdx.y / p.c.Hkv, h = blockIdx.y % p.c.Hkv, t0 = (int)(blockIdx.x / parts) * p.tq;
+    // operand A first: its latency passes under the query codes'
+    int page[kWaveTiles];
+    int4_v m[kWaveTiles][D / 64];
+    const int table_end = min(p.nb, p.c.max_blocks);
+#pragma unroll
+    for (int i = 0; i < kWaveTiles; ++i) {
+        const int blk = blk0 + 16 * (kWaveTiles * wave + i) + n;
+        page[i] = blk < table_end ? kv8_page(p.c, b, blk) : -1;
+        const signed char* at = p.c.k_sum + ((size_t)max(page[i], 0) * p.c.Hkv + h) * D + 16 * g4;
+#pragma unroll
+        for (int k = 0; k < D / 64; ++k) m[i][k] = *reinterpret_cast<const int4_v*>(at + 64 * k);
     }
-    p.score[row * p.nb + blk] = score;
+    const Kv8Seq sq = kv8_seq(p.c, p.len, p.n_new, b, p.T);
+    const int nt = min(p.tq, sq.n + sq.t0 - t0), front = sq.len - (sq.n + sq.t0);
+    if (nt <= 0) return;
+    if (blk0 >= min((front + t0 + nt - 1) / kKvBlock, p.nb)) return;  // no query's own block has a score
+    const half_t* q = p.q.data + b * p.q.b + (long long)h * p.G * p.q.h + (long long)t0 * p.q.t;
+    if (tid < nt) most[tid] = 1;
+    __syncthreads();
+    // max |q| of each query's group, as the bits of its fp16: infinities and NaN are at least 0x7c00
+    for (int i = tid; i < nt * p.G * (D / 8); i += 256) {
+        const int row = i / (D / 8);
+        const half8_t x = *reinterpret_cast<const half8_t*>(q + row / p.G * p.q.t + row % p.G * p.q.h + i % (D / 8) * 8);
+        int a = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a = max(a, (int)(__builtin_bit_cast(unsigned short, (half_t)x[j]) & 0x7fff));
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) a = max(a, __shfl_xor(a, o));  // 8 lanes are of one row
+        if ((i & 7) == 0) atomicMax(&most[row / p.G], a);
+    }
+    int best = INT_MIN;  // one query of many heads: the maximum over its rounds
+    for (int col0 = 0; col0 < nt * p.G; col0 += kKvScoreCols) {
+        const int cols = min(kKvScoreCols, nt * p.G - col0);
+        __syncthreads();
+        for (int i = tid; i < cols * (D / 8); i += 256) {
+            const int col = i / (D / 8), row = col0 + col, big = most[row / p.G];
+            const half8_t x = *reinterpret_cast<const half8_t*>(q + row / p.G * p.q.t + row % p.G * p.q.h + i % (D / 8) * 8);
+            // a group with an infinity or NaN has no order: all its codes are 0
+            const float a = big < 0x7c00 ? (float)__builtin_bit_cast(half_t, (unsigned short)big) : 1.f, r = 1.f / a;
+            unsigned y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = kv8_code(big < 0x7c00 ? (float)x[j] : 0.f, a, r);
+            // code + 128 to code: the other sign bit
+            *reinterpret_cast<uint2*>(&qs[col * kRow + i % (D / 8) * 8]) =
+                uint2{kv8_pack(y[0], y[1], y[2], y[3]) ^ 0x80808080u, kv8_pack(y[4], y[5], y[6], y[7]) ^ 0x80808080u};
+        }
+        __syncthreads();
+        for (int ct = 0; 16 * ct < cols; ++ct) {
+            int4_v acc[kWaveTiles] = {};
+            // rows behind the last hold what they held: their scores are not looked at
+#pragma unroll
+            for (int k = 0; k < D / 64; ++k) {
+                const int4_v qf = *reinterpret_cast<const int4_v*>(&qs[(16 * ct + n) * kRow + 64 * k + 16 * g4]);
+#pragma unroll
+                for (int i = 0; i < kWaveTiles; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(m[i][k], qf, acc[i], 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < kWaveTiles; ++i) *reinterpret_cast<int4_v*>(&sc[16 * ct + n][16 * (kWaveTiles * wave + i) + 4 * g4]) = acc[i];
+        }
+        __syncthreads();
+        if (nt * p.G <= kKvScoreCols) {
+            for (int i = tid; i < nt * kKvScoreBlocks; i += 256) {
+                const int t = i / kKvScoreBlocks, j = i % kKvScoreBlocks;
+                int x = sc[t * p.G][j];
+                for (int g = 1; g < p.G; ++g) x = max(x, sc[t * p.G + g][j]);
+                sc[t * p.G][j] = x;
+            }
+        } else if (tid < kKvScoreBlocks) {  // one query: the maximum of all rounds
+            for (int g = 0; g < cols; ++g) best = max(best, sc[g][tid]);
+            sc[0][tid] = best;
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < nt * kKvScoreBlocks; i += 256) {
+        const int t = i / kKvScoreBlocks, blk = blk0 + i % kKvScoreBlocks;
+        const int pos = front + t0 + t;
+        if (pos < 0 || blk >= min(pos / kKvBlock, p.nb)) continue;
+        const int at = kv8_page(p.c, b, blk);
+        float x = -INFINITY;  // a block without a page
+        if (at >= 0) x = (float)sc[t * p.G][i % kKvScoreBlocks] * p.c.k_sum_scale[(size_t)at * p.c.Hkv + h];
+        // NaN: a block that holds an infinity or NaN
+        p.score[((size_t)blockIdx.y * p.T + t0 + t) * p.nb + blk] = x == x ? x : -INFINITY;
+    }
 }
 
 // A score as a whole number of the same order; 0 is below every score.
@@ -88,92 +133,115 @@ __device__ __forceinline__ unsigned kv8_order(float x) {
 }
 
 // Workgroup (t, b Hkv + h): the `top` best of the row's blocks, the lowest index first among
-// equals, listed ascending.  Four rounds over the scores' bytes find the last value that is kept.
-__global__ void __launch_bounds__(256)
+// equals, listed ascending.  The last value that is kept is found bit by bit from the top, by
+// counting the values that are at least as large (ballots; one barrier a bit), and no further than
+// where exactly `top` are.  A thread holds kN values (blocks i kThreads + thread) in registers; with
+// more blocks it reads them again for each bit.
+constexpr int kKvPickN = 8;
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads)
 kv8_pick_kernel(Kv8SelectArgs p) {
-    __shared__ int hist[256];
-    __shared__ int found[2];  // the round's byte, and how many of it are still to be kept
-    __shared__ int sums[2][4];
-    const int b = blockIdx.y / p.c.Hkv, t = blockIdx.x, tid = threadIdx.x;
+    constexpr int kWaves = kThreads / 64, kHeld = kKvPickN * kThreads;
+    __shared__ int count[2][kWaves];
+    __shared__ int sums[2][kWaves];
+    const int b = blockIdx.y / p.c.Hkv, t = blockIdx.x, tid = threadIdx.x, wave = tid >> 6;
+    const size_t row = (size_t)blockIdx.y * p.T + t;
+    const float* score = p.score + row * p.nb;
+    float held[kKvPickN];
+#pragma unroll
+    for (int j = 0; j < kKvPickN; ++j) held[j] = score[min(j * kThreads + tid, p.nb - 1)];
     const Kv8Seq sq = kv8_seq(p.c, p.len, p.n_new, b, p.T);
     if (t >= sq.n + sq.t0) return;
     const int pos = sq.len - (sq.n + sq.t0) + t;
-    const size_t row = (size_t)blockIdx.y * p.T + t;
     int* out = p.blocks + row * p.top;
     const int n = pos < 0 ? 0 : pos / kKvBlock + 1;
-    const int kept = min(n, p.top);
-    for (int i = kept + tid; i < p.top; i += 256) out[i] = -1;
+    for (int i = min(n, p.top) + tid; i < p.top; i += kThreads) out[i] = -1;
     if (n <= p.top) {
-        for (int i = tid; i < n; i += 256) out[i] = i;
+        for (int i = tid; i < n; i += kThreads) out[i] = i;
         return;
     }
-    const float* score = p.score + row * p.nb;
-    auto order = [&](int i) {
-        return i < p.first || i >= n - 1 - p.recent ? 0xffffffffu : i < p.nb ? kv8_order(score[i]) : 0u;
+    auto order = [&](int i, float x) {
+        return i < p.first || i >= n - 1 - p.recent ? 0xffffffffu : i < p.nb ? kv8_order(x) : 0u;
     };
-    unsigned value = 0;
-    int left = p.top;  // of the values that share the bytes found so far, how many are kept
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        hist[tid] = 0;
-        __syncthreads();
-        for (int i = tid; i < n; i += 256) {
-            const unsigned u = order(i);
-            if (shift == 24 || u >> (shift + 8) == value >> (shift + 8)) atomicAdd(&hist[u >> shift & 255], 1);
+    unsigned u[kKvPickN];
+#pragma unroll
+    for (int j = 0; j < kKvPickN; ++j) u[j] = j * kThreads + tid < n ? order(j * kThreads + tid, held[j]) : 0u;
+    auto at_least = [&](unsigned v, int slot) {  // v > 0
+        int x = 0;
+#pragma unroll
+        for (int j = 0; j < kKvPickN; ++j) x += __popcll(__ballot(u[j] >= v));
+        for (int i0 = kHeld; i0 < n; i0 += kThreads) {
+            const int i = i0 + tid;
+            x += __popcll(__ballot(i < n && order(i, i < p.nb ? score[i] : 0.f) >= v));
         }
+        if ((tid & 63) == 0) count[slot][wave] = x;
         __syncthreads();
-        if (tid == 0) {
-            int i = 255;
-            while (hist[i] < left) left -= hist[i--];
-            found[0] = i;
-            found[1] = left;
+        x = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) x += count[slot][w];
+        return x;
+    };
+    unsigned value = 0;  // at least `top` values are at least this
+    int have = n;
+    for (int bit = 31; bit >= 0 && have != p.top; --bit) {
+        const unsigned v = value | 1u << bit;
+        const int x = at_least(v, bit & 1);
+        if (x >= p.top) {
+            value = v;
+            have = x;
         }
-        __syncthreads();
-        value |= (unsigned)found[0] << shift;
-        left = found[1];
-        __syncthreads();
     }
-    // those above `value`, and the first `left` equal to it, in order
+    // where more than `top` are: those above `value`, and the first of the others
+    const bool all = have == p.top;
+    const int left = all ? n : p.top - (value == 0xffffffffu ? 0 : at_least(value + 1, 1));
     int done = 0, equal = 0;
-    for (int i0 = 0; i0 < n; i0 += 256) {
-        const int i = i0 + tid;
-        const unsigned u = i < n ? order(i) : 0;
-        const bool eq = i < n && u == value;
+    auto emit = [&](int i, unsigned x) {
+        const bool eq = i < n && x == value;
         const unsigned long long eqs = __ballot(eq), below = (1ull << (tid & 63)) - 1;
-        if ((tid & 63) == 0) sums[0][tid >> 6] = __popcll(eqs);
+        __syncthreads();
+        if ((tid & 63) == 0) sums[0][wave] = __popcll(eqs);
         __syncthreads();
         int before = equal + __popcll(eqs & below);
-        for (int w = 0; w < tid >> 6; ++w) before += sums[0][w];
-        const bool take = i < n && (u > value || (eq && before < left));
+        for (int w = 0; w < wave; ++w) before += sums[0][w];
+        const bool take = i < n && (x > value || (eq && before < left));
         const unsigned long long takes = __ballot(take);
-        if ((tid & 63) == 0) sums[1][tid >> 6] = __popcll(takes);
+        if ((tid & 63) == 0) sums[1][wave] = __popcll(takes);
         __syncthreads();
         int at = done + __popcll(takes & below);
-        for (int w = 0; w < tid >> 6; ++w) at += sums[1][w];
+        for (int w = 0; w < wave; ++w) at += sums[1][w];
         if (take) out[at] = i;
-        for (int w = 0; w < 4; ++w) {
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
             equal += sums[0][w];
             done += sums[1][w];
         }
-        __syncthreads();
+    };
+#pragma unroll
+    for (int j = 0; j < kKvPickN; ++j)
+        if (j * kThreads < n) emit(j * kThreads + tid, u[j]);
+    for (int i0 = kHeld; i0 < n; i0 += kThreads) {
+        const int i = i0 + tid;
+        emit(i, i < n ? order(i, i < p.nb ? score[i] : 0.f) : 0u);
     }
 }
 
-inline size_t kv8_select_qc_bytes(int B, int T, int Hq, int D) { return ((size_t)B * T * Hq * D + 255) / 256 * 256; }
-inline size_t kv8_select_bytes(int B, int T, int Hq, int Hkv, int D, int nb) {
-    return kv8_select_qc_bytes(B, T, Hq, D) + (size_t)B * Hkv * T * nb * 4;
-}
+inline size_t kv8_select_bytes(int B, int T, int Hkv, int nb) { return (size_t)B * Hkv * T * nb * 4; }
 
 template <int D>
 hipError_t kv8_select_d(const Kv8SelectArgs& p, hipStream_t stream) {
+    const int parts = (p.nb + kKvScoreBlocks - 1) / kKvScoreBlocks;
+    const dim3 grid((unsigned)((p.T + p.tq - 1) / p.tq * parts), (unsigned)(p.c.B * p.c.Hkv));
+    hipLaunchKernelGGL(kv8_score_kernel<D>, grid, dim3(256), 0, stream, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    // one wave a row where its registers hold the row's scores, else 16
     const dim3 rows((unsigned)p.T, (unsigned)(p.c.B * p.c.Hkv));
-    hipLaunchKernelGGL(kv8_qcode_kernel<D>, rows, dim3(256), 0, stream, p);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    const dim3 grid((unsigned)((p.nb + 255) / 256 * p.T), (unsigned)(p.c.B * p.c.Hkv));
-    hipLaunchKernelGGL(kv8_score_kernel<D>, grid, dim3(256), p.G * D, stream, p);
-    e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(kv8_pick_kernel, rows, dim3(256), 0, stream, p);
+    if (p.nb <= kKvPickN * 64)
+        hipLaunchKernelGGL(kv8_pick_kernel<64>, rows, dim3(64), 0, stream, p);
+    else if (p.nb <= kKvPickN * 256)
+        hipLaunchKernelGGL(kv8_pick_kernel<256>, rows, dim3(256), 0, stream, p);
+    else
+        hipLaunchKernelGGL(kv8_pick_kernel<1024>, rows, dim3(1024), 0, stream, p);
     return hipGetLastError();
 }
 
@@ -181,8 +249,8 @@ hipError_t kv8_select_d(const Kv8SelectArgs& p, hipStream_t stream) {
 
 hipError_t kv8_select(const Kv8& c, const Rows16& q, const int* len, const int* n_new, int T, int Hq, int top, int first,
                       int recent, int* blocks, int nb, void* ws, hipStream_t stream) {
-    const Kv8SelectArgs p{c, q, len, n_new, (signed char*)ws, (float*)((char*)ws + kv8_select_qc_bytes(c.B, T, Hq, c.D)),
-                          blocks, T, Hq, Hq / c.Hkv, top, first, recent, nb};
+    const int G = Hq / c.Hkv, tq = G <= kKvScoreCols ? kKvScoreCols / G : 1;
+    const Kv8SelectArgs p{c, q, len, n_new, (float*)ws, blocks, T, Hq, G, top, first, recent, nb, tq < T ? tq : T};
     if (c.D == 64) return kv8_select_d<64>(p, stream);
     if (c.D == 128) return kv8_select_d<128>(p, stream);
     return kv8_select_d<256>(p, stream);
@@ -191,7 +259,7 @@ hipError_t kv8_select(const Kv8& c, const Rows16& q, const int* len, const int* 
 size_t kv8_ws_bytes(int B, int T, int Hq, int Hkv, int D, int nb, int top) {
     const bool list = top > 0;
     const size_t part = kv8_part_bytes(B, T, Hq, Hkv, D, kv8_splits(kv8_tiles(B, T, Hq, Hkv, list), list ? top : nb));
-    const size_t sel = list ? kv8_select_bytes(B, T, Hq, Hkv, D, nb) : 0;
+    const size_t sel = list ? kv8_select_bytes(B, T, Hkv, nb) : 0;
     return part > sel ? part : sel;
 }
 
