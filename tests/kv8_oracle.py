@@ -35,6 +35,8 @@ class Head:
             parts.append(c * s)
             read.append(r)
         rest = x[self.n // BLOCK * BLOCK:]
+        self.steps = torch.cat([torch.full((BLOCK,), s, dtype=torch.float64) for s in self.scales] +
+                               [torch.ones(len(rest), dtype=torch.float64)])  # of a key's values: v / step is what is multiplied
         self.values = torch.cat(parts + [rest.double()])
         self.read = torch.cat(read + [rest])  # fp16, bit for bit
 
@@ -47,11 +49,14 @@ class Head:
         return m, np.float32(scale)
 
 
-def attend(q, K, V, keys, scale, gate=None):
+def attend(q, K, V, steps, keys, scale, gate=None):
     """q [D], K, V [n, D] values in 64 bits, keys: the positions seen (a list, repeats count).  The
     output in 64 bits and the most that a kernel with fp16 weights and fp32 sums may be off,
     element by element, the output's own rounding included:
-      weights       a rounding to fp16: 2^-11 of each
+      weights       a rounding to fp16: 2^-11 of each.  What is rounded is p_j step_j in units where the
+                    largest of a row is 2^12 or more, and what is multiplied v_j / step_j.  Below 2^-14
+                    fp16's steps are 2^-24, so a weight may be off by 2^-25 whatever its size: that
+                    is 2^-37 of the largest p_j step_j, times |v_j| / step_j, summed over the keys
       scores        an fp32 dot of D terms, the factor and log2 of the value scale: (D + 8) 2^-24 of
                     sum |q k| scale; and of the score itself, twice; exp2's argument and result: 2^-21
       sums          n terms in fp32: n 2^-23 at the most
@@ -61,7 +66,7 @@ def attend(q, K, V, keys, scale, gate=None):
     D = q.shape[0]
     if not keys:
         return torch.zeros(D, dtype=torch.float64), torch.full((D,), 2.0 ** -25, dtype=torch.float64)
-    k, v, q = K[keys], V[keys], q.double()
+    k, v, q, step = K[keys], V[keys], q.double(), steps[keys]
     s = (k @ q) * scale
     p = torch.exp(s - s.max())
     p = p / p.sum()
@@ -69,6 +74,7 @@ def attend(q, K, V, keys, scale, gate=None):
     size = p @ v.abs()
     ds = (D + 8) * 2.0 ** -24 * float((k.abs() @ q.abs()).max()) * scale + 2 ** -23 * float(s.abs().max()) + 2.0 ** -21
     tol = (2.0 ** -11 + 2 * (math.expm1(ds) + len(keys) * 2.0 ** -23)) * size
+    tol = tol + 2.0 ** -37 * float((p * step).max()) * (v.abs() / step[:, None]).sum(0)
     if gate is not None:
         g = 1 / (1 + torch.exp(-gate.double()))
         o, tol = o * g, (tol + 2.0 ** -20 * o.abs()) * g

@@ -65,7 +65,7 @@ def expect(q, k, v, lens, n_new, causal, gate=None, scale=None, lists=None, page
     for b in range(B):
         n, L = n_new[b], lens[b]
         for h in range(H):
-            K, V = ko.Head(k[b, h, :L]).values, ko.Head(v[b, h, :L]).values
+            K, V = ko.Head(k[b, h, :L]).values, ko.Head(v[b, h, :L])
             for t in range(n):
                 p = L - n + t
                 see = list(range(p + 1 if causal else L)) if p >= 0 or not causal else []
@@ -75,7 +75,7 @@ def expect(q, k, v, lens, n_new, causal, gate=None, scale=None, lists=None, page
                     see = [j for j in see if pages[b][j // 64] or j >= L // 64 * 64]
                 for g in range(G):
                     hq = h * G + g
-                    want[b, hq, t], tol[b, hq, t] = ko.attend(q[b, hq, t], K, V, see, scale, None if gate is None else gate[b, hq, t])
+                    want[b, hq, t], tol[b, hq, t] = ko.attend(q[b, hq, t], K, V.values, V.steps, see, scale, None if gate is None else gate[b, hq, t])
     return want, tol
 
 

@@ -189,62 +189,64 @@ __device__ __forceinline__ void kv8_open_block(Kv8State<D, NT>& st, const Kv8& c
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) w[nt][a] = mfma16(kf, st.q[nt][2 * i + x], w[nt][a]);
                 }
-        half8_t v[D / 16];
+        kv8_softmax<D, NT, 2>(st, w, p0, {c2, 0.f, 1.f}, true);
+        half8_t p[NT];
 #pragma unroll
-        for (int m = 0; m < D / 32; ++m)
-#pragma unroll
-            for (int o = 0; o < 2; ++o) v[2 * m + o] = vp[(s * (D / 32) + m) * 128 + o];
+        for (int nt = 0; nt < NT; ++nt) p[nt] = kv8_weights<2>(w[nt], 0);
         uint4_v keep;  // elements of rows that there are
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int key = 32 * s + 16 * (j >> 1) + 4 * g4 + 2 * (j & 1);
             keep[j] = (key < n ? 0xffffu : 0u) | (key + 1 < n ? 0xffff0000u : 0u);
         }
-        ushort8_t big = {};
 #pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt) {
-            v[dt] = __builtin_bit_cast(half8_t, __builtin_bit_cast(uint4_v, v[dt]) & keep);
-            big = __builtin_elementwise_max(big, __builtin_bit_cast(ushort8_t, v[dt]) & (unsigned short)0x7fff);
-        }
-        int most = 0;
+        for (int m = 0; m < D / 32; m += 2) {  // 64 d at a time
+            half8_t v[4];
+            ushort8_t big = {};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) most = max(most, (int)big[j]);
-        const bool bad = __any(most >= 0x7c00);
-        if (bad) {
+            for (int x = 0; x < 4; ++x) v[x] = vp[(s * (D / 32) + m + (x >> 1)) * 128 + (x & 1)];
 #pragma unroll
-            for (int dt = 0; dt < D / 16; ++dt)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[dt][j] = kv8_bad(v[dt][j]) ? (half_t)0.f : v[dt][j];
-        }
-        kv8_softmax<D, NT, 2>(st, w, p0, {c2, 0.f, 1.f}, true);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const half8_t p = kv8_weights<2>(w[nt], 0);
-#pragma unroll
-            for (int dt = 0; dt < D / 16; ++dt) st.o[nt][dt] = mfma16(v[dt], p, st.o[nt][dt]);
-        }
-        if (!bad) continue;
-        const half_t* vo = c.v_open + at;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll 1
-            for (int x = 0; x < 32; ++x) {
-                const int j = x >> 2, g = x & 3, key = 16 * (j >> 2) + 4 * g + (j & 3);
-                float wj = 0.f;
-#pragma unroll
-                for (int a = 0; a < 2; ++a)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) wj = j == 4 * a + r ? w[nt][a][r] : wj;
-                wj = __shfl(wj, 16 * g + (lane & 15));
-                if (p0 + key > st.limit[nt]) continue;
-#pragma unroll
-                for (int dt = 0; dt < D / 16; ++dt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const half_t y = vo[kv8_v_at<D>(32 * s + key, 16 * dt + 4 * g4 + e)];
-                        if (kv8_bad(y)) st.o[nt][dt][e] += wj * (float)y;
-                    }
+            for (int x = 0; x < 4; ++x) {
+                v[x] = __builtin_bit_cast(half8_t, __builtin_bit_cast(uint4_v, v[x]) & keep);
+                big = __builtin_elementwise_max(big, __builtin_bit_cast(ushort8_t, v[x]) & (unsigned short)0x7fff);
             }
+            int most = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) most = max(most, (int)big[j]);
+            const bool bad = __any(most >= 0x7c00);
+            if (bad) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[x][j] = kv8_bad(v[x][j]) ? (half_t)0.f : v[x][j];
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) st.o[nt][2 * m + x] = mfma16(v[x], p[nt], st.o[nt][2 * m + x]);
+            if (!bad) continue;
+            const half_t* vo = c.v_open + at;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll 1
+                for (int y = 0; y < 32; ++y) {
+                    const int j = y >> 2, g = y & 3, key = 16 * (j >> 2) + 4 * g + (j & 3);
+                    float wj = 0.f;
+#pragma unroll
+                    for (int a = 0; a < 2; ++a)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) wj = j == 4 * a + r ? w[nt][a][r] : wj;
+                    wj = __shfl(wj, 16 * g + (lane & 15));
+                    if (p0 + key > st.limit[nt]) continue;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const half_t z = vo[kv8_v_at<D>(32 * s + key, 16 * (2 * m + x) + 4 * g4 + e)];
+                            if (kv8_bad(z)) st.o[nt][2 * m + x][e] += wj * (float)z;
+                        }
+                }
+        }
     }
 }
 
@@ -474,6 +476,139 @@ kv8_row_kernel(Kv8AttnArgs p) {
 
 constexpr int kKvMaxSplits = 128;
 
+// Many rows: a workgroup is 4 waves of 16 NT query rows each over one split of their blocks.  A
+// stage of kKeys keys and their values (16 KiB of codes at the most) goes from memory to registers
+// two stages ahead, is turned into fp16 operands once for all waves, and lies in one of two LDS
+// buffers in operand order, so every LDS access is 16 consecutive bytes a lane and a code is
+// converted once per 64 NT rows.  One barrier a stage.
+template <int D, int NT>
+struct Kv8Tile {
+    static constexpr int kKeys = D == 256 ? 32 : 64, kParts = kKvBlock / kKeys;
+    static constexpr int kUnits = kKeys * D / 16;          // 16-code units of K (or V) a stage
+    static constexpr int kN = kUnits / 256;                // of them a thread moves
+    static constexpr int kRows = 64 * NT;
+    static constexpr int kLds = 2 * 2 * kKeys * D * 2;     // 2 buffers x (K, V) of fp16
+};
+template <int D, int NT>
+__global__ void __launch_bounds__(256, 2)
+kv8_tile_kernel(Kv8AttnArgs p, int tiles, int streams) {
+    using C = Kv8Tile<D, NT>;
+    __shared__ __align__(16) half8_t buf[2][4 * C::kUnits];  // K's halves, then V's
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g4 = lane >> 4, n = lane & 15;
+    const Kv8& c = p.c;
+    // Workgroups go round the 8 XCDs: all tiles of one (head, split), which read the same keys, on
+    // one of them where there are enough to share out, the last (longest) tiles first.
+    int stream, rank;
+    if ((streams & 7) == 0) {
+        const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3, per = streams >> 3;
+        stream = xcd * per + slot % per;
+        rank = slot / per;
+    } else {
+        stream = blockIdx.x % streams;
+        rank = blockIdx.x / streams;
+    }
+    const int tile = tiles - 1 - rank, bh = stream / p.nsplit, split = stream % p.nsplit;
+    const int b = bh / c.Hkv, h = bh % c.Hkv;
+    const Kv8Seq sq = kv8_seq(c, p.len, p.n_new, b, p.T);
+    const int front = sq.len - (sq.n + sq.t0);  // position of row t = 0
+    const int row_end = min(p.T, sq.n + sq.t0) * p.G;
+    if (tile * C::kRows >= row_end) return;
+
+    Kv8State<D, NT> st;
+    const int row0 = tile * C::kRows + wave * 16 * NT;
+    const int see = kv8_begin<D, NT>(st, p, sq, b, h, row0, row_end);
+    const int least = kv8_least<D, NT>(st, row0, row_end);
+    // the last key that any row of the workgroup sees
+    const int all = p.causal ? min(front + (min(row_end, (tile + 1) * C::kRows) - 1) / p.G, sq.len - 1) : sq.len - 1;
+    const int nb = all < 0 ? 0 : all / kKvBlock + 1;
+    const int n_full = min(sq.len / kKvBlock, nb);
+    const int per = (nb + p.nsplit - 1) / p.nsplit;
+    const int end = min(nb, (split + 1) * per);
+    int i = split * per, blk = 0, page = -1, part = 0;
+    const bool open = i <= n_full && n_full < end;
+    auto next = [&]() {  // the split's next full block that has a page
+        for (page = -1; page < 0 && i < min(end, n_full); ++i) {
+            blk = i;
+            page = kv8_page(c, b, blk);
+        }
+    };
+
+    struct Stage {
+        int p0;  // first key, -1: none
+        float sk, sv;
+    };
+    uint4 rk[C::kN], rv[C::kN];
+    auto load = [&]() -> Stage {  // codes of the stage at (page, part) to registers, and on to the next
+        if (page < 0) return {-1, 0.f, 0.f};
+        const size_t head = (size_t)page * c.Hkv + h;
+        const uint4* kp = reinterpret_cast<const uint4*>(c.k + head * (kKvBlock * D)) + part * C::kUnits + tid;
+        const uint4* vp = reinterpret_cast<const uint4*>(c.v + head * (kKvBlock * D)) + part * C::kUnits + tid;
+#pragma unroll
+        for (int x = 0; x < C::kN; ++x) rk[x] = kp[x * 256];
+#pragma unroll
+        for (int x = 0; x < C::kN; ++x) rv[x] = vp[x * 256];
+        const Stage s = {blk * kKvBlock + part * C::kKeys, c.k_scale[head], c.v_scale[head]};
+        if (++part == C::kParts) {
+            part = 0;
+            next();
+        }
+        return s;
+    };
+    auto store = [&](int to) {  // registers to LDS as fp16
+#pragma unroll
+        for (int x = 0; x < C::kN; ++x) {
+            const int at = ((tid >> 6) + 4 * x) * 128 + lane;
+            buf[to][at] = kv8_halves(rk[x].x, rk[x].y);
+            buf[to][at + 64] = kv8_halves(rk[x].z, rk[x].w);
+            buf[to][2 * C::kUnits + at] = kv8_halves(rv[x].x, rv[x].y);
+            buf[to][2 * C::kUnits + at + 64] = kv8_halves(rv[x].z, rv[x].w);
+        }
+    };
+    next();
+    Stage now = load();
+    if (now.p0 >= 0) store(0);
+    Stage then = load();
+    lds_barrier();
+    for (int u = 0; now.p0 >= 0; u ^= 1) {
+        if (then.p0 >= 0) store(u ^ 1);
+        const Stage after = load();
+        if (now.p0 <= see) {
+            const half8_t* kb = &buf[u][lane];
+            const half8_t* vb = kb + 2 * C::kUnits;
+            const Kv8Scale sc = {p.c2 * now.sk, __builtin_amdgcn_logf(now.sv), __builtin_amdgcn_rcpf(now.sv)};
+            kv8_keys<D, NT, C::kKeys / 16>(
+                st, now.p0, sc, now.p0 + C::kKeys - 1 > least,
+                [&](int a, int x, int s) { return kb[((a * (D / 64) + x) * 2 + s) * 64]; },
+                [&](int s, int m, int o) { return vb[((s * (D / 32) + m) * 2 + o) * 64]; }, []() {});
+        }
+        lds_barrier();
+        now = then;
+        then = after;
+    }
+    if (open && see >= n_full * kKvBlock) kv8_open_block<D, NT>(st, c, b, h, n_full, sq.len - n_full * kKvBlock, p.c2);
+
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const float l = sum_xor32(sum_xor16(st.l[nt]));
+        const int row = row0 + 16 * nt + n;
+        if (row >= row_end) continue;
+        if (p.nsplit > 1) {
+            if (l != 0.f) {
+                float* at = kv8_part<D>(p, bh, row, split) + 4 * g4;
+#pragma unroll
+                for (int dt = 0; dt < D / 16; ++dt) *reinterpret_cast<float4_t*>(at + 16 * dt) = st.o[nt][dt];
+            }
+            if (g4 == 0) *reinterpret_cast<float2*>(kv8_pair<D>(p, bh, row, split)) = float2{st.m[nt], l};
+        } else {
+            const int t = row / p.G, hq = h * p.G + row % p.G;
+#pragma unroll
+            for (int dt = 0; dt < D / 16; ++dt)
+                kv8_store4(p, b, hq, t, 16 * dt + 4 * g4, st.o[nt][dt], l, kv8_gate4(p, b, hq, t, 16 * dt + 4 * g4));
+        }
+    }
+}
+
 // Joins the splits of 1024 / D rows: workgroup (rows, b Hkv + h), D / 4 lanes a row.  Every address
 // is known at once, so that the loads wait for memory together and not for each other: a row's
 // maxima and sums, its first splits' sums (unread where they were not written), its gate.
@@ -534,53 +669,74 @@ kv8_join_kernel(Kv8AttnArgs p) {
     kv8_store4(p, b, hq, t, 4 * x, y, l, gate);
 }
 
-// Key splits of one tile: as many workgroups as the chip takes twice, not fewer than 4 blocks each.
-inline int kv8_splits(long long tiles, int items) {
-    const long long want = (1024 + tiles - 1) / tiles;
+// How a call's rows are cut into tiles and its keys into splits.
+struct Kv8Plan {
+    int rows;       // of a tile
+    long long tiles;  // of one K/V head
+    int nsplit;
+};
+// One tile of 16 rows where there are no more (and for listed blocks, one query's heads), else
+// workgroups of 64 or 128 rows.  items: blocks of the longest sequence, or of a list.
+inline Kv8Plan kv8_plan(int B, int T, int Hq, int Hkv, int items, bool list) {
+    const long long G = Hq / Hkv, rows = T * G;
+    Kv8Plan q;
+    q.rows = list || rows <= 16 ? 16 : rows <= 64 ? 64 : 128;
+    q.tiles = list ? T * ((G + 15) / 16) : (rows + q.rows - 1) / q.rows;
+    const long long all = q.tiles * B * Hkv;
+    // row tiles: as many workgroups as the chip takes twice, not fewer than 4 blocks each; the others
+    // as many as it takes once
+    const long long want = q.rows == 16 ? (1024 + all - 1) / all : 512 / all;
     const long long most = (items + 3) / 4;
     const long long n = want < most ? want : most;
-    return (int)(n < kKvMaxSplits ? n : kKvMaxSplits);
+    q.nsplit = (int)(n < 1 ? 1 : n < kKvMaxSplits ? n : kKvMaxSplits);
+    return q;
 }
-inline long long kv8_tiles(int B, int T, int Hq, int Hkv, bool list) {
-    const long long G = Hq / Hkv;
-    return (long long)B * Hkv * (list ? (long long)T * ((G + 15) / 16) : (T * G + 15) / 16);
-}
-inline size_t kv8_part_bytes(int B, int T, int Hq, int Hkv, int D, int nsplit) {
+inline size_t kv8_part_bytes(int B, int T, int Hq, int D, int nsplit) {
     return nsplit > 1 ? (size_t)B * T * Hq * nsplit * (D + 2) * 4 : 0;
 }
 
 template <int D, bool kList>
-hipError_t kv8_attn_d(Kv8AttnArgs p, hipStream_t stream) {
-    const long long tiles = kv8_tiles(1, p.T, p.G, 1, kList);
-    const dim3 grid((unsigned)tiles, (unsigned)(p.c.B * p.c.Hkv), (unsigned)p.nsplit);
-    hipLaunchKernelGGL((kv8_row_kernel<D, kList>), grid, dim3(256), 0, stream, p);
-    hipError_t e = hipGetLastError();
+hipError_t kv8_attn_d(const Kv8AttnArgs& p, const Kv8Plan& q, hipStream_t stream) {
+    const int BH = p.c.B * p.c.Hkv;
+    if (kList || q.rows == 16) {
+        const dim3 grid((unsigned)q.tiles, (unsigned)BH, (unsigned)p.nsplit);
+        hipLaunchKernelGGL((kv8_row_kernel<D, kList>), grid, dim3(256), 0, stream, p);
+    } else {
+        const dim3 grid((unsigned)(q.tiles * BH * p.nsplit));
+        if (q.rows == 64)
+            hipLaunchKernelGGL((kv8_tile_kernel<D, 1>), grid, dim3(256), 0, stream, p, (int)q.tiles, BH * p.nsplit);
+        else
+            hipLaunchKernelGGL((kv8_tile_kernel<D, 2>), grid, dim3(256), 0, stream, p, (int)q.tiles, BH * p.nsplit);
+    }
+    const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.nsplit == 1) return e;
     constexpr int kRows = 1024 / D;
-    const dim3 rows((unsigned)((p.T * p.G + kRows - 1) / kRows), (unsigned)(p.c.B * p.c.Hkv));
+    const dim3 rows((unsigned)((p.T * p.G + kRows - 1) / kRows), (unsigned)BH);
     hipLaunchKernelGGL(kv8_join_kernel<D>, rows, dim3(256), 0, stream, p);
     return hipGetLastError();
 }
 template <bool kList>
-hipError_t kv8_attn_any(const Kv8AttnArgs& p, hipStream_t stream) {
-    if (p.c.D == 64) return kv8_attn_d<64, kList>(p, stream);
-    if (p.c.D == 128) return kv8_attn_d<128, kList>(p, stream);
-    return kv8_attn_d<256, kList>(p, stream);
+hipError_t kv8_attn_any(const Kv8AttnArgs& p, const Kv8Plan& q, hipStream_t stream) {
+    if (p.c.D == 64) return kv8_attn_d<64, kList>(p, q, stream);
+    if (p.c.D == 128) return kv8_attn_d<128, kList>(p, q, stream);
+    return kv8_attn_d<256, kList>(p, q, stream);
 }
 
 }  // namespace
 
 hipError_t kv8_attn(const Kv8& c, const Rows16& q, const Rows16& gate, const Rows16& o, const int* len, const int* n_new,
                     int T, int Hq, int nb_hint, float scale, int causal, void* ws, hipStream_t stream) {
-    const int nsplit = kv8_splits(kv8_tiles(c.B, T, Hq, c.Hkv, false), nb_hint);
-    return kv8_attn_any<false>({c, q, gate, o, len, n_new, nullptr, (float*)ws, T, Hq, Hq / c.Hkv, 0, nsplit, causal, scale * kLog2e}, stream);
+    const Kv8Plan plan = kv8_plan(c.B, T, Hq, c.Hkv, nb_hint, false);
+    return kv8_attn_any<false>({c, q, gate, o, len, n_new, nullptr, (float*)ws, T, Hq, Hq / c.Hkv, 0, plan.nsplit, causal, scale * kLog2e},
+                               plan, stream);
 }
 
 hipError_t kv8_attn_blocks(const Kv8& c, const Rows16& q, const Rows16& gate, const Rows16& o, const int* len,
                            const int* n_new, int T, int Hq, const int* blocks, int top, float scale, void* ws,
                            hipStream_t stream) {
-    const int nsplit = kv8_splits(kv8_tiles(c.B, T, Hq, c.Hkv, true), top);
-    return kv8_attn_any<true>({c, q, gate, o, len, n_new, blocks, (float*)ws, T, Hq, Hq / c.Hkv, top, nsplit, 1, scale * kLog2e}, stream);
+    const Kv8Plan plan = kv8_plan(c.B, T, Hq, c.Hkv, top, true);
+    return kv8_attn_any<true>({c, q, gate, o, len, n_new, blocks, (float*)ws, T, Hq, Hq / c.Hkv, top, plan.nsplit, 1, scale * kLog2e}, plan,
+                              stream);
 }
 
 }  // namespace tsa
