@@ -57,6 +57,13 @@ __device__ __forceinline__ unsigned kv8_pack(unsigned b0, unsigned b1, unsigned 
     return __builtin_amdgcn_perm(__builtin_amdgcn_perm(b3, b2, 0x0c0c0400u), __builtin_amdgcn_perm(b1, b0, 0x0c0c0400u), 0x05040100u);
 }
 
+// A value at an address that is the same on all lanes and that the kernel does not write: a scalar
+// load (the compiler takes a vector load where it cannot see that).
+template <typename T>
+__device__ __forceinline__ T kv8_uniform(const T* p) {
+    return *(const __attribute__((address_space(4))) T*)(uintptr_t)p;
+}
+
 // A sequence's tokens: `len` of them, the last `n` new; rows of a call's T start at new row `t0`
 // (rows before it would lie in front of the sequence).  Every count is clamped to what the cache
 // and the call hold, so that no value of the device arrays leads out of bounds.
@@ -66,8 +73,8 @@ struct Kv8Seq {
 __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8& c, const int* __restrict__ len, const int* __restrict__ n_new,
                                           int b, int T) {
     Kv8Seq s;
-    s.len = min(max(len[b], 0), c.max_blocks * kKvBlock);
-    const int n = n_new ? min(max(n_new[b], 0), T) : T;
+    s.len = min(max(kv8_uniform(len + b), 0), c.max_blocks * kKvBlock);
+    const int n = n_new ? min(max(kv8_uniform(n_new + b), 0), T) : T;
     s.n = min(n, s.len);
     s.t0 = n - s.n;
     return s;
@@ -76,6 +83,12 @@ __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8& c, const int* __restrict__ 
 // The page of block `blk` of sequence b, -1 where the table names none.
 __device__ __forceinline__ int kv8_page(const Kv8& c, int b, int blk) {
     const int p = c.table[(size_t)b * c.max_blocks + blk];
+    return p >= 0 && p < c.n_pages ? p : -1;
+}
+
+// The same, sequence and block being the same on all lanes.
+__device__ __forceinline__ int kv8_uniform_page(const Kv8& c, int b, int blk) {
+    const int p = kv8_uniform(c.table + (size_t)b * c.max_blocks + blk);
     return p >= 0 && p < c.n_pages ? p : -1;
 }
 

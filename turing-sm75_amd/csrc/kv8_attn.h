@@ -55,16 +55,51 @@ struct Kv8State {
     int limit[NT];          // last key the row sees, -1: none
 };
 
-// Scales of a block as the softmax takes them: the score's factor (scale log2(e) sk), log2(sv) and
+// A block's scales as the softmax takes them: the score's factor (scale log2(e) sk), log2(sv) and
 // 1 / sv.
 struct Kv8Scale {
     float f, lsv, isv;
 };
-__device__ __forceinline__ Kv8Scale kv8_scale(const Kv8& c, int page, int h, float c2) {
-    const size_t head = (size_t)page * c.Hkv + h;
-    const float sv = c.v_scale[head];
-    return {c2 * c.k_scale[head], __builtin_amdgcn_logf(sv), __builtin_amdgcn_rcpf(sv)};
-}
+
+// The full blocks of a wave's work, in turn.  Each lane looks one of the next 64 items up (an entry
+// of the list, or the item itself; its page; its scales), so that a block's are lane reads and no
+// load waits for another once in 64 blocks.
+template <bool kList>
+struct Kv8Walk {
+    int item, end, step;   // the next 64 are item + step * lane, below end
+    int nb, n_full;        // blocks that are seen, and the full ones of them
+    int open;              // how often the open block came up
+    unsigned long long todo;
+    int blks, pages;       // of this lane's item
+    Kv8Scale scales;
+
+    __device__ __forceinline__ void look(const Kv8& c, int b, int h, const int* list, float c2) {
+        const int i = item + step * (int)(threadIdx.x & 63);
+        blks = i < end ? (kList ? list[i] : i) : -1;
+        if (kList || n_full < nb) open += __popcll(__ballot(blks >= n_full && blks < nb));
+        const bool is = blks >= 0 && blks < n_full;
+        pages = is ? kv8_page(c, b, blks) : -1;
+        const size_t head = (size_t)max(pages, 0) * c.Hkv + h;
+        const float sk = c.k_scale[head], sv = c.v_scale[head];
+        scales = {c2 * sk, __builtin_amdgcn_logf(sv), __builtin_amdgcn_rcpf(sv)};
+        todo = __ballot(pages >= 0);
+        item += 64 * step;
+    }
+    // The next block; false when there is none.
+    __device__ __forceinline__ bool next(const Kv8& c, int b, int h, const int* list, float c2, int& blk, int& page, Kv8Scale& sc) {
+        while (todo == 0) {
+            if (item >= end) return false;
+            look(c, b, h, list, c2);
+        }
+        const int l = __builtin_ctzll(todo);
+        todo &= todo - 1;
+        auto read = [&](float x) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), l)); };
+        blk = __builtin_amdgcn_readlane(blks, l);
+        page = __builtin_amdgcn_readlane(pages, l);
+        sc = {read(scales.f), read(scales.lsv), read(scales.isv)};
+        return true;
+    }
+};
 
 // Scores (w: raw q . k') to weights for 16 KA keys from p0 on: raises the running maximum where a
 // score passes it by more than the slack, rescaling what there is, and adds to the row sums.
@@ -86,10 +121,9 @@ __device__ __forceinline__ void kv8_softmax(Kv8State<D, NT>& st, float4_t (&w)[N
         for (int a = 0; a < KA; ++a)
 #pragma unroll
             for (int r = 0; r < 4; ++r) big = fmaxf(big, w[nt][a][r]);
-        big = max_xor32(max_xor16(big));
-        big = __builtin_fmaf(big, sc.f, sc.lsv);
+        big = __builtin_fmaf(big, sc.f, sc.lsv);  // of this lane's keys
         if (__any(big > st.m[nt] + kKvSlack)) {
-            const float m_new = fmaxf(st.m[nt], big);
+            const float m_new = fmaxf(st.m[nt], max_xor32(max_xor16(big)));
             const float alpha = m_new == st.m[nt] ? 1.f : fast_exp2(st.m[nt] - m_new);
             st.m[nt] = m_new;
             st.l[nt] *= alpha;
@@ -118,8 +152,7 @@ __device__ __forceinline__ void kv8_softmax(Kv8State<D, NT>& st, float4_t (&w)[N
 // Weights of key tiles 2 s and 2 s + 1 as operand B.
 template <int KA>
 __device__ __forceinline__ half8_t kv8_weights(const float4_t (&w)[KA], int s) {
-    return half8_t{(half_t)w[2 * s][0],     (half_t)w[2 * s][1],     (half_t)w[2 * s][2],     (half_t)w[2 * s][3],
-                   (half_t)w[2 * s + 1][0], (half_t)w[2 * s + 1][1], (half_t)w[2 * s + 1][2], (half_t)w[2 * s + 1][3]};
+    return __builtin_convertvector(__builtin_shufflevector(w[2 * s], w[2 * s + 1], 0, 1, 2, 3, 4, 5, 6, 7), half8_t);
 }
 
 // 16 KA keys: kload(a, i, s) and vload(s, m, o) give the operands; between() is called where the
@@ -158,6 +191,61 @@ __device__ __forceinline__ void kv8_keys(Kv8State<D, NT>& st, int p0, const Kv8S
                 for (int nt = 0; nt < NT; ++nt) st.o[nt][2 * m + o] = mfma16(vf, p[nt], st.o[nt][2 * m + o]);
             }
     }
+}
+
+// The same from operands in LDS (kb, vb: this lane's of K and V), read a few ahead of their products;
+// between(e) is called among K's.  The queries' last kQl steps lie in LDS too (qb: this lane's).
+template <int D, int NT, int KA, int kQl, class Between>
+__device__ __forceinline__ void kv8_lds_keys(Kv8State<D, NT>& st, int p0, const Kv8Scale& sc, bool masked, const half8_t* kb,
+                                             const half8_t* vb, const half8_t* qb, Between between) {
+    constexpr int kOps = KA * (D / 32), kAhead = D == 256 ? 3 : 6, kQr = D / 32 - kQl;
+    float4_t w[NT][KA];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int a = 0; a < KA; ++a) w[nt][a] = float4_t{0.f, 0.f, 0.f, 0.f};
+    half8_t op[kOps], ql[D / 32][NT];
+    auto read_k = [&](int e) {  // key tile e % KA, step e / KA
+        const int a = e % KA, x = e / KA;
+        op[e] = kb[((a * (D / 64) + x / 2) * 2 + x % 2) * 64];
+    };
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) read_k(e);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int e = 0; e < kOps; ++e) {
+        if (e + kAhead < kOps) read_k(e + kAhead);
+        // a step of queries from LDS two products before its first
+        if (kQl && (e + 2) % KA == 0 && (e + 2) / KA >= kQr && e + 2 < kOps) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) ql[(e + 2) / KA][nt] = qb[(((e + 2) / KA - kQr) * NT + nt) * 64];
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+            w[nt][e % KA] = mfma16(op[e], e / KA < kQr ? st.q[nt][e / KA] : ql[e / KA][nt], w[nt][e % KA]);
+        between(e);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    auto read_v = [&](int e) { op[e] = vb[e * 64]; };  // (s, m, o) in order
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) read_v(e);
+    kv8_softmax<D, NT, KA>(st, w, p0, sc, masked);
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int s = 0; s < KA / 2; ++s) {
+        half8_t p[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) p[nt] = kv8_weights<KA>(w[nt], s);
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) {
+            const int e = s * (D / 16) + dt;
+            if (e + kAhead < kOps) read_v(e + kAhead);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) st.o[nt][dt] = mfma16(op[e], p[nt], st.o[nt][dt]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    __builtin_amdgcn_s_setprio(0);
 }
 
 // The open block from the ring: n of its rows are the sequence's, those behind are whatever the
@@ -281,6 +369,16 @@ __device__ __forceinline__ int kv8_begin(Kv8State<D, NT>& st, const Kv8AttnArgs&
     return __builtin_amdgcn_readfirstlane(see);
 }
 
+// The queries have arrived: said in front of a loop that only reads them, the loop waits for none
+// of the loads that it has under way itself.
+template <int D, int NT>
+__device__ __forceinline__ void kv8_arrived(Kv8State<D, NT>& st) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) asm volatile("" : "+v"(st.q[nt][i]));
+}
+
 // The last key that every row of the tile sees.
 template <int D, int NT>
 __device__ __forceinline__ int kv8_least(const Kv8State<D, NT>& st, int row0, int row_end) {
@@ -327,15 +425,12 @@ template <int D>
 struct Kv8Regs {
     static constexpr int kKeys = D == 256 ? 32 : 64, kN = kKeys * D / 1024;
     uint4 k[kN], v[kN];
-    float sk, sv;
 
     __device__ __forceinline__ void load_k(const Kv8& c, int page, int h, int part) {
         const size_t head = (size_t)page * c.Hkv + h;
         const uint4* kp = reinterpret_cast<const uint4*>(c.k + head * (kKvBlock * D)) + part * (kN * 64) + (threadIdx.x & 63);
 #pragma unroll
         for (int i = 0; i < kN; ++i) k[i] = kp[i * 64];
-        sk = c.k_scale[head];
-        sv = c.v_scale[head];
     }
     __device__ __forceinline__ void load_v(const Kv8& c, int page, int h, int part) {
         const size_t head = (size_t)page * c.Hkv + h;
@@ -382,18 +477,11 @@ kv8_row_kernel(Kv8AttnArgs p) {
     const int per = (items + p.nsplit - 1) / p.nsplit;
     const int end = min(items, (split + 1) * per);
     const int* list = kList ? p.blocks + (((size_t)b * c.Hkv + h) * p.T + row0 / p.G) * p.top : nullptr;
-    int open = 0;  // how often the open block is among this wave's
-    int i = split * per + wave, blk = 0, page = -1;
-    // the next of this wave's full blocks that has a page; i is behind it
+    Kv8Walk<kList> walk = {split * per + wave, end, 4, nb, n_full, 0, 0};
+    int blk = 0, page = -1;
+    Kv8Scale sc = {};
     auto next = [&]() {
-        for (page = -1; page < 0 && i < end; i += 4) {
-            blk = kList ? list[i] : i;
-            if (blk < 0 || blk >= nb) continue;
-            if (blk >= n_full)
-                ++open;
-            else
-                page = kv8_page(c, b, blk);
-        }
+        if (!walk.next(c, b, h, list, p.c2, blk, page, sc)) page = -1;
     };
     // rows of one query see whole blocks but the last; several queries' last one or two are masked
     const int least = kv8_least<D, 1>(st, row0, row_end);
@@ -403,16 +491,17 @@ kv8_row_kernel(Kv8AttnArgs p) {
         Kv8Regs<D> x;
         x.load_k(c, page, h, 0);
         x.load_v(c, page, h, 0);
+        kv8_arrived<D, 1>(st);
         while (page >= 0) {
             const int now = blk, here = page;
-            const Kv8Scale sc = {p.c2 * x.sk, __builtin_amdgcn_logf(x.sv), __builtin_amdgcn_rcpf(x.sv)};
+            const Kv8Scale scale = sc;
 #pragma unroll
             for (int part = 0; part < kParts; ++part) {
                 const bool last = part == kParts - 1;
                 if (last) next();
                 const int to = last ? page : here;
                 kv8_keys<D, 1, Kv8Regs<D>::kKeys / 16>(
-                    st, now * kKvBlock + part * Kv8Regs<D>::kKeys, sc, masked(now),
+                    st, now * kKvBlock + part * Kv8Regs<D>::kKeys, scale, masked(now),
                     [&](int a, int i, int s) {
                         const uint4& k = x.k[a * (D / 64) + i];
                         return s ? kv8_halves(k.z, k.w) : kv8_halves(k.x, k.y);
@@ -428,7 +517,7 @@ kv8_row_kernel(Kv8AttnArgs p) {
             }
         }
     }
-    for (; open > 0; --open) kv8_open_block<D, 1>(st, c, b, h, n_full, sq.len - n_full * kKvBlock, p.c2);
+    for (; walk.open > 0; --walk.open) kv8_open_block<D, 1>(st, c, b, h, n_full, sq.len - n_full * kKvBlock, p.c2);
 
     // the four waves' sums, relative to their common maximum
     st.l[0] = sum_xor32(sum_xor16(st.l[0]));
@@ -487,26 +576,31 @@ struct Kv8Tile {
     static constexpr int kUnits = kKeys * D / 16;          // 16-code units of K (or V) a stage
     static constexpr int kN = kUnits / 256;                // of them a thread moves
     static constexpr int kRows = 64 * NT;
-    static constexpr int kLds = 2 * 2 * kKeys * D * 2;     // 2 buffers x (K, V) of fp16
+    static constexpr int kQl = D == 256 && NT == 2 ? 2 : 0;  // steps of the queries kept in LDS: registers for the rest
 };
 template <int D, int NT>
 __global__ void __launch_bounds__(256, 2)
 kv8_tile_kernel(Kv8AttnArgs p, int tiles, int streams) {
     using C = Kv8Tile<D, NT>;
     __shared__ __align__(16) half8_t buf[2][4 * C::kUnits];  // K's halves, then V's
+    __shared__ __align__(16) half8_t qs[C::kQl ? 4 : 1][C::kQl ? C::kQl * NT : 1][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g4 = lane >> 4, n = lane & 15;
     const Kv8& c = p.c;
-    // Workgroups go round the 8 XCDs: all tiles of one (head, split), which read the same keys, on
-    // one of them where there are enough to share out, the last (longest) tiles first.
+    // Workgroups go round the 8 XCDs.  The tiles of one (head, split) read the same keys: they go to
+    // one XCD, the last (longest) tiles of its heads first, or where the heads and splits are no
+    // multiple of 8, each XCD takes an eighth of all in a row.
     int stream, rank;
+    const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
     if ((streams & 7) == 0) {
-        const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3, per = streams >> 3;
+        const int per = streams >> 3;
         stream = xcd * per + slot % per;
         rank = slot / per;
     } else {
-        stream = blockIdx.x % streams;
-        rank = blockIdx.x / streams;
+        const int at = xcd * (int)(gridDim.x >> 3) + slot;
+        if (at >= streams * tiles) return;
+        stream = at / tiles;
+        rank = at % tiles;
     }
     const int tile = tiles - 1 - rank, bh = stream / p.nsplit, split = stream % p.nsplit;
     const int b = bh / c.Hkv, h = bh % c.Hkv;
@@ -525,22 +619,21 @@ kv8_tile_kernel(Kv8AttnArgs p, int tiles, int streams) {
     const int n_full = min(sq.len / kKvBlock, nb);
     const int per = (nb + p.nsplit - 1) / p.nsplit;
     const int end = min(nb, (split + 1) * per);
-    int i = split * per, blk = 0, page = -1, part = 0;
-    const bool open = i <= n_full && n_full < end;
-    auto next = [&]() {  // the split's next full block that has a page
-        for (page = -1; page < 0 && i < min(end, n_full); ++i) {
-            blk = i;
-            page = kv8_page(c, b, blk);
-        }
+    const bool open = split * per <= n_full && n_full < end;
+    Kv8Walk<false> walk = {split * per, min(end, n_full), 1, n_full, n_full, 0, 0};
+    int blk = 0, page = -1, part = 0;
+    Kv8Scale sc = {};
+    auto next = [&]() {
+        if (!walk.next(c, b, h, nullptr, p.c2, blk, page, sc)) page = -1;
     };
 
     struct Stage {
         int p0;  // first key, -1: none
-        float sk, sv;
+        Kv8Scale sc;
     };
     uint4 rk[C::kN], rv[C::kN];
     auto load = [&]() -> Stage {  // codes of the stage at (page, part) to registers, and on to the next
-        if (page < 0) return {-1, 0.f, 0.f};
+        if (page < 0) return {-1, {}};
         const size_t head = (size_t)page * c.Hkv + h;
         const uint4* kp = reinterpret_cast<const uint4*>(c.k + head * (kKvBlock * D)) + part * C::kUnits + tid;
         const uint4* vp = reinterpret_cast<const uint4*>(c.v + head * (kKvBlock * D)) + part * C::kUnits + tid;
@@ -548,44 +641,56 @@ kv8_tile_kernel(Kv8AttnArgs p, int tiles, int streams) {
         for (int x = 0; x < C::kN; ++x) rk[x] = kp[x * 256];
 #pragma unroll
         for (int x = 0; x < C::kN; ++x) rv[x] = vp[x * 256];
-        const Stage s = {blk * kKvBlock + part * C::kKeys, c.k_scale[head], c.v_scale[head]};
+        const Stage s = {blk * kKvBlock + part * C::kKeys, sc};
         if (++part == C::kParts) {
             part = 0;
             next();
         }
         return s;
     };
-    auto store = [&](int to) {  // registers to LDS as fp16
+    // Unit x of the registers (K's, then V's) to LDS as fp16.
+    auto store = [&](int to, int x) {
+        const bool isv = x >= C::kN;
+        const uint4& r = isv ? rv[x - C::kN] : rk[x];
+        half8_t* at = &buf[to][(isv ? 2 * C::kUnits : 0) + ((tid >> 6) + 4 * (isv ? x - C::kN : x)) * 128 + lane];
+        at[0] = kv8_halves(r.x, r.y);
+        at[64] = kv8_halves(r.z, r.w);
+    };
+    auto store_all = [&](int to) {
 #pragma unroll
-        for (int x = 0; x < C::kN; ++x) {
-            const int at = ((tid >> 6) + 4 * x) * 128 + lane;
-            buf[to][at] = kv8_halves(rk[x].x, rk[x].y);
-            buf[to][at + 64] = kv8_halves(rk[x].z, rk[x].w);
-            buf[to][2 * C::kUnits + at] = kv8_halves(rv[x].x, rv[x].y);
-            buf[to][2 * C::kUnits + at + 64] = kv8_halves(rv[x].z, rv[x].w);
-        }
+        for (int x = 0; x < 2 * C::kN; ++x) store(to, x);
     };
     next();
     Stage now = load();
-    if (now.p0 >= 0) store(0);
+    if (now.p0 >= 0) store_all(0);
     Stage then = load();
+    kv8_arrived<D, NT>(st);
+    half8_t* ql = &qs[C::kQl ? wave : 0][0][lane];  // a wave reads its own only
+#pragma unroll
+    for (int x = 0; x < C::kQl; ++x)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) ql[(x * NT + nt) * 64] = st.q[nt][D / 32 - C::kQl + x];
     lds_barrier();
     for (int u = 0; now.p0 >= 0; u ^= 1) {
-        if (then.p0 >= 0) store(u ^ 1);
+        const half8_t* kb = &buf[u][lane];
+        const half8_t* vb = kb + 2 * C::kUnits;
+        // The next stage's codes are converted among the products of K's operands, and the one after
+        // that is sent for behind them.  (Behind the last stage the registers hold old codes; what
+        // is written is not read.)  A wave that sees none of the stage's keys, on the diagonal, runs
+        // them masked: a branch round the products would cost it a copy of all its sums.
+        kv8_lds_keys<D, NT, C::kKeys / 16, C::kQl>(st, now.p0, now.sc, now.p0 + C::kKeys - 1 > least, kb, vb, ql, [&](int e) {
+            constexpr int kOps = C::kKeys / 16 * (D / 32), kEvery = kOps / (4 * C::kN);
+            if (e % kEvery == kEvery - 1 && e / kEvery < 2 * C::kN) store(u ^ 1, e / kEvery);
+        });
         const Stage after = load();
-        if (now.p0 <= see) {
-            const half8_t* kb = &buf[u][lane];
-            const half8_t* vb = kb + 2 * C::kUnits;
-            const Kv8Scale sc = {p.c2 * now.sk, __builtin_amdgcn_logf(now.sv), __builtin_amdgcn_rcpf(now.sv)};
-            kv8_keys<D, NT, C::kKeys / 16>(
-                st, now.p0, sc, now.p0 + C::kKeys - 1 > least,
-                [&](int a, int x, int s) { return kb[((a * (D / 64) + x) * 2 + s) * 64]; },
-                [&](int s, int m, int o) { return vb[((s * (D / 32) + m) * 2 + o) * 64]; }, []() {});
-        }
         lds_barrier();
         now = then;
         then = after;
     }
+#pragma unroll
+    for (int x = 0; x < C::kQl; ++x)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) st.q[nt][D / 32 - C::kQl + x] = ql[(x * NT + nt) * 64];
     if (open && see >= n_full * kKvBlock) kv8_open_block<D, NT>(st, c, b, h, n_full, sq.len - n_full * kKvBlock, p.c2);
 
 #pragma unroll
@@ -702,7 +807,7 @@ hipError_t kv8_attn_d(const Kv8AttnArgs& p, const Kv8Plan& q, hipStream_t stream
         const dim3 grid((unsigned)q.tiles, (unsigned)BH, (unsigned)p.nsplit);
         hipLaunchKernelGGL((kv8_row_kernel<D, kList>), grid, dim3(256), 0, stream, p);
     } else {
-        const dim3 grid((unsigned)(q.tiles * BH * p.nsplit));
+        const dim3 grid((unsigned)((q.tiles * BH * p.nsplit + 7) / 8 * 8));
         if (q.rows == 64)
             hipLaunchKernelGGL((kv8_tile_kernel<D, 1>), grid, dim3(256), 0, stream, p, (int)q.tiles, BH * p.nsplit);
         else

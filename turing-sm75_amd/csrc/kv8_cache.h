@@ -42,7 +42,7 @@ __device__ __forceinline__ void kv8_write_block(const Kv8& c, const half_t* __re
     const int p0 = blk * kKvBlock;
     const int r0 = max(start - p0, 0);           // rows before it are in the ring
     const int r1 = min(sq.len - p0, kKvBlock);   // rows behind it are not there yet
-    const int page = r1 == kKvBlock ? kv8_page(c, b, blk) : -1;
+    const int page = r1 == kKvBlock ? kv8_uniform_page(c, b, blk) : -1;
     half_t* ring = (kV ? c.v_open : c.k_open) + kv8_open_at<D>(c, b, h, blk);
     const half_t* in = rows + (long long)(sq.t0 + p0 - start) * st;  // row r at in + r * st
     half8_t x[kN][4];
@@ -193,8 +193,8 @@ kv8_read_kernel(Kv8 c, const int* __restrict__ len, const int* __restrict__ star
     const bool isv = blockIdx.y & 1;
     const Rows16& x = isv ? v : k;
     if (!x.data) return;
-    const int n = min(max(len[b], 0), c.max_blocks * kKvBlock);
-    const int first = start ? max(start[b], 0) : 0;
+    const int n = min(max(kv8_uniform(len + b), 0), c.max_blocks * kKvBlock);
+    const int first = start ? max(kv8_uniform(start + b), 0) : 0;
     if (first >= n) return;
     const int blk = first / kKvBlock + blockIdx.x;
     if (blk >= c.max_blocks) return;
@@ -210,7 +210,7 @@ kv8_read_kernel(Kv8 c, const int* __restrict__ len, const int* __restrict__ star
 #pragma unroll
             for (int j = 0; j < 2; ++j) y[i][j] = ring[2 * (tid + i * kThreads) + j];
     } else {
-        const int page = kv8_page(c, b, blk);
+        const int page = kv8_uniform_page(c, b, blk);
         if (page < 0) return;
         const size_t head = (size_t)page * c.Hkv + h;
         const uint4* codes = reinterpret_cast<const uint4*>((isv ? c.v : c.k) + head * (kKvBlock * D));
