@@ -46,13 +46,13 @@ __device__ __forceinline__ bool kv8_bad(half_t x) {
     return (__builtin_bit_cast(unsigned short, x) & 0x7c00) == 0x7c00;
 }
 
-// A wave's state for NT tiles of 16 query rows: lane l owns row l % 16 of each.
-template <int D, int NT>
-struct Kv8State {
-    half8_t q[NT][D / 32];  // operand B: step (i, s) holds d = 64 i + 16 (l / 16) + 8 s + 0 .. 7
-    float4_t o[NT][D / 16]; // O^T: d = 16 dt + 4 (l / 16) + r
-    float m[NT], l[NT];     // l: this lane's keys only
-    int limit[NT];          // last key the row sees, -1: none
+// A wave's state for a tile of 16 query rows: lane l owns row l % 16.
+template <int D>
+struct Kv8Rows {
+    half8_t q[D / 32];   // operand B: step (i, s) holds d = 64 i + 16 (l / 16) + 8 s + 0 .. 7
+    float4_t o[D / 16];  // O^T: d = 16 dt + 4 (l / 16) + r
+    float m, l;          // l: this lane's keys only
+    int limit;           // last key the row sees, -1: none
 };
 
 // A block's scales as the softmax takes them: the score's factor (scale log2(e) sk), log2(sv) and
@@ -104,50 +104,46 @@ struct Kv8Walk {
 // Scores (w: raw q . k') to weights for 16 KA keys from p0 on: raises the running maximum where a
 // score passes it by more than the slack, rescaling what there is, and adds to the row sums.
 // `masked` (the same on all lanes): some row may not see all of the keys.
-template <int D, int NT, int KA>
-__device__ __forceinline__ void kv8_softmax(Kv8State<D, NT>& st, float4_t (&w)[NT][KA], int p0, const Kv8Scale& sc,
-                                            bool masked) {
-    const int k0 = p0 + 4 * ((threadIdx.x & 63) >> 4);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        if (masked) {
-#pragma unroll
-            for (int a = 0; a < KA; ++a)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) w[nt][a][r] = k0 + 16 * a + r <= st.limit[nt] ? w[nt][a][r] : -INFINITY;
-        }
-        float big = -INFINITY;
+template <int D, int KA>
+__device__ __forceinline__ void kv8_softmax(Kv8Rows<D>& st, float4_t (&w)[KA], int p0, const Kv8Scale& sc, bool masked) {
+    const int left = st.limit - p0 - 4 * (int)((threadIdx.x & 63) >> 4);  // key 16 a + r is seen up to this
+    if (masked) {
 #pragma unroll
         for (int a = 0; a < KA; ++a)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) big = fmaxf(big, w[nt][a][r]);
-        big = __builtin_fmaf(big, sc.f, sc.lsv);  // of this lane's keys
-        if (__any(big > st.m[nt] + kKvSlack)) {
-            const float m_new = fmaxf(st.m[nt], max_xor32(max_xor16(big)));
-            const float alpha = m_new == st.m[nt] ? 1.f : fast_exp2(st.m[nt] - m_new);
-            st.m[nt] = m_new;
-            st.l[nt] *= alpha;
-#pragma unroll
-            for (int dt = 0; dt < D / 16; ++dt) st.o[nt][dt] *= alpha;
-        }
-        const float c = sc.lsv - (st.m[nt] == -INFINITY ? 0.f : st.m[nt] - kKvBias);
-        float sum = 0.f;
-#pragma unroll
-        for (int a = 0; a < KA; ++a)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) w[nt][a][r] = fast_exp2(__builtin_fmaf(w[nt][a][r], sc.f, c));
-        if (masked) {  // again: of a block of scale NaN, a key that is not seen weighs 0
-#pragma unroll
-            for (int a = 0; a < KA; ++a)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) w[nt][a][r] = k0 + 16 * a + r <= st.limit[nt] ? w[nt][a][r] : 0.f;
-        }
-#pragma unroll
-        for (int a = 0; a < KA; ++a)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) sum += w[nt][a][r];
-        st.l[nt] += sum == 0.f ? 0.f : sum * sc.isv;
+            for (int r = 0; r < 4; ++r) w[a][r] = 16 * a + r <= left ? w[a][r] : -INFINITY;
     }
+    float big = -INFINITY;
+#pragma unroll
+    for (int a = 0; a < KA; ++a)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) big = fmaxf(big, w[a][r]);
+    big = __builtin_fmaf(big, sc.f, sc.lsv);  // of this lane's keys
+    if (__any(big > st.m + kKvSlack)) {
+        const float m_new = fmaxf(st.m, max_xor32(max_xor16(big)));
+        const float alpha = m_new == st.m ? 1.f : fast_exp2(st.m - m_new);
+        st.m = m_new;
+        st.l *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) st.o[dt] *= alpha;
+    }
+    const float c = sc.lsv - (st.m == -INFINITY ? 0.f : st.m - kKvBias);
+    float sum = 0.f;
+#pragma unroll
+    for (int a = 0; a < KA; ++a)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) w[a][r] = fast_exp2(__builtin_fmaf(w[a][r], sc.f, c));
+    if (masked) {  // again: of a block of scale NaN, a key that is not seen weighs 0
+#pragma unroll
+        for (int a = 0; a < KA; ++a)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) w[a][r] = 16 * a + r <= left ? w[a][r] : 0.f;
+    }
+#pragma unroll
+    for (int a = 0; a < KA; ++a)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum += w[a][r];
+    st.l += sum == 0.f ? 0.f : sum * sc.isv;
 }
 // Weights of key tiles 2 s and 2 s + 1 as operand B.
 template <int KA>
@@ -158,7 +154,7 @@ __device__ __forceinline__ half8_t kv8_weights(const float4_t (&w)[KA], int s) {
 // 16 KA keys: kload(a, i, s) and vload(s, m, o) give the operands; between() is called where the
 // keys' operands are done with.
 template <int D, int NT, int KA, class KLoad, class VLoad, class Between>
-__device__ __forceinline__ void kv8_keys(Kv8State<D, NT>& st, int p0, const Kv8Scale& sc, bool masked, KLoad kload,
+__device__ __forceinline__ void kv8_keys(Kv8Rows<D> (&st)[NT], int p0, const Kv8Scale& sc, bool masked, KLoad kload,
                                          VLoad vload, Between between) {
     float4_t w[NT][KA];
 #pragma unroll
@@ -173,10 +169,11 @@ __device__ __forceinline__ void kv8_keys(Kv8State<D, NT>& st, int p0, const Kv8S
             for (int a = 0; a < KA; ++a) {
                 const half8_t kf = kload(a, i, s);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) w[nt][a] = mfma16(kf, st.q[nt][2 * i + s], w[nt][a]);
+                for (int nt = 0; nt < NT; ++nt) w[nt][a] = mfma16(kf, st[nt].q[2 * i + s], w[nt][a]);
             }
     between();
-    kv8_softmax<D, NT, KA>(st, w, p0, sc, masked);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) kv8_softmax<D, KA>(st[nt], w[nt], p0, sc, masked);
 #pragma unroll
     for (int s = 0; s < KA / 2; ++s) {
         half8_t p[NT];
@@ -188,7 +185,7 @@ __device__ __forceinline__ void kv8_keys(Kv8State<D, NT>& st, int p0, const Kv8S
             for (int o = 0; o < 2; ++o) {
                 const half8_t vf = vload(s, m, o);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) st.o[nt][2 * m + o] = mfma16(vf, p[nt], st.o[nt][2 * m + o]);
+                for (int nt = 0; nt < NT; ++nt) st[nt].o[2 * m + o] = mfma16(vf, p[nt], st[nt].o[2 * m + o]);
             }
     }
 }
@@ -196,7 +193,7 @@ __device__ __forceinline__ void kv8_keys(Kv8State<D, NT>& st, int p0, const Kv8S
 // The same from operands in LDS (kb, vb: this lane's of K and V), read a few ahead of their products;
 // between(e) is called among K's.  The queries' last kQl steps lie in LDS too (qb: this lane's).
 template <int D, int NT, int KA, int kQl, class Between>
-__device__ __forceinline__ void kv8_lds_keys(Kv8State<D, NT>& st, int p0, const Kv8Scale& sc, bool masked, const half8_t* kb,
+__device__ __forceinline__ void kv8_lds_keys(Kv8Rows<D> (&st)[NT], int p0, const Kv8Scale& sc, bool masked, const half8_t* kb,
                                              const half8_t* vb, const half8_t* qb, Between between) {
     constexpr int kOps = KA * (D / 32), kAhead = D == 256 ? 3 : 6, kQr = D / 32 - kQl;
     float4_t w[NT][KA];
@@ -204,7 +201,7 @@ __device__ __forceinline__ void kv8_lds_keys(Kv8State<D, NT>& st, int p0, const 
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int a = 0; a < KA; ++a) w[nt][a] = float4_t{0.f, 0.f, 0.f, 0.f};
-    half8_t op[kOps], ql[D / 32][NT];
+    half8_t op[kOps], ql[NT];
     auto read_k = [&](int e) {  // key tile e % KA, step e / KA
         const int a = e % KA, x = e / KA;
         op[e] = kb[((a * (D / 64) + x / 2) * 2 + x % 2) * 64];
@@ -215,21 +212,21 @@ __device__ __forceinline__ void kv8_lds_keys(Kv8State<D, NT>& st, int p0, const 
 #pragma unroll
     for (int e = 0; e < kOps; ++e) {
         if (e + kAhead < kOps) read_k(e + kAhead);
-        // a step of queries from LDS two products before its first
-        if (kQl && (e + 2) % KA == 0 && (e + 2) / KA >= kQr && e + 2 < kOps) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) ql[(e + 2) / KA][nt] = qb[(((e + 2) / KA - kQr) * NT + nt) * 64];
-        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
-            w[nt][e % KA] = mfma16(op[e], e / KA < kQr ? st.q[nt][e / KA] : ql[e / KA][nt], w[nt][e % KA]);
+            w[nt][e % KA] = mfma16(op[e], e / KA < kQr ? st[nt].q[e / KA] : ql[nt], w[nt][e % KA]);
+        if (kQl && (e + 1) % KA == 0 && (e + 1) / KA >= kQr && e + 1 < kOps) {  // the next step's queries
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) ql[nt] = qb[(((e + 1) / KA - kQr) * NT + nt) * 64];
+        }
         between(e);
         __builtin_amdgcn_sched_barrier(0);
     }
     auto read_v = [&](int e) { op[e] = vb[e * 64]; };  // (s, m, o) in order
 #pragma unroll
     for (int e = 0; e < kAhead; ++e) read_v(e);
-    kv8_softmax<D, NT, KA>(st, w, p0, sc, masked);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) kv8_softmax<D, KA>(st[nt], w[nt], p0, sc, masked);
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int s = 0; s < KA / 2; ++s) {
@@ -241,7 +238,7 @@ __device__ __forceinline__ void kv8_lds_keys(Kv8State<D, NT>& st, int p0, const 
             const int e = s * (D / 16) + dt;
             if (e + kAhead < kOps) read_v(e + kAhead);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) st.o[nt][dt] = mfma16(op[e], p[nt], st.o[nt][dt]);
+            for (int nt = 0; nt < NT; ++nt) st[nt].o[dt] = mfma16(op[e], p[nt], st[nt].o[dt]);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
@@ -251,8 +248,8 @@ __device__ __forceinline__ void kv8_lds_keys(Kv8State<D, NT>& st, int p0, const 
 // The open block from the ring: n of its rows are the sequence's, those behind are whatever the
 // ring held.  Values that are not finite are left out of the matrix products, where a masked key's
 // weight 0 would turn them into NaN for every query, and added for the queries that see them.
-template <int D, int NT>
-__device__ __forceinline__ void kv8_open_block(Kv8State<D, NT>& st, const Kv8& c, int b, int h, int blk, int n, float c2) {
+template <int D>
+__device__ __forceinline__ void kv8_open_block(Kv8Rows<D>& st, const Kv8& c, int b, int h, int blk, int n, float c2) {
     typedef unsigned uint4_v __attribute__((ext_vector_type(4)));
     typedef unsigned short ushort8_t __attribute__((ext_vector_type(8)));
     const int lane = threadIdx.x & 63, g4 = lane >> 4;
@@ -262,25 +259,15 @@ __device__ __forceinline__ void kv8_open_block(Kv8State<D, NT>& st, const Kv8& c
 #pragma unroll 1
     for (int s = 0; 32 * s < n; ++s) {  // half a block at a time
         const int p0 = blk * kKvBlock + 32 * s;
-        float4_t w[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int a = 0; a < 2; ++a) w[nt][a] = float4_t{0.f, 0.f, 0.f, 0.f};
+        float4_t w[2] = {float4_t{0.f, 0.f, 0.f, 0.f}, float4_t{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
         for (int i = 0; i < D / 64; ++i)
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
-                for (int a = 0; a < 2; ++a) {
-                    const half8_t kf = kp[((2 * s + a) * (D / 64) + i) * 128 + x];
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) w[nt][a] = mfma16(kf, st.q[nt][2 * i + x], w[nt][a]);
-                }
-        kv8_softmax<D, NT, 2>(st, w, p0, {c2, 0.f, 1.f}, true);
-        half8_t p[NT];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) p[nt] = kv8_weights<2>(w[nt], 0);
+                for (int a = 0; a < 2; ++a) w[a] = mfma16(kp[((2 * s + a) * (D / 64) + i) * 128 + x], st.q[2 * i + x], w[a]);
+        kv8_softmax<D, 2>(st, w, p0, {c2, 0.f, 1.f}, true);
+        const half8_t p = kv8_weights<2>(w, 0);
         uint4_v keep;  // elements of rows that there are
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -309,86 +296,80 @@ __device__ __forceinline__ void kv8_open_block(Kv8State<D, NT>& st, const Kv8& c
                     for (int j = 0; j < 8; ++j) v[x][j] = kv8_bad(v[x][j]) ? (half_t)0.f : v[x][j];
             }
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) st.o[nt][2 * m + x] = mfma16(v[x], p[nt], st.o[nt][2 * m + x]);
+            for (int x = 0; x < 4; ++x) st.o[2 * m + x] = mfma16(v[x], p, st.o[2 * m + x]);
             if (!bad) continue;
             const half_t* vo = c.v_open + at;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll 1
-                for (int y = 0; y < 32; ++y) {
-                    const int j = y >> 2, g = y & 3, key = 16 * (j >> 2) + 4 * g + (j & 3);
-                    float wj = 0.f;
+            for (int y = 0; y < 32; ++y) {
+                const int j = y >> 2, g = y & 3, key = 16 * (j >> 2) + 4 * g + (j & 3);
+                float wj = 0.f;
 #pragma unroll
-                    for (int a = 0; a < 2; ++a)
+                for (int a = 0; a < 2; ++a)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) wj = j == 4 * a + r ? w[nt][a][r] : wj;
-                    wj = __shfl(wj, 16 * g + (lane & 15));
-                    if (p0 + key > st.limit[nt]) continue;
+                    for (int r = 0; r < 4; ++r) wj = j == 4 * a + r ? w[a][r] : wj;
+                wj = __shfl(wj, 16 * g + (lane & 15));
+                if (p0 + key > st.limit) continue;
 #pragma unroll
-                    for (int x = 0; x < 4; ++x)
+                for (int x = 0; x < 4; ++x)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const half_t z = vo[kv8_v_at<D>(32 * s + key, 16 * (2 * m + x) + 4 * g4 + e)];
-                            if (kv8_bad(z)) st.o[nt][2 * m + x][e] += wj * (float)z;
-                        }
-                }
+                    for (int e = 0; e < 4; ++e) {
+                        const half_t z = vo[kv8_v_at<D>(32 * s + key, 16 * (2 * m + x) + 4 * g4 + e)];
+                        if (kv8_bad(z)) st.o[2 * m + x][e] += wj * (float)z;
+                    }
+            }
         }
     }
 }
 
-// The rows of a tile: row0 + 0 .. of the T G rows t G + g of a K/V head's group.  Loads the queries
-// of NT tiles of 16 from row0 on and clears the state; returns the last key that any row sees.
+// The queries of 16 of the T G rows t G + g of a K/V head's group, from row0 on.
+template <int D>
+__device__ __forceinline__ void kv8_queries(Kv8Rows<D>& st, const Kv8AttnArgs& p, int b, int h, int row0, int row_end) {
+    const int lane = threadIdx.x & 63, g4 = lane >> 4, row = row0 + (lane & 15), t = row / p.G, g = row % p.G;
+    const half_t* qr = p.q.data + b * p.q.b + (long long)(h * p.G + g) * p.q.h + t * p.q.t;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+            st.q[2 * i + s] = row < row_end ? *reinterpret_cast<const half8_t*>(qr + 64 * i + 16 * g4 + 8 * s) : half8_t{};
+}
+// NT tiles from row0 on with nothing summed yet, and which keys they see: the last that any row
+// does (`most`) and the last that all do (`least`).
 template <int D, int NT>
-__device__ __forceinline__ int kv8_begin(Kv8State<D, NT>& st, const Kv8AttnArgs& p, const Kv8Seq& sq, int b, int h, int row0,
-                                         int row_end) {
-    const int lane = threadIdx.x & 63, g4 = lane >> 4, n = lane & 15;
-    int see = -1;
+__device__ __forceinline__ void kv8_begin(Kv8Rows<D> (&st)[NT], const Kv8AttnArgs& p, const Kv8Seq& sq, int b, int h, int row0,
+                                          int row_end, int& most, int& least) {
+    most = -1;
+    least = INT_MAX;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int row = row0 + 16 * nt + n;
-        const int t = row / p.G, g = row % p.G;
+        kv8_queries<D>(st[nt], p, b, h, row0 + 16 * nt, row_end);
+        const int row = row0 + 16 * nt + (int)(threadIdx.x & 15);
         const bool is = row < row_end;
-        const int pos = sq.len - (sq.n + sq.t0) + t;  // below 0: in front of the sequence
-        st.limit[nt] = !is ? -1 : p.causal ? min(pos, sq.len - 1) : sq.len - 1;
-        see = max(see, st.limit[nt]);
-        const half_t* qr = p.q.data + b * p.q.b + (long long)(h * p.G + g) * p.q.h + t * p.q.t;
+        const int pos = sq.len - (sq.n + sq.t0) + row / p.G;  // below 0: in front of the sequence
+        st[nt].limit = !is ? -1 : p.causal ? min(pos, sq.len - 1) : sq.len - 1;
+        most = max(most, st[nt].limit);
+        if (is) least = min(least, st[nt].limit);
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i)
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-                st.q[nt][2 * i + s] = is ? *reinterpret_cast<const half8_t*>(qr + 64 * i + 16 * g4 + 8 * s) : half8_t{};
-#pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt) st.o[nt][dt] = float4_t{0.f, 0.f, 0.f, 0.f};
-        st.m[nt] = -INFINITY;
-        st.l[nt] = 0.f;
+        for (int dt = 0; dt < D / 16; ++dt) st[nt].o[dt] = float4_t{0.f, 0.f, 0.f, 0.f};
+        st[nt].m = -INFINITY;
+        st[nt].l = 0.f;
     }
 #pragma unroll
-    for (int x = 1; x < 16; x <<= 1) see = max(see, __shfl_xor(see, x));
-    return __builtin_amdgcn_readfirstlane(see);
+    for (int x = 1; x < 16; x <<= 1) {
+        most = max(most, __shfl_xor(most, x));
+        least = min(least, __shfl_xor(least, x));
+    }
+    most = __builtin_amdgcn_readfirstlane(most);
+    least = __builtin_amdgcn_readfirstlane(least);
 }
 
 // The queries have arrived: said in front of a loop that only reads them, the loop waits for none
 // of the loads that it has under way itself.
 template <int D, int NT>
-__device__ __forceinline__ void kv8_arrived(Kv8State<D, NT>& st) {
+__device__ __forceinline__ void kv8_arrived(Kv8Rows<D> (&st)[NT]) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) asm volatile("" : "+v"(st.q[nt][i]));
-}
-
-// The last key that every row of the tile sees.
-template <int D, int NT>
-__device__ __forceinline__ int kv8_least(const Kv8State<D, NT>& st, int row0, int row_end) {
-    int least = INT_MAX;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-        if (row0 + 16 * nt + (int)(threadIdx.x & 15) < row_end) least = min(least, st.limit[nt]);
-#pragma unroll
-    for (int x = 1; x < 16; x <<= 1) least = min(least, __shfl_xor(least, x));
-    return __builtin_amdgcn_readfirstlane(least);
+        for (int i = 0; i < D / 32; ++i) asm volatile("" : "+v"(st[nt].q[i]));
 }
 
 // Where a split's sums of a row lie: [row][split][D] sums, behind all of them (m, l) pairs.
@@ -469,8 +450,9 @@ kv8_row_kernel(Kv8AttnArgs p) {
     row_end = min(row_end, (sq.n + sq.t0) * p.G);
     if (row0 >= row_end) return;
 
-    Kv8State<D, 1> st;
-    const int see = kv8_begin<D, 1>(st, p, sq, b, h, row0, row_end);
+    Kv8Rows<D> rows[1], &st = rows[0];
+    int see, least;
+    kv8_begin<D, 1>(rows, p, sq, b, h, row0, row_end, see, least);
     const int nb = see / kKvBlock + (see >= 0 ? 1 : 0);  // blocks that any row sees
     const int n_full = min(sq.len / kKvBlock, nb);
     const int items = kList ? p.top : nb;
@@ -484,14 +466,13 @@ kv8_row_kernel(Kv8AttnArgs p) {
         if (!walk.next(c, b, h, list, p.c2, blk, page, sc)) page = -1;
     };
     // rows of one query see whole blocks but the last; several queries' last one or two are masked
-    const int least = kv8_least<D, 1>(st, row0, row_end);
     auto masked = [&](int k) { return (k + 1) * kKvBlock - 1 > least; };
     next();
     if (page >= 0) {
         Kv8Regs<D> x;
         x.load_k(c, page, h, 0);
         x.load_v(c, page, h, 0);
-        kv8_arrived<D, 1>(st);
+        kv8_arrived<D, 1>(rows);
         while (page >= 0) {
             const int now = blk, here = page;
             const Kv8Scale scale = sc;
@@ -501,7 +482,7 @@ kv8_row_kernel(Kv8AttnArgs p) {
                 if (last) next();
                 const int to = last ? page : here;
                 kv8_keys<D, 1, Kv8Regs<D>::kKeys / 16>(
-                    st, now * kKvBlock + part * Kv8Regs<D>::kKeys, scale, masked(now),
+                    rows, now * kKvBlock + part * Kv8Regs<D>::kKeys, scale, masked(now),
                     [&](int a, int i, int s) {
                         const uint4& k = x.k[a * (D / 64) + i];
                         return s ? kv8_halves(k.z, k.w) : kv8_halves(k.x, k.y);
@@ -517,31 +498,31 @@ kv8_row_kernel(Kv8AttnArgs p) {
             }
         }
     }
-    for (; walk.open > 0; --walk.open) kv8_open_block<D, 1>(st, c, b, h, n_full, sq.len - n_full * kKvBlock, p.c2);
+    for (; walk.open > 0; --walk.open) kv8_open_block<D>(st, c, b, h, n_full, sq.len - n_full * kKvBlock, p.c2);
 
     // the four waves' sums, relative to their common maximum
-    st.l[0] = sum_xor32(sum_xor16(st.l[0]));
+    st.l = sum_xor32(sum_xor16(st.l));
     if (g4 == 0) {
-        ml[wave][0][n] = st.m[0];
-        ml[wave][1][n] = st.l[0];
+        ml[wave][0][n] = st.m;
+        ml[wave][1][n] = st.l;
     }
     __syncthreads();
     {
         const float m = fmaxf(fmaxf(ml[0][0][n], ml[1][0][n]), fmaxf(ml[2][0][n], ml[3][0][n]));
-        const float f = st.m[0] == m ? 1.f : fast_exp2(st.m[0] - m);
+        const float f = st.m == m ? 1.f : fast_exp2(st.m - m);
 #pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt) st.o[0][dt] *= f;
+        for (int dt = 0; dt < D / 16; ++dt) st.o[dt] *= f;
     }
     if (wave >= 2) {
 #pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt) *reinterpret_cast<float4_t*>(&acc[wave & 1][n][16 * dt + 4 * g4]) = st.o[0][dt];
+        for (int dt = 0; dt < D / 16; ++dt) *reinterpret_cast<float4_t*>(&acc[wave & 1][n][16 * dt + 4 * g4]) = st.o[dt];
     }
     __syncthreads();
     if (wave < 2) {
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt) {
             float4_t* at = reinterpret_cast<float4_t*>(&acc[wave][n][16 * dt + 4 * g4]);
-            *at += st.o[0][dt];
+            *at += st.o[dt];
         }
     }
     __syncthreads();
@@ -565,25 +546,28 @@ kv8_row_kernel(Kv8AttnArgs p) {
 
 constexpr int kKvMaxSplits = 128;
 
-// Many rows: a workgroup is 4 waves of 16 NT query rows each over one split of their blocks.  A
+// Many rows: a workgroup is kWaves waves of 16 NT query rows each over one split of their blocks.  A
 // stage of kKeys keys and their values (16 KiB of codes at the most) goes from memory to registers
 // two stages ahead, is turned into fp16 operands once for all waves, and lies in one of two LDS
 // buffers in operand order, so every LDS access is 16 consecutive bytes a lane and a code is
-// converted once per 64 NT rows.  One barrier a stage.
+// converted once per 16 NT kWaves rows.  One barrier a stage.  Two waves a SIMD: two workgroups of 4
+// waves a CU, or at D = 256, NT = 2 one of 8 (a thread then holds half as many codes, without which
+// the 128 sums and 64 query registers spill).
 template <int D, int NT>
 struct Kv8Tile {
+    static constexpr int kWaves = D == 256 && NT == 2 ? 8 : 4, kThreads = 64 * kWaves;
     static constexpr int kKeys = D == 256 ? 32 : 64, kParts = kKvBlock / kKeys;
     static constexpr int kUnits = kKeys * D / 16;          // 16-code units of K (or V) a stage
-    static constexpr int kN = kUnits / 256;                // of them a thread moves
-    static constexpr int kRows = 64 * NT;
-    static constexpr int kQl = D == 256 && NT == 2 ? 2 : 0;  // steps of the queries kept in LDS: registers for the rest
+    static constexpr int kN = kUnits / kThreads;           // of them a thread moves
+    static constexpr int kRows = 16 * NT * kWaves;
+    static constexpr int kQl = D == 256 && NT == 2 ? 3 : 0;  // steps of the queries kept in LDS, likewise
 };
 template <int D, int NT>
-__global__ void __launch_bounds__(256, 2)
+__global__ void __launch_bounds__((Kv8Tile<D, NT>::kThreads), 2)
 kv8_tile_kernel(Kv8AttnArgs p, int tiles, int streams) {
     using C = Kv8Tile<D, NT>;
     __shared__ __align__(16) half8_t buf[2][4 * C::kUnits];  // K's halves, then V's
-    __shared__ __align__(16) half8_t qs[C::kQl ? 4 : 1][C::kQl ? C::kQl * NT : 1][64];
+    __shared__ __align__(16) half8_t qs[C::kQl ? C::kWaves : 1][C::kQl ? C::kQl * NT : 1][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g4 = lane >> 4, n = lane & 15;
     const Kv8& c = p.c;
@@ -609,10 +593,10 @@ kv8_tile_kernel(Kv8AttnArgs p, int tiles, int streams) {
     const int row_end = min(p.T, sq.n + sq.t0) * p.G;
     if (tile * C::kRows >= row_end) return;
 
-    Kv8State<D, NT> st;
+    Kv8Rows<D> st[NT];
     const int row0 = tile * C::kRows + wave * 16 * NT;
-    const int see = kv8_begin<D, NT>(st, p, sq, b, h, row0, row_end);
-    const int least = kv8_least<D, NT>(st, row0, row_end);
+    int see, least;
+    kv8_begin<D, NT>(st, p, sq, b, h, row0, row_end, see, least);
     // the last key that any row of the workgroup sees
     const int all = p.causal ? min(front + (min(row_end, (tile + 1) * C::kRows) - 1) / p.G, sq.len - 1) : sq.len - 1;
     const int nb = all < 0 ? 0 : all / kKvBlock + 1;
@@ -638,9 +622,9 @@ kv8_tile_kernel(Kv8AttnArgs p, int tiles, int streams) {
         const uint4* kp = reinterpret_cast<const uint4*>(c.k + head * (kKvBlock * D)) + part * C::kUnits + tid;
         const uint4* vp = reinterpret_cast<const uint4*>(c.v + head * (kKvBlock * D)) + part * C::kUnits + tid;
 #pragma unroll
-        for (int x = 0; x < C::kN; ++x) rk[x] = kp[x * 256];
+        for (int x = 0; x < C::kN; ++x) rk[x] = kp[x * C::kThreads];
 #pragma unroll
-        for (int x = 0; x < C::kN; ++x) rv[x] = vp[x * 256];
+        for (int x = 0; x < C::kN; ++x) rv[x] = vp[x * C::kThreads];
         const Stage s = {blk * kKvBlock + part * C::kKeys, sc};
         if (++part == C::kParts) {
             part = 0;
@@ -652,7 +636,7 @@ kv8_tile_kernel(Kv8AttnArgs p, int tiles, int streams) {
     auto store = [&](int to, int x) {
         const bool isv = x >= C::kN;
         const uint4& r = isv ? rv[x - C::kN] : rk[x];
-        half8_t* at = &buf[to][(isv ? 2 * C::kUnits : 0) + ((tid >> 6) + 4 * (isv ? x - C::kN : x)) * 128 + lane];
+        half8_t* at = &buf[to][(isv ? 2 * C::kUnits : 0) + ((tid >> 6) + C::kWaves * (isv ? x - C::kN : x)) * 128 + lane];
         at[0] = kv8_halves(r.x, r.y);
         at[64] = kv8_halves(r.z, r.w);
     };
@@ -669,7 +653,7 @@ kv8_tile_kernel(Kv8AttnArgs p, int tiles, int streams) {
 #pragma unroll
     for (int x = 0; x < C::kQl; ++x)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) ql[(x * NT + nt) * 64] = st.q[nt][D / 32 - C::kQl + x];
+        for (int nt = 0; nt < NT; ++nt) ql[(x * NT + nt) * 64] = st[nt].q[D / 32 - C::kQl + x];
     lds_barrier();
     for (int u = 0; now.p0 >= 0; u ^= 1) {
         const half8_t* kb = &buf[u][lane];
@@ -687,29 +671,31 @@ kv8_tile_kernel(Kv8AttnArgs p, int tiles, int streams) {
         now = then;
         then = after;
     }
+    if (open && see >= n_full * kKvBlock) {
 #pragma unroll
-    for (int x = 0; x < C::kQl; ++x)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) st.q[nt][D / 32 - C::kQl + x] = ql[(x * NT + nt) * 64];
-    if (open && see >= n_full * kKvBlock) kv8_open_block<D, NT>(st, c, b, h, n_full, sq.len - n_full * kKvBlock, p.c2);
+        for (int nt = 0; nt < NT; ++nt) {
+            kv8_queries<D>(st[nt], p, b, h, row0 + 16 * nt, row_end);  // again: not held through the loop's end
+            kv8_open_block<D>(st[nt], c, b, h, n_full, sq.len - n_full * kKvBlock, p.c2);
+        }
+    }
 
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const float l = sum_xor32(sum_xor16(st.l[nt]));
+        const float l = sum_xor32(sum_xor16(st[nt].l));
         const int row = row0 + 16 * nt + n;
         if (row >= row_end) continue;
         if (p.nsplit > 1) {
             if (l != 0.f) {
                 float* at = kv8_part<D>(p, bh, row, split) + 4 * g4;
 #pragma unroll
-                for (int dt = 0; dt < D / 16; ++dt) *reinterpret_cast<float4_t*>(at + 16 * dt) = st.o[nt][dt];
+                for (int dt = 0; dt < D / 16; ++dt) *reinterpret_cast<float4_t*>(at + 16 * dt) = st[nt].o[dt];
             }
-            if (g4 == 0) *reinterpret_cast<float2*>(kv8_pair<D>(p, bh, row, split)) = float2{st.m[nt], l};
+            if (g4 == 0) *reinterpret_cast<float2*>(kv8_pair<D>(p, bh, row, split)) = float2{st[nt].m, l};
         } else {
             const int t = row / p.G, hq = h * p.G + row % p.G;
 #pragma unroll
             for (int dt = 0; dt < D / 16; ++dt)
-                kv8_store4(p, b, hq, t, 16 * dt + 4 * g4, st.o[nt][dt], l, kv8_gate4(p, b, hq, t, 16 * dt + 4 * g4));
+                kv8_store4(p, b, hq, t, 16 * dt + 4 * g4, st[nt].o[dt], l, kv8_gate4(p, b, hq, t, 16 * dt + 4 * g4));
         }
     }
 }
@@ -781,16 +767,16 @@ struct Kv8Plan {
     int nsplit;
 };
 // One tile of 16 rows where there are no more (and for listed blocks, one query's heads), else
-// workgroups of 64 or 128 rows.  items: blocks of the longest sequence, or of a list.
-inline Kv8Plan kv8_plan(int B, int T, int Hq, int Hkv, int items, bool list) {
+// workgroups of 64, or of 128 (256 at D = 256) rows.  items: blocks of the longest sequence, or of a list.
+inline Kv8Plan kv8_plan(int B, int T, int Hq, int Hkv, int D, int items, bool list) {
     const long long G = Hq / Hkv, rows = T * G;
     Kv8Plan q;
-    q.rows = list || rows <= 16 ? 16 : rows <= 64 ? 64 : 128;
+    q.rows = list || rows <= 16 ? 16 : rows <= 64 ? 64 : D == 256 ? 256 : 128;
     q.tiles = list ? T * ((G + 15) / 16) : (rows + q.rows - 1) / q.rows;
     const long long all = q.tiles * B * Hkv;
     // row tiles: as many workgroups as the chip takes twice, not fewer than 4 blocks each; the others
     // as many as it takes once
-    const long long want = q.rows == 16 ? (1024 + all - 1) / all : 512 / all;
+    const long long want = q.rows == 16 ? (1024 + all - 1) / all : (q.rows == 256 ? 256 : 512) / all;
     const long long most = (items + 3) / 4;
     const long long n = want < most ? want : most;
     q.nsplit = (int)(n < 1 ? 1 : n < kKvMaxSplits ? n : kKvMaxSplits);
@@ -809,9 +795,9 @@ hipError_t kv8_attn_d(const Kv8AttnArgs& p, const Kv8Plan& q, hipStream_t stream
     } else {
         const dim3 grid((unsigned)((q.tiles * BH * p.nsplit + 7) / 8 * 8));
         if (q.rows == 64)
-            hipLaunchKernelGGL((kv8_tile_kernel<D, 1>), grid, dim3(256), 0, stream, p, (int)q.tiles, BH * p.nsplit);
+            hipLaunchKernelGGL((kv8_tile_kernel<D, 1>), grid, dim3(Kv8Tile<D, 1>::kThreads), 0, stream, p, (int)q.tiles, BH * p.nsplit);
         else
-            hipLaunchKernelGGL((kv8_tile_kernel<D, 2>), grid, dim3(256), 0, stream, p, (int)q.tiles, BH * p.nsplit);
+            hipLaunchKernelGGL((kv8_tile_kernel<D, 2>), grid, dim3(Kv8Tile<D, 2>::kThreads), 0, stream, p, (int)q.tiles, BH * p.nsplit);
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.nsplit == 1) return e;
@@ -831,7 +817,7 @@ hipError_t kv8_attn_any(const Kv8AttnArgs& p, const Kv8Plan& q, hipStream_t stre
 
 hipError_t kv8_attn(const Kv8& c, const Rows16& q, const Rows16& gate, const Rows16& o, const int* len, const int* n_new,
                     int T, int Hq, int nb_hint, float scale, int causal, void* ws, hipStream_t stream) {
-    const Kv8Plan plan = kv8_plan(c.B, T, Hq, c.Hkv, nb_hint, false);
+    const Kv8Plan plan = kv8_plan(c.B, T, Hq, c.Hkv, c.D, nb_hint, false);
     return kv8_attn_any<false>({c, q, gate, o, len, n_new, nullptr, (float*)ws, T, Hq, Hq / c.Hkv, 0, plan.nsplit, causal, scale * kLog2e},
                                plan, stream);
 }
@@ -839,7 +825,7 @@ hipError_t kv8_attn(const Kv8& c, const Rows16& q, const Rows16& gate, const Row
 hipError_t kv8_attn_blocks(const Kv8& c, const Rows16& q, const Rows16& gate, const Rows16& o, const int* len,
                            const int* n_new, int T, int Hq, const int* blocks, int top, float scale, void* ws,
                            hipStream_t stream) {
-    const Kv8Plan plan = kv8_plan(c.B, T, Hq, c.Hkv, top, true);
+    const Kv8Plan plan = kv8_plan(c.B, T, Hq, c.Hkv, c.D, top, true);
     return kv8_attn_any<true>({c, q, gate, o, len, n_new, blocks, (float*)ws, T, Hq, Hq / c.Hkv, top, plan.nsplit, 1, scale * kLog2e}, plan,
                               stream);
 }
