@@ -133,11 +133,13 @@ __device__ __forceinline__ void kv8_softmax(Kv8Rows<D>& st, float4_t (&w)[KA], i
     for (int a = 0; a < KA; ++a)
 #pragma unroll
         for (int r = 0; r < 4; ++r) w[a][r] = fast_exp2(__builtin_fmaf(w[a][r], sc.f, c));
-    if (masked) {  // again: of a block of scale NaN, a key that is not seen weighs 0
+    if (masked && !(sc.f == sc.f && sc.lsv == sc.lsv)) {  // of a block of scale NaN, a key that is not seen weighs 0
+        int again = left;
+        asm volatile("" : "+v"(again));  // compared here, and not kept from above on every path
 #pragma unroll
         for (int a = 0; a < KA; ++a)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) w[a][r] = 16 * a + r <= left ? w[a][r] : 0.f;
+            for (int r = 0; r < 4; ++r) w[a][r] = 16 * a + r <= again ? w[a][r] : 0.f;
     }
 #pragma unroll
     for (int a = 0; a < KA; ++a)
@@ -190,18 +192,16 @@ __device__ __forceinline__ void kv8_keys(Kv8Rows<D> (&st)[NT], int p0, const Kv8
     }
 }
 
-// The same from operands in LDS (kb, vb: this lane's of K and V), read a few ahead of their products;
-// between(e) is called among K's.  The queries' last kQl steps lie in LDS too (qb: this lane's).
-template <int D, int NT, int KA, int kQl, class Between>
-__device__ __forceinline__ void kv8_lds_keys(Kv8Rows<D> (&st)[NT], int p0, const Kv8Scale& sc, bool masked, const half8_t* kb,
-                                             const half8_t* vb, const half8_t* qb, Between between) {
-    constexpr int kOps = KA * (D / 32), kAhead = D == 256 ? 3 : 6, kQr = D / 32 - kQl;
-    float4_t w[NT][KA];
+// The same in two parts from operands in LDS (kb, vb: this lane's of K and V), read kAhead before
+// their products.  Scores: between(e) is called among the products.
+template <int D, int NT, int KA, int kAhead, class Between>
+__device__ __forceinline__ void kv8_lds_scores(const Kv8Rows<D> (&st)[NT], float4_t (&w)[NT][KA], const half8_t* kb, Between between) {
+    constexpr int kOps = KA * (D / 32);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int a = 0; a < KA; ++a) w[nt][a] = float4_t{0.f, 0.f, 0.f, 0.f};
-    half8_t op[kOps], ql[NT];
+    half8_t op[kOps];
     auto read_k = [&](int e) {  // key tile e % KA, step e / KA
         const int a = e % KA, x = e / KA;
         op[e] = kb[((a * (D / 64) + x / 2) * 2 + x % 2) * 64];
@@ -214,35 +214,26 @@ __device__ __forceinline__ void kv8_lds_keys(Kv8Rows<D> (&st)[NT], int p0, const
         if (e + kAhead < kOps) read_k(e + kAhead);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
-            w[nt][e % KA] = mfma16(op[e], e / KA < kQr ? st[nt].q[e / KA] : ql[nt], w[nt][e % KA]);
-        if (kQl && (e + 1) % KA == 0 && (e + 1) / KA >= kQr && e + 1 < kOps) {  // the next step's queries
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) ql[nt] = qb[(((e + 1) / KA - kQr) * NT + nt) * 64];
-        }
+            w[nt][e % KA] = mfma16(op[e], st[nt].q[e / KA], w[nt][e % KA]);
         between(e);
         __builtin_amdgcn_sched_barrier(0);
     }
-    auto read_v = [&](int e) { op[e] = vb[e * 64]; };  // (s, m, o) in order
+}
+// Sums: p are the weights of key steps of 32.
+template <int D, int NT, int KS, int kAhead>
+__device__ __forceinline__ void kv8_lds_sums(Kv8Rows<D> (&st)[NT], const half8_t (&p)[NT][KS], const half8_t* vb) {
+    constexpr int kOps = KS * (D / 16);
+    half8_t op[kOps];
 #pragma unroll
-    for (int e = 0; e < kAhead; ++e) read_v(e);
+    for (int e = 0; e < kAhead; ++e) op[e] = vb[e * 64];
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) kv8_softmax<D, KA>(st[nt], w[nt], p0, sc, masked);
-    __builtin_amdgcn_s_setprio(1);
+    for (int e = 0; e < kOps; ++e) {  // (s, m, o) in order
+        if (e + kAhead < kOps) op[e + kAhead] = vb[(e + kAhead) * 64];
 #pragma unroll
-    for (int s = 0; s < KA / 2; ++s) {
-        half8_t p[NT];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) p[nt] = kv8_weights<KA>(w[nt], s);
-#pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt) {
-            const int e = s * (D / 16) + dt;
-            if (e + kAhead < kOps) read_v(e + kAhead);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) st[nt].o[dt] = mfma16(op[e], p[nt], st[nt].o[dt]);
-            __builtin_amdgcn_sched_barrier(0);
-        }
+        for (int nt = 0; nt < NT; ++nt) st[nt].o[e % (D / 16)] = mfma16(op[e], p[nt][e / (D / 16)], st[nt].o[e % (D / 16)]);
+        __builtin_amdgcn_sched_barrier(0);
     }
-    __builtin_amdgcn_s_setprio(0);
 }
 
 // The open block from the ring: n of its rows are the sequence's, those behind are whatever the
@@ -299,6 +290,7 @@ __device__ __forceinline__ void kv8_open_block(Kv8Rows<D>& st, const Kv8& c, int
             for (int x = 0; x < 4; ++x) st.o[2 * m + x] = mfma16(v[x], p, st.o[2 * m + x]);
             if (!bad) continue;
             const half_t* vo = c.v_open + at;
+            float4_t more[4] = {};  // (not on the sums themselves, which are to stay in place)
 #pragma unroll 1
             for (int y = 0; y < 32; ++y) {
                 const int j = y >> 2, g = y & 3, key = 16 * (j >> 2) + 4 * g + (j & 3);
@@ -314,9 +306,11 @@ __device__ __forceinline__ void kv8_open_block(Kv8Rows<D>& st, const Kv8& c, int
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const half_t z = vo[kv8_v_at<D>(32 * s + key, 16 * (2 * m + x) + 4 * g4 + e)];
-                        if (kv8_bad(z)) st.o[2 * m + x][e] += wj * (float)z;
+                        if (kv8_bad(z)) more[x][e] += wj * (float)z;
                     }
             }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) st.o[2 * m + x] += more[x];
         }
     }
 }
@@ -546,157 +540,515 @@ kv8_row_kernel(Kv8AttnArgs p) {
 
 constexpr int kKvMaxSplits = 128;
 
-// Many rows: a workgroup is kWaves waves of 16 NT query rows each over one split of their blocks.  A
-// stage of kKeys keys and their values (16 KiB of codes at the most) goes from memory to registers
-// two stages ahead, is turned into fp16 operands once for all waves, and lies in one of two LDS
-// buffers in operand order, so every LDS access is 16 consecutive bytes a lane and a code is
-// converted once per 16 NT kWaves rows.  One barrier a stage.  Two waves a SIMD: two workgroups of 4
-// waves a CU, or at D = 256, NT = 2 one of 8 (a thread then holds half as many codes, without which
-// the 128 sums and 64 query registers spill).
+// Which tile, (sequence, head) and split a workgroup of the kernels below has.  Workgroups go round
+// the 8 XCDs.  The tiles of one (head, split) read the same keys: they go to one XCD, the last
+// (longest) tiles of its heads first, or where the heads and splits are no multiple of 8, each XCD
+// takes an eighth of all in a row.
+struct Kv8Place {
+    int tile, bh, b, h, split;
+    __device__ __forceinline__ bool find(const Kv8AttnArgs& p, int tiles, int streams) {
+        int stream, rank;
+        const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
+        if ((streams & 7) == 0) {
+            const int per = streams >> 3;
+            stream = xcd * per + slot % per;
+            rank = slot / per;
+        } else {
+            const int at = xcd * (int)(gridDim.x >> 3) + slot;
+            if (at >= streams * tiles) return false;
+            stream = at / tiles;
+            rank = at % tiles;
+        }
+        tile = tiles - 1 - rank;
+        bh = stream / p.nsplit;
+        split = stream % p.nsplit;
+        b = bh / p.c.Hkv;
+        h = bh % p.c.Hkv;
+        return true;
+    }
+};
+
+// The blocks of a split of a tile of rows [first, end): those that some row sees, shared out.
+struct Kv8Share {
+    int n_full;   // full blocks that are seen
+    bool open;    // the open block is this split's
+    Kv8Walk<false> walk;
+    __device__ __forceinline__ void find(const Kv8AttnArgs& p, const Kv8Seq& sq, int last_row, int split) {
+        const int front = sq.len - (sq.n + sq.t0);  // position of row t = 0
+        const int all = p.causal ? min(front + last_row / p.G, sq.len - 1) : sq.len - 1;
+        const int nb = all < 0 ? 0 : all / kKvBlock + 1;
+        n_full = min(sq.len / kKvBlock, nb);
+        const int per = (nb + p.nsplit - 1) / p.nsplit, end = min(nb, (split + 1) * per);
+        open = split * per <= n_full && n_full < end;
+        walk = {split * per, min(end, n_full), 1, n_full, n_full, 0, 0};
+    }
+};
+
+// A wave's finished rows, or a split's sums of them.
+template <int D, int NT>
+__device__ __forceinline__ void kv8_finish(Kv8Rows<D> (&st)[NT], const Kv8AttnArgs& p, const Kv8Place& at, int row0, int row_end) {
+    const int lane = threadIdx.x & 63, g4 = lane >> 4;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const float l = sum_xor32(sum_xor16(st[nt].l));
+        const int row = row0 + 16 * nt + (lane & 15);
+        if (row >= row_end) continue;
+        if (p.nsplit > 1) {
+            if (l != 0.f) {
+                float* part = kv8_part<D>(p, at.bh, row, at.split) + 4 * g4;
+#pragma unroll
+                for (int dt = 0; dt < D / 16; ++dt) *reinterpret_cast<float4_t*>(part + 16 * dt) = st[nt].o[dt];
+            }
+            if (g4 == 0) *reinterpret_cast<float2*>(kv8_pair<D>(p, at.bh, row, at.split)) = float2{st[nt].m, l};
+        } else {
+            const int t = row / p.G, hq = at.h * p.G + row % p.G;
+#pragma unroll
+            for (int dt = 0; dt < D / 16; ++dt)
+                kv8_store4(p, at.b, hq, t, 16 * dt + 4 * g4, st[nt].o[dt], l, kv8_gate4(p, at.b, hq, t, 16 * dt + 4 * g4));
+        }
+    }
+}
+
+// A stage of keys on its way from memory to LDS.
+struct Kv8Stage {
+    int p0 = -1;  // first key, -1: none
+    int page = 0, part = 0;
+    Kv8Scale sc = {};
+};
+// The next stage of a walk in parts of kParts a block.
+template <int kParts, class Walk>
+__device__ __forceinline__ void kv8_step(Kv8Stage& s, Walk& walk, const Kv8& c, int b, int h, float c2) {
+    if (s.p0 >= 0 && s.part + 1 < kParts) {
+        s.p0 += kKvBlock / kParts;
+        ++s.part;
+        return;
+    }
+    int blk;
+    s.p0 = walk.next(c, b, h, nullptr, c2, blk, s.page, s.sc) ? blk * kKvBlock : -1;
+    s.part = 0;
+}
+
+// More rows than a tile: a workgroup is 4 waves of 16 NT query rows each over one split of their
+// blocks.  A stage of kKeys keys and their values (16 KiB of codes at the most) goes from memory to
+// registers two stages ahead, is turned into fp16 operands once for all waves, and lies in one of
+// two LDS buffers in operand order, so every LDS access is 16 consecutive bytes a lane and a code
+// is converted once per 64 NT rows.  One barrier a stage.
 template <int D, int NT>
 struct Kv8Tile {
-    static constexpr int kWaves = D == 256 && NT == 2 ? 8 : 4, kThreads = 64 * kWaves;
     static constexpr int kKeys = D == 256 ? 32 : 64, kParts = kKvBlock / kKeys;
-    static constexpr int kUnits = kKeys * D / 16;          // 16-code units of K (or V) a stage
-    static constexpr int kN = kUnits / kThreads;           // of them a thread moves
-    static constexpr int kRows = 16 * NT * kWaves;
-    static constexpr int kQl = D == 256 && NT == 2 ? 3 : 0;  // steps of the queries kept in LDS, likewise
+    static constexpr int kUnits = kKeys * D / 16;  // 16-code units of K (or V) a stage
+    static constexpr int kN = kUnits / 256;        // of them a thread moves
+    static constexpr int kRows = 64 * NT;
 };
 template <int D, int NT>
-__global__ void __launch_bounds__((Kv8Tile<D, NT>::kThreads), 2)
+__global__ void __launch_bounds__(256, 2)
 kv8_tile_kernel(Kv8AttnArgs p, int tiles, int streams) {
     using C = Kv8Tile<D, NT>;
+    constexpr int KA = C::kKeys / 16, kAhead = D == 256 ? 3 : 6;
     __shared__ __align__(16) half8_t buf[2][4 * C::kUnits];  // K's halves, then V's
-    __shared__ __align__(16) half8_t qs[C::kQl ? C::kWaves : 1][C::kQl ? C::kQl * NT : 1][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int g4 = lane >> 4, n = lane & 15;
     const Kv8& c = p.c;
-    // Workgroups go round the 8 XCDs.  The tiles of one (head, split) read the same keys: they go to
-    // one XCD, the last (longest) tiles of its heads first, or where the heads and splits are no
-    // multiple of 8, each XCD takes an eighth of all in a row.
-    int stream, rank;
-    const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
-    if ((streams & 7) == 0) {
-        const int per = streams >> 3;
-        stream = xcd * per + slot % per;
-        rank = slot / per;
-    } else {
-        const int at = xcd * (int)(gridDim.x >> 3) + slot;
-        if (at >= streams * tiles) return;
-        stream = at / tiles;
-        rank = at % tiles;
-    }
-    const int tile = tiles - 1 - rank, bh = stream / p.nsplit, split = stream % p.nsplit;
-    const int b = bh / c.Hkv, h = bh % c.Hkv;
-    const Kv8Seq sq = kv8_seq(c, p.len, p.n_new, b, p.T);
-    const int front = sq.len - (sq.n + sq.t0);  // position of row t = 0
+    Kv8Place at;
+    if (!at.find(p, tiles, streams)) return;
+    const Kv8Seq sq = kv8_seq(c, p.len, p.n_new, at.b, p.T);
     const int row_end = min(p.T, sq.n + sq.t0) * p.G;
-    if (tile * C::kRows >= row_end) return;
+    if (at.tile * C::kRows >= row_end) return;
 
     Kv8Rows<D> st[NT];
-    const int row0 = tile * C::kRows + wave * 16 * NT;
+    const int row0 = at.tile * C::kRows + wave * 16 * NT;
     int see, least;
-    kv8_begin<D, NT>(st, p, sq, b, h, row0, row_end, see, least);
-    // the last key that any row of the workgroup sees
-    const int all = p.causal ? min(front + (min(row_end, (tile + 1) * C::kRows) - 1) / p.G, sq.len - 1) : sq.len - 1;
-    const int nb = all < 0 ? 0 : all / kKvBlock + 1;
-    const int n_full = min(sq.len / kKvBlock, nb);
-    const int per = (nb + p.nsplit - 1) / p.nsplit;
-    const int end = min(nb, (split + 1) * per);
-    const bool open = split * per <= n_full && n_full < end;
-    Kv8Walk<false> walk = {split * per, min(end, n_full), 1, n_full, n_full, 0, 0};
-    int blk = 0, page = -1, part = 0;
-    Kv8Scale sc = {};
-    auto next = [&]() {
-        if (!walk.next(c, b, h, nullptr, p.c2, blk, page, sc)) page = -1;
-    };
+    kv8_begin<D, NT>(st, p, sq, at.b, at.h, row0, row_end, see, least);
+    Kv8Share share;
+    share.find(p, sq, min(row_end, (at.tile + 1) * C::kRows) - 1, at.split);
 
-    struct Stage {
-        int p0;  // first key, -1: none
-        Kv8Scale sc;
-    };
     uint4 rk[C::kN], rv[C::kN];
-    auto load = [&]() -> Stage {  // codes of the stage at (page, part) to registers, and on to the next
-        if (page < 0) return {-1, {}};
-        const size_t head = (size_t)page * c.Hkv + h;
-        const uint4* kp = reinterpret_cast<const uint4*>(c.k + head * (kKvBlock * D)) + part * C::kUnits + tid;
-        const uint4* vp = reinterpret_cast<const uint4*>(c.v + head * (kKvBlock * D)) + part * C::kUnits + tid;
+    auto load = [&](const Kv8Stage& s) {
+        if (s.p0 < 0) return;
+        const size_t head = (size_t)s.page * c.Hkv + at.h;
+        const uint4* kp = reinterpret_cast<const uint4*>(c.k + head * (kKvBlock * D)) + s.part * C::kUnits + tid;
+        const uint4* vp = reinterpret_cast<const uint4*>(c.v + head * (kKvBlock * D)) + s.part * C::kUnits + tid;
 #pragma unroll
-        for (int x = 0; x < C::kN; ++x) rk[x] = kp[x * C::kThreads];
+        for (int x = 0; x < C::kN; ++x) rk[x] = kp[x * 256];
 #pragma unroll
-        for (int x = 0; x < C::kN; ++x) rv[x] = vp[x * C::kThreads];
-        const Stage s = {blk * kKvBlock + part * C::kKeys, sc};
-        if (++part == C::kParts) {
-            part = 0;
-            next();
-        }
-        return s;
+        for (int x = 0; x < C::kN; ++x) rv[x] = vp[x * 256];
     };
     // Unit x of the registers (K's, then V's) to LDS as fp16.
     auto store = [&](int to, int x) {
         const bool isv = x >= C::kN;
         const uint4& r = isv ? rv[x - C::kN] : rk[x];
-        half8_t* at = &buf[to][(isv ? 2 * C::kUnits : 0) + ((tid >> 6) + C::kWaves * (isv ? x - C::kN : x)) * 128 + lane];
-        at[0] = kv8_halves(r.x, r.y);
-        at[64] = kv8_halves(r.z, r.w);
+        half8_t* u = &buf[to][(isv ? 2 * C::kUnits : 0) + ((tid >> 6) + 4 * (isv ? x - C::kN : x)) * 128 + lane];
+        u[0] = kv8_halves(r.x, r.y);
+        u[64] = kv8_halves(r.z, r.w);
     };
-    auto store_all = [&](int to) {
+    Kv8Stage now, then, after;
+    auto step = [&](Kv8Stage& s) { kv8_step<C::kParts>(s, share.walk, c, at.b, at.h, p.c2); };
+    step(now);
+    load(now);
+    if (now.p0 >= 0) {
 #pragma unroll
-        for (int x = 0; x < 2 * C::kN; ++x) store(to, x);
-    };
-    next();
-    Stage now = load();
-    if (now.p0 >= 0) store_all(0);
-    Stage then = load();
+        for (int x = 0; x < 2 * C::kN; ++x) store(0, x);
+    }
+    then = now;
+    if (now.p0 >= 0) step(then);
+    load(then);
     kv8_arrived<D, NT>(st);
-    half8_t* ql = &qs[C::kQl ? wave : 0][0][lane];  // a wave reads its own only
-#pragma unroll
-    for (int x = 0; x < C::kQl; ++x)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) ql[(x * NT + nt) * 64] = st[nt].q[D / 32 - C::kQl + x];
     lds_barrier();
     for (int u = 0; now.p0 >= 0; u ^= 1) {
         const half8_t* kb = &buf[u][lane];
-        const half8_t* vb = kb + 2 * C::kUnits;
+        float4_t w[NT][KA];
         // The next stage's codes are converted among the products of K's operands, and the one after
         // that is sent for behind them.  (Behind the last stage the registers hold old codes; what
         // is written is not read.)  A wave that sees none of the stage's keys, on the diagonal, runs
         // them masked: a branch round the products would cost it a copy of all its sums.
-        kv8_lds_keys<D, NT, C::kKeys / 16, C::kQl>(st, now.p0, now.sc, now.p0 + C::kKeys - 1 > least, kb, vb, ql, [&](int e) {
-            constexpr int kOps = C::kKeys / 16 * (D / 32), kEvery = kOps / (4 * C::kN);
+        kv8_lds_scores<D, NT, KA, kAhead>(st, w, kb, [&](int e) {
+            constexpr int kEvery = KA * (D / 32) / (4 * C::kN);
             if (e % kEvery == kEvery - 1 && e / kEvery < 2 * C::kN) store(u ^ 1, e / kEvery);
         });
-        const Stage after = load();
+        after = then;
+        if (then.p0 >= 0) step(after);
+        load(after);
+        half8_t wp[NT][KA / 2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            kv8_softmax<D, KA>(st[nt], w[nt], now.p0, now.sc, now.p0 + C::kKeys - 1 > least);
+#pragma unroll
+            for (int s = 0; s < KA / 2; ++s) wp[nt][s] = kv8_weights<KA>(w[nt], s);
+        }
+        kv8_lds_sums<D, NT, KA / 2, kAhead>(st, wp, kb + 2 * C::kUnits);
         lds_barrier();
         now = then;
         then = after;
     }
-    if (open && see >= n_full * kKvBlock) {
+    if (share.open && see >= share.n_full * kKvBlock) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            kv8_queries<D>(st[nt], p, b, h, row0 + 16 * nt, row_end);  // again: not held through the loop's end
-            kv8_open_block<D>(st[nt], c, b, h, n_full, sq.len - n_full * kKvBlock, p.c2);
+            kv8_queries<D>(st[nt], p, at.b, at.h, row0 + 16 * nt, row_end);  // again: not held through the loop's end
+            kv8_open_block<D>(st[nt], c, at.b, at.h, share.n_full, sq.len - share.n_full * kKvBlock, p.c2);
         }
     }
+    kv8_finish<D, NT>(st, p, at, row0, row_end);
+}
 
+// ---- Many rows at D = 128 and 256 ----
+// v_mfma_f32_32x32x16_f16 in place of the 16-row one: half the instructions for the same products,
+// and its sums stay where they are over the branch that rescales them (two tiles of 16 rows moved
+// all sums in every stage).  Lane l owns query row l % 32 and half h = l / 32 of the keys.  Register
+// 4 a + e of a score tile of 32 keys holds key kv8_key32(a) + 4 h + e: K's rows are put in that
+// order in LDS, so that the weights of registers 8 x .. 8 x + 7 are the keys of the 8 consecutive
+// codes g4 = 2 x + h of a V unit.
+__device__ __forceinline__ constexpr int kv8_key32(int a) { return 16 * (a & 1) + 4 * (a & 2); }
+
+template <int D>
+struct Kv8Rows32 {
+    half8_t q[D / 16];    // operand B: step u holds d = 16 u + 8 h + 0 .. 7
+    float16_t o[D / 32];  // O^T: d = 32 m + 8 (r / 4) + 4 h + r % 4 in register r
+    float m, l;           // l: this lane's keys only
+    int limit;            // last key the row sees, -1: none
+};
+
+// kv8_softmax for 32 KT keys.
+template <int D, int KT>
+__device__ __forceinline__ void kv8_softmax32(Kv8Rows32<D>& st, float16_t (&w)[KT], int p0, const Kv8Scale& sc, bool masked) {
+    const int left = st.limit - p0 - 4 * (int)((threadIdx.x & 63) >> 5);
+    if (masked) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const float l = sum_xor32(sum_xor16(st[nt].l));
-        const int row = row0 + 16 * nt + n;
-        if (row >= row_end) continue;
-        if (p.nsplit > 1) {
-            if (l != 0.f) {
-                float* at = kv8_part<D>(p, bh, row, split) + 4 * g4;
+        for (int t = 0; t < KT; ++t)
 #pragma unroll
-                for (int dt = 0; dt < D / 16; ++dt) *reinterpret_cast<float4_t*>(at + 16 * dt) = st[nt].o[dt];
-            }
-            if (g4 == 0) *reinterpret_cast<float2*>(kv8_pair<D>(p, bh, row, split)) = float2{st[nt].m, l};
-        } else {
-            const int t = row / p.G, hq = h * p.G + row % p.G;
+            for (int r = 0; r < 16; ++r) w[t][r] = 32 * t + kv8_key32(r >> 2) + (r & 3) <= left ? w[t][r] : -INFINITY;
+    }
+    float big = -INFINITY;
 #pragma unroll
-            for (int dt = 0; dt < D / 16; ++dt)
-                kv8_store4(p, b, hq, t, 16 * dt + 4 * g4, st[nt].o[dt], l, kv8_gate4(p, b, hq, t, 16 * dt + 4 * g4));
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) big = fmaxf(big, w[t][r]);
+    big = __builtin_fmaf(big, sc.f, sc.lsv);  // of this lane's keys
+    if (__any(big > st.m + kKvSlack)) {
+        const float m_new = fmaxf(st.m, max_xor32(big));
+        const float alpha = m_new == st.m ? 1.f : fast_exp2(st.m - m_new);
+        st.m = m_new;
+        st.l *= alpha;
+#pragma unroll
+        for (int m = 0; m < D / 32; ++m)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) st.o[m][r] *= alpha;
+    }
+    const float c = sc.lsv - (st.m == -INFINITY ? 0.f : st.m - kKvBias);
+    float sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) w[t][r] = fast_exp2(__builtin_fmaf(w[t][r], sc.f, c));
+    if (masked && !(sc.f == sc.f && sc.lsv == sc.lsv)) {  // of a block of scale NaN, a key that is not seen weighs 0
+        int again = left;
+        asm volatile("" : "+v"(again));  // compared here, and not kept from above on every path
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) w[t][r] = 32 * t + kv8_key32(r >> 2) + (r & 3) <= again ? w[t][r] : 0.f;
+    }
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum += w[t][r];
+    st.l += sum == 0.f ? 0.f : sum * sc.isv;
+}
+// Weights of registers 8 x .. 8 x + 7 of a score tile as operand B.
+__device__ __forceinline__ half8_t kv8_weights32(const float16_t& w, int x) {
+    typedef float float8_v __attribute__((ext_vector_type(8)));
+    const float8_v y = x ? __builtin_shufflevector(w, w, 8, 9, 10, 11, 12, 13, 14, 15) : __builtin_shufflevector(w, w, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_convertvector(y, half8_t);
+}
+
+// Where a lane's row of queries starts (its half of each step of 16 d).
+__device__ __forceinline__ const half_t* kv8_query32(const Kv8AttnArgs& p, int b, int h, int row) {
+    const int t = row / p.G, g = row % p.G;
+    return p.q.data + b * p.q.b + (long long)(h * p.G + g) * p.q.h + t * p.q.t + 8 * ((threadIdx.x & 63) >> 5);
+}
+
+// kv8_open_block for 32 rows, whose queries are read from qr (is_row: the lane's row is one): held in
+// registers with the sums they would spill at D = 256.
+template <int D>
+__device__ __forceinline__ void kv8_open_block32(Kv8Rows32<D>& st, const half_t* qr, bool is_row, const Kv8& c, int b, int h, int blk,
+                                                 int n, float c2) {
+    const int lane = threadIdx.x & 63, hi = lane >> 5, x32 = lane & 31;
+    const size_t at = kv8_open_at<D>(c, b, h, blk);
+    const half_t* ko = c.k_open + at;
+    const half_t* vo = c.v_open + at;
+    const int row = kv8_key32(x32 >> 3) + 4 * ((x32 >> 2) & 1) + (x32 & 3);  // this lane's key as operand A
+#pragma unroll 1
+    for (int s = 0; 32 * s < n; ++s) {  // half a block at a time
+        const int p0 = blk * kKvBlock + 32 * s;
+        float16_t w[1] = {};
+#pragma unroll
+        for (int u = 0; u < D / 16; ++u) {
+            const half8_t q = is_row ? *reinterpret_cast<const half8_t*>(qr + 16 * u) : half8_t{};
+            w[0] = mfma32(*reinterpret_cast<const half8_t*>(ko + kv8_k_at<D>(32 * s + row, 16 * u + 8 * hi)), q, w[0]);
+            if (u % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // a few loads at a time
         }
+        kv8_softmax32<D, 1>(st, w, p0, {c2, 0.f, 1.f}, true);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {  // 16 keys at a time
+            const half8_t p = kv8_weights32(w[0], x);
+            const int g4 = 2 * x + hi;  // keys 16 i + 4 g4 + e
+#pragma unroll
+            for (int m = 0; m < D / 32; ++m) {
+                half8_t v = *reinterpret_cast<const half8_t*>(vo + kv8_v_at<D>(32 * s + 4 * g4, 32 * m + x32));
+                bool bad = false;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const bool is = 32 * s + 16 * (j >> 2) + 4 * g4 + (j & 3) < n;
+                    const bool off = kv8_bad(v[j]);
+                    bad |= is && off;
+                    if (!is || off) v[j] = (half_t)0.f;
+                }
+                st.o[m] = mfma32(v, p, st.o[m]);
+                if (!__any(bad)) continue;
+                float16_t more = {};  // (not on the sums themselves, which are to stay in place)
+#pragma unroll 1
+                for (int y = 0; y < 16; ++y) {  // a key: register 8 x + j of half g
+                    const int j = y >> 1, g = y & 1, key = 16 * (j >> 2) + 4 * (2 * x + g) + (j & 3);
+                    float wj = 0.f;
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) wj = j == r ? w[0][8 * x + r] : wj;
+                    wj = __shfl(wj, 32 * g + x32);
+                    if (p0 + key > st.limit) continue;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const half_t z = vo[kv8_v_at<D>(32 * s + key, 32 * m + 8 * (r >> 2) + 4 * hi + (r & 3))];
+                        if (kv8_bad(z)) more[r] += wj * (float)z;
+                    }
+                }
+                st.o[m] += more;
+            }
+        }
+    }
+}
+
+// A workgroup is 8 waves of 32 rows over one split of their blocks.  A stage of kKeys keys goes from
+// memory to registers two stages ahead (a unit of K and one of V a thread), is turned into fp16
+// operands once for all waves, and lies in one of two LDS buffers in operand order.  One barrier a
+// stage.
+// Bound by the card's power at D = 128 (prompt of 8192, 32 heads: 0.65 ms at 1.8 GHz, 0.84 PFLOP/s;
+// the fp16 kernel of attn_fwd.hip, 0.57 ms at 1.6 GHz): two groups of waves taking turns at matrix
+// and vector instructions needed 13 % fewer cycles and the same time.  At D = 256 (512 tokens over
+// 16384, 24/4 heads: 0.23 ms, 0.89 PFLOP/s) by LDS, which the operands of 32 rows keep busy for as
+// long as the matrix units; the two groups' second barrier a stage cost it 8 %.
+template <int D>
+struct Kv8Wide {
+    static constexpr int kRows = 32 * 8;
+    static constexpr int kKeys = D == 256 ? 32 : 64, kParts = kKvBlock / kKeys, KT = kKeys / 32;
+    static constexpr int kUnits = kKeys * D / 16;  // 512: of K and of V, one a thread
+    static constexpr int kAhead = D == 256 ? 3 : 4;  // operands read ahead of their products
+    // At D = 256 128 sums and 64 registers of queries leave too few for the rest: the queries' last
+    // steps are kept in LDS and read as operands with K's.
+    static constexpr int kQl = D == 256 ? 6 : 0, kQr = D / 16 - kQl;
+    static_assert(kUnits == 512, "a thread moves one unit of K and one of V a stage");
+};
+template <int D>
+__global__ void __launch_bounds__(512, 2)
+kv8_wide_kernel(Kv8AttnArgs p, int tiles, int streams) {
+    using C = Kv8Wide<D>;
+    constexpr int KT = C::KT;
+    __shared__ __align__(16) half8_t kbuf[2][2 * C::kUnits];
+    __shared__ __align__(16) half8_t vbuf[2][2 * C::kUnits];
+    __shared__ __align__(16) half8_t qbuf[C::kQl ? 8 : 1][C::kQl ? C::kQl : 1][64];
+    const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Kv8& c = p.c;
+    Kv8Place at;
+    if (!at.find(p, tiles, streams)) return;
+    const Kv8Seq sq = kv8_seq(c, p.len, p.n_new, at.b, p.T);
+    const int row_end = min(p.T, sq.n + sq.t0) * p.G;
+    if (at.tile * C::kRows >= row_end) return;
+
+    Kv8Rows32<D> st;
+    int row = at.tile * C::kRows + wave * 32 + (lane & 31);
+    const half_t* qr = kv8_query32(p, at.b, at.h, row);
+#pragma unroll
+    for (int u = 0; u < D / 16; ++u) st.q[u] = row < row_end ? *reinterpret_cast<const half8_t*>(qr + 16 * u) : half8_t{};
+    const int pos = sq.len - (sq.n + sq.t0) + row / p.G;  // below 0: in front of the sequence
+    st.limit = row >= row_end ? -1 : p.causal ? min(pos, sq.len - 1) : sq.len - 1;
+    int see = st.limit, least = row < row_end ? st.limit : INT_MAX;  // the last key that any, that every row sees
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+        see = max(see, __shfl_xor(see, x));
+        least = min(least, __shfl_xor(least, x));
+    }
+    see = __builtin_amdgcn_readfirstlane(see);
+    least = __builtin_amdgcn_readfirstlane(least);
+#pragma unroll
+    for (int m = 0; m < D / 32; ++m) st.o[m] = float16_t{};
+    st.m = -INFINITY;
+    st.l = 0.f;
+    Kv8Share share;
+    share.find(p, sq, min(row_end, (at.tile + 1) * C::kRows) - 1, at.split);
+
+    uint4 rk, rv;
+    auto load = [&](const Kv8Stage& s) {
+        if (s.p0 < 0) return;
+        const size_t head = ((size_t)s.page * c.Hkv + at.h) * (kKvBlock * D);
+        rk = reinterpret_cast<const uint4*>(c.k + head)[s.part * C::kUnits + tid];
+        rv = reinterpret_cast<const uint4*>(c.v + head)[s.part * C::kUnits + tid];
+    };
+    // Where this thread's unit goes.  K: key 16 a + rr (a = tile / (D / 64)) of score tile a / 2, d =
+    // 16 u + 0 .. 15: step u, halves 0 and 1, the key's row.  V: d = 32 m + dd and + 16, codes g4 of
+    // half block s: step x = g4 / 2, half g4 % 2.
+    const int g4 = (lane >> 4) & 3, rr = lane & 15, tile = tid >> 6;
+    const int ka = tile / (D / 64), ku = tile % (D / 64) * 4 + g4, quad = rr >> 2;
+    // score row of a key: register groups 0, 1, 2, 3 hold quads h, 4 + h, 2 + h, 6 + h
+    const int krow = 8 * (2 * (quad >> 1) + (ka & 1)) + 4 * (quad & 1) + (rr & 3);
+    const int kto = (ka / 2 * (D / 16) + ku) * 64 + krow;
+    const int vto = (tile * 2 + (g4 >> 1)) * 64 + (g4 & 1) * 32 + rr;
+    auto store_k = [&](int u) {
+        kbuf[u][kto] = kv8_halves(rk.x, rk.y);
+        kbuf[u][kto + 32] = kv8_halves(rk.z, rk.w);
+    };
+    auto store_v = [&](int u) {
+        vbuf[u][vto] = kv8_halves(rv.x, rv.y);
+        vbuf[u][vto + 16] = kv8_halves(rv.z, rv.w);
+    };
+    Kv8Stage now, then, after;
+    auto step = [&](Kv8Stage& s) { kv8_step<C::kParts>(s, share.walk, c, at.b, at.h, p.c2); };
+    step(then);
+    if (then.p0 >= 0) {
+        constexpr int kOps = KT * (D / 16);
+        half8_t op[kOps], wp[2 * KT] = {};
+        float16_t w[KT];
+        half8_t* ql = &qbuf[C::kQl ? wave : 0][0][lane];  // a wave reads its own only
+        // A stage's scores, with the next one's codes converted and written among the products.
+        // (Behind the last stage the registers hold old codes; what is written is not read.)
+        auto scores = [&](int u) {
+            const half8_t* kb = &kbuf[u][lane];
+            half8_t qop[D / 16];
+            auto read_k = [&](int e) {  // tile e % KT, step e / KT
+                op[e] = kb[(e % KT * (D / 16) + e / KT) * 64];
+                if (e % KT == 0 && e / KT >= C::kQr) qop[e / KT] = ql[(e / KT - C::kQr) * 64];
+            };
+#pragma unroll
+            for (int t = 0; t < KT; ++t) w[t] = float16_t{};
+#pragma unroll
+            for (int e = 0; e < C::kAhead; ++e) read_k(e);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int e = 0; e < kOps; ++e) {
+                if (e + C::kAhead < kOps) read_k(e + C::kAhead);
+                w[e % KT] = mfma32(op[e], e / KT < C::kQr ? st.q[e / KT] : qop[e / KT], w[e % KT]);
+                if (e == kOps / 4) store_k(u ^ 1);
+                if (e == kOps / 2) store_v(u ^ 1);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        auto softmax = [&]() {
+            kv8_softmax32<D, KT>(st, w, now.p0, now.sc, now.p0 + C::kKeys - 1 > least);
+#pragma unroll
+            for (int x = 0; x < 2 * KT; ++x) wp[x] = kv8_weights32(w[x / 2], x % 2);
+        };
+        // A stage's sums.  Product e: half block e / (D / 16), d block m, key step x (in LDS: half, m, x).
+        auto sums = [&](int u) {
+            const half8_t* vb = &vbuf[u][lane];
+#pragma unroll
+            for (int e = 0; e < C::kAhead; ++e) op[e] = vb[e * 64];
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int e = 0; e < kOps; ++e) {
+                if (e + C::kAhead < kOps) op[e + C::kAhead] = vb[(e + C::kAhead) * 64];
+                const int s = e / (D / 16), m = e % (D / 16) / 2, x = e % 2;
+                st.o[m] = mfma32(op[e], wp[2 * s + x], st.o[m]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        load(then);
+        store_k(0);
+        store_v(0);
+        after = then;
+        step(after);
+        load(after);
+#pragma unroll
+        for (int u = 0; u < D / 16; ++u) asm volatile("" : "+v"(st.q[u]));  // arrived (see kv8_arrived)
+#pragma unroll
+        for (int x = 0; x < C::kQl; ++x) ql[x * 64] = st.q[C::kQr + x];
+        lds_barrier();
+        int u = 0;
+        do {  // (its end behind the barrier: left among the products, the sums were moved in every stage)
+            now = then;
+            then = after;
+            scores(u);
+            if (then.p0 >= 0) step(after);
+            load(after);
+            softmax();
+            __builtin_amdgcn_s_setprio(1);
+            sums(u);
+            __builtin_amdgcn_s_setprio(0);
+            lds_barrier();
+            u ^= 1;
+        } while (then.p0 >= 0);
+    }
+    asm volatile("" : "+v"(row));  // what follows from it below is computed again, not held through the loop
+    if (share.open && see >= share.n_full * kKvBlock) {
+        kv8_open_block32<D>(st, kv8_query32(p, at.b, at.h, row), row < row_end, c, at.b, at.h, share.n_full, sq.len - share.n_full * kKvBlock, p.c2);
+    }
+    const float l = sum_xor32(st.l);
+    if (row >= row_end) return;
+    if (p.nsplit > 1) {
+        if (l != 0.f) {
+            float* part = kv8_part<D>(p, at.bh, row, at.split) + 4 * hi;
+#pragma unroll
+            for (int m = 0; m < D / 32; ++m)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    *reinterpret_cast<float4_t*>(part + 32 * m + 8 * r) =
+                        float4_t{st.o[m][4 * r], st.o[m][4 * r + 1], st.o[m][4 * r + 2], st.o[m][4 * r + 3]};
+        }
+        if (hi == 0) *reinterpret_cast<float2*>(kv8_pair<D>(p, at.bh, row, at.split)) = float2{st.m, l};
+    } else {
+        const int t = row / p.G, hq = at.h * p.G + row % p.G;
+#pragma unroll
+        for (int m = 0; m < D / 32; ++m)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int d = 32 * m + 8 * r + 4 * hi;
+                kv8_store4(p, at.b, hq, t, d, float4_t{st.o[m][4 * r], st.o[m][4 * r + 1], st.o[m][4 * r + 2], st.o[m][4 * r + 3]}, l,
+                           kv8_gate4(p, at.b, hq, t, d));
+            }
     }
 }
 
@@ -767,11 +1119,11 @@ struct Kv8Plan {
     int nsplit;
 };
 // One tile of 16 rows where there are no more (and for listed blocks, one query's heads), else
-// workgroups of 64, or of 128 (256 at D = 256) rows.  items: blocks of the longest sequence, or of a list.
+// workgroups of 64 rows, or more at D = 64 of 128 and at D = 128 and 256 of 256.  items: blocks of the longest sequence, or of a list.
 inline Kv8Plan kv8_plan(int B, int T, int Hq, int Hkv, int D, int items, bool list) {
     const long long G = Hq / Hkv, rows = T * G;
     Kv8Plan q;
-    q.rows = list || rows <= 16 ? 16 : rows <= 64 ? 64 : D == 256 ? 256 : 128;
+    q.rows = list || rows <= 16 ? 16 : rows <= 64 ? 64 : D == 64 ? 128 : 256;
     q.tiles = list ? T * ((G + 15) / 16) : (rows + q.rows - 1) / q.rows;
     const long long all = q.tiles * B * Hkv;
     // row tiles: as many workgroups as the chip takes twice, not fewer than 4 blocks each; the others
@@ -794,10 +1146,13 @@ hipError_t kv8_attn_d(const Kv8AttnArgs& p, const Kv8Plan& q, hipStream_t stream
         hipLaunchKernelGGL((kv8_row_kernel<D, kList>), grid, dim3(256), 0, stream, p);
     } else {
         const dim3 grid((unsigned)((q.tiles * BH * p.nsplit + 7) / 8 * 8));
+        const int streams = BH * p.nsplit;
         if (q.rows == 64)
-            hipLaunchKernelGGL((kv8_tile_kernel<D, 1>), grid, dim3(Kv8Tile<D, 1>::kThreads), 0, stream, p, (int)q.tiles, BH * p.nsplit);
+            hipLaunchKernelGGL((kv8_tile_kernel<D, 1>), grid, dim3(256), 0, stream, p, (int)q.tiles, streams);
+        else if constexpr (D == 64)
+            hipLaunchKernelGGL((kv8_tile_kernel<D, 2>), grid, dim3(256), 0, stream, p, (int)q.tiles, streams);
         else
-            hipLaunchKernelGGL((kv8_tile_kernel<D, 2>), grid, dim3(Kv8Tile<D, 2>::kThreads), 0, stream, p, (int)q.tiles, BH * p.nsplit);
+            hipLaunchKernelGGL(kv8_wide_kernel<D>, grid, dim3(512), 0, stream, p, (int)q.tiles, streams);
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.nsplit == 1) return e;
