@@ -396,7 +396,7 @@ __device__ __forceinline__ half4_t kv8_gate4(const Kv8AttnArgs& p, int b, int hq
 }
 
 // Keys that a wave of the row kernel takes at a time, and their codes in registers.
-template <int D>
+template <int D, bool kOnce>
 struct Kv8Regs {
     static constexpr int kKeys = D == 256 ? 32 : 64, kN = kKeys * D / 1024;
     uint4 k[kN], v[kN];
@@ -405,40 +405,48 @@ struct Kv8Regs {
         const size_t head = (size_t)page * c.Hkv + h;
         const uint4* kp = reinterpret_cast<const uint4*>(c.k + head * (kKvBlock * D)) + part * (kN * 64) + (threadIdx.x & 63);
 #pragma unroll
-        for (int i = 0; i < kN; ++i) k[i] = kp[i * 64];
+        for (int i = 0; i < kN; ++i) k[i] = kv8_codes<kOnce>(kp + i * 64);
     }
     __device__ __forceinline__ void load_v(const Kv8& c, int page, int h, int part) {
         const size_t head = (size_t)page * c.Hkv + h;
         const uint4* vp = reinterpret_cast<const uint4*>(c.v + head * (kKvBlock * D)) + part * (kN * 64) + (threadIdx.x & 63);
 #pragma unroll
-        for (int i = 0; i < kN; ++i) v[i] = vp[i * 64];
+        for (int i = 0; i < kN; ++i) v[i] = kv8_codes<kOnce>(vp + i * 64);
     }
 };
 
-// Few rows: workgroup (tile, b Hkv + h, split), one tile of 16 query rows of a K/V head's group over
+// Few rows: a workgroup is one tile of a head and a split: one tile of 16 query rows of a K/V head's group over
 // the split's share of their blocks, the blocks dealt to the four waves in turn.  A wave's
 // next keys are on their way to registers as soon as its last ones have been multiplied, its next
 // values likewise.
 // kList: a tile is one query's heads (16 at a time) over its listed blocks; otherwise rows are
 // t G + g over all the sequence's blocks.
+// Listed: neighbouring queries share most of their blocks, so an eighth of all tiles in a row goes to
+// each XCD (workgroups go round them), whose L2 then serves the blocks again (700 queries of 16
+// blocks, 24/4 heads, D = 256: %%% us).
 template <int D, bool kList>
 __global__ void __launch_bounds__(256, 2)
-kv8_row_kernel(Kv8AttnArgs p) {
-    constexpr int kParts = kKvBlock / Kv8Regs<D>::kKeys, kRow = D + 4;
+kv8_row_kernel(Kv8AttnArgs p, int tiles) {
+    using Regs = Kv8Regs<D, !kList>;
+    constexpr int kParts = kKvBlock / Regs::kKeys, kRow = D + 4;
     __shared__ __align__(16) float acc[2][16][kRow];
     __shared__ float ml[4][2][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g4 = lane >> 4, n = lane & 15;
     const Kv8& c = p.c;
-    const int b = blockIdx.y / c.Hkv, h = blockIdx.y % c.Hkv, split = blockIdx.z;
+    int at = blockIdx.x;
+    if constexpr (kList) at = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
+    if (at >= tiles * c.B * c.Hkv * p.nsplit) return;
+    const int tile = at % tiles, bh = at / tiles % (c.B * c.Hkv), split = at / tiles / (c.B * c.Hkv);
+    const int b = bh / c.Hkv, h = bh % c.Hkv;
     const Kv8Seq sq = kv8_seq(c, p.len, p.n_new, b, p.T);
     int row0, row_end;
     if constexpr (kList) {
-        const int per = (p.G + 15) / 16, t = blockIdx.x / per;
-        row0 = t * p.G + blockIdx.x % per * 16;
+        const int per = (p.G + 15) / 16, t = tile / per;
+        row0 = t * p.G + tile % per * 16;
         row_end = (t + 1) * p.G;
     } else {
-        row0 = blockIdx.x * 16;
+        row0 = tile * 16;
         row_end = p.T * p.G;
     }
     row_end = min(row_end, (sq.n + sq.t0) * p.G);
@@ -463,7 +471,7 @@ kv8_row_kernel(Kv8AttnArgs p) {
     auto masked = [&](int k) { return (k + 1) * kKvBlock - 1 > least; };
     next();
     if (page >= 0) {
-        Kv8Regs<D> x;
+        Regs x;
         x.load_k(c, page, h, 0);
         x.load_v(c, page, h, 0);
         kv8_arrived<D, 1>(rows);
@@ -475,8 +483,8 @@ kv8_row_kernel(Kv8AttnArgs p) {
                 const bool last = part == kParts - 1;
                 if (last) next();
                 const int to = last ? page : here;
-                kv8_keys<D, 1, Kv8Regs<D>::kKeys / 16>(
-                    rows, now * kKvBlock + part * Kv8Regs<D>::kKeys, scale, masked(now),
+                kv8_keys<D, 1, Regs::kKeys / 16>(
+                    rows, now * kKvBlock + part * Regs::kKeys, scale, masked(now),
                     [&](int a, int i, int s) {
                         const uint4& k = x.k[a * (D / 64) + i];
                         return s ? kv8_halves(k.z, k.w) : kv8_halves(k.x, k.y);
@@ -529,8 +537,8 @@ kv8_row_kernel(Kv8AttnArgs p) {
         for (int w = 0; w < 4; ++w) l += ml[w][0][r] == m ? ml[w][1][r] : ml[w][1][r] * fast_exp2(ml[w][0][r] - m);
         const float4_t y = *reinterpret_cast<const float4_t*>(&acc[0][r][d]) + *reinterpret_cast<const float4_t*>(&acc[1][r][d]);
         if (p.nsplit > 1) {
-            if (l != 0.f) *reinterpret_cast<float4_t*>(kv8_part<D>(p, blockIdx.y, row0 + r, split) + d) = y;
-            if (d == 0) *reinterpret_cast<float2*>(kv8_pair<D>(p, blockIdx.y, row0 + r, split)) = float2{m, l};
+            if (l != 0.f) *reinterpret_cast<float4_t*>(kv8_part<D>(p, bh, row0 + r, split) + d) = y;
+            if (d == 0) *reinterpret_cast<float2*>(kv8_pair<D>(p, bh, row0 + r, split)) = float2{m, l};
         } else {
             const int t = (row0 + r) / p.G, hq = h * p.G + (row0 + r) % p.G;
             kv8_store4(p, b, hq, t, d, y, l, kv8_gate4(p, b, hq, t, d));
@@ -1142,8 +1150,8 @@ template <int D, bool kList>
 hipError_t kv8_attn_d(const Kv8AttnArgs& p, const Kv8Plan& q, hipStream_t stream) {
     const int BH = p.c.B * p.c.Hkv;
     if (kList || q.rows == 16) {
-        const dim3 grid((unsigned)q.tiles, (unsigned)BH, (unsigned)p.nsplit);
-        hipLaunchKernelGGL((kv8_row_kernel<D, kList>), grid, dim3(256), 0, stream, p);
+        const dim3 grid((unsigned)((q.tiles * BH * p.nsplit + 7) / 8 * 8));
+        hipLaunchKernelGGL((kv8_row_kernel<D, kList>), grid, dim3(256), 0, stream, p, (int)q.tiles);
     } else {
         const dim3 grid((unsigned)((q.tiles * BH * p.nsplit + 7) / 8 * 8));
         const int streams = BH * p.nsplit;
