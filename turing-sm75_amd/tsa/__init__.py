@@ -545,12 +545,13 @@ class Kv8Cache:
             torch.full((B, blocks), -1, dtype=torch.int32, device=device)
         self.B, self.Hkv, self.D, self.n_pages, self.max_blocks = B, Hkv, D, n_pages, blocks
         self.max_len = blocks * KV8_BLOCK
-        self.device = self.k.device
+        self.device, self.index, self.counts_shape = self.k.device, self.k.get_device(), (B,)
         self.view = TsaKv8(*(_ptr(getattr(self, n)) for n, _ in TsaKv8._fields_[:9]), B, Hkv, D, n_pages, blocks)
         self._ref = ctypes.byref(self.view)
 
 
-# a tsa_rows as bytes: data, strides of b, h and t
+# a tsa_rows as bytes: data, strides of b, h and t.  ctypes passes bytes as a pointer to them, so a
+# call's views need no object of their own.
 _ROWS = struct.Struct("@P3q")
 assert _ROWS.size == ctypes.sizeof(TsaRows)
 
@@ -561,42 +562,36 @@ def _rows(t, shape, name, cache):
     torch = _torch or _t()
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if t.dtype is not torch.float16 or t.device != cache.device or t.shape != shape or t.stride(3) != 1:
-        raise ValueError(f"{name}: expected fp16 {tuple(shape)} on {cache.device} with consecutive row elements, got "
-                         f"{tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}")
-    return _ROWS.pack(t.data_ptr(), *t.stride()[:3])
+    if t.dtype is torch.float16 and t.get_device() == cache.index and t.shape == shape:
+        b, h, r, d = t.stride()
+        if d == 1:
+            return _ROWS.pack(t.data_ptr(), b, h, r)
+    raise ValueError(f"{name}: expected fp16 {tuple(shape)} on {cache.device} with consecutive row elements, got "
+                     f"{tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}")
 
 
 def _counts(t, name, cache):
     torch = _torch or _t()
-    if t is None:
-        return None
-    if t.dtype is not torch.int32 or t.device != cache.device or t.shape != (cache.B,) or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.get_device() != cache.index or t.shape != cache.counts_shape or not t.is_contiguous():
         raise ValueError(f"{name}: expected a contiguous int32 tensor of {cache.B} on {cache.device}, got "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
     return t.data_ptr()
 
 
-class _on:
-    """The cache's device as the current one for the length of a call, where it is another."""
-
-    def __init__(self, device):
-        torch = _torch or _t()
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *a):
-        if self.guard is not None:
-            self.guard.__exit__(*a)
-
-
 def _len(t, cache):
-    if t is None:
+    if not isinstance(t, (_torch or _t()).Tensor):
         raise TypeError("len must be a torch.Tensor")
     return _counts(t, "len", cache)
+
+
+def _kv8_call(fn, cache, stream, *args):
+    """The entry point on the cache's device, made the current one for the call where it is another."""
+    torch = _torch or _t()
+    if torch._C._cuda_getDevice() == cache.index:
+        _check(fn(cache._ref, *args, torch._C._cuda_getCurrentRawStream(cache.index) if stream is None else stream.cuda_stream))
+    else:
+        with torch.cuda.device(cache.index):
+            _check(fn(cache._ref, *args, _stream(stream)))
 
 
 def kv8_write(cache, k, v, len, n_new=None, stream=None):
@@ -605,10 +600,8 @@ def kv8_write(cache, k, v, len, n_new=None, stream=None):
     says how many of the T rows are tokens, the rest is padding."""
     T = k.shape[2]
     shape = (cache.B, cache.Hkv, T, cache.D)
-    r = (TsaRows * 2).from_buffer(bytearray(_rows(k, shape, "k", cache) + _rows(v, shape, "v", cache)))
-    with _on(cache.device):
-        _check(load().tsa_kv8_write(cache._ref, ctypes.byref(r), ctypes.byref(r, 32), _len(len, cache),
-                                    _counts(n_new, "n_new", cache), T, _stream(stream)))
+    _kv8_call(load().tsa_kv8_write, cache, stream, _rows(k, shape, "k", cache), _rows(v, shape, "v", cache), _len(len, cache),
+              None if n_new is None else _counts(n_new, "n_new", cache), T)
 
 
 def kv8_read(cache, len, S=None, start=None, k_out=None, v_out=None, stream=None):
@@ -620,14 +613,19 @@ def kv8_read(cache, len, S=None, start=None, k_out=None, v_out=None, stream=None
         S = k_out.shape[2] if k_out is not None else v_out.shape[2] if v_out is not None else cache.max_len
     shape = (cache.B, cache.Hkv, S, cache.D)
     if k_out is None and v_out is None:
-        k_out, v_out = (torch.zeros(shape, dtype=torch.float16, device=cache.device) for _ in range(2))
-    packs = [None if t is None else _rows(t, shape, n, cache) for t, n in ((k_out, "k_out"), (v_out, "v_out"))]
-    r = (TsaRows * 2).from_buffer(bytearray(b"".join(p or bytes(32) for p in packs)))
-    with _on(cache.device):
-        _check(load().tsa_kv8_read(cache._ref, _len(len, cache), _counts(start, "start", cache), S,
-                                   ctypes.byref(r) if packs[0] else None, ctypes.byref(r, 32) if packs[1] else None,
-                                   _stream(stream)))
+        k_out, v_out = (_zeros(shape, cache, stream) for _ in range(2))
+    _kv8_call(load().tsa_kv8_read, cache, stream, _len(len, cache), None if start is None else _counts(start, "start", cache), S,
+              None if k_out is None else _rows(k_out, shape, "k_out", cache),
+              None if v_out is None else _rows(v_out, shape, "v_out", cache))
     return k_out, v_out
+
+
+def _zeros(shape, cache, stream, dtype=None, value=0):
+    """An output with a value where nothing will be written, filled on the stream that writes it."""
+    torch = _torch or _t()
+    s = torch.cuda.current_stream(cache.device) if stream is None else stream
+    with torch.cuda.stream(s):
+        return torch.full(shape, value, dtype=dtype or torch.float16, device=cache.device)
 
 
 def kv8_workspace_bytes(cache, T, Hq, max_len=None, top=0) -> int:
@@ -636,54 +634,50 @@ def kv8_workspace_bytes(cache, T, Hq, max_len=None, top=0) -> int:
     return int(load().tsa_kv8_workspace_bytes(cache._ref, T, Hq, cache.max_len if max_len is None else max_len, top))
 
 
-def _queries(q, cache, gate, out, extra):
+def _queries(q, cache, gate, out, n_new, stream):
     """Views of q, gate and out, the output, and Hq, T; made before anything is launched."""
-    torch = _torch or _t()
     if q.dim() != 4:
         raise ValueError(f"q: expected [B, Hq, T, D], got {tuple(q.shape)}")
-    shape = (cache.B, q.shape[1], q.shape[2], cache.D)
-    packed = _rows(q, shape, "q", cache)
-    if gate is not None:
-        packed += _rows(gate, shape, "gate", cache)
-    else:
-        packed += bytes(32)
+    _, Hq, T, _ = q.shape
+    shape = (cache.B, Hq, T, cache.D)
+    qp = _rows(q, shape, "q", cache)
+    gp = None if gate is None else _rows(gate, shape, "gate", cache)
     if out is None:
-        out = torch.zeros(shape, dtype=torch.float16, device=cache.device) if extra else \
-            torch.empty(shape, dtype=torch.float16, device=cache.device)
-    r = (TsaRows * 3).from_buffer(bytearray(packed + _rows(out, shape, "out", cache)))
-    return r, ctypes.byref(r, 32) if gate is not None else None, out, shape[1], shape[2]
+        out = _zeros(shape, cache, stream) if n_new is not None else \
+            (_torch or _t()).empty(shape, dtype=q.dtype, device=cache.device)
+    return qp, gp, _rows(out, shape, "out", cache), out, Hq, T
 
 
 def _ws(ws, cache, T, Hq, max_len, top, stream):
+    """Pointer and bytes of the caller's workspace, or of one for this call (and the tensor itself, to
+    be held until the call is made)."""
     if ws is None:
         ws = _scratch(kv8_workspace_bytes(cache, T, Hq, max_len, top), cache.device, stream)
-    elif ws.device != cache.device or not ws.is_contiguous():
+    elif ws.get_device() != cache.index or not ws.is_contiguous():
         raise ValueError(f"ws: expected a contiguous tensor on {cache.device}, got one on {ws.device}")
-    return ws
+    return ws.data_ptr(), ws.numel() * ws.element_size(), ws
 
 
 def attn_kv8_fwd(q, cache, len, n_new=None, gate=None, out=None, scale=None, causal=True, max_len=None, ws=None,
                  stream=None):
     """Attention of q [B, Hq, T, D], the last n_new tokens of each sequence (default T each), over the
     cache that holds them already: softmax(scale q K^T) V over the keys up to each query's own
-    (causal) or all len of them, times sigmoid(gate) if given.  Hq % Hkv == 0.  Rows of padding (t >= n_new) are left
-    as they were (0 in an output made here).  max_len: no sequence is longer (a tighter split of the
-    keys; results do not depend on it)."""
-    r, gp, out, Hq, T = _queries(q, cache, gate, out, n_new is not None)
+    (causal) or all len of them, times sigmoid(gate) if given.  Hq % Hkv == 0.  Rows of padding
+    (t >= n_new) are left as they were (0 in an output made here).  max_len: no sequence is longer (a
+    tighter split of the keys; results do not depend on it)."""
+    qp, gp, op, out, Hq, T = _queries(q, cache, gate, out, n_new, stream)
     if max_len is None:
         max_len = cache.max_len
-    with _on(cache.device):
-        ws = _ws(ws, cache, T, Hq, max_len, 0, stream)
-        _check(load().tsa_attn_kv8_fwd(
-            cache._ref, ctypes.byref(r), gp, ctypes.byref(r, 64), _len(len, cache), _counts(n_new, "n_new", cache), T, Hq,
-            max_len, 1.0 / math.sqrt(cache.D) if scale is None else float(scale), int(bool(causal)), _ptr(ws),
-            ws.numel() * ws.element_size(), _stream(stream)))
+    wp, wn, ws = _ws(ws, cache, T, Hq, max_len, 0, stream)
+    _kv8_call(load().tsa_attn_kv8_fwd, cache, stream, qp, gp, op, _len(len, cache),
+              None if n_new is None else _counts(n_new, "n_new", cache), T, Hq, max_len,
+              1.0 / math.sqrt(cache.D) if scale is None else float(scale), 1 if causal else 0, wp, wn)
     return out
 
 
 def _blocks(blocks, cache, T, top):
     torch = _torch or _t()
-    if blocks.dtype is not torch.int32 or blocks.device != cache.device or not blocks.is_contiguous() or \
+    if blocks.dtype is not torch.int32 or blocks.get_device() != cache.index or not blocks.is_contiguous() or \
             blocks.shape != (cache.B, cache.Hkv, T, top):
         raise ValueError(f"blocks: expected contiguous int32 {(cache.B, cache.Hkv, T, top)} on {cache.device}, got "
                          f"{tuple(blocks.shape)} {blocks.dtype} on {blocks.device}")
@@ -693,21 +687,21 @@ def _blocks(blocks, cache, T, top):
 def kv8_select(q, cache, len, top, n_new=None, first=1, recent=1, out=None, max_len=None, ws=None, stream=None):
     """The blocks [B, Hkv, T, top] int32 that each query of q [B, Hq, T, D] attends to: the first
     `first`, its own and the `recent` before it, and the best by score, ascending, -1 behind the last.
-    max_len: no sequence is longer (blocks behind it have no score)."""
+    Rows of padding are left as they were (-1 in an output made here).  max_len: no sequence is longer
+    (blocks behind it have no score)."""
     torch = _torch or _t()
     if q.dim() != 4:
         raise ValueError(f"q: expected [B, Hq, T, D], got {tuple(q.shape)}")
     _, Hq, T, _ = q.shape
-    r = TsaRows.from_buffer(bytearray(_rows(q, (cache.B, Hq, T, cache.D), "q", cache)))
+    qp = _rows(q, (cache.B, Hq, T, cache.D), "q", cache)
     if out is None:
-        out = torch.full((cache.B, cache.Hkv, T, top), -1, dtype=torch.int32, device=cache.device)
+        out = _zeros((cache.B, cache.Hkv, T, top), cache, stream, torch.int32, -1)
     if max_len is None:
         max_len = cache.max_len
-    with _on(cache.device):
-        ws = _ws(ws, cache, T, Hq, max_len, top, stream)
-        _check(load().tsa_kv8_select(
-            cache._ref, ctypes.byref(r), _len(len, cache), _counts(n_new, "n_new", cache), T, Hq, top, first, recent,
-            _blocks(out, cache, T, top), max_len, _ptr(ws), ws.numel() * ws.element_size(), _stream(stream)))
+    wp, wn, ws = _ws(ws, cache, T, Hq, max_len, top, stream)
+    _kv8_call(load().tsa_kv8_select, cache, stream, qp, _len(len, cache),
+              None if n_new is None else _counts(n_new, "n_new", cache), T, Hq, top, first, recent, _blocks(out, cache, T, top),
+              max_len, wp, wn)
     return out
 
 
@@ -715,12 +709,10 @@ def attn_kv8_blocks_fwd(q, cache, len, blocks, n_new=None, gate=None, out=None, 
     """attn_kv8_fwd (causal) over the listed blocks [B, Hkv, T, top] only (of kv8_select, or the
     caller's own: entries that are no block up to the query's own are passed over, a block listed
     twice counts twice)."""
-    r, gp, out, Hq, T = _queries(q, cache, gate, out, n_new is not None)
+    qp, gp, op, out, Hq, T = _queries(q, cache, gate, out, n_new, stream)
     top = blocks.shape[-1]
-    with _on(cache.device):
-        ws = _ws(ws, cache, T, Hq, 1, top, stream)
-        _check(load().tsa_attn_kv8_blocks_fwd(
-            cache._ref, ctypes.byref(r), gp, ctypes.byref(r, 64), _len(len, cache), _counts(n_new, "n_new", cache), T, Hq,
-            _blocks(blocks, cache, T, top), top, 1.0 / math.sqrt(cache.D) if scale is None else float(scale), _ptr(ws),
-            ws.numel() * ws.element_size(), _stream(stream)))
+    wp, wn, ws = _ws(ws, cache, T, Hq, 1, top, stream)
+    _kv8_call(load().tsa_attn_kv8_blocks_fwd, cache, stream, qp, gp, op, _len(len, cache),
+              None if n_new is None else _counts(n_new, "n_new", cache), T, Hq, _blocks(blocks, cache, T, top), top,
+              1.0 / math.sqrt(cache.D) if scale is None else float(scale), wp, wn)
     return out
