@@ -453,7 +453,8 @@ def as_lists(blocks):
 
 @pytest.mark.parametrize("D,G,T,top,first,recent", [(64, 1, 1, 4, 1, 1), (128, 6, 1, 7, 1, 2), (256, 6, 3, 16, 0, 0), (64, 20, 2, 3, 2, 0),
                                                     (128, 2, 40, 5, 1, 1), (256, 3, 1, 64, 1, 1), (64, 2, 70, 1, 0, 0),
-                                                    (64, 100, 1, 6, 1, 1), (128, 48, 3, 5, 0, 1), (64, 16, 5, 9, 1, 1)])
+                                                    (64, 100, 1, 6, 1, 1), (128, 48, 3, 5, 0, 1), (64, 16, 5, 9, 1, 1),
+                                                    (64, 2, 230, 3, 1, 1), (256, 3, 215, 5, 0, 1), (128, 17, 110, 4, 1, 0)])
 def test_select_and_attend(dev, D, G, T, top, first, recent):
     gen = torch.Generator().manual_seed(D + 7 * G + T + top)
     H = 2

@@ -61,10 +61,10 @@ struct Kv8Scale {
     float f, lsv, isv;
 };
 
-// The full blocks of a wave's work, in turn.  Each lane looks one of the next 64 items up (an entry
-// of the list, or the item itself; its page; its scales), so that a block's are lane reads and no
-// load waits for another once in 64 blocks.
-template <bool kList>
+// The full blocks of a wave's work, in turn.  Each lane looks one of the next 64 items up (part
+// item % kParts of a block: an entry of the list, or item / kParts itself; its page; its scales), so
+// that a block's are lane reads and no load waits for another but once in 64 items.
+template <bool kList, int kParts>
 struct Kv8Walk {
     int item, end, step;   // the next 64 are item + step * lane, below end
     int nb, n_full;        // blocks that are seen, and the full ones of them
@@ -75,8 +75,9 @@ struct Kv8Walk {
 
     __device__ __forceinline__ void look(const Kv8& c, int b, int h, const int* list, float c2) {
         const int i = item + step * (int)(threadIdx.x & 63);
-        blks = i < end ? (kList ? list[i] : i) : -1;
-        if (kList || n_full < nb) open += __popcll(__ballot(blks >= n_full && blks < nb));
+        blks = i < end ? (kList ? list[i / kParts] : i / kParts) : -1;
+        // the open block is taken whole, with its first part
+        if (kList || n_full < nb) open += __popcll(__ballot(blks >= n_full && blks < nb && i % kParts == 0));
         const bool is = blks >= 0 && blks < n_full;
         pages = is ? kv8_page(c, b, blks) : -1;
         const size_t head = (size_t)max(pages, 0) * c.Hkv + h;
@@ -86,13 +87,15 @@ struct Kv8Walk {
         item += 64 * step;
     }
     // The next block; false when there is none.
-    __device__ __forceinline__ bool next(const Kv8& c, int b, int h, const int* list, float c2, int& blk, int& page, Kv8Scale& sc) {
+    __device__ __forceinline__ bool next(const Kv8& c, int b, int h, const int* list, float c2, int& blk, int& part, int& page,
+                                         Kv8Scale& sc) {
         while (todo == 0) {
             if (item >= end) return false;
             look(c, b, h, list, c2);
         }
         const int l = __builtin_ctzll(todo);
         todo &= todo - 1;
+        part = (item - 64 * step + l * step) % kParts;
         auto read = [&](float x) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), l)); };
         blk = __builtin_amdgcn_readlane(blks, l);
         page = __builtin_amdgcn_readlane(pages, l);
@@ -415,27 +418,101 @@ struct Kv8Regs {
     }
 };
 
-// Few rows: a workgroup is one tile of a head and a split: one tile of 16 query rows of a K/V head's group over
-// the split's share of their blocks, the blocks dealt to the four waves in turn.  A wave's
-// next keys are on their way to registers as soon as its last ones have been multiplied, its next
-// values likewise.
+constexpr int kKvMaxSplits = 128;
+
+// Which tile, (sequence, head) and split a workgroup of the kernels below has.  Workgroups go round
+// the 8 XCDs.  The tiles of one (head, split) read the same keys: they go to one XCD, the last
+// (longest) tiles of its heads first, or where the heads and splits are no multiple of 8, each XCD
+// takes an eighth of all in a row.
+struct Kv8Place {
+    int tile, bh, b, h, split;
+    __device__ __forceinline__ bool find(const Kv8AttnArgs& p, int tiles, int streams) {
+        int stream, rank;
+        const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
+        if ((streams & 7) == 0) {
+            const int per = streams >> 3;
+            stream = xcd * per + slot % per;
+            rank = slot / per;
+        } else {
+            const int at = xcd * (int)(gridDim.x >> 3) + slot;
+            if (at >= streams * tiles) return false;
+            stream = at / tiles;
+            rank = at % tiles;
+        }
+        tile = tiles - 1 - rank;
+        bh = stream / p.nsplit;
+        split = stream % p.nsplit;
+        b = bh / p.c.Hkv;
+        h = bh % p.c.Hkv;
+        return true;
+    }
+};
+
+// The blocks of a split of a tile of rows [first, end): those that some row sees, shared out.
+struct Kv8Share {
+    int n_full;   // full blocks that are seen
+    bool open;    // the open block is this split's
+    Kv8Walk<false, 1> walk;
+    __device__ __forceinline__ void find(const Kv8AttnArgs& p, const Kv8Seq& sq, int last_row, int split) {
+        const int front = sq.len - (sq.n + sq.t0);  // position of row t = 0
+        const int all = p.causal ? min(front + last_row / p.G, sq.len - 1) : sq.len - 1;
+        const int nb = all < 0 ? 0 : all / kKvBlock + 1;
+        n_full = min(sq.len / kKvBlock, nb);
+        const int per = (nb + p.nsplit - 1) / p.nsplit, end = min(nb, (split + 1) * per);
+        open = split * per <= n_full && n_full < end;
+        walk = {split * per, min(end, n_full), 1, n_full, n_full, 0, 0};
+    }
+};
+
+// A wave's finished rows, or a split's sums of them.
+template <int D, int NT>
+__device__ __forceinline__ void kv8_finish(Kv8Rows<D> (&st)[NT], const Kv8AttnArgs& p, const Kv8Place& at, int row0, int row_end) {
+    const int lane = threadIdx.x & 63, g4 = lane >> 4;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const float l = sum_xor32(sum_xor16(st[nt].l));
+        const int row = row0 + 16 * nt + (lane & 15);
+        if (row >= row_end) continue;
+        if (p.nsplit > 1) {
+            if (l != 0.f) {
+                float* part = kv8_part<D>(p, at.bh, row, at.split) + 4 * g4;
+#pragma unroll
+                for (int dt = 0; dt < D / 16; ++dt) *reinterpret_cast<float4_t*>(part + 16 * dt) = st[nt].o[dt];
+            }
+            if (g4 == 0) *reinterpret_cast<float2*>(kv8_pair<D>(p, at.bh, row, at.split)) = float2{st[nt].m, l};
+        } else {
+            const int t = row / p.G, hq = at.h * p.G + row % p.G;
+#pragma unroll
+            for (int dt = 0; dt < D / 16; ++dt)
+                kv8_store4(p, at.b, hq, t, 16 * dt + 4 * g4, st[nt].o[dt], l, kv8_gate4(p, at.b, hq, t, 16 * dt + 4 * g4));
+        }
+    }
+}
+
+// Few rows: tiles of 16 query rows of a K/V head's group over one split of their blocks, a stage of
+// keys (half a block at D = 256, else a block) at a time.  A wave's next keys are on their way to
+// registers as soon as its last ones have been multiplied, its next values likewise.
+// kWaves = 4: a workgroup is one tile and split, the stages dealt to its waves in turn and their
+// sums joined; 1: a wave is a tile by itself, and nothing is joined.
 // kList: a tile is one query's heads (16 at a time) over its listed blocks; otherwise rows are
-// t G + g over all the sequence's blocks.
-// Listed: neighbouring queries share most of their blocks, so an eighth of all tiles in a row goes to
-// each XCD (workgroups go round them), whose L2 then serves the blocks again (700 queries of 16
-// blocks, 24/4 heads, D = 256: %%% us).
-template <int D, bool kList>
+// t G + g over all the sequence's blocks.  Neighbouring queries share most of their listed blocks:
+// an eighth of all tiles in a row goes to each XCD (workgroups go round them), whose L2 then serves
+// the blocks again (700 queries of 16 blocks, 24/4 heads, D = 256: 115 -> 109 us; a wave a tile 102).
+// Bound by memory with one query a sequence (32 of up to 32768 keys, D = 256: 283 us, 5.7 TB/s);
+// where queries share their blocks by the vector instructions that turn codes into fp16.
+template <int D, bool kList, int kWaves>
 __global__ void __launch_bounds__(256, 2)
 kv8_row_kernel(Kv8AttnArgs p, int tiles) {
     using Regs = Kv8Regs<D, !kList>;
     constexpr int kParts = kKvBlock / Regs::kKeys, kRow = D + 4;
-    __shared__ __align__(16) float acc[2][16][kRow];
+    __shared__ __align__(16) float acc[kWaves == 4 ? 2 : 1][kWaves == 4 ? 16 : 1][kRow];
     __shared__ float ml[4][2][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g4 = lane >> 4, n = lane & 15;
     const Kv8& c = p.c;
     int at = blockIdx.x;
     if constexpr (kList) at = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
+    if constexpr (kWaves == 1) at = 4 * at + wave;
     if (at >= tiles * c.B * c.Hkv * p.nsplit) return;
     const int tile = at % tiles, bh = at / tiles % (c.B * c.Hkv), split = at / tiles / (c.B * c.Hkv);
     const int b = bh / c.Hkv, h = bh % c.Hkv;
@@ -457,51 +534,49 @@ kv8_row_kernel(Kv8AttnArgs p, int tiles) {
     kv8_begin<D, 1>(rows, p, sq, b, h, row0, row_end, see, least);
     const int nb = see / kKvBlock + (see >= 0 ? 1 : 0);  // blocks that any row sees
     const int n_full = min(sq.len / kKvBlock, nb);
-    const int items = kList ? p.top : nb;
+    const int items = (kList ? p.top : nb) * kParts;
     const int per = (items + p.nsplit - 1) / p.nsplit;
     const int end = min(items, (split + 1) * per);
     const int* list = kList ? p.blocks + (((size_t)b * c.Hkv + h) * p.T + row0 / p.G) * p.top : nullptr;
-    Kv8Walk<kList> walk = {split * per + wave, end, 4, nb, n_full, 0, 0};
-    int blk = 0, page = -1;
+    Kv8Walk<kList, kParts> walk = {split * per + (kWaves == 4 ? wave : 0), end, kWaves, nb, n_full, 0, 0};
+    int blk = 0, part = 0, page = -1;
     Kv8Scale sc = {};
     auto next = [&]() {
-        if (!walk.next(c, b, h, list, p.c2, blk, page, sc)) page = -1;
+        if (!walk.next(c, b, h, list, p.c2, blk, part, page, sc)) page = -1;
     };
-    // rows of one query see whole blocks but the last; several queries' last one or two are masked
-    auto masked = [&](int k) { return (k + 1) * kKvBlock - 1 > least; };
     next();
     if (page >= 0) {
         Regs x;
-        x.load_k(c, page, h, 0);
-        x.load_v(c, page, h, 0);
+        x.load_k(c, page, h, part);
+        x.load_v(c, page, h, part);
         kv8_arrived<D, 1>(rows);
         while (page >= 0) {
-            const int now = blk, here = page;
+            // rows of one query see whole blocks but the last; several queries' last one or two are masked
+            const int p0 = blk * kKvBlock + part * Regs::kKeys;
             const Kv8Scale scale = sc;
-#pragma unroll
-            for (int part = 0; part < kParts; ++part) {
-                const bool last = part == kParts - 1;
-                if (last) next();
-                const int to = last ? page : here;
-                kv8_keys<D, 1, Regs::kKeys / 16>(
-                    rows, now * kKvBlock + part * Regs::kKeys, scale, masked(now),
-                    [&](int a, int i, int s) {
-                        const uint4& k = x.k[a * (D / 64) + i];
-                        return s ? kv8_halves(k.z, k.w) : kv8_halves(k.x, k.y);
-                    },
-                    [&](int s, int m, int o) {
-                        const uint4& v = x.v[s * (D / 32) + m];
-                        return o ? kv8_halves(v.z, v.w) : kv8_halves(v.x, v.y);
-                    },
-                    [&]() {
-                        if (to >= 0) x.load_k(c, to, h, last ? 0 : part + 1);
-                    });
-                if (to >= 0) x.load_v(c, to, h, last ? 0 : part + 1);
-            }
+            next();
+            kv8_keys<D, 1, Regs::kKeys / 16>(
+                rows, p0, scale, p0 + Regs::kKeys - 1 > least,
+                [&](int a, int i, int s) {
+                    const uint4& k = x.k[a * (D / 64) + i];
+                    return s ? kv8_halves(k.z, k.w) : kv8_halves(k.x, k.y);
+                },
+                [&](int s, int m, int o) {
+                    const uint4& v = x.v[s * (D / 32) + m];
+                    return o ? kv8_halves(v.z, v.w) : kv8_halves(v.x, v.y);
+                },
+                [&]() {
+                    if (page >= 0) x.load_k(c, page, h, part);
+                });
+            if (page >= 0) x.load_v(c, page, h, part);
         }
     }
     for (; walk.open > 0; --walk.open) kv8_open_block<D>(st, c, b, h, n_full, sq.len - n_full * kKvBlock, p.c2);
 
+    if constexpr (kWaves == 1) {
+        kv8_finish<D, 1>(rows, p, {tile, bh, b, h, split}, row0, row_end);
+        return;
+    }
     // the four waves' sums, relative to their common maximum
     st.l = sum_xor32(sum_xor16(st.l));
     if (g4 == 0) {
@@ -546,77 +621,6 @@ kv8_row_kernel(Kv8AttnArgs p, int tiles) {
     }
 }
 
-constexpr int kKvMaxSplits = 128;
-
-// Which tile, (sequence, head) and split a workgroup of the kernels below has.  Workgroups go round
-// the 8 XCDs.  The tiles of one (head, split) read the same keys: they go to one XCD, the last
-// (longest) tiles of its heads first, or where the heads and splits are no multiple of 8, each XCD
-// takes an eighth of all in a row.
-struct Kv8Place {
-    int tile, bh, b, h, split;
-    __device__ __forceinline__ bool find(const Kv8AttnArgs& p, int tiles, int streams) {
-        int stream, rank;
-        const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
-        if ((streams & 7) == 0) {
-            const int per = streams >> 3;
-            stream = xcd * per + slot % per;
-            rank = slot / per;
-        } else {
-            const int at = xcd * (int)(gridDim.x >> 3) + slot;
-            if (at >= streams * tiles) return false;
-            stream = at / tiles;
-            rank = at % tiles;
-        }
-        tile = tiles - 1 - rank;
-        bh = stream / p.nsplit;
-        split = stream % p.nsplit;
-        b = bh / p.c.Hkv;
-        h = bh % p.c.Hkv;
-        return true;
-    }
-};
-
-// The blocks of a split of a tile of rows [first, end): those that some row sees, shared out.
-struct Kv8Share {
-    int n_full;   // full blocks that are seen
-    bool open;    // the open block is this split's
-    Kv8Walk<false> walk;
-    __device__ __forceinline__ void find(const Kv8AttnArgs& p, const Kv8Seq& sq, int last_row, int split) {
-        const int front = sq.len - (sq.n + sq.t0);  // position of row t = 0
-        const int all = p.causal ? min(front + last_row / p.G, sq.len - 1) : sq.len - 1;
-        const int nb = all < 0 ? 0 : all / kKvBlock + 1;
-        n_full = min(sq.len / kKvBlock, nb);
-        const int per = (nb + p.nsplit - 1) / p.nsplit, end = min(nb, (split + 1) * per);
-        open = split * per <= n_full && n_full < end;
-        walk = {split * per, min(end, n_full), 1, n_full, n_full, 0, 0};
-    }
-};
-
-// A wave's finished rows, or a split's sums of them.
-template <int D, int NT>
-__device__ __forceinline__ void kv8_finish(Kv8Rows<D> (&st)[NT], const Kv8AttnArgs& p, const Kv8Place& at, int row0, int row_end) {
-    const int lane = threadIdx.x & 63, g4 = lane >> 4;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const float l = sum_xor32(sum_xor16(st[nt].l));
-        const int row = row0 + 16 * nt + (lane & 15);
-        if (row >= row_end) continue;
-        if (p.nsplit > 1) {
-            if (l != 0.f) {
-                float* part = kv8_part<D>(p, at.bh, row, at.split) + 4 * g4;
-#pragma unroll
-                for (int dt = 0; dt < D / 16; ++dt) *reinterpret_cast<float4_t*>(part + 16 * dt) = st[nt].o[dt];
-            }
-            if (g4 == 0) *reinterpret_cast<float2*>(kv8_pair<D>(p, at.bh, row, at.split)) = float2{st[nt].m, l};
-        } else {
-            const int t = row / p.G, hq = at.h * p.G + row % p.G;
-#pragma unroll
-            for (int dt = 0; dt < D / 16; ++dt)
-                kv8_store4(p, at.b, hq, t, 16 * dt + 4 * g4, st[nt].o[dt], l, kv8_gate4(p, at.b, hq, t, 16 * dt + 4 * g4));
-        }
-    }
-}
-
 // A stage of keys on its way from memory to LDS.
 struct Kv8Stage {
     int p0 = -1;  // first key, -1: none
@@ -631,16 +635,18 @@ __device__ __forceinline__ void kv8_step(Kv8Stage& s, Walk& walk, const Kv8& c, 
         ++s.part;
         return;
     }
-    int blk;
-    s.p0 = walk.next(c, b, h, nullptr, c2, blk, s.page, s.sc) ? blk * kKvBlock : -1;
+    int blk, part;
+    s.p0 = walk.next(c, b, h, nullptr, c2, blk, part, s.page, s.sc) ? blk * kKvBlock : -1;
     s.part = 0;
 }
 
 // More rows than a tile: a workgroup is 4 waves of 16 NT query rows each over one split of their
 // blocks.  A stage of kKeys keys and their values (16 KiB of codes at the most) goes from memory to
-// registers two stages ahead, is turned into fp16 operands once for all waves, and lies in one of
-// two LDS buffers in operand order, so every LDS access is 16 consecutive bytes a lane and a code
-// is converted once per 64 NT rows.  One barrier a stage.
+// registers, is turned into fp16 operands once for all waves, and lies in one of two LDS buffers in
+// operand order, so every LDS access is 16 consecutive bytes a lane and a code is converted once
+// per 64 NT rows.  One barrier a stage.  Two sets of registers are filled in turn, three stages
+// ahead of their use: 18 rows over 8 sequences of 16384, 24/4 heads, D = 256, need the bandwidth
+// (one set 68 us, two, past the caches, 65).
 template <int D, int NT>
 struct Kv8Tile {
     static constexpr int kKeys = D == 256 ? 32 : 64, kParts = kKvBlock / kKeys;
@@ -648,7 +654,8 @@ struct Kv8Tile {
     static constexpr int kN = kUnits / 256;        // of them a thread moves
     static constexpr int kRows = 64 * NT;
 };
-template <int D, int NT>
+// kOnce: a (sequence, head) is one tile.
+template <int D, int NT, bool kOnce>
 __global__ void __launch_bounds__(256, 2)
 kv8_tile_kernel(Kv8AttnArgs p, int tiles, int streams) {
     using C = Kv8Tile<D, NT>;
@@ -669,63 +676,76 @@ kv8_tile_kernel(Kv8AttnArgs p, int tiles, int streams) {
     Kv8Share share;
     share.find(p, sq, min(row_end, (at.tile + 1) * C::kRows) - 1, at.split);
 
-    uint4 rk[C::kN], rv[C::kN];
-    auto load = [&](const Kv8Stage& s) {
+    struct Set {
+        uint4 k[C::kN], v[C::kN];
+    } r[2];
+    auto load = [&](Set& x, const Kv8Stage& s) {
         if (s.p0 < 0) return;
         const size_t head = (size_t)s.page * c.Hkv + at.h;
         const uint4* kp = reinterpret_cast<const uint4*>(c.k + head * (kKvBlock * D)) + s.part * C::kUnits + tid;
         const uint4* vp = reinterpret_cast<const uint4*>(c.v + head * (kKvBlock * D)) + s.part * C::kUnits + tid;
 #pragma unroll
-        for (int x = 0; x < C::kN; ++x) rk[x] = kp[x * 256];
+        for (int i = 0; i < C::kN; ++i) x.k[i] = kv8_codes<kOnce>(kp + i * 256);
 #pragma unroll
-        for (int x = 0; x < C::kN; ++x) rv[x] = vp[x * 256];
+        for (int i = 0; i < C::kN; ++i) x.v[i] = kv8_codes<kOnce>(vp + i * 256);
     };
-    // Unit x of the registers (K's, then V's) to LDS as fp16.
-    auto store = [&](int to, int x) {
-        const bool isv = x >= C::kN;
-        const uint4& r = isv ? rv[x - C::kN] : rk[x];
-        half8_t* u = &buf[to][(isv ? 2 * C::kUnits : 0) + ((tid >> 6) + 4 * (isv ? x - C::kN : x)) * 128 + lane];
-        u[0] = kv8_halves(r.x, r.y);
-        u[64] = kv8_halves(r.z, r.w);
+    // Unit i of a set (K's, then V's) to LDS as fp16.
+    auto store = [&](int to, const Set& x, int i) {
+        const bool isv = i >= C::kN;
+        const uint4& y = isv ? x.v[i - C::kN] : x.k[i];
+        half8_t* u = &buf[to][(isv ? 2 * C::kUnits : 0) + ((tid >> 6) + 4 * (isv ? i - C::kN : i)) * 128 + lane];
+        u[0] = kv8_halves(y.x, y.y);
+        u[64] = kv8_halves(y.z, y.w);
     };
-    Kv8Stage now, then, after;
+    // The stages, `now` in buffer 0 and the next two in the sets.  One behind the last keeps its
+    // scales and has no key that a row sees.
+    constexpr int kNone = INT_MAX / 2;
+    Kv8Stage now, next[2];
     auto step = [&](Kv8Stage& s) { kv8_step<C::kParts>(s, share.walk, c, at.b, at.h, p.c2); };
     step(now);
-    load(now);
     if (now.p0 >= 0) {
+        load(r[0], now);
 #pragma unroll
-        for (int x = 0; x < 2 * C::kN; ++x) store(0, x);
-    }
-    then = now;
-    if (now.p0 >= 0) step(then);
-    load(then);
-    kv8_arrived<D, NT>(st);
-    lds_barrier();
-    for (int u = 0; now.p0 >= 0; u ^= 1) {
-        const half8_t* kb = &buf[u][lane];
-        float4_t w[NT][KA];
-        // The next stage's codes are converted among the products of K's operands, and the one after
-        // that is sent for behind them.  (Behind the last stage the registers hold old codes; what
-        // is written is not read.)  A wave that sees none of the stage's keys, on the diagonal, runs
-        // them masked: a branch round the products would cost it a copy of all its sums.
-        kv8_lds_scores<D, NT, KA, kAhead>(st, w, kb, [&](int e) {
-            constexpr int kEvery = KA * (D / 32) / (4 * C::kN);
-            if (e % kEvery == kEvery - 1 && e / kEvery < 2 * C::kN) store(u ^ 1, e / kEvery);
-        });
-        after = then;
-        if (then.p0 >= 0) step(after);
-        load(after);
-        half8_t wp[NT][KA / 2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            kv8_softmax<D, KA>(st[nt], w[nt], now.p0, now.sc, now.p0 + C::kKeys - 1 > least);
-#pragma unroll
-            for (int s = 0; s < KA / 2; ++s) wp[nt][s] = kv8_weights<KA>(w[nt], s);
-        }
-        kv8_lds_sums<D, NT, KA / 2, kAhead>(st, wp, kb + 2 * C::kUnits);
+        for (int i = 0; i < 2 * C::kN; ++i) store(0, r[0], i);
+        next[0] = now;
+        step(next[0]);
+        load(r[0], next[0]);
+        next[1] = next[0];
+        if (next[0].p0 >= 0) step(next[1]);
+        load(r[1], next[1]);
+        kv8_arrived<D, NT>(st);
         lds_barrier();
-        now = then;
-        then = after;
+        do {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {  // the stage in buffer u
+                const half8_t* kb = &buf[u][lane];
+                float4_t w[NT][KA];
+                // The next stage's codes are converted among the products of K's operands, and its
+                // set is filled again behind them.  (Behind the last stage the registers hold old
+                // codes; what is written is not seen.)  A wave that sees none of the stage's keys, on
+                // the diagonal, runs them masked: a branch round the products, or a way out of the
+                // loop between its halves, would cost it a copy of all its sums.
+                kv8_lds_scores<D, NT, KA, kAhead>(st, w, kb, [&](int e) {
+                    constexpr int kEvery = KA * (D / 32) / (4 * C::kN);
+                    if (e % kEvery == kEvery - 1 && e / kEvery < 2 * C::kN) store(u ^ 1, r[u], e / kEvery);
+                });
+                Kv8Stage after = next[u ^ 1];
+                if (after.p0 >= 0) step(after);
+                load(r[u], after);
+                const int p0 = now.p0 < 0 ? kNone : now.p0;
+                half8_t wp[NT][KA / 2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    kv8_softmax<D, KA>(st[nt], w[nt], p0, now.sc, p0 + C::kKeys - 1 > least);
+#pragma unroll
+                    for (int s = 0; s < KA / 2; ++s) wp[nt][s] = kv8_weights<KA>(w[nt], s);
+                }
+                kv8_lds_sums<D, NT, KA / 2, kAhead>(st, wp, kb + 2 * C::kUnits);
+                lds_barrier();
+                now = next[u];
+                next[u] = after;
+            }
+        } while (now.p0 >= 0);
     }
     if (share.open && see >= share.n_full * kKvBlock) {
 #pragma unroll
@@ -1120,6 +1140,10 @@ kv8_join_kernel(Kv8AttnArgs p) {
     kv8_store4(p, b, hq, t, 4 * x, y, l, gate);
 }
 
+// Listed tiles from which on a wave takes one by itself: as many as the chip has room for waves of
+// the kernel (fewer leave SIMDs empty, and a tile's four waves are joined instead).
+constexpr int kKvWaveTiles = 2048;
+
 // How a call's rows are cut into tiles and its keys into splits.
 struct Kv8Plan {
     int rows;       // of a tile
@@ -1131,13 +1155,14 @@ struct Kv8Plan {
 inline Kv8Plan kv8_plan(int B, int T, int Hq, int Hkv, int D, int items, bool list) {
     const long long G = Hq / Hkv, rows = T * G;
     Kv8Plan q;
-    q.rows = list || rows <= 16 ? 16 : rows <= 64 ? 64 : D == 64 ? 128 : 256;
+    q.rows = list || rows <= 16 ? 16 : rows <= (D == 64 ? 64 : 128) ? 64 : D == 64 ? 128 : 256;
     q.tiles = list ? T * ((G + 15) / 16) : (rows + q.rows - 1) / q.rows;
     const long long all = q.tiles * B * Hkv;
-    // row tiles: as many workgroups as the chip takes twice, not fewer than 4 blocks each; the others
-    // as many as it takes once
-    const long long want = q.rows == 16 ? (1024 + all - 1) / all : (q.rows == 256 ? 256 : 512) / all;
-    const long long most = (items + 3) / 4;
+    // row tiles: as many workgroups as the chip takes twice, but two stages of keys a wave at the
+    // least; the others as many as it takes once, but 4 blocks at the least
+    const bool few = q.rows == 16;
+    const long long want = few ? (1024 + all - 1) / all : (q.rows == 256 ? 256 : 512) / all;
+    const long long most = few ? ((long long)items * (D == 256 ? 2 : 1) + 7) / 8 : (items + 3) / 4;
     const long long n = want < most ? want : most;
     q.nsplit = (int)(n < 1 ? 1 : n < kKvMaxSplits ? n : kKvMaxSplits);
     return q;
@@ -1150,15 +1175,23 @@ template <int D, bool kList>
 hipError_t kv8_attn_d(const Kv8AttnArgs& p, const Kv8Plan& q, hipStream_t stream) {
     const int BH = p.c.B * p.c.Hkv;
     if (kList || q.rows == 16) {
-        const dim3 grid((unsigned)((q.tiles * BH * p.nsplit + 7) / 8 * 8));
-        hipLaunchKernelGGL((kv8_row_kernel<D, kList>), grid, dim3(256), 0, stream, p, (int)q.tiles);
+        const long long n = q.tiles * BH * p.nsplit;
+        if (kList && n >= kKvWaveTiles) {
+            const dim3 grid((unsigned)((n + 31) / 32 * 8));
+            hipLaunchKernelGGL((kv8_row_kernel<D, kList, 1>), grid, dim3(256), 0, stream, p, (int)q.tiles);
+        } else {
+            const dim3 grid((unsigned)((n + 7) / 8 * 8));
+            hipLaunchKernelGGL((kv8_row_kernel<D, kList, 4>), grid, dim3(256), 0, stream, p, (int)q.tiles);
+        }
     } else {
         const dim3 grid((unsigned)((q.tiles * BH * p.nsplit + 7) / 8 * 8));
         const int streams = BH * p.nsplit;
-        if (q.rows == 64)
-            hipLaunchKernelGGL((kv8_tile_kernel<D, 1>), grid, dim3(256), 0, stream, p, (int)q.tiles, streams);
+        if (q.rows == 64 && q.tiles == 1)
+            hipLaunchKernelGGL((kv8_tile_kernel<D, 1, true>), grid, dim3(256), 0, stream, p, (int)q.tiles, streams);
+        else if (q.rows == 64)
+            hipLaunchKernelGGL((kv8_tile_kernel<D, 1, false>), grid, dim3(256), 0, stream, p, (int)q.tiles, streams);
         else if constexpr (D == 64)
-            hipLaunchKernelGGL((kv8_tile_kernel<D, 2>), grid, dim3(256), 0, stream, p, (int)q.tiles, streams);
+            hipLaunchKernelGGL((kv8_tile_kernel<D, 2, false>), grid, dim3(256), 0, stream, p, (int)q.tiles, streams);
         else
             hipLaunchKernelGGL(kv8_wide_kernel<D>, grid, dim3(512), 0, stream, p, (int)q.tiles, streams);
     }

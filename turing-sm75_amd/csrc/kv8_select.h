@@ -60,24 +60,36 @@ kv8_score_kernel(Kv8SelectArgs p) {
     const half_t* q = p.q.data + b * p.q.b + (long long)h * p.G * p.q.h + (long long)t0 * p.q.t;
     if (tid < nt) most[tid] = 1;
     __syncthreads();
-    // max |q| of each query's group, as the bits of its fp16: infinities and NaN are at least 0x7c00
-    for (int i = tid; i < nt * p.G * (D / 8); i += 256) {
+    // max |q| of each query's group, as the bits of its fp16: infinities and NaN are at least 0x7c00.
+    // Up to 48 rows stay in registers for their codes.
+    constexpr int kHeld = kKvScoreCols * (D / 8) / 256 + (kKvScoreCols * (D / 8) % 256 ? 1 : 0);
+    half8_t held[kHeld];
+    auto load = [&](int i) {
         const int row = i / (D / 8);
-        const half8_t x = *reinterpret_cast<const half8_t*>(q + row / p.G * p.q.t + row % p.G * p.q.h + i % (D / 8) * 8);
+        return *reinterpret_cast<const half8_t*>(q + row / p.G * p.q.t + row % p.G * p.q.h + i % (D / 8) * 8);
+    };
+    const int parts8 = nt * p.G * (D / 8);  // of 8 elements
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) held[j] = tid + 256 * j < parts8 ? load(tid + 256 * j) : half8_t{};
+    auto raise = [&](int i, half8_t x) {
+        const int row = i / (D / 8);
         int a = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) a = max(a, (int)(__builtin_bit_cast(unsigned short, (half_t)x[j]) & 0x7fff));
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) a = max(a, __shfl_xor(a, o));  // 8 lanes are of one row
         if ((i & 7) == 0) atomicMax(&most[row / p.G], a);
-    }
+    };
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j)
+        if (tid + 256 * j < parts8) raise(tid + 256 * j, held[j]);
+    for (int i = tid + 256 * kHeld; i < parts8; i += 256) raise(i, load(i));
     int best = INT_MIN;  // one query of many heads: the maximum over its rounds
     for (int col0 = 0; col0 < nt * p.G; col0 += kKvScoreCols) {
         const int cols = min(kKvScoreCols, nt * p.G - col0);
         __syncthreads();
-        for (int i = tid; i < cols * (D / 8); i += 256) {
+        auto code = [&](int i, half8_t x) {
             const int col = i / (D / 8), row = col0 + col, big = most[row / p.G];
-            const half8_t x = *reinterpret_cast<const half8_t*>(q + row / p.G * p.q.t + row % p.G * p.q.h + i % (D / 8) * 8);
             // a group with an infinity or NaN has no order: all its codes are 0
             const float a = big < 0x7c00 ? (float)__builtin_bit_cast(half_t, (unsigned short)big) : 1.f, r = 1.f / a;
             unsigned y[8];
@@ -86,7 +98,10 @@ kv8_score_kernel(Kv8SelectArgs p) {
             // code + 128 to code: the other sign bit
             *reinterpret_cast<uint2*>(&qs[col * kRow + i % (D / 8) * 8]) =
                 uint2{kv8_pack(y[0], y[1], y[2], y[3]) ^ 0x80808080u, kv8_pack(y[4], y[5], y[6], y[7]) ^ 0x80808080u};
-        }
+        };
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j)
+            if (tid + 256 * j < cols * (D / 8)) code(tid + 256 * j, col0 ? load(tid + 256 * j + col0 * (D / 8)) : held[j]);
         __syncthreads();
         for (int ct = 0; 16 * ct < cols; ++ct) {
             int4_v acc[kWaveTiles] = {};
@@ -133,25 +148,25 @@ __device__ __forceinline__ unsigned kv8_order(float x) {
 }
 
 // Workgroup (t, b Hkv + h): the `top` best of the row's blocks, the lowest index first among
-// equals, listed ascending.  The last value that is kept is found bit by bit from the top, by
-// counting the values that are at least as large (ballots; one barrier a bit), and no further than
-// where exactly `top` are.  A thread holds kN values (blocks i kThreads + thread) in registers; with
-// more blocks it reads them again for each bit.
-constexpr int kKvPickN = 8;
-template <int kThreads>
+// equals, listed ascending.  The last value that is kept is found from the top, two bits at a time,
+// by counting the values that are at least as large (ballots; one barrier a round), and no further
+// than where exactly `top` are.  A thread holds kN values (blocks i kThreads + thread) in registers; with
+// more blocks it reads them again in each round.
+template <int kThreads, int kN>
 __global__ void __launch_bounds__(kThreads)
 kv8_pick_kernel(Kv8SelectArgs p) {
-    constexpr int kWaves = kThreads / 64, kHeld = kKvPickN * kThreads;
-    __shared__ int count[2][kWaves];
+    constexpr int kWaves = kThreads / 64, kHeld = kN * kThreads;
+    __shared__ int count[3][3];  // of three rounds in turn: one's, the next one's being cleared
     __shared__ int sums[2][kWaves];
     const int b = blockIdx.y / p.c.Hkv, t = blockIdx.x, tid = threadIdx.x, wave = tid >> 6;
     const size_t row = (size_t)blockIdx.y * p.T + t;
     const float* score = p.score + row * p.nb;
-    float held[kKvPickN];
+    float held[kN];
 #pragma unroll
-    for (int j = 0; j < kKvPickN; ++j) held[j] = score[min(j * kThreads + tid, p.nb - 1)];
+    for (int j = 0; j < kN; ++j) held[j] = score[min(j * kThreads + tid, p.nb - 1)];
     const Kv8Seq sq = kv8_seq(p.c, p.len, p.n_new, b, p.T);
     if (t >= sq.n + sq.t0) return;
+    if (tid < 9) count[tid / 3][tid % 3] = 0;
     const int pos = sq.len - (sq.n + sq.t0) + t;
     int* out = p.blocks + row * p.top;
     const int n = pos < 0 ? 0 : pos / kKvBlock + 1;
@@ -163,37 +178,53 @@ kv8_pick_kernel(Kv8SelectArgs p) {
     auto order = [&](int i, float x) {
         return i < p.first || i >= n - 1 - p.recent ? 0xffffffffu : i < p.nb ? kv8_order(x) : 0u;
     };
-    unsigned u[kKvPickN];
+    unsigned u[kN];
 #pragma unroll
-    for (int j = 0; j < kKvPickN; ++j) u[j] = j * kThreads + tid < n ? order(j * kThreads + tid, held[j]) : 0u;
-    auto at_least = [&](unsigned v, int slot) {  // v > 0
-        int x = 0;
+    for (int j = 0; j < kN; ++j) u[j] = j * kThreads + tid < n ? order(j * kThreads + tid, held[j]) : 0u;
+    // how many values are at least v[0], v[1], v[2] (all above 0)
+    auto at_least = [&](const unsigned (&v)[3], int (&x)[3], int slot) {
+        x[0] = x[1] = x[2] = 0;
+        auto add = [&](unsigned y) {
 #pragma unroll
-        for (int j = 0; j < kKvPickN; ++j) x += __popcll(__ballot(u[j] >= v));
+            for (int k = 0; k < 3; ++k) x[k] += __popcll(__ballot(y >= v[k]));
+        };
+#pragma unroll
+        for (int j = 0; j < kN; ++j) add(u[j]);
         for (int i0 = kHeld; i0 < n; i0 += kThreads) {
             const int i = i0 + tid;
-            x += __popcll(__ballot(i < n && order(i, i < p.nb ? score[i] : 0.f) >= v));
+            add(i < n ? order(i, i < p.nb ? score[i] : 0.f) : 0u);
         }
-        if ((tid & 63) == 0) count[slot][wave] = x;
-        __syncthreads();
-        x = 0;
+        if constexpr (kWaves > 1) {
+            // a round's counts were last read two barriers before they are cleared
+            if ((tid & 63) < 3) atomicAdd(&count[slot][tid & 63], (tid & 63) == 0 ? x[0] : (tid & 63) == 1 ? x[1] : x[2]);
+            if (tid >= 64 && tid < 67) count[(slot + 1) % 3][tid - 64] = 0;
+            __syncthreads();
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) x += count[slot][w];
-        return x;
+            for (int k = 0; k < 3; ++k) x[k] = count[slot][k];
+        }
     };
     unsigned value = 0;  // at least `top` values are at least this
-    int have = n;
-    for (int bit = 31; bit >= 0 && have != p.top; --bit) {
-        const unsigned v = value | 1u << bit;
-        const int x = at_least(v, bit & 1);
-        if (x >= p.top) {
-            value = v;
-            have = x;
-        }
+    int have = n, slot = 0;
+    __syncthreads();
+    for (int bit = 30; bit >= 0 && have != p.top; bit -= 2, slot = (slot + 1) % 3) {
+        const unsigned v[3] = {value | 1u << bit, value | 2u << bit, value | 3u << bit};
+        int x[3];
+        at_least(v, x, slot);
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+            if (x[k] >= p.top) {
+                value = v[k];
+                have = x[k];
+            }
     }
     // where more than `top` are: those above `value`, and the first of the others
-    const bool all = have == p.top;
-    const int left = all ? n : p.top - (value == 0xffffffffu ? 0 : at_least(value + 1, 1));
+    int left = n;
+    if (have != p.top) {
+        const unsigned v[3] = {value + 1, value + 1, value + 1};
+        int x[3] = {0, 0, 0};
+        if (value != 0xffffffffu) at_least(v, x, slot);
+        left = p.top - x[0];
+    }
     int done = 0, equal = 0;
     auto emit = [&](int i, unsigned x) {
         const bool eq = i < n && x == value;
@@ -217,7 +248,7 @@ kv8_pick_kernel(Kv8SelectArgs p) {
         }
     };
 #pragma unroll
-    for (int j = 0; j < kKvPickN; ++j)
+    for (int j = 0; j < kN; ++j)
         if (j * kThreads < n) emit(j * kThreads + tid, u[j]);
     for (int i0 = kHeld; i0 < n; i0 += kThreads) {
         const int i = i0 + tid;
@@ -234,14 +265,15 @@ hipError_t kv8_select_d(const Kv8SelectArgs& p, hipStream_t stream) {
     hipLaunchKernelGGL(kv8_score_kernel<D>, grid, dim3(256), 0, stream, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    // one wave a row where its registers hold the row's scores, else 16
+    // one wave a row where its registers hold the row's scores, else 16 (32 rows of 2048 scores: 4
+    // waves of 8 values a thread 11.9 us, 16 of 2 10.6)
     const dim3 rows((unsigned)p.T, (unsigned)(p.c.B * p.c.Hkv));
-    if (p.nb <= kKvPickN * 64)
-        hipLaunchKernelGGL(kv8_pick_kernel<64>, rows, dim3(64), 0, stream, p);
-    else if (p.nb <= kKvPickN * 256)
-        hipLaunchKernelGGL(kv8_pick_kernel<256>, rows, dim3(256), 0, stream, p);
+    if (p.nb <= 512)
+        hipLaunchKernelGGL((kv8_pick_kernel<64, 8>), rows, dim3(64), 0, stream, p);
+    else if (p.nb <= 2048)
+        hipLaunchKernelGGL((kv8_pick_kernel<1024, 2>), rows, dim3(1024), 0, stream, p);
     else
-        hipLaunchKernelGGL(kv8_pick_kernel<1024>, rows, dim3(1024), 0, stream, p);
+        hipLaunchKernelGGL((kv8_pick_kernel<1024, 8>), rows, dim3(1024), 0, stream, p);
     return hipGetLastError();
 }
 
