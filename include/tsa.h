@@ -307,7 +307,7 @@ int tsa_kv8_write(const tsa_kv8* cache, const tsa_rows* k, const tsa_rows* v, co
                   const int32_t* n_new, int T, void* stream);
 
 /* Reads positions start .. start + S - 1 of each sequence back as fp16 (start: int32 [B] on the
- * device, NULL for 0; k, v [B][Hkv][S][D], either may be NULL).  Rows of positions behind the
+ * device, at least 0, NULL for 0; k, v [B][Hkv][S][D], either may be NULL).  Rows of positions behind the
  * sequence or without a page are left as they were. */
 int tsa_kv8_read(const tsa_kv8* cache, const int32_t* len, const int32_t* start, int S, const tsa_rows* k,
                  const tsa_rows* v, void* stream);
@@ -333,7 +333,7 @@ int tsa_attn_kv8_fwd(const tsa_kv8* cache, const tsa_rows* q, const tsa_rows* ga
  * sum_d qc[d] k_sum[d], a whole number, times k_sum_scale (one fp32 product).  A query at position
  * p keeps, of the blocks 0 .. p / 64: the first `first`, its own and the `recent` before it, and
  * then the best scores, the lowest index first among equals, up to `top` in all
- * (top >= first + recent + 1).  A full block that holds an infinity or NaN, or has no page, scores
+ * (first + recent + 1 <= top <= 2^24).  A full block that holds an infinity or NaN, or has no page, scores
  * below every other; a group with an infinity or NaN scores every block 0.
  * blocks: int32 [B][Hkv][T][top], ascending, -1 behind the last; rows of padding are left as they
  * were.  Blocks behind max_len have no score. */

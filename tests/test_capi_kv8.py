@@ -100,6 +100,8 @@ def test_sizes():
     assert select(max_len=0) == tsa.TSA_ERR_SHAPE
     assert select(top=0) == tsa.TSA_ERR_SHAPE
     assert sparse(top=0) == tsa.TSA_ERR_SHAPE
+    assert select(top=(1 << 24) + 1) == tsa.TSA_ERR_SHAPE
+    assert sparse(top=(1 << 31) - 1) == tsa.TSA_ERR_SHAPE
     assert select(first=-1) == tsa.TSA_ERR_SHAPE
 
 

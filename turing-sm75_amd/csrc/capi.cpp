@@ -373,6 +373,9 @@ int check_kv8_queries(const tsa_kv8* c, int T, int Hq) {
     return TSA_OK;
 }
 
+// Entries of a list: the kernels count parts of blocks in ints.
+bool fits_top(int top) { return top >= 1 && top <= 1 << 24; }
+
 int kv8_nb(const tsa_kv8* c, int max_len) {
     const int nb = (int)((max_len + 63LL) / 64);
     return nb < c->max_blocks ? nb : c->max_blocks;
@@ -416,7 +419,7 @@ extern "C" int tsa_kv8_read(const tsa_kv8* cache, const int32_t* len, const int3
 }
 
 extern "C" size_t tsa_kv8_workspace_bytes(const tsa_kv8* cache, int T, int Hq, int max_len, int top) {
-    if (check_kv8(cache) || check_kv8_queries(cache, T, Hq) || max_len < 1 || top < 0) return 0;
+    if (check_kv8(cache) || check_kv8_queries(cache, T, Hq) || max_len < 1 || (top != 0 && !fits_top(top))) return 0;
     return tsa::kv8_ws_bytes(cache->B, T, Hq, cache->Hkv, cache->D, kv8_nb(cache, max_len), top);
 }
 
@@ -441,7 +444,7 @@ extern "C" int tsa_kv8_select(const tsa_kv8* cache, const tsa_rows* q, const int
     if (rc) return rc;
     if (!len || !blocks) return TSA_ERR_NULL;
     if ((rc = check_kv8_queries(cache, T, Hq))) return rc;
-    if (max_len < 1 || top < 1 || first < 0 || recent < 0) return TSA_ERR_SHAPE;
+    if (max_len < 1 || !fits_top(top) || first < 0 || recent < 0) return TSA_ERR_SHAPE;
     if ((long long)first + recent + 1 > top) return TSA_ERR_ARG;
     const int B = cache->B, nb = kv8_nb(cache, max_len);
     if ((rc = check_rows(q, B, Hq, T, false))) return rc;
@@ -457,7 +460,7 @@ extern "C" int tsa_attn_kv8_blocks_fwd(const tsa_kv8* cache, const tsa_rows* q, 
     const int rc = check_kv8_attn(cache, q, gate, o, len, T, Hq, scale);
     if (rc) return rc;
     if (!blocks) return TSA_ERR_NULL;
-    if (top < 1) return TSA_ERR_SHAPE;
+    if (!fits_top(top)) return TSA_ERR_SHAPE;
     const int B = cache->B;
     const size_t need = tsa::kv8_ws_bytes(B, T, Hq, cache->Hkv, cache->D, 1, top);
     if (need && (!ws || ws_bytes < need)) return TSA_ERR_WORKSPACE;

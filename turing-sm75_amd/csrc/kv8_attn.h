@@ -1176,10 +1176,14 @@ hipError_t kv8_attn_d(const Kv8AttnArgs& p, const Kv8Plan& q, hipStream_t stream
     const int BH = p.c.B * p.c.Hkv;
     if (kList || q.rows == 16) {
         const long long n = q.tiles * BH * p.nsplit;
-        if (kList && n >= kKvWaveTiles) {
-            const dim3 grid((unsigned)((n + 31) / 32 * 8));
-            hipLaunchKernelGGL((kv8_row_kernel<D, kList, 1>), grid, dim3(256), 0, stream, p, (int)q.tiles);
-        } else {
+        bool wave = false;
+        if constexpr (kList) {
+            if ((wave = n >= kKvWaveTiles)) {
+                const dim3 grid((unsigned)((n + 31) / 32 * 8));
+                hipLaunchKernelGGL((kv8_row_kernel<D, true, 1>), grid, dim3(256), 0, stream, p, (int)q.tiles);
+            }
+        }
+        if (!wave) {
             const dim3 grid((unsigned)((n + 7) / 8 * 8));
             hipLaunchKernelGGL((kv8_row_kernel<D, kList, 4>), grid, dim3(256), 0, stream, p, (int)q.tiles);
         }
