@@ -96,6 +96,7 @@ def test_sizes():
         assert call(Hq=0) == tsa.TSA_ERR_SHAPE
         assert call(Hq=3) == tsa.TSA_ERR_SHAPE  # no multiple of the K/V heads
         assert call(T=1 << 30) == tsa.TSA_ERR_SHAPE
+        assert call(cache(B=1, Hkv=1), T=1, Hq=65537) == tsa.TSA_ERR_SHAPE
     assert attn(max_len=0) == tsa.TSA_ERR_SHAPE
     assert select(max_len=0) == tsa.TSA_ERR_SHAPE
     assert select(top=0) == tsa.TSA_ERR_SHAPE
@@ -126,6 +127,9 @@ def test_workspace():
     assert top >= 4 << 14  # a score for each block
     assert select(c, T=1, Hq=8, max_len=1 << 20, top=64, ws_bytes=top - 1) == tsa.TSA_ERR_WORKSPACE
     assert sparse(c, T=1, Hq=8, top=64, ws=None) == tsa.TSA_ERR_WORKSPACE
+    assert attn(c, T=1, Hq=8, max_len=1 << 20, ws=P + 8, ws_bytes=need) == tsa.TSA_ERR_ARG
+    assert select(c, T=1, Hq=8, max_len=1 << 20, top=64, ws=P + 4, ws_bytes=top) == tsa.TSA_ERR_ARG
+    assert sparse(c, T=1, Hq=8, top=64, ws=P + 8) == tsa.TSA_ERR_ARG
     for bad in (dict(T=0), dict(Hq=0), dict(max_len=0), dict(top=-1)):
         a = dict(T=1, Hq=8, max_len=64, top=0)
         a.update(bad)

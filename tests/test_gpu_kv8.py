@@ -414,6 +414,47 @@ def test_not_finite_behind_the_mask(dev, T):
                         assert bool(o[:, :, t].isnan().all()), (where, what, side, t)
 
 
+@pytest.mark.parametrize("D,T", [(128, 30), (128, 150), (256, 50), (256, 150)])
+def test_not_finite_behind_the_mask_of_many_rows(dev, D, T):
+    """The same for two heads of T tokens, whose rows share tiles with rows that see the bad key: an open
+    key's infinity and NaN, and a full block that holds one."""
+    gen = torch.Generator().manual_seed(D + T)
+    L = 64 * 3 + 40
+    for where, what, side in ((L - 3, math.nan, "k"), (L - 3, math.nan, "v"), (L - 3, -math.inf, "v"), (190, math.inf, "k"), (190, math.nan, "v")):
+        k, v = keys(gen, 1, 1, L, D)
+        q = rand(gen, 1, 2, T, D)
+        x = k if side == "k" else v
+        x[0, 0, where, 5] = what
+        o = tsa.attn_kv8_fwd(q.to(dev), fill(dev, k, v, [L]), ints([L], dev)).cpu()
+        first = where if where >= 192 else 128
+        x[0, 0, where, 5] = 0
+        if where < 192:
+            x[0, 0, 128:192] = 0
+        want, tol = expect(q, k, v, [L], [T], True)
+        clean = max(0, min(T, first - (L - T)))  # queries in front of the first bad key
+        check_out(o[:, :, :clean], want[:, :, :clean], tol[:, :, :clean], (where, what, side))
+        bad = o[:, :, clean:]
+        if side == "v" and where >= 192:
+            assert bool((bad[..., 5].isnan() if what != what else bad[..., 5] == what).all()), (where, what)
+            for d in (4, 6):
+                check_out(bad[..., d], want[:, :, clean:, d], tol[:, :, clean:, d], (where, what, d))
+        else:
+            assert bool(bad.isnan().all()), (where, what, side)
+
+
+@pytest.mark.parametrize("D,G,T", [(64, 2, 4), (64, 1, 100), (128, 1, 40), (128, 2, 140), (256, 1, 3), (256, 2, 140)])
+def test_scores_that_underflow(dev, D, G, T):
+    """A scale so small that its product with a block's step is 0: every key that a query sees weighs
+    the same, and one that it does not see nothing."""
+    gen = torch.Generator().manual_seed(D + T)
+    L = 64 * 3 + 30
+    k, v = rand(gen, 1, 1, L, D) * 2.0 ** -20, rand(gen, 1, 1, L, D)
+    c = fill(dev, k, v, [L])
+    q = rand(gen, 1, G, T, D)
+    want, tol = expect(q, k, v, [L], [T], True, scale=1e-40)
+    check_out(tsa.attn_kv8_fwd(q.to(dev), c, ints([L], dev), scale=1e-40).cpu(), want, tol, (D, G, T))
+
+
 def test_garbage_behind_the_sequence(dev):
     """What the ring and pages hold behind a sequence (here NaN) is not looked at."""
     gen = torch.Generator().manual_seed(25)

@@ -65,7 +65,7 @@ extern "C" const char* tsa_strerror(int code) {
         case TSA_ERR_UNSUPPORTED: return "shape not supported by this library (attention: D in {64,128,256}; GDN: dk = dv = 128, chunk = 64)";
         case TSA_ERR_WORKSPACE: return "workspace is NULL or smaller than the required size";
         case TSA_ERR_LAUNCH: return "the HIP runtime rejected a kernel launch";
-        case TSA_ERR_ARG: return "invalid argument (causal not 0/1, scale not finite / not > 0, eps not finite / not > 0, 8-bit cache: misaligned rows, or top < first + recent + 1)";
+        case TSA_ERR_ARG: return "invalid argument (causal not 0/1, scale not finite / not > 0, eps not finite / not > 0, 8-bit cache: a misaligned buffer, or top < first + recent + 1)";
         case TSA_ERR_SCRATCH: return "the shapes need more than the 64 MiB device scratch of tsa_gdn_chunked_fwd_noalloc (use tsa_gdn_chunked_fwd with a workspace)";
         default: return "unknown tsa error code";
     }
@@ -366,15 +366,20 @@ tsa::Rows16 as_rows(const tsa_rows* r, int B, int H, int T) {
     return {static_cast<_Float16*>(r->data), B > 1 ? r->stride_b : 0, H > 1 ? r->stride_h : 0, T > 1 ? r->stride_t : 0};
 }
 
-// Queries: rows per K/V head and workgroups must fit an int.
+// Queries: rows per K/V head and workgroups must fit an int, and a group's elements too.
 int check_kv8_queries(const tsa_kv8* c, int T, int Hq) {
-    if (T < 1 || Hq < 1 || Hq % c->Hkv != 0) return TSA_ERR_SHAPE;
+    if (T < 1 || Hq < 1 || Hq % c->Hkv != 0 || Hq / c->Hkv > 65536) return TSA_ERR_SHAPE;
     if (!fits_int(c->B, Hq, T) || !fits_int(T, c->max_blocks)) return TSA_ERR_SHAPE;
     return TSA_OK;
 }
 
 // Entries of a list: the kernels count parts of blocks in ints.
 bool fits_top(int top) { return top >= 1 && top <= 1 << 24; }
+
+int check_ws(const void* ws, size_t ws_bytes, size_t need) {
+    if (need && (!ws || ws_bytes < need)) return TSA_ERR_WORKSPACE;
+    return need && !aligned16(ws) ? TSA_ERR_ARG : TSA_OK;
+}
 
 int kv8_nb(const tsa_kv8* c, int max_len) {
     const int nb = (int)((max_len + 63LL) / 64);
@@ -426,13 +431,13 @@ extern "C" size_t tsa_kv8_workspace_bytes(const tsa_kv8* cache, int T, int Hq, i
 extern "C" int tsa_attn_kv8_fwd(const tsa_kv8* cache, const tsa_rows* q, const tsa_rows* gate, const tsa_rows* o,
                                 const int32_t* len, const int32_t* n_new, int T, int Hq, int max_len, float scale,
                                 int causal, void* ws, size_t ws_bytes, void* stream) {
-    const int rc = check_kv8_attn(cache, q, gate, o, len, T, Hq, scale);
+    int rc = check_kv8_attn(cache, q, gate, o, len, T, Hq, scale);
     if (rc) return rc;
     if (max_len < 1) return TSA_ERR_SHAPE;
     if (causal != 0 && causal != 1) return TSA_ERR_ARG;
     const int B = cache->B, nb = kv8_nb(cache, max_len);
     const size_t need = tsa::kv8_ws_bytes(B, T, Hq, cache->Hkv, cache->D, nb, 0);
-    if (need && (!ws || ws_bytes < need)) return TSA_ERR_WORKSPACE;
+    if ((rc = check_ws(ws, ws_bytes, need))) return rc;
     return from_hip(tsa::kv8_attn(as_kv8(cache), as_rows(q, B, Hq, T), as_rows(gate, B, Hq, T), as_rows(o, B, Hq, T), len,
                                   n_new, T, Hq, nb, scale, causal, ws, as_stream(stream)));
 }
@@ -449,7 +454,7 @@ extern "C" int tsa_kv8_select(const tsa_kv8* cache, const tsa_rows* q, const int
     const int B = cache->B, nb = kv8_nb(cache, max_len);
     if ((rc = check_rows(q, B, Hq, T, false))) return rc;
     const size_t need = tsa::kv8_ws_bytes(B, T, Hq, cache->Hkv, cache->D, nb, top);
-    if (need && (!ws || ws_bytes < need)) return TSA_ERR_WORKSPACE;
+    if ((rc = check_ws(ws, ws_bytes, need))) return rc;
     return from_hip(tsa::kv8_select(as_kv8(cache), as_rows(q, B, Hq, T), len, n_new, T, Hq, top, first, recent, blocks, nb,
                                     ws, as_stream(stream)));
 }
@@ -457,13 +462,13 @@ extern "C" int tsa_kv8_select(const tsa_kv8* cache, const tsa_rows* q, const int
 extern "C" int tsa_attn_kv8_blocks_fwd(const tsa_kv8* cache, const tsa_rows* q, const tsa_rows* gate, const tsa_rows* o,
                                        const int32_t* len, const int32_t* n_new, int T, int Hq, const int32_t* blocks,
                                        int top, float scale, void* ws, size_t ws_bytes, void* stream) {
-    const int rc = check_kv8_attn(cache, q, gate, o, len, T, Hq, scale);
+    int rc = check_kv8_attn(cache, q, gate, o, len, T, Hq, scale);
     if (rc) return rc;
     if (!blocks) return TSA_ERR_NULL;
     if (!fits_top(top)) return TSA_ERR_SHAPE;
     const int B = cache->B;
     const size_t need = tsa::kv8_ws_bytes(B, T, Hq, cache->Hkv, cache->D, 1, top);
-    if (need && (!ws || ws_bytes < need)) return TSA_ERR_WORKSPACE;
+    if ((rc = check_ws(ws, ws_bytes, need))) return rc;
     return from_hip(tsa::kv8_attn_blocks(as_kv8(cache), as_rows(q, B, Hq, T), as_rows(gate, B, Hq, T), as_rows(o, B, Hq, T),
                                          len, n_new, T, Hq, blocks, top, scale, ws, as_stream(stream)));
 }

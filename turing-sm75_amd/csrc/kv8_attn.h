@@ -136,7 +136,7 @@ __device__ __forceinline__ void kv8_softmax(Kv8Rows<D>& st, float4_t (&w)[KA], i
     for (int a = 0; a < KA; ++a)
 #pragma unroll
         for (int r = 0; r < 4; ++r) w[a][r] = fast_exp2(__builtin_fmaf(w[a][r], sc.f, c));
-    if (masked && !(sc.f == sc.f && sc.lsv == sc.lsv)) {  // of a block of scale NaN, a key that is not seen weighs 0
+    if (masked && !(sc.f > 0.f && sc.lsv == sc.lsv)) {  // a key that is not seen weighs 0 (-inf times NaN, or times a factor that underflowed)
         int again = left;
         asm volatile("" : "+v"(again));  // compared here, and not kept from above on every path
 #pragma unroll
@@ -806,7 +806,7 @@ __device__ __forceinline__ void kv8_softmax32(Kv8Rows32<D>& st, float16_t (&w)[K
     for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) w[t][r] = fast_exp2(__builtin_fmaf(w[t][r], sc.f, c));
-    if (masked && !(sc.f == sc.f && sc.lsv == sc.lsv)) {  // of a block of scale NaN, a key that is not seen weighs 0
+    if (masked && !(sc.f > 0.f && sc.lsv == sc.lsv)) {  // a key that is not seen weighs 0 (-inf times NaN, or times a factor that underflowed)
         int again = left;
         asm volatile("" : "+v"(again));  // compared here, and not kept from above on every path
 #pragma unroll
