@@ -329,6 +329,34 @@ def test_attention_over_long_caches(dev, D, G, T, length):
         check_out(o.cpu(), want, tol, max_len)
 
 
+@pytest.mark.parametrize("D,H,G,T,lens", [
+    (64, 1, 2, 2, [(37 * b) % 401 for b in range(70)]),
+    (128, 2, 3, 1, [64, 1, 1300, 63, 0, 65, 128, 700]),
+    (256, 3, 2, 3, [900, 5, 0, 64, 1500]),
+    (256, 1, 6, 1, [2500, 2500, 2500]),
+    (64, 1, 2, 1, [70000, 100, 3]),
+], ids=["70", "8", "5", "3", "long"])
+def test_attention_over_sequences_of_a_large_cache(dev, D, H, G, T, lens):
+    """A cache that could hold much more: all sequences' keys are dealt out to the workgroups, whose
+    segments end anywhere and pass over sequences that are empty or without new tokens."""
+    gen = torch.Generator().manual_seed(D + len(lens))
+    B = len(lens)
+    new = [0 if b % 5 == 3 else T - (b % 7 == 2 and T > 1) for b in range(B)]
+    k, v = keys(gen, B, H, max(lens), D)
+    c, page = tsa.Kv8Cache(B, H, D, 1 << 18, n_pages=sum(n // 64 for n in lens) + 1, device=dev), 0
+    for b, n in enumerate(lens):
+        c.table[b, :n // 64] = torch.arange(page, page + n // 64, dtype=torch.int32, device=dev)
+        page += n // 64
+    tsa.kv8_write(c, k.to(dev), v.to(dev), ints(lens, dev), ints(lens, dev))
+    q, gate = rand(gen, B, H * G, T, D), rand(gen, B, H * G, T, D)
+    out = torch.full(q.shape, 9.0, dtype=torch.float16, device=dev)
+    tsa.attn_kv8_fwd(q.to(dev), c, ints(lens, dev), ints(new, dev), gate=gate.to(dev), out=out)
+    want, tol = expect(q, k, v, lens, new, True, gate)
+    for b in range(B):
+        assert bool((out[b, :, new[b]:] == 9).all())
+        check_out(out[b, :, :new[b]].cpu(), want[b, :, :new[b]], tol[b, :, :new[b]], b)
+
+
 def test_attention_ragged_and_padded(dev):
     """A padded batch: rows of padding stay as they were, slots without new tokens are untouched."""
     gen = torch.Generator().manual_seed(21)

@@ -27,11 +27,11 @@ BUDGETS = [
     (r"kv8_write_kernelILi(64|128)E", 2, 4, 128, 18 << 10),
     (r"kv8_write_kernelILi256E", 1, 3, 168, 18 << 10),
     (r"kv8_read_kernel", 3, 4, 128, 33 << 10),
-    (r"kv8_row_kernelILi64E", 3, 4, 128, 40 << 10),
-    (r"kv8_row_kernelILi(128|256)E", 6, 2, 256, 40 << 10),
+    (r"kv8_row_kernelILi64E", 4, 4, 128, 40 << 10),
+    (r"kv8_row_kernelILi(128|256)E", 8, 2, 256, 40 << 10),
     (r"kv8_tile_kernel", 7, 2, 256, 64 << 10),
     (r"kv8_wide_kernel", 2, 2, 256, 160 << 10),
-    (r"kv8_join_kernel", 3, 3, 168, 16 << 10),
+    (r"kv8_join_kernel", 6, 3, 168, 16 << 10),
     (r"kv8_score_kernel", 3, 4, 128, 40 << 10),
     (r"kv8_pick_kernel", 3, 8, 64, 4 << 10),
 ]

@@ -425,7 +425,7 @@ extern "C" int tsa_kv8_read(const tsa_kv8* cache, const int32_t* len, const int3
 
 extern "C" size_t tsa_kv8_workspace_bytes(const tsa_kv8* cache, int T, int Hq, int max_len, int top) {
     if (check_kv8(cache) || check_kv8_queries(cache, T, Hq) || max_len < 1 || (top != 0 && !fits_top(top))) return 0;
-    return tsa::kv8_ws_bytes(cache->B, T, Hq, cache->Hkv, cache->D, kv8_nb(cache, max_len), top);
+    return tsa::kv8_ws_bytes(as_kv8(cache), T, Hq, kv8_nb(cache, max_len), top);
 }
 
 extern "C" int tsa_attn_kv8_fwd(const tsa_kv8* cache, const tsa_rows* q, const tsa_rows* gate, const tsa_rows* o,
@@ -436,7 +436,7 @@ extern "C" int tsa_attn_kv8_fwd(const tsa_kv8* cache, const tsa_rows* q, const t
     if (max_len < 1) return TSA_ERR_SHAPE;
     if (causal != 0 && causal != 1) return TSA_ERR_ARG;
     const int B = cache->B, nb = kv8_nb(cache, max_len);
-    const size_t need = tsa::kv8_ws_bytes(B, T, Hq, cache->Hkv, cache->D, nb, 0);
+    const size_t need = tsa::kv8_ws_bytes(as_kv8(cache), T, Hq, nb, 0);
     if ((rc = check_ws(ws, ws_bytes, need))) return rc;
     return from_hip(tsa::kv8_attn(as_kv8(cache), as_rows(q, B, Hq, T), as_rows(gate, B, Hq, T), as_rows(o, B, Hq, T), len,
                                   n_new, T, Hq, nb, scale, causal, ws, as_stream(stream)));
@@ -453,7 +453,7 @@ extern "C" int tsa_kv8_select(const tsa_kv8* cache, const tsa_rows* q, const int
     if ((long long)first + recent + 1 > top) return TSA_ERR_ARG;
     const int B = cache->B, nb = kv8_nb(cache, max_len);
     if ((rc = check_rows(q, B, Hq, T, false))) return rc;
-    const size_t need = tsa::kv8_ws_bytes(B, T, Hq, cache->Hkv, cache->D, nb, top);
+    const size_t need = tsa::kv8_ws_bytes(as_kv8(cache), T, Hq, nb, top);
     if ((rc = check_ws(ws, ws_bytes, need))) return rc;
     return from_hip(tsa::kv8_select(as_kv8(cache), as_rows(q, B, Hq, T), len, n_new, T, Hq, top, first, recent, blocks, nb,
                                     ws, as_stream(stream)));
@@ -467,7 +467,7 @@ extern "C" int tsa_attn_kv8_blocks_fwd(const tsa_kv8* cache, const tsa_rows* q, 
     if (!blocks) return TSA_ERR_NULL;
     if (!fits_top(top)) return TSA_ERR_SHAPE;
     const int B = cache->B;
-    const size_t need = tsa::kv8_ws_bytes(B, T, Hq, cache->Hkv, cache->D, 1, top);
+    const size_t need = tsa::kv8_ws_bytes(as_kv8(cache), T, Hq, 1, top);
     if ((rc = check_ws(ws, ws_bytes, need))) return rc;
     return from_hip(tsa::kv8_attn_blocks(as_kv8(cache), as_rows(q, B, Hq, T), as_rows(gate, B, Hq, T), as_rows(o, B, Hq, T),
                                          len, n_new, T, Hq, blocks, top, scale, ws, as_stream(stream)));

@@ -120,7 +120,7 @@ hipError_t kv8_read(const Kv8& c, const int* len, const int* start, int S, const
                     hipStream_t stream);
 // Workspace of an attention call (blocks of its keys: nb) or, with top > 0, of a selection and
 // the attention over it.
-size_t kv8_ws_bytes(int B, int T, int Hq, int Hkv, int D, int nb, int top);
+size_t kv8_ws_bytes(const Kv8& c, int T, int Hq, int nb, int top);
 // nb_hint: the longest sequence's blocks as the caller knows it; any length is right.
 hipError_t kv8_attn(const Kv8& c, const Rows16& q, const Rows16& gate, const Rows16& o, const int* len,
                     const int* n_new, int T, int Hq, int nb_hint, float scale, int causal, void* ws,

@@ -23,8 +23,9 @@ struct Kv8AttnArgs {
     Kv8 c;
     Rows16 q, gate, o;
     const int *len, *n_new, *blocks;
-    float* part;  // split keys: [B][Hkv][rows][nsplit][D] sums, then as many (m, l) pairs
+    float *part, *pair;  // split keys: D sums for each slot (see kv8_slot), and a pair (m, l)
     int T, Hq, G, top, nsplit, causal;
+    int share;  // above 0: the keys of all sequences are dealt to so many workgroups a head (Kv8Deal)
     float c2;  // scale log2(e)
 };
 
@@ -369,16 +370,19 @@ __device__ __forceinline__ void kv8_arrived(Kv8Rows<D> (&st)[NT]) {
         for (int i = 0; i < D / 32; ++i) asm volatile("" : "+v"(st[nt].q[i]));
 }
 
-// Where a split's sums of a row lie: [row][split][D] sums, behind all of them (m, l) pairs.
-template <int D>
-__device__ __forceinline__ float* kv8_part(const Kv8AttnArgs& p, size_t bh, int row, int split) {
-    return p.part + ((bh * p.T * p.G + row) * p.nsplit + split) * D;
+// Where a split's sums of a row lie: slot [row of all][split], or where all sequences' keys are dealt
+// out [head][segment][row], workgroup w's segment of sequence b being w + b.
+__device__ __forceinline__ size_t kv8_slot(const Kv8AttnArgs& p, size_t bh, int row, int split) {
+    return (bh * p.T * p.G + row) * p.nsplit + split;
+}
+__device__ __forceinline__ size_t kv8_dealt_slot(const Kv8AttnArgs& p, int h, int seg, int row) {
+    return ((size_t)h * (p.share + p.c.B) + seg) * (p.T * p.G) + row;
 }
 template <int D>
-__device__ __forceinline__ float* kv8_pair(const Kv8AttnArgs& p, size_t bh, int row, int split) {
-    const size_t rows = (size_t)p.c.B * p.c.Hkv * p.T * p.G;
-    return p.part + rows * p.nsplit * D + ((bh * p.T * p.G + row) * p.nsplit + split) * 2;
+__device__ __forceinline__ float* kv8_part(const Kv8AttnArgs& p, size_t slot) {
+    return p.part + slot * D;
 }
+__device__ __forceinline__ float2* kv8_pair(const Kv8AttnArgs& p, size_t slot) { return reinterpret_cast<float2*>(p.pair) + slot; }
 
 // 4 consecutive d of a finished row, times the gate.
 __device__ __forceinline__ void kv8_store4(const Kv8AttnArgs& p, int b, int hq, int t, int d, float4_t y, float l, half4_t gate) {
@@ -475,11 +479,11 @@ __device__ __forceinline__ void kv8_finish(Kv8Rows<D> (&st)[NT], const Kv8AttnAr
         if (row >= row_end) continue;
         if (p.nsplit > 1) {
             if (l != 0.f) {
-                float* part = kv8_part<D>(p, at.bh, row, at.split) + 4 * g4;
+                float* part = kv8_part<D>(p, kv8_slot(p, at.bh, row, at.split)) + 4 * g4;
 #pragma unroll
                 for (int dt = 0; dt < D / 16; ++dt) *reinterpret_cast<float4_t*>(part + 16 * dt) = st[nt].o[dt];
             }
-            if (g4 == 0) *reinterpret_cast<float2*>(kv8_pair<D>(p, at.bh, row, at.split)) = float2{st[nt].m, l};
+            if (g4 == 0) *kv8_pair(p, kv8_slot(p, at.bh, row, at.split)) = float2{st[nt].m, l};
         } else {
             const int t = row / p.G, hq = at.h * p.G + row % p.G;
 #pragma unroll
@@ -488,6 +492,81 @@ __device__ __forceinline__ void kv8_finish(Kv8Rows<D> (&st)[NT], const Kv8AttnAr
         }
     }
 }
+
+// All sequences' keys dealt out: one head's, in the order of the sequences, are cut into as many
+// workgroups' as the chip takes, so that all of them have as much to do whatever the lengths are (24/4
+// heads, D = 256: 32 sequences of 16385 to 32768 keys 283 us with 8 splits each, 264 dealt out; 24 of
+// 32768, 272 and 259; 32 of 24576, 250 both).  They are counted in rounds, in which each of a
+// workgroup's 4 waves takes a part; a sequence has one at least, and no more than kKvMaxSplits segments.
+template <int kParts>
+struct Kv8Deal {
+    int groups, per, odd;  // workgroups; rounds of each, the first `odd` having one more
+    int total, before;     // rounds of all sequences, of those before one
+    int lane_own, lane_end;  // a lane's sequence's rounds, and those up to its end
+
+    static __device__ __forceinline__ int rounds(const Kv8AttnArgs& p, int b) {
+        const int n = p.n_new ? min(max(p.n_new[b], 0), p.T) : p.T;
+        const int len = min(max(p.len[b], 0), p.c.max_blocks * kKvBlock);
+        return n > 0 ? max(((len + kKvBlock - 1) / kKvBlock * kParts + 3) / 4, 1) : 0;
+    }
+    // 64 sequences from b0 on; the rounds of all of them.
+    __device__ __forceinline__ int look(const Kv8AttnArgs& p, int b0) {
+        const int lane = threadIdx.x & 63;
+        lane_own = b0 + lane < p.c.B ? rounds(p, b0 + lane) : 0;
+        lane_end = lane_own;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int z = __shfl_up(lane_end, o);
+            lane_end += lane >= o ? z : 0;
+        }
+        return __builtin_amdgcn_readlane(lane_end, 63);
+    }
+    __device__ __forceinline__ void find(const Kv8AttnArgs& p) {
+        int most = 0;
+        total = 0;
+        for (int b0 = 0; b0 < p.c.B; b0 += 64) {
+            total += look(p, b0);
+            most = max(most, lane_own);
+        }
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) most = max(most, __shfl_xor(most, o));
+        most = __builtin_amdgcn_readfirstlane(most);
+        groups = max(1, min(p.share, total / max(2, (most + kKvMaxSplits - 3) / (kKvMaxSplits - 2))));
+        per = total / groups;
+        odd = total % groups;
+    }
+    // The first round of a workgroup, and the workgroup of a round.
+    __device__ __forceinline__ int front(int w) const { return w * per + min(w, odd); }
+    __device__ __forceinline__ int group(int x) const {
+        const int y = odd * (per + 1);
+        return x < y ? x / (per + 1) : odd + (x - y) / max(per, 1);
+    }
+    // The sequence that a round (below total) is of; `before` is its own.
+    __device__ __forceinline__ int seek(const Kv8AttnArgs& p, int x) {
+        before = 0;
+        for (int b0 = 0;; b0 += 64) {
+            const int all = p.c.B > 64 ? look(p, b0) : total;
+            if (x < before + all) {
+                const int l = __builtin_ctzll(__ballot(before + lane_end > x));
+                before += __builtin_amdgcn_readlane(lane_end - lane_own, l);
+                return b0 + l;
+            }
+            before += all;
+        }
+    }
+    // The rounds of sequence b; `before` is its own.
+    __device__ __forceinline__ int own(const Kv8AttnArgs& p, int b) {
+        before = 0;
+        for (int b0 = 0;; b0 += 64) {
+            const int all = p.c.B > 64 ? look(p, b0) : total;
+            if (b < b0 + 64) {
+                before += __builtin_amdgcn_readlane(lane_end - lane_own, b - b0);
+                return __builtin_amdgcn_readlane(lane_own, b - b0);
+            }
+            before += all;
+        }
+    }
+};
 
 // Few rows: tiles of 16 query rows of a K/V head's group over one split of their blocks, a stage of
 // keys (half a block at D = 256, else a block) at a time.  A wave's next keys are on their way to
@@ -498,9 +577,10 @@ __device__ __forceinline__ void kv8_finish(Kv8Rows<D> (&st)[NT], const Kv8AttnAr
 // t G + g over all the sequence's blocks.  Neighbouring queries share most of their listed blocks:
 // an eighth of all tiles in a row goes to each XCD (workgroups go round them), whose L2 then serves
 // the blocks again (700 queries of 16 blocks, 24/4 heads, D = 256: 115 -> 109 us; a wave a tile 102).
-// Bound by memory with one query a sequence (32 of up to 32768 keys, D = 256: 283 us, 5.7 TB/s);
+// Bound by memory with one query a sequence (32 of 16385 to 32768 keys, D = 256: 264 us, 6.1 TB/s);
 // where queries share their blocks by the vector instructions that turn codes into fp16.
-template <int D, bool kList, int kWaves>
+// kDeal: all sequences' keys are dealt out, and a workgroup goes through its segments.
+template <int D, bool kList, int kWaves, bool kDeal>
 __global__ void __launch_bounds__(256, 2)
 kv8_row_kernel(Kv8AttnArgs p, int tiles) {
     using Regs = Kv8Regs<D, !kList>;
@@ -513,111 +593,144 @@ kv8_row_kernel(Kv8AttnArgs p, int tiles) {
     int at = blockIdx.x;
     if constexpr (kList) at = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
     if constexpr (kWaves == 1) at = 4 * at + wave;
-    if (at >= tiles * c.B * c.Hkv * p.nsplit) return;
-    const int tile = at % tiles, bh = at / tiles % (c.B * c.Hkv), split = at / tiles / (c.B * c.Hkv);
-    const int b = bh / c.Hkv, h = bh % c.Hkv;
-    const Kv8Seq sq = kv8_seq(c, p.len, p.n_new, b, p.T);
-    int row0, row_end;
-    if constexpr (kList) {
-        const int per = (p.G + 15) / 16, t = tile / per;
-        row0 = t * p.G + tile % per * 16;
-        row_end = (t + 1) * p.G;
+    int tile = 0, b, h, split = 0, bh = 0;
+    Kv8Deal<kParts> deal;
+    int from = 0, to = 0;  // this workgroup's rounds
+    if constexpr (kDeal) {
+        h = at % c.Hkv;
+        deal.find(p);
+        // neighbours an eighth of the keys apart (next to each other 268 us for the 32 sequences, 264)
+        split = at / c.Hkv;
+        split = split % 8 * (p.share / 8) + split / 8;
+        if (split >= deal.groups) return;
+        from = deal.front(split);
+        to = deal.front(split + 1);
+        if (from == to) return;
+        b = deal.seek(p, from);
     } else {
-        row0 = tile * 16;
-        row_end = p.T * p.G;
+        if (at >= tiles * c.B * c.Hkv * p.nsplit) return;
+        tile = at % tiles, bh = at / tiles % (c.B * c.Hkv), split = at / tiles / (c.B * c.Hkv);
+        b = bh / c.Hkv, h = bh % c.Hkv;
     }
-    row_end = min(row_end, (sq.n + sq.t0) * p.G);
-    if (row0 >= row_end) return;
-
-    Kv8Rows<D> rows[1], &st = rows[0];
-    int see, least;
-    kv8_begin<D, 1>(rows, p, sq, b, h, row0, row_end, see, least);
-    const int nb = see / kKvBlock + (see >= 0 ? 1 : 0);  // blocks that any row sees
-    const int n_full = min(sq.len / kKvBlock, nb);
-    const int items = (kList ? p.top : nb) * kParts;
-    const int per = (items + p.nsplit - 1) / p.nsplit;
-    const int end = min(items, (split + 1) * per);
-    const int* list = kList ? p.blocks + (((size_t)b * c.Hkv + h) * p.T + row0 / p.G) * p.top : nullptr;
-    Kv8Walk<kList, kParts> walk = {split * per + (kWaves == 4 ? wave : 0), end, kWaves, nb, n_full, 0, 0};
-    int blk = 0, part = 0, page = -1;
-    Kv8Scale sc = {};
-    auto next = [&]() {
-        if (!walk.next(c, b, h, list, p.c2, blk, part, page, sc)) page = -1;
-    };
-    next();
-    if (page >= 0) {
-        Regs x;
-        x.load_k(c, page, h, part);
-        x.load_v(c, page, h, part);
-        kv8_arrived<D, 1>(rows);
-        while (page >= 0) {
-            // rows of one query see whole blocks but the last; several queries' last one or two are masked
-            const int p0 = blk * kKvBlock + part * Regs::kKeys;
-            const Kv8Scale scale = sc;
-            next();
-            kv8_keys<D, 1, Regs::kKeys / 16>(
-                rows, p0, scale, p0 + Regs::kKeys - 1 > least,
-                [&](int a, int i, int s) {
-                    const uint4& k = x.k[a * (D / 64) + i];
-                    return s ? kv8_halves(k.z, k.w) : kv8_halves(k.x, k.y);
-                },
-                [&](int s, int m, int o) {
-                    const uint4& v = x.v[s * (D / 32) + m];
-                    return o ? kv8_halves(v.z, v.w) : kv8_halves(v.x, v.y);
-                },
-                [&]() {
-                    if (page >= 0) x.load_k(c, page, h, part);
-                });
-            if (page >= 0) x.load_v(c, page, h, part);
-        }
-    }
-    for (; walk.open > 0; --walk.open) kv8_open_block<D>(st, c, b, h, n_full, sq.len - n_full * kKvBlock, p.c2);
-
-    if constexpr (kWaves == 1) {
-        kv8_finish<D, 1>(rows, p, {tile, bh, b, h, split}, row0, row_end);
-        return;
-    }
-    // the four waves' sums, relative to their common maximum
-    st.l = sum_xor32(sum_xor16(st.l));
-    if (g4 == 0) {
-        ml[wave][0][n] = st.m;
-        ml[wave][1][n] = st.l;
-    }
-    __syncthreads();
-    {
-        const float m = fmaxf(fmaxf(ml[0][0][n], ml[1][0][n]), fmaxf(ml[2][0][n], ml[3][0][n]));
-        const float f = st.m == m ? 1.f : fast_exp2(st.m - m);
-#pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt) st.o[dt] *= f;
-    }
-    if (wave >= 2) {
-#pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt) *reinterpret_cast<float4_t*>(&acc[wave & 1][n][16 * dt + 4 * g4]) = st.o[dt];
-    }
-    __syncthreads();
-    if (wave < 2) {
-#pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt) {
-            float4_t* at = reinterpret_cast<float4_t*>(&acc[wave][n][16 * dt + 4 * g4]);
-            *at += st.o[dt];
-        }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < min(16, row_end - row0) * (D / 4); i += 256) {
-        const int r = i / (D / 4), d = i % (D / 4) * 4;
-        float m = -INFINITY, l = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) m = fmaxf(m, ml[w][0][r]);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) l += ml[w][0][r] == m ? ml[w][1][r] : ml[w][1][r] * fast_exp2(ml[w][0][r] - m);
-        const float4_t y = *reinterpret_cast<const float4_t*>(&acc[0][r][d]) + *reinterpret_cast<const float4_t*>(&acc[1][r][d]);
-        if (p.nsplit > 1) {
-            if (l != 0.f) *reinterpret_cast<float4_t*>(kv8_part<D>(p, bh, row0 + r, split) + d) = y;
-            if (d == 0) *reinterpret_cast<float2*>(kv8_pair<D>(p, bh, row0 + r, split)) = float2{m, l};
+    for (;;) {  // segments of a deal, else once
+        const Kv8Seq sq = kv8_seq(c, p.len, p.n_new, b, p.T);
+        int row0, row_end;
+        if constexpr (kList) {
+            const int per = (p.G + 15) / 16, t = tile / per;
+            row0 = t * p.G + tile % per * 16;
+            row_end = (t + 1) * p.G;
         } else {
-            const int t = (row0 + r) / p.G, hq = h * p.G + (row0 + r) % p.G;
-            kv8_store4(p, b, hq, t, d, y, l, kv8_gate4(p, b, hq, t, d));
+            row0 = tile * 16;
+            row_end = p.T * p.G;
         }
+        row_end = min(row_end, (sq.n + sq.t0) * p.G);
+        if (!kDeal && row0 >= row_end) return;
+
+        Kv8Rows<D> rows[1], &st = rows[0];
+        int see, least;
+        kv8_begin<D, 1>(rows, p, sq, b, h, row0, row_end, see, least);
+        const int nb = see / kKvBlock + (see >= 0 ? 1 : 0);  // blocks that any row sees
+        const int n_full = min(sq.len / kKvBlock, nb);
+        const int items = (kList ? p.top : nb) * kParts;
+        int begin, end;
+        if constexpr (kDeal) {
+            begin = max(from - deal.before, 0) * 4;
+            end = min((to - deal.before) * 4, items);
+        } else {
+            const int per = (items + p.nsplit - 1) / p.nsplit;
+            begin = split * per;
+            end = min(items, begin + per);
+        }
+        const int* list = kList ? p.blocks + (((size_t)b * c.Hkv + h) * p.T + row0 / p.G) * p.top : nullptr;
+        Kv8Walk<kList, kParts> walk = {begin + (kWaves == 4 ? wave : 0), end, kWaves, nb, n_full, 0, 0};
+        int blk = 0, part = 0, page = -1;
+        Kv8Scale sc = {};
+        auto next = [&]() {
+            if (!walk.next(c, b, h, list, p.c2, blk, part, page, sc)) page = -1;
+        };
+        next();
+        if (page >= 0) {
+            Regs x;
+            x.load_k(c, page, h, part);
+            x.load_v(c, page, h, part);
+            kv8_arrived<D, 1>(rows);
+            while (page >= 0) {
+                // rows of one query see whole blocks but the last; several queries' last one or two are masked
+                const int p0 = blk * kKvBlock + part * Regs::kKeys;
+                const Kv8Scale scale = sc;
+                next();
+                kv8_keys<D, 1, Regs::kKeys / 16>(
+                    rows, p0, scale, p0 + Regs::kKeys - 1 > least,
+                    [&](int a, int i, int s) {
+                        const uint4& k = x.k[a * (D / 64) + i];
+                        return s ? kv8_halves(k.z, k.w) : kv8_halves(k.x, k.y);
+                    },
+                    [&](int s, int m, int o) {
+                        const uint4& v = x.v[s * (D / 32) + m];
+                        return o ? kv8_halves(v.z, v.w) : kv8_halves(v.x, v.y);
+                    },
+                    [&]() {
+                        if (page >= 0) x.load_k(c, page, h, part);
+                    });
+                if (page >= 0) x.load_v(c, page, h, part);
+            }
+        }
+        for (; walk.open > 0; --walk.open) kv8_open_block<D>(st, c, b, h, n_full, sq.len - n_full * kKvBlock, p.c2);
+
+        if constexpr (kWaves == 1) {
+            kv8_finish<D, 1>(rows, p, {tile, bh, b, h, split}, row0, row_end);
+            return;
+        }
+        // the four waves' sums, relative to their common maximum
+        st.l = sum_xor32(sum_xor16(st.l));
+        if (g4 == 0) {
+            ml[wave][0][n] = st.m;
+            ml[wave][1][n] = st.l;
+        }
+        __syncthreads();
+        {
+            const float m = fmaxf(fmaxf(ml[0][0][n], ml[1][0][n]), fmaxf(ml[2][0][n], ml[3][0][n]));
+            const float f = st.m == m ? 1.f : fast_exp2(st.m - m);
+    #pragma unroll
+            for (int dt = 0; dt < D / 16; ++dt) st.o[dt] *= f;
+        }
+        if (wave >= 2) {
+    #pragma unroll
+            for (int dt = 0; dt < D / 16; ++dt) *reinterpret_cast<float4_t*>(&acc[wave & 1][n][16 * dt + 4 * g4]) = st.o[dt];
+        }
+        __syncthreads();
+        if (wave < 2) {
+    #pragma unroll
+            for (int dt = 0; dt < D / 16; ++dt) {
+                float4_t* at = reinterpret_cast<float4_t*>(&acc[wave][n][16 * dt + 4 * g4]);
+                *at += st.o[dt];
+            }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < min(16, row_end - row0) * (D / 4); i += 256) {
+            const int r = i / (D / 4), d = i % (D / 4) * 4;
+            float m = -INFINITY, l = 0.f;
+    #pragma unroll
+            for (int w = 0; w < 4; ++w) m = fmaxf(m, ml[w][0][r]);
+    #pragma unroll
+            for (int w = 0; w < 4; ++w) l += ml[w][0][r] == m ? ml[w][1][r] : ml[w][1][r] * fast_exp2(ml[w][0][r] - m);
+            const float4_t y = *reinterpret_cast<const float4_t*>(&acc[0][r][d]) + *reinterpret_cast<const float4_t*>(&acc[1][r][d]);
+            if (kDeal || p.nsplit > 1) {
+                const size_t slot = kDeal ? kv8_dealt_slot(p, h, split + b, row0 + r) : kv8_slot(p, bh, row0 + r, split);
+                if (l != 0.f) *reinterpret_cast<float4_t*>(kv8_part<D>(p, slot) + d) = y;
+                if (d == 0) *kv8_pair(p, slot) = float2{m, l};
+            } else {
+                const int t = (row0 + r) / p.G, hq = h * p.G + (row0 + r) % p.G;
+                kv8_store4(p, b, hq, t, d, y, l, kv8_gate4(p, b, hq, t, d));
+            }
+        }
+        if constexpr (!kDeal) return;
+        do {  // the next sequence, if any of its rounds are this workgroup's
+            deal.before += Kv8Deal<kParts>::rounds(p, b);
+            if (deal.before >= to) return;
+            ++b;
+        } while (Kv8Deal<kParts>::rounds(p, b) == 0);
+        __syncthreads();
     }
 }
 
@@ -1058,7 +1171,7 @@ kv8_wide_kernel(Kv8AttnArgs p, int tiles, int streams) {
     if (row >= row_end) return;
     if (p.nsplit > 1) {
         if (l != 0.f) {
-            float* part = kv8_part<D>(p, at.bh, row, at.split) + 4 * hi;
+            float* part = kv8_part<D>(p, kv8_slot(p, at.bh, row, at.split)) + 4 * hi;
 #pragma unroll
             for (int m = 0; m < D / 32; ++m)
 #pragma unroll
@@ -1066,7 +1179,7 @@ kv8_wide_kernel(Kv8AttnArgs p, int tiles, int streams) {
                     *reinterpret_cast<float4_t*>(part + 32 * m + 8 * r) =
                         float4_t{st.o[m][4 * r], st.o[m][4 * r + 1], st.o[m][4 * r + 2], st.o[m][4 * r + 3]};
         }
-        if (hi == 0) *reinterpret_cast<float2*>(kv8_pair<D>(p, at.bh, row, at.split)) = float2{st.m, l};
+        if (hi == 0) *kv8_pair(p, kv8_slot(p, at.bh, row, at.split)) = float2{st.m, l};
     } else {
         const int t = row / p.G, hq = at.h * p.G + row % p.G;
 #pragma unroll
@@ -1083,7 +1196,7 @@ kv8_wide_kernel(Kv8AttnArgs p, int tiles, int streams) {
 // Joins the splits of 1024 / D rows: workgroup (rows, b Hkv + h), D / 4 lanes a row.  Every address
 // is known at once, so that the loads wait for memory together and not for each other: a row's
 // maxima and sums, its first splits' sums (unread where they were not written), its gate.
-template <int D>
+template <int D, bool kDeal>
 __global__ void __launch_bounds__(256)
 kv8_join_kernel(Kv8AttnArgs p) {
     constexpr int kLanes = D / 4, kRows = 256 / kLanes, kAhead = 16;
@@ -1092,14 +1205,25 @@ kv8_join_kernel(Kv8AttnArgs p) {
     const int b = blockIdx.y / c.Hkv, h = blockIdx.y % c.Hkv;
     const int r = threadIdx.x / kLanes, x = threadIdx.x % kLanes, n_rows = p.T * p.G;
     const int row = min((int)blockIdx.x * kRows + r, n_rows - 1);
-    const float2* pair = reinterpret_cast<const float2*>(kv8_pair<D>(p, blockIdx.y, row, 0));
-    const float4_t* at = reinterpret_cast<const float4_t*>(kv8_part<D>(p, blockIdx.y, row, 0)) + x;
+    int n = p.nsplit;
+    size_t slot = kv8_slot(p, blockIdx.y, row, 0), step = 1;
+    if constexpr (kDeal) {
+        using Deal = Kv8Deal<kKvBlock / Kv8Regs<D, true>::kKeys>;
+        Deal deal;
+        deal.find(p);
+        const int own = deal.own(p, b), first = deal.group(deal.before);
+        n = own ? deal.group(deal.before + own - 1) - first + 1 : 1;
+        slot = kv8_dealt_slot(p, h, first + b, row);
+        step = n_rows;
+    }
+    const float2* pair = kv8_pair(p, slot);
+    const float4_t* at = reinterpret_cast<const float4_t*>(kv8_part<D>(p, slot)) + x;
     float2 ml[kKvMaxSplits / kLanes];
 #pragma unroll
-    for (int i = 0; i < kKvMaxSplits / kLanes; ++i) ml[i] = pair[min(x + i * kLanes, p.nsplit - 1)];
+    for (int i = 0; i < kKvMaxSplits / kLanes; ++i) ml[i] = pair[min(x + i * kLanes, n - 1) * step];
     float4_t part[kAhead];
 #pragma unroll
-    for (int s = 0; s < kAhead; ++s) part[s] = at[(size_t)min(s, p.nsplit - 1) * (D / 4)];
+    for (int s = 0; s < kAhead; ++s) part[s] = at[min(s, n - 1) * step * (D / 4)];
     const int t = row / p.G, hq = h * p.G + row % p.G;
     const half4_t gate = kv8_gate4(p, b, hq, t, 4 * x);
     const Kv8Seq sq = kv8_seq(c, p.len, p.n_new, b, p.T);
@@ -1107,7 +1231,7 @@ kv8_join_kernel(Kv8AttnArgs p) {
     float m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int i = 0; i < kKvMaxSplits / kLanes; ++i) {
-        if (x + i * kLanes >= p.nsplit) ml[i] = float2{-INFINITY, 0.f};
+        if (x + i * kLanes >= n) ml[i] = float2{-INFINITY, 0.f};
         m = fmaxf(m, ml[i].x);
     }
 #pragma unroll
@@ -1117,7 +1241,7 @@ kv8_join_kernel(Kv8AttnArgs p) {
         float f = ml[i].y == 0.f ? 0.f : ml[i].x == m ? 1.f : fast_exp2(ml[i].x - m);
         if (ml[i].y != ml[i].y) f = ml[i].y;  // a row of NaN, whatever its maximum
         l += ml[i].y == 0.f ? 0.f : f * ml[i].y;
-        if (x + i * kLanes < p.nsplit) fs[r][x + i * kLanes] = f;
+        if (x + i * kLanes < n) fs[r][x + i * kLanes] = f;
     }
 #pragma unroll
     for (int o = 1; o < kLanes; o <<= 1) l += __shfl_xor(l, o);
@@ -1129,13 +1253,13 @@ kv8_join_kernel(Kv8AttnArgs p) {
     };
 #pragma unroll
     for (int s = 0; s < kAhead; ++s)
-        if (s < p.nsplit) add(part[s], fs[r][s]);
-    for (int s0 = kAhead; s0 < p.nsplit; s0 += kAhead) {
+        if (s < n) add(part[s], fs[r][s]);
+    for (int s0 = kAhead; s0 < n; s0 += kAhead) {
 #pragma unroll
-        for (int s = 0; s < kAhead; ++s) part[s] = at[(size_t)min(s0 + s, p.nsplit - 1) * (D / 4)];
+        for (int s = 0; s < kAhead; ++s) part[s] = at[min(s0 + s, n - 1) * step * (D / 4)];
 #pragma unroll
         for (int s = 0; s < kAhead; ++s)
-            if (s0 + s < p.nsplit) add(part[s], fs[r][s0 + s]);
+            if (s0 + s < n) add(part[s], fs[r][s0 + s]);
     }
     kv8_store4(p, b, hq, t, 4 * x, y, l, gate);
 }
@@ -1149,43 +1273,55 @@ struct Kv8Plan {
     int rows;       // of a tile
     long long tiles;  // of one K/V head
     int nsplit;
+    int share;      // above 0: keys are dealt to so many workgroups a head
 };
 // One tile of 16 rows where there are no more (and for listed blocks, one query's heads), else
-// workgroups of 64 rows, or more at D = 64 of 128 and at D = 128 and 256 of 256.  items: blocks of the longest sequence, or of a list.
-inline Kv8Plan kv8_plan(int B, int T, int Hq, int Hkv, int D, int items, bool list) {
-    const long long G = Hq / Hkv, rows = T * G;
+// workgroups of 64 rows, or more at D = 64 of 128 and at D = 128 and 256 of 256.  items: blocks of the
+// longest sequence, or of a list.
+inline Kv8Plan kv8_plan(const Kv8& c, int T, int Hq, int items, bool list) {
+    const long long G = Hq / c.Hkv, rows = T * G;
     Kv8Plan q;
-    q.rows = list || rows <= 16 ? 16 : rows <= (D == 64 ? 64 : 128) ? 64 : D == 64 ? 128 : 256;
+    q.rows = list || rows <= 16 ? 16 : rows <= (c.D == 64 ? 64 : 128) ? 64 : c.D == 64 ? 128 : 256;
     q.tiles = list ? T * ((G + 15) / 16) : (rows + q.rows - 1) / q.rows;
-    const long long all = q.tiles * B * Hkv;
+    const long long all = q.tiles * c.B * c.Hkv;
     // row tiles: as many workgroups as the chip takes twice, but two stages of keys a wave at the
     // least; the others as many as it takes once, but 4 blocks at the least
     const bool few = q.rows == 16;
+    const int parts = c.D == 256 ? 2 : 1;
     const long long want = few ? (1024 + all - 1) / all : (q.rows == 256 ? 256 : 512) / all;
-    const long long most = few ? ((long long)items * (D == 256 ? 2 : 1) + 7) / 8 : (items + 3) / 4;
+    const long long most = few ? ((long long)items * parts + 7) / 8 : (items + 3) / 4;
     const long long n = want < most ? want : most;
     q.nsplit = (int)(n < 1 ? 1 : n < kKvMaxSplits ? n : kKvMaxSplits);
+    // Several sequences whose keys fill the chip: dealt out (parts are counted in ints).  Where two
+    // stages a wave are the bound, most workgroups would have two short segments one after the other.
+    q.share = few && !list && c.B > 1 && want > 1 && want < most && c.B * ((long long)c.max_blocks * parts + 4) < INT_MAX
+                  ? 1024 / c.Hkv & ~7 : 0;
     return q;
 }
-inline size_t kv8_part_bytes(int B, int T, int Hq, int D, int nsplit) {
-    return nsplit > 1 ? (size_t)B * T * Hq * nsplit * (D + 2) * 4 : 0;
+inline size_t kv8_slots(const Kv8& c, int T, int Hq, const Kv8Plan& q) {
+    return (q.share ? q.share + c.B : q.nsplit > 1 ? (size_t)c.B * q.nsplit : 0) * T * Hq;
 }
+inline size_t kv8_part_bytes(const Kv8& c, int T, int Hq, const Kv8Plan& q) { return kv8_slots(c, T, Hq, q) * (c.D + 2) * 4; }
 
 template <int D, bool kList>
 hipError_t kv8_attn_d(const Kv8AttnArgs& p, const Kv8Plan& q, hipStream_t stream) {
     const int BH = p.c.B * p.c.Hkv;
     if (kList || q.rows == 16) {
         const long long n = q.tiles * BH * p.nsplit;
-        bool wave = false;
+        bool done = false;
         if constexpr (kList) {
-            if ((wave = n >= kKvWaveTiles)) {
+            if ((done = n >= kKvWaveTiles)) {
                 const dim3 grid((unsigned)((n + 31) / 32 * 8));
-                hipLaunchKernelGGL((kv8_row_kernel<D, true, 1>), grid, dim3(256), 0, stream, p, (int)q.tiles);
+                hipLaunchKernelGGL((kv8_row_kernel<D, true, 1, false>), grid, dim3(256), 0, stream, p, (int)q.tiles);
             }
         }
-        if (!wave) {
+        if constexpr (!kList) {
+            if ((done = p.share > 0))
+                hipLaunchKernelGGL((kv8_row_kernel<D, false, 4, true>), dim3((unsigned)(p.share * p.c.Hkv)), dim3(256), 0, stream, p, 1);
+        }
+        if (!done) {
             const dim3 grid((unsigned)((n + 7) / 8 * 8));
-            hipLaunchKernelGGL((kv8_row_kernel<D, kList, 4>), grid, dim3(256), 0, stream, p, (int)q.tiles);
+            hipLaunchKernelGGL((kv8_row_kernel<D, kList, 4, false>), grid, dim3(256), 0, stream, p, (int)q.tiles);
         }
     } else {
         const dim3 grid((unsigned)((q.tiles * BH * p.nsplit + 7) / 8 * 8));
@@ -1200,10 +1336,16 @@ hipError_t kv8_attn_d(const Kv8AttnArgs& p, const Kv8Plan& q, hipStream_t stream
             hipLaunchKernelGGL(kv8_wide_kernel<D>, grid, dim3(512), 0, stream, p, (int)q.tiles, streams);
     }
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || p.nsplit == 1) return e;
+    if (e != hipSuccess || (p.nsplit == 1 && !p.share)) return e;
     constexpr int kRows = 1024 / D;
     const dim3 rows((unsigned)((p.T * p.G + kRows - 1) / kRows), (unsigned)BH);
-    hipLaunchKernelGGL(kv8_join_kernel<D>, rows, dim3(256), 0, stream, p);
+    if constexpr (!kList) {
+        if (p.share) {
+            hipLaunchKernelGGL((kv8_join_kernel<D, true>), rows, dim3(256), 0, stream, p);
+            return hipGetLastError();
+        }
+    }
+    hipLaunchKernelGGL((kv8_join_kernel<D, false>), rows, dim3(256), 0, stream, p);
     return hipGetLastError();
 }
 template <bool kList>
@@ -1217,17 +1359,19 @@ hipError_t kv8_attn_any(const Kv8AttnArgs& p, const Kv8Plan& q, hipStream_t stre
 
 hipError_t kv8_attn(const Kv8& c, const Rows16& q, const Rows16& gate, const Rows16& o, const int* len, const int* n_new,
                     int T, int Hq, int nb_hint, float scale, int causal, void* ws, hipStream_t stream) {
-    const Kv8Plan plan = kv8_plan(c.B, T, Hq, c.Hkv, c.D, nb_hint, false);
-    return kv8_attn_any<false>({c, q, gate, o, len, n_new, nullptr, (float*)ws, T, Hq, Hq / c.Hkv, 0, plan.nsplit, causal, scale * kLog2e},
-                               plan, stream);
+    const Kv8Plan plan = kv8_plan(c, T, Hq, nb_hint, false);
+    float* part = (float*)ws;
+    return kv8_attn_any<false>({c, q, gate, o, len, n_new, nullptr, part, part ? part + kv8_slots(c, T, Hq, plan) * c.D : nullptr, T, Hq,
+                                Hq / c.Hkv, 0, plan.nsplit, causal, plan.share, scale * kLog2e}, plan, stream);
 }
 
 hipError_t kv8_attn_blocks(const Kv8& c, const Rows16& q, const Rows16& gate, const Rows16& o, const int* len,
                            const int* n_new, int T, int Hq, const int* blocks, int top, float scale, void* ws,
                            hipStream_t stream) {
-    const Kv8Plan plan = kv8_plan(c.B, T, Hq, c.Hkv, c.D, top, true);
-    return kv8_attn_any<true>({c, q, gate, o, len, n_new, blocks, (float*)ws, T, Hq, Hq / c.Hkv, top, plan.nsplit, 1, scale * kLog2e}, plan,
-                              stream);
+    const Kv8Plan plan = kv8_plan(c, T, Hq, top, true);
+    float* part = (float*)ws;
+    return kv8_attn_any<true>({c, q, gate, o, len, n_new, blocks, part, part ? part + kv8_slots(c, T, Hq, plan) * c.D : nullptr, T, Hq,
+                               Hq / c.Hkv, top, plan.nsplit, 1, plan.share, scale * kLog2e}, plan, stream);
 }
 
 }  // namespace tsa

@@ -288,10 +288,10 @@ hipError_t kv8_select(const Kv8& c, const Rows16& q, const int* len, const int* 
     return kv8_select_d<256>(p, stream);
 }
 
-size_t kv8_ws_bytes(int B, int T, int Hq, int Hkv, int D, int nb, int top) {
+size_t kv8_ws_bytes(const Kv8& c, int T, int Hq, int nb, int top) {
     const bool list = top > 0;
-    const size_t part = kv8_part_bytes(B, T, Hq, D, kv8_plan(B, T, Hq, Hkv, D, list ? top : nb, list).nsplit);
-    const size_t sel = list ? kv8_select_bytes(B, T, Hkv, nb) : 0;
+    const size_t part = kv8_part_bytes(c, T, Hq, kv8_plan(c, T, Hq, list ? top : nb, list));
+    const size_t sel = list ? kv8_select_bytes(c.B, T, c.Hkv, nb) : 0;
     return part > sel ? part : sel;
 }
 
