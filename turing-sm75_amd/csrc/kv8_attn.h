@@ -964,25 +964,28 @@ __device__ __forceinline__ void kv8_open_block32(Kv8Rows32<D>& st, const half_t*
         for (int u = 0; u < D / 16; ++u) {
             const half8_t q = is_row ? *reinterpret_cast<const half8_t*>(qr + 16 * u) : half8_t{};
             w[0] = mfma32(*reinterpret_cast<const half8_t*>(ko + kv8_k_at<D>(32 * s + row, 16 * u + 8 * hi)), q, w[0]);
-            if (u % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // a few loads at a time
+            if (u % 8 == 7) __builtin_amdgcn_sched_barrier(0);  // some loads at a time
         }
         kv8_softmax32<D, 1>(st, w, p0, {c2, 0.f, 1.f}, true);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {  // 16 keys at a time
             const half8_t p = kv8_weights32(w[0], x);
             const int g4 = 2 * x + hi;  // keys 16 i + 4 g4 + e
+            half8_t v[D / 32];
+#pragma unroll
+            for (int m = 0; m < D / 32; ++m) v[m] = *reinterpret_cast<const half8_t*>(vo + kv8_v_at<D>(32 * s + 4 * g4, 32 * m + x32));
+            __builtin_amdgcn_sched_barrier(0);  // the loads wait for memory together (39 open rows at D = 256: 20 us, 7)
 #pragma unroll
             for (int m = 0; m < D / 32; ++m) {
-                half8_t v = *reinterpret_cast<const half8_t*>(vo + kv8_v_at<D>(32 * s + 4 * g4, 32 * m + x32));
                 bool bad = false;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const bool is = 32 * s + 16 * (j >> 2) + 4 * g4 + (j & 3) < n;
-                    const bool off = kv8_bad(v[j]);
+                    const bool off = kv8_bad(v[m][j]);
                     bad |= is && off;
-                    if (!is || off) v[j] = (half_t)0.f;
+                    if (!is || off) v[m][j] = (half_t)0.f;
                 }
-                st.o[m] = mfma32(v, p, st.o[m]);
+                st.o[m] = mfma32(v[m], p, st.o[m]);
                 if (!__any(bad)) continue;
                 float16_t more = {};  // (not on the sums themselves, which are to stay in place)
 #pragma unroll 1
@@ -1285,12 +1288,17 @@ inline Kv8Plan kv8_plan(const Kv8& c, int T, int Hq, int items, bool list) {
     q.tiles = list ? T * ((G + 15) / 16) : (rows + q.rows - 1) / q.rows;
     const long long all = q.tiles * c.B * c.Hkv;
     // row tiles: as many workgroups as the chip takes twice, but two stages of keys a wave at the
-    // least; the others as many as it takes once, but 4 blocks at the least
+    // least; the others as many as it takes once, but 2 blocks at the least (500 tokens of one head,
+    // D = 256: 4 blocks 40 us, 2 31; 300 tokens over 2300, 4 heads, D = 128: 26, 24), or 4 of 64 rows (8
+    // sequences of 2777, 5 tokens, 16/2 heads, D = 64: 4 blocks 12.5 us, 2 14.3)
     const bool few = q.rows == 16;
     const int parts = c.D == 256 ? 2 : 1;
     const long long want = few ? (1024 + all - 1) / all : (q.rows == 256 ? 256 : 512) / all;
-    const long long most = few ? ((long long)items * parts + 7) / 8 : (items + 3) / 4;
-    const long long n = want < most ? want : most;
+    const long long most = few ? ((long long)items * parts + 7) / 8 : q.rows == 64 ? (items + 3) / 4 : (items + 1) / 2;
+    long long n = want < most ? want : most;
+    // The sums of splits of 256 rows that fill the chip take as long to write and join as 8 blocks to
+    // multiply (7 x 640 tokens, 6/2 heads, D = 256: 56 us in 2 splits, 51 in one).
+    if (q.rows == 256 && n > 1 && items * (n - 1) * 256 <= 8 * all * n * n) n = 1;
     q.nsplit = (int)(n < 1 ? 1 : n < kKvMaxSplits ? n : kKvMaxSplits);
     // Several sequences whose keys fill the chip: dealt out (parts are counted in ints).  Where two
     // stages a wave are the bound, most workgroups would have two short segments one after the other.
