@@ -1012,10 +1012,10 @@ __device__ __forceinline__ void kv8_open_block32(Kv8Rows32<D>& st, const half_t*
 // memory to registers two stages ahead (a unit of K and one of V a thread), is turned into fp16
 // operands once for all waves, and lies in one of two LDS buffers in operand order.  One barrier a
 // stage.
-// Bound by the card's power at D = 128 (prompt of 8192, 32 heads: 0.65 ms at 1.8 GHz, 0.84 PFLOP/s;
-// the fp16 kernel of attn_fwd.hip, 0.57 ms at 1.6 GHz): two groups of waves taking turns at matrix
+// Bound by the card's power at D = 128 (prompt of 8192, 32 heads: 0.56 ms, 0.98 PFLOP/s, 1.8 GHz; the
+// fp16 kernel of attn_fwd.hip, 0.53-0.55 ms at 1.6 GHz): two groups of waves taking turns at matrix
 // and vector instructions needed 13 % fewer cycles and the same time.  At D = 256 (512 tokens over
-// 16384, 24/4 heads: 0.23 ms, 0.89 PFLOP/s) by LDS, which the operands of 32 rows keep busy for as
+// 16384, 24/4 heads: 0.21 ms, 0.95 PFLOP/s) by LDS, which the operands of 32 rows keep busy for as
 // long as the matrix units; the two groups' second barrier a stage cost it 8 %.
 template <int D>
 struct Kv8Wide {
