@@ -315,7 +315,7 @@ int tsa_kv8_read(const tsa_kv8* cache, const int32_t* len, const int32_t* start,
 /* Workspace bytes of the calls below for T rows of Hq query heads; max_len: no sequence is longer
  * (at most 64 * max_blocks).  top = 0: tsa_attn_kv8_fwd; top > 0: tsa_kv8_select and
  * tsa_attn_kv8_blocks_fwd, which may share one workspace.  0 for invalid arguments, and where no
- * workspace is needed.  A workspace is 16-byte aligned.  Hq / Hkv is at most 65536.  Calls that share a workspace must be ordered on one stream. */
+ * workspace is needed; enough for calls of a smaller max_len as well.  A workspace is 16-byte aligned.  Hq / Hkv is at most 65536.  Calls that share a workspace must be ordered on one stream. */
 size_t tsa_kv8_workspace_bytes(const tsa_kv8* cache, int T, int Hq, int max_len, int top);
 
 /* Attention of T new tokens per sequence over the cache that holds them already (write first):

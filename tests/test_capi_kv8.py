@@ -136,6 +136,16 @@ def test_workspace():
         assert lib.tsa_kv8_workspace_bytes(ref(c), a["T"], a["Hq"], a["max_len"], a["top"]) == 0
 
 
+def test_workspace_serves_shorter_lengths():
+    """A workspace sized for the longest sequences serves calls with a smaller max_len."""
+    lib = tsa.load()
+    for D in (64, 128, 256):
+        for B, Hkv, Hq, T in ((1, 4, 24, 1), (3, 2, 8, 2), (32, 4, 24, 1), (7, 1, 1, 1), (100, 3, 9, 1), (42, 1, 1, 200), (6, 7, 7, 200), (2, 5, 20, 33)):
+            c = cache(B=B, Hkv=Hkv, D=D, n_pages=8, max_blocks=1 << 12)
+            sizes = [lib.tsa_kv8_workspace_bytes(ref(c), T, Hq, 64 * nb, 0) for nb in list(range(1, 200)) + [500, 1 << 11, 1 << 12]]
+            assert sizes == sorted(sizes), (D, B, Hkv, Hq, T)
+
+
 def test_cache_object_refuses():
     for kw in (dict(B=0), dict(Hkv=0), dict(D=96), dict(max_len=0), dict(n_pages=0), dict(device="cpu")):
         a = dict(B=1, Hkv=1, D=64, max_len=64)

@@ -546,11 +546,13 @@ struct Kv8Deal {
         before = 0;
         for (int b0 = 0;; b0 += 64) {
             const int all = p.c.B > 64 ? look(p, b0) : total;
-            if (x < before + all) {
-                const int l = __builtin_ctzll(__ballot(before + lane_end > x));
+            const unsigned long long is = __ballot(before + lane_end > x);
+            if (is != 0) {
+                const int l = __builtin_ctzll(is);
                 before += __builtin_amdgcn_readlane(lane_end - lane_own, l);
                 return b0 + l;
             }
+            if (b0 + 64 >= p.c.B) return p.c.B;  // (the lengths changed under the call)
             before += all;
         }
     }
@@ -607,6 +609,7 @@ kv8_row_kernel(Kv8AttnArgs p, int tiles) {
         to = deal.front(split + 1);
         if (from == to) return;
         b = deal.seek(p, from);
+        if (b >= c.B) return;
     } else {
         if (at >= tiles * c.B * c.Hkv * p.nsplit) return;
         tile = at % tiles, bh = at / tiles % (c.B * c.Hkv), split = at / tiles / (c.B * c.Hkv);
@@ -728,7 +731,7 @@ kv8_row_kernel(Kv8AttnArgs p, int tiles) {
         do {  // the next sequence, if any of its rounds are this workgroup's
             deal.before += Kv8Deal<kParts>::rounds(p, b);
             if (deal.before >= to) return;
-            ++b;
+            if (++b >= c.B) return;
         } while (Kv8Deal<kParts>::rounds(p, b) == 0);
         __syncthreads();
     }
@@ -1215,7 +1218,7 @@ kv8_join_kernel(Kv8AttnArgs p) {
         Deal deal;
         deal.find(p);
         const int own = deal.own(p, b), first = deal.group(deal.before);
-        n = own ? deal.group(deal.before + own - 1) - first + 1 : 1;
+        n = own ? min(deal.group(deal.before + own - 1) - first + 1, kKvMaxSplits) : 1;
         slot = kv8_dealt_slot(p, h, first + b, row);
         step = n_rows;
     }
@@ -1277,6 +1280,7 @@ struct Kv8Plan {
     long long tiles;  // of one K/V head
     int nsplit;
     int share;      // above 0: keys are dealt to so many workgroups a head
+    int splits;     // no call with fewer items has more
 };
 // One tile of 16 rows where there are no more (and for listed blocks, one query's heads), else
 // workgroups of 64 rows, or more at D = 64 of 128 and at D = 128 and 256 of 256.  items: blocks of the
@@ -1296,10 +1300,12 @@ inline Kv8Plan kv8_plan(const Kv8& c, int T, int Hq, int items, bool list) {
     const long long want = few ? (1024 + all - 1) / all : (q.rows == 256 ? 256 : 512) / all;
     const long long most = few ? ((long long)items * parts + 7) / 8 : q.rows == 64 ? (items + 3) / 4 : (items + 1) / 2;
     long long n = want < most ? want : most;
+    n = n < 1 ? 1 : n < kKvMaxSplits ? n : kKvMaxSplits;
+    q.splits = (int)n;
     // The sums of splits of 256 rows that fill the chip take as long to write and join as 8 blocks to
     // multiply (7 x 640 tokens, 6/2 heads, D = 256: 56 us in 2 splits, 51 in one).
     if (q.rows == 256 && n > 1 && items * (n - 1) * 256 <= 8 * all * n * n) n = 1;
-    q.nsplit = (int)(n < 1 ? 1 : n < kKvMaxSplits ? n : kKvMaxSplits);
+    q.nsplit = (int)n;
     // Several sequences whose keys fill the chip: dealt out (parts are counted in ints).  Where two
     // stages a wave are the bound, most workgroups would have two short segments one after the other.
     q.share = few && !list && c.B > 1 && want > 1 && want < most && c.B * ((long long)c.max_blocks * parts + 4) < INT_MAX
@@ -1309,7 +1315,11 @@ inline Kv8Plan kv8_plan(const Kv8& c, int T, int Hq, int items, bool list) {
 inline size_t kv8_slots(const Kv8& c, int T, int Hq, const Kv8Plan& q) {
     return (q.share ? q.share + c.B : q.nsplit > 1 ? (size_t)c.B * q.nsplit : 0) * T * Hq;
 }
-inline size_t kv8_part_bytes(const Kv8& c, int T, int Hq, const Kv8Plan& q) { return kv8_slots(c, T, Hq, q) * (c.D + 2) * 4; }
+// Enough for every call with no more items too.
+inline size_t kv8_part_bytes(const Kv8& c, int T, int Hq, const Kv8Plan& q) {
+    const size_t own = kv8_slots(c, T, Hq, q), fewer = q.splits > 1 ? (size_t)c.B * q.splits * T * Hq : 0;
+    return (own > fewer ? own : fewer) * (c.D + 2) * 4;
+}
 
 template <int D, bool kList>
 hipError_t kv8_attn_d(const Kv8AttnArgs& p, const Kv8Plan& q, hipStream_t stream) {
