@@ -712,7 +712,9 @@ def test_another_stream(dev):
     s.wait_stream(torch.cuda.current_stream())
     tsa.attn_kv8_fwd(args[2], c, n, out=o, stream=s)
     tsa.attn_kv8_blocks_fwd(args[2], c, n, blocks, out=oq, stream=s)
+    own = tsa.attn_kv8_fwd(args[2], c, n, stream=s)
     s.synchronize()
+    assert torch.equal(own, o)
     want, tol = expect(q, k, v, [L], [1], True)
     check_out(o.cpu(), want, tol, "dense")
     lists = chosen(q, k, [L], [1], 8, 1, 1)

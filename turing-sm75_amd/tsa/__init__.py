@@ -643,8 +643,13 @@ def _queries(q, cache, gate, out, n_new, stream):
     qp = _rows(q, shape, "q", cache)
     gp = None if gate is None else _rows(gate, shape, "gate", cache)
     if out is None:
-        out = _zeros(shape, cache, stream) if n_new is not None else \
-            (_torch or _t()).empty(shape, dtype=q.dtype, device=cache.device)
+        if n_new is not None:
+            out = _zeros(shape, cache, stream)
+        elif stream is None:
+            out = (_torch or _t()).empty(shape, dtype=q.dtype, device=cache.device)
+        else:  # memory that no other stream's earlier work still uses
+            with (_torch or _t()).cuda.stream(stream):
+                out = _t().empty(shape, dtype=q.dtype, device=cache.device)
     return qp, gp, _rows(out, shape, "out", cache), out, Hq, T
 
 
