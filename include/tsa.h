@@ -279,7 +279,19 @@ int tsa_ggml_gated_delta_net(const tsa_tensor* q, const tsa_tensor* k, const tsa
  * rows behind them being padding that is neither read nor written.  New token t of a sequence is
  * at position len - n_new + t.  len is taken as at most 64 * max_blocks and at least 0, n_new as
  * at most T and at least 0; new tokens in front of position 0 (n_new > len) are not written and
- * see no key.  After a write, a sequence may be cut back (a smaller len) by up to 64 tokens.
+ * see no key.
+ *
+ * Cutting back: a sequence goes on from a smaller len, if that is a whole number of blocks or not
+ * below its lowest length.  The open blocks hold the last two blocks that the sequence wrote itself:
+ * the lowest length begins as the length its own writes begin at (0, or the tokens it took over in
+ * another sequence's pages); a write up to length M raises it to 64 * ((M - 1) / 64 - 1) if that is
+ * more; a cut below it, to a whole number of blocks, makes it that.  So it follows the longest
+ * length, and does not fall again when less is written after a cut.  Rejected drafts are always
+ * within it: of at most 64 tokens behind what was accepted, cut to no less than that.  Any other
+ * length is not told from a valid one and gives wrong keys and values (rows that the open blocks do
+ * not hold any more): to go on from there, cut to the whole block in front of it and write the
+ * rest again.  What is written behind a cut goes to the table's pages: where another sequence reads
+ * those too, name pages of this one's own first.
  * Calls on one cache must be ordered on one stream (or by the caller's events). ---- */
 typedef struct tsa_kv8 {
     void* k;

@@ -1,0 +1,88 @@
+"""The 8-bit K/V cache on the GPU: uses at the edge of what its header allows, against the same
+definitions and bounds as test_gpu_kv8.py."""
+import random
+
+import pytest
+import torch
+
+import kv8_oracle as ko
+import tsa
+from test_gpu_kv8 import check_out, check_rows, expect, ints, keys, rand
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------------------
+# cutting back, again and again
+# ---------------------------------------------------------------------------------------
+def check_holds(c, k, v, lens, what, dev):
+    """The cache's sequences are k[b], v[b] [H, len, D], bit for bit."""
+    kg, vg = (x.cpu() for x in tsa.kv8_read(c, ints(lens, dev), S=max(max(lens), 1)))
+    for b, n in enumerate(lens):
+        for h in range(c.Hkv):
+            check_rows(kg[b, h, :n], ko.Head(k[b][h, :n]).read, (what, b, h, "k"))
+            check_rows(vg[b, h, :n], ko.Head(v[b][h, :n]).read, (what, b, h, "v"))
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_cut_back_many_times(dev, seed):
+    """Writes of every size and cuts in turn, several between two writes, to any length from the lowest
+    on and to whole blocks below it: each time the sequence goes on as if what was cut had never come."""
+    rng = random.Random(seed)
+    gen = torch.Generator().manual_seed(50 + seed)
+    D, H, cap = (64, 128, 256, 64)[seed], 2, 640
+    c = tsa.Kv8Cache(1, H, D, cap, device=dev)
+    k, v, lowest = torch.zeros(H, 0, D).half(), torch.zeros(H, 0, D).half(), 0
+    for i in range(14):
+        T = min(rng.choice([1, 1, 2, 5, 17, 63, 64, 65, 128, 129, 200]), cap - k.shape[1])
+        if T == 0:
+            k, v, lowest = k[:, :64], v[:, :64], 64
+            continue
+        kn, vn = (x[0] for x in keys(gen, 1, H, T, D))
+        k, v = torch.cat([k, kn], 1), torch.cat([v, vn], 1)
+        n = k.shape[1]
+        tsa.kv8_write(c, kn[None].to(dev), vn[None].to(dev), ints([n], dev))
+        lowest = max(lowest, 64 * ((n - 1) // 64 - 1))
+        check_holds(c, [k], [v], [n], (seed, i, "written"), dev)
+        for _ in range(rng.randint(0, 2)):
+            n = k.shape[1]
+            n = 64 * rng.randint(0, n // 64) if rng.random() < 0.3 else rng.randint(min(lowest, n), n)
+            k, v, lowest = k[:, :n], v[:, :n], min(lowest, n)
+            check_holds(c, [k], [v], [n], (seed, i, "cut"), dev)
+    n = k.shape[1]
+    q = rand(gen, 1, 2 * H, 1, D)
+    want, tol = expect(q, k[None], v[None], [n], [1], True) if n else (torch.zeros_like(q).double(), torch.zeros_like(q).double())
+    check_out(tsa.attn_kv8_fwd(q.to(dev), c, ints([n], dev)).cpu(), want, tol, seed)
+
+
+def test_cut_back_behind_a_shared_prefix(dev):
+    """A sequence that took over 128 tokens in another's pages is cut back to no less than those, and to
+    a whole block inside them with pages of its own named first: the other sequence keeps its bytes."""
+    gen = torch.Generator().manual_seed(61)
+    D, H = 64, 2
+    k, v = keys(gen, 2, H, 360, D)
+    k[1, :, :128], v[1, :, :128] = k[0, :, :128], v[0, :, :128]
+    c = tsa.Kv8Cache(2, H, D, 320, n_pages=9, device=dev)
+    c.table.copy_(ints([[0, 1, 2, 3, -1], [0, 1, 4, 5, 6]], dev))
+
+    def write(at, new):
+        T = max(new)
+        kn, vn = (torch.stack([x[b, :, at[b]:at[b] + T] for b in range(2)]) for x in (k, v))
+        tsa.kv8_write(c, kn.to(dev), vn.to(dev), ints([a + n for a, n in zip(at, new)], dev), ints(new, dev))
+
+    write([0, 128], [128, 0])
+    write([128, 128], [70, 5])
+    lens = [198, 133]
+    check_holds(c, k, v, lens, "written", dev)
+    pages = [getattr(c, x)[:4].clone() for x in ("k", "v", "k_scale", "v_scale", "k_sum", "k_sum_scale")]
+    for n, T in ((130, 60), (128, 100), (192, 7)):  # the lowest length is 128 each time
+        check_holds(c, k, v, [198, n], ("cut", n), dev)
+        k[1:, :, n:], v[1:, :, n:] = keys(gen, 1, H, 360 - n, D)
+        write([198, n], [0, T])
+        check_holds(c, k, v, [198, n + T], ("on from", n), dev)
+    c.table[1, 1] = 7
+    k[1:, :, 64:], v[1:, :, 64:] = keys(gen, 1, H, 296, D)
+    write([198, 64], [0, 150])
+    check_holds(c, k, v, [198, 214], "on from a whole block", dev)
+    for x, before in zip(("k", "v", "k_scale", "v_scale", "k_sum", "k_sum_scale"), pages):
+        assert torch.equal(getattr(c, x)[:4], before), x

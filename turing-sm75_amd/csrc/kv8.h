@@ -3,8 +3,11 @@
 //
 // A block is 64 tokens of one sequence.  A full block of one K/V head is 64 x D codes, a byte
 // each (code + 128, code = rint(127 x / max|x|) in -127 .. 127), with one fp32 scale max|x| / 127.
-// The tokens behind the last full block are fp16 rows in a ring of two blocks per sequence, so a
-// sequence may be cut back by up to a block.
+// The tokens behind the last full block are fp16 rows in a ring of two blocks per sequence, block i
+// in slot i % 2.  A write keeps its rows of the last block that it touches and of the one before, so
+// a sequence may be cut back to any length in the two blocks at its longest length's end, as far as
+// it wrote them itself; further back only to whole blocks, which need no row of the ring.  (After
+// 129 tokens, a cut to 65 and one more, block 0 is still not in the ring: slot 0 is block 2's.)
 //
 // Both are laid out as the operands of v_mfma_f32_16x16x32_f16 (lane l holds row l % 16 and 8
 // consecutive k at 8 * (l / 16)), so that a wave reads 1 KiB of consecutive codes per load, 16
