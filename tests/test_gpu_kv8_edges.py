@@ -86,3 +86,31 @@ def test_cut_back_behind_a_shared_prefix(dev):
     check_holds(c, k, v, [198, 214], "on from a whole block", dev)
     for x, before in zip(("k", "v", "k_scale", "v_scale", "k_sum", "k_sum_scale"), pages):
         assert torch.equal(getattr(c, x)[:4], before), x
+
+
+# ---------------------------------------------------------------------------------------
+# rows that see no key
+# ---------------------------------------------------------------------------------------
+FORMS = [(64, 2, 3), (128, 6, 1), (256, 1, 5), (64, 1, 40), (128, 2, 30), (256, 3, 20), (64, 3, 70), (128, 2, 170), (256, 1, 300)]
+
+
+@pytest.mark.parametrize("D,G,T", FORMS)
+@pytest.mark.parametrize("causal", [True, False])
+def test_rows_in_front_of_the_sequence(dev, D, G, T, causal):
+    """More new tokens than the sequence has: those in front of position 0 see no key, with the causal
+    mask and without it, and their rows are 0; the others attend as ever."""
+    gen = torch.Generator().manual_seed(D + T)
+    lens, new = [max(1, T // 2), 1, 0, T], [T, T, T, T]
+    B = len(lens)
+    k, v = keys(gen, B, 1, T, D)
+    c = tsa.Kv8Cache(B, 1, D, T, device=dev)
+    tsa.kv8_write(c, k.to(dev), v.to(dev), ints(lens, dev), ints(lens, dev))
+    q = rand(gen, B, G, T, D)
+    for counts in (None, ints(new, dev)):
+        out = torch.full(q.shape, 9.0, dtype=torch.float16, device=dev)
+        tsa.attn_kv8_fwd(q.to(dev), c, ints(lens, dev), counts, out=out, causal=causal)
+        for b, n in enumerate(lens):
+            assert not bool(out[b, :, :T - n].any()), (b, causal)
+            if n:
+                want, tol = expect(q[b:b + 1, :, T - n:], k[b:b + 1], v[b:b + 1], [n], [n], causal)
+                check_out(out[b:b + 1, :, T - n:].cpu(), want, tol, (b, causal))

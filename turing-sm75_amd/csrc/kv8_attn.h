@@ -330,6 +330,11 @@ __device__ __forceinline__ void kv8_queries(Kv8Rows<D>& st, const Kv8AttnArgs& p
         for (int s = 0; s < 2; ++s)
             st.q[2 * i + s] = row < row_end ? *reinterpret_cast<const half8_t*>(qr + 64 * i + 16 * g4 + 8 * s) : half8_t{};
 }
+// The last key that query row t G + g sees.  A row in front of position 0 sees none, causal or not.
+__device__ __forceinline__ int kv8_limit(const Kv8AttnArgs& p, const Kv8Seq& sq, int row) {
+    const int pos = sq.len - (sq.n + sq.t0) + row / p.G;
+    return pos < 0 ? -1 : p.causal ? min(pos, sq.len - 1) : sq.len - 1;
+}
 // NT tiles from row0 on with nothing summed yet, and which keys they see: the last that any row
 // does (`most`) and the last that all do (`least`).
 template <int D, int NT>
@@ -342,8 +347,7 @@ __device__ __forceinline__ void kv8_begin(Kv8Rows<D> (&st)[NT], const Kv8AttnArg
         kv8_queries<D>(st[nt], p, b, h, row0 + 16 * nt, row_end);
         const int row = row0 + 16 * nt + (int)(threadIdx.x & 15);
         const bool is = row < row_end;
-        const int pos = sq.len - (sq.n + sq.t0) + row / p.G;  // below 0: in front of the sequence
-        st[nt].limit = !is ? -1 : p.causal ? min(pos, sq.len - 1) : sq.len - 1;
+        st[nt].limit = is ? kv8_limit(p, sq, row) : -1;
         most = max(most, st[nt].limit);
         if (is) least = min(least, st[nt].limit);
 #pragma unroll
@@ -1052,8 +1056,7 @@ kv8_wide_kernel(Kv8AttnArgs p, int tiles, int streams) {
     const half_t* qr = kv8_query32(p, at.b, at.h, row);
 #pragma unroll
     for (int u = 0; u < D / 16; ++u) st.q[u] = row < row_end ? *reinterpret_cast<const half8_t*>(qr + 16 * u) : half8_t{};
-    const int pos = sq.len - (sq.n + sq.t0) + row / p.G;  // below 0: in front of the sequence
-    st.limit = row >= row_end ? -1 : p.causal ? min(pos, sq.len - 1) : sq.len - 1;
+    st.limit = row < row_end ? kv8_limit(p, sq, row) : -1;
     int see = st.limit, least = row < row_end ? st.limit : INT_MAX;  // the last key that any, that every row sees
 #pragma unroll
     for (int x = 1; x < 32; x <<= 1) {
