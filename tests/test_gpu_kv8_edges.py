@@ -1,5 +1,6 @@
 """The 8-bit K/V cache on the GPU: uses at the edge of what its header allows, against the same
 definitions and bounds as test_gpu_kv8.py."""
+import math
 import random
 
 import pytest
@@ -7,7 +8,7 @@ import torch
 
 import kv8_oracle as ko
 import tsa
-from test_gpu_kv8 import check_out, check_rows, expect, ints, keys, rand
+from test_gpu_kv8 import check_out, check_rows, expect, fill, ints, keys, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -89,7 +90,7 @@ def test_cut_back_behind_a_shared_prefix(dev):
 
 
 # ---------------------------------------------------------------------------------------
-# rows that see no key
+# rows that see no key, infinities in open keys, output over the queries
 # ---------------------------------------------------------------------------------------
 FORMS = [(64, 2, 3), (128, 6, 1), (256, 1, 5), (64, 1, 40), (128, 2, 30), (256, 3, 20), (64, 3, 70), (128, 2, 170), (256, 1, 300)]
 
@@ -114,3 +115,64 @@ def test_rows_in_front_of_the_sequence(dev, D, G, T, causal):
             if n:
                 want, tol = expect(q[b:b + 1, :, T - n:], k[b:b + 1], v[b:b + 1], [n], [n], causal)
                 check_out(out[b:b + 1, :, T - n:].cpu(), want, tol, (b, causal))
+
+
+@pytest.mark.parametrize("D,G,T", FORMS)
+@pytest.mark.parametrize("what", [math.inf, -math.inf])
+def test_infinite_key_in_the_open_block(dev, D, G, T, what):
+    """A query's score with it is an infinity of its own sign: below every other, the key weighs 0 and
+    the rest stays; above them, the row is NaN.  Queries in front of it see neither."""
+    gen = torch.Generator().manual_seed(D + G + T)
+    L = 64 * max(3, T // 64 + 1) + 40
+    where = L - 1 - T // 2 if T < 40 else L - 20
+    k, v = keys(gen, 1, 1, L, D)
+    q = rand(gen, 1, G, T, D)
+    q[..., 5] = torch.where(q[..., 5] < 0, -1, 1) * q[..., 5].abs().clamp_min(0.01)
+    k[0, 0, where, 5] = what
+    o = tsa.attn_kv8_fwd(q.to(dev), fill(dev, k, v, [L]), ints([L], dev)).cpu()
+    k[0, 0, where, 5] = 0
+    K, V = ko.Head(k[0, 0]).values, ko.Head(v[0, 0])
+    for g in range(G):
+        for t in range(T):
+            p = L - T + t
+            if p >= where and float(q[0, g, t, 5]) * what > 0:
+                assert bool(o[0, g, t].isnan().all()), (g, t)
+            else:
+                see = [j for j in range(p + 1) if j != where]
+                want, tol = ko.attend(q[0, g, t], K, V.values, V.steps, see, 1 / math.sqrt(D))
+                check_out(o[0, g, t], want, tol, (g, t))
+
+
+@pytest.mark.parametrize("D,G,T", FORMS)
+def test_output_over_the_queries(dev, D, G, T):
+    """o = q in every form, its keys split or not: the same bytes as in a buffer of its own."""
+    gen = torch.Generator().manual_seed(2 * D + T)
+    for H, L in ((2, T + 70), (1, T + 2500)):
+        k, v = (x.to(dev) for x in keys(gen, 2, H, L, D))
+        n = ints([L, L - 50], dev)
+        c = tsa.Kv8Cache(2, H, D, L, device=dev)
+        tsa.kv8_write(c, k, v, n, n)
+        buf = rand(gen, 2, T, H * G, 2 * D).to(dev)  # a token-major projection of q and gate
+        q, gate = buf[..., :D].transpose(1, 2), buf[..., D:].transpose(1, 2)
+        blocks = tsa.kv8_select(q, c, n, 4)
+        for call in (lambda **kw: tsa.attn_kv8_fwd(q, c, n, gate=gate, **kw), lambda **kw: tsa.attn_kv8_blocks_fwd(q, c, n, blocks, gate=gate, **kw)):
+            before = q.clone()
+            want = call()
+            call(out=q)
+            assert torch.equal(q, want), (H, L)
+            q.copy_(before)
+
+
+def test_output_over_the_queries_of_many_listed_tiles(dev):
+    """The form that takes a listed tile a wave, and a group of more heads than a tile has."""
+    gen = torch.Generator().manual_seed(71)
+    D, H, G, T, L = 64, 2, 17, 600, 900
+    k, v = (x.to(dev) for x in keys(gen, 1, H, L, D))
+    n = ints([L], dev)
+    c = tsa.Kv8Cache(1, H, D, L, device=dev)
+    tsa.kv8_write(c, k, v, n)
+    q = rand(gen, 1, H * G, T, D).to(dev)
+    blocks = tsa.kv8_select(q, c, n, 3)
+    want = tsa.attn_kv8_blocks_fwd(q, c, n, blocks)
+    tsa.attn_kv8_blocks_fwd(q, c, n, blocks, out=q)
+    assert torch.equal(q, want)
