@@ -42,10 +42,6 @@ __device__ __forceinline__ int kv8_v_at(int r, int d) {
     return ((((r >> 5) * (D / 32) + (d >> 5)) * 4 + ((r >> 2) & 3)) * 16 + (d & 15)) * 16 + ((d >> 4) & 1) * 8 +
            ((r >> 4) & 1) * 4 + (r & 3);
 }
-template <int D>
-__device__ __forceinline__ int kv8_at(bool isv, int r, int d) {
-    return isv ? kv8_v_at<D>(r, d) : kv8_k_at<D>(r, d);
-}
 
 // 127 x / a as a division would round it (with r = 1 / a rounded, one correction of y r by its exact
 // remainder gives the correctly rounded quotient), then to a whole number, ties to even: the sum
