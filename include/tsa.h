@@ -327,7 +327,9 @@ int tsa_kv8_read(const tsa_kv8* cache, const int32_t* len, const int32_t* start,
 /* Workspace bytes of the calls below for T rows of Hq query heads; max_len: no sequence is longer
  * (at most 64 * max_blocks).  top = 0: tsa_attn_kv8_fwd; top > 0: tsa_kv8_select and
  * tsa_attn_kv8_blocks_fwd, which may share one workspace.  0 for invalid arguments, and where no
- * workspace is needed; enough for calls of a smaller max_len as well.  A workspace is 16-byte aligned.  Hq / Hkv is at most 65536.  Calls that share a workspace must be ordered on one stream. */
+ * workspace is needed; enough for calls of a smaller max_len as well.  A workspace is 16-byte
+ * aligned.  Hq / Hkv is at most 65536, B * Hq * T at most 2^31 - 1.  Calls that share a workspace must be
+ * ordered on one stream. */
 size_t tsa_kv8_workspace_bytes(const tsa_kv8* cache, int T, int Hq, int max_len, int top);
 
 /* Attention of T new tokens per sequence over the cache that holds them already (write first):
@@ -348,7 +350,7 @@ int tsa_attn_kv8_fwd(const tsa_kv8* cache, const tsa_rows* q, const tsa_rows* ga
  * (first + recent + 1 <= top <= 2^24).  A full block that holds an infinity or NaN, or has no page, scores
  * below every other; a group with an infinity or NaN scores every block 0.
  * blocks: int32 [B][Hkv][T][top], ascending, -1 behind the last; rows of padding are left as they
- * were.  Blocks behind max_len have no score. */
+ * were.  Blocks behind max_len have no score; T times its blocks is at most 2^31 - 1. */
 int tsa_kv8_select(const tsa_kv8* cache, const tsa_rows* q, const int32_t* len, const int32_t* n_new, int T, int Hq,
                    int top, int first, int recent, int32_t* blocks, int max_len, void* ws, size_t ws_bytes,
                    void* stream);

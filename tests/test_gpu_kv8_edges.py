@@ -176,3 +176,23 @@ def test_output_over_the_queries_of_many_listed_tiles(dev):
     want = tsa.attn_kv8_blocks_fwd(q, c, n, blocks)
     tsa.attn_kv8_blocks_fwd(q, c, n, blocks, out=q)
     assert torch.equal(q, want)
+
+
+@pytest.mark.parametrize("D,T", [(64, 300), (128, 260)])
+def test_long_queries_over_a_large_capacity(dev, D, T):
+    """Queries and blocks of capacity whose product passes 32 bits, with a few blocks in use; a selection
+    with a max_len that holds every sequence."""
+    gen = torch.Generator().manual_seed(81)
+    L = T + 150
+    k, v = keys(gen, 1, 1, L, D)
+    c = tsa.Kv8Cache(1, 1, D, 64 << 23, n_pages=8, device=dev)
+    c.table[0, :8] = torch.arange(8, dtype=torch.int32, device=dev)
+    tsa.kv8_write(c, k.to(dev), v.to(dev), ints([L], dev))
+    q = rand(gen, 1, 1, T, D)
+    want, tol = expect(q, k, v, [L], [T], True)
+    check_out(tsa.attn_kv8_fwd(q.to(dev), c, ints([L], dev)).cpu(), want, tol, "dense")
+    blocks = tsa.kv8_select(q.to(dev), c, ints([L], dev), 100, max_len=L)
+    check_out(tsa.attn_kv8_blocks_fwd(q.to(dev), c, ints([L], dev), blocks).cpu(), want, tol, "sparse")
+    with pytest.raises(tsa.TsaError) as e:
+        tsa.kv8_select(q.to(dev), c, ints([L], dev), 100)
+    assert e.value.code == tsa.TSA_ERR_SHAPE

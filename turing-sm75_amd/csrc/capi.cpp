@@ -366,11 +366,10 @@ tsa::Rows16 as_rows(const tsa_rows* r, int B, int H, int T) {
     return {static_cast<_Float16*>(r->data), B > 1 ? r->stride_b : 0, H > 1 ? r->stride_h : 0, T > 1 ? r->stride_t : 0};
 }
 
-// Queries: rows per K/V head and workgroups must fit an int, and a group's elements too.
+// Queries: rows of all heads must fit an int, and a group's elements too.
 int check_kv8_queries(const tsa_kv8* c, int T, int Hq) {
     if (T < 1 || Hq < 1 || Hq % c->Hkv != 0 || Hq / c->Hkv > 65536) return TSA_ERR_SHAPE;
-    if (!fits_int(c->B, Hq, T) || !fits_int(T, c->max_blocks)) return TSA_ERR_SHAPE;
-    return TSA_OK;
+    return fits_int(c->B, Hq, T) ? TSA_OK : TSA_ERR_SHAPE;
 }
 
 // Entries of a list: the kernels count parts of blocks in ints.
@@ -425,7 +424,8 @@ extern "C" int tsa_kv8_read(const tsa_kv8* cache, const int32_t* len, const int3
 
 extern "C" size_t tsa_kv8_workspace_bytes(const tsa_kv8* cache, int T, int Hq, int max_len, int top) {
     if (check_kv8(cache) || check_kv8_queries(cache, T, Hq) || max_len < 1 || (top != 0 && !fits_top(top))) return 0;
-    return tsa::kv8_ws_bytes(as_kv8(cache), T, Hq, kv8_nb(cache, max_len), top);
+    const int nb = kv8_nb(cache, max_len);
+    return top != 0 && !fits_int(T, nb) ? 0 : tsa::kv8_ws_bytes(as_kv8(cache), T, Hq, nb, top);
 }
 
 extern "C" int tsa_attn_kv8_fwd(const tsa_kv8* cache, const tsa_rows* q, const tsa_rows* gate, const tsa_rows* o,
@@ -452,6 +452,7 @@ extern "C" int tsa_kv8_select(const tsa_kv8* cache, const tsa_rows* q, const int
     if (max_len < 1 || !fits_top(top) || first < 0 || recent < 0) return TSA_ERR_SHAPE;
     if ((long long)first + recent + 1 > top) return TSA_ERR_ARG;
     const int B = cache->B, nb = kv8_nb(cache, max_len);
+    if (!fits_int(T, nb)) return TSA_ERR_SHAPE;  // a query's scores of all blocks: the launch's workgroups
     if ((rc = check_rows(q, B, Hq, T, false))) return rc;
     const size_t need = tsa::kv8_ws_bytes(as_kv8(cache), T, Hq, nb, top);
     if ((rc = check_ws(ws, ws_bytes, need))) return rc;
