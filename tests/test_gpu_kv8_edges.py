@@ -196,3 +196,18 @@ def test_long_queries_over_a_large_capacity(dev, D, T):
     with pytest.raises(tsa.TsaError) as e:
         tsa.kv8_select(q.to(dev), c, ints([L], dev), 100)
     assert e.value.code == tsa.TSA_ERR_SHAPE
+
+
+@pytest.mark.parametrize("G,T", [(1, 65), (2, 40), (8, 16), (4, 32)])
+@pytest.mark.parametrize("blocks", [64, 4096, 4097])
+def test_tiles_of_medium_row_counts(dev, G, T, blocks):
+    """65 to 128 rows at D = 64: two tiles of 64 rows, and with max_len behind 4096 blocks one of 128."""
+    gen = torch.Generator().manual_seed(90 + T)
+    lens = [T + 777]
+    k, v = keys(gen, 1, 1, lens[0], 64)
+    c = tsa.Kv8Cache(1, 1, 64, 64 * blocks, device=dev)
+    tsa.kv8_write(c, k.to(dev), v.to(dev), ints(lens, dev))
+    q = rand(gen, 1, G, T, 64)
+    o = tsa.attn_kv8_fwd(q.to(dev), c, ints(lens, dev))
+    want, tol = expect(q, k, v, lens, [T], True)
+    check_out(o.cpu(), want, tol, (G, T, blocks))

@@ -1285,13 +1285,21 @@ struct Kv8Plan {
     int share;      // above 0: keys are dealt to so many workgroups a head
     int splits;     // no call with fewer items has more
 };
+// At D = 64 65 to 128 rows are two tiles of 64 where the call has at most this many blocks (a
+// sequence's by the K/V heads), and one of 128 above.  Up to 16 blocks a CU the call waits more than it
+// computes, and twice the workgroups wait less (96 rows, 8 x 2777 keys, 2 heads: 20.2 us with 128 rows, 16.0
+// with 64; 1 x 32000, 4 heads: 36.0, 26.9; at 4096 blocks 25.5 to 38.6, 26.7 to 33.2); with more, two tiles
+// convert every code twice (32 x 8000, 2 heads: 38.7, 42.1).
+constexpr long long kKvSmallTileBlocks = 4096;
+
 // One tile of 16 rows where there are no more (and for listed blocks, one query's heads), else
 // workgroups of 64 rows, or more at D = 64 of 128 and at D = 128 and 256 of 256.  items: blocks of the
 // longest sequence, or of a list.
 inline Kv8Plan kv8_plan(const Kv8& c, int T, int Hq, int items, bool list) {
     const long long G = Hq / c.Hkv, rows = T * G;
     Kv8Plan q;
-    q.rows = list || rows <= 16 ? 16 : rows <= (c.D == 64 ? 64 : 128) ? 64 : c.D == 64 ? 128 : 256;
+    const bool small = rows <= 64 || (rows <= 128 && (c.D != 64 || (long long)c.B * c.Hkv * items <= kKvSmallTileBlocks));
+    q.rows = list || rows <= 16 ? 16 : small ? 64 : c.D == 64 ? 128 : 256;
     q.tiles = list ? T * ((G + 15) / 16) : (rows + q.rows - 1) / q.rows;
     const long long all = q.tiles * c.B * c.Hkv;
     // row tiles: as many workgroups as the chip takes twice, but two stages of keys a wave at the
