@@ -63,9 +63,12 @@ __device__ __forceinline__ T kv8_uniform(const T* p) {
     return *(const __attribute__((address_space(4))) T*)(uintptr_t)p;
 }
 
-// 16 codes.  kOnce: no other workgroup of the call reads them, and they pass the caches by
-// (attention of one token each for 32 sequences of up to 32768, D = 256: 308 -> 283 us; where
-// queries share their blocks, 115 -> 184 us).
+// 16 codes.  kOnce: no other workgroup of the call reads them, unless sequences share their pages, and
+// they pass the caches by (attention of one token each for 32 sequences of up to 32768, D = 256: 308 ->
+// 283 us; where queries share their blocks, 115 -> 184 us).  Sequences that share pages pay for it: the
+// host does not see their tables, and pages of a sequence's own are taken for the common case (32 x
+// 32768, 24/4 heads, D = 256: own pages 378 us past the caches and 403 through them, all pages shared
+// 194 and 132).
 template <bool kOnce>
 __device__ __forceinline__ uint4 kv8_codes(const uint4* p) {
     typedef unsigned uint4_v __attribute__((ext_vector_type(4)));
