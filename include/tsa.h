@@ -337,7 +337,7 @@ size_t tsa_kv8_workspace_bytes(const tsa_kv8* cache, int T, int Hq, int max_len,
  * times sigmoid(gate) when gate is not NULL.  q, gate, o [B][Hq][T][D], Hq % Hkv == 0, query head
  * h reads K/V head h / (Hq / Hkv); D in {64, 128, 256}.  A query that sees no key gets 0.  o may
  * be q.  max_len: no sequence is longer; it decides only how the keys are split over workgroups
- * (results for longer ones are right as well). */
+ * (results for longer ones are right as well; last bits may depend on it). */
 int tsa_attn_kv8_fwd(const tsa_kv8* cache, const tsa_rows* q, const tsa_rows* gate, const tsa_rows* o,
                      const int32_t* len, const int32_t* n_new, int T, int Hq, int max_len, float scale, int causal,
                      void* ws, size_t ws_bytes, void* stream);
@@ -350,7 +350,8 @@ int tsa_attn_kv8_fwd(const tsa_kv8* cache, const tsa_rows* q, const tsa_rows* ga
  * (first + recent + 1 <= top <= 2^24).  A full block that holds an infinity or NaN, or has no page, scores
  * below every other; a group with an infinity or NaN scores every block 0.
  * blocks: int32 [B][Hkv][T][top], ascending, -1 behind the last; rows of padding are left as they
- * were.  Blocks behind max_len have no score; T times its blocks is at most 2^31 - 1. */
+ * were.  Blocks behind max_len have no score and come last: it is to be no less than any sequence's
+ * length, in replays of a captured call too.  T times its blocks is at most 2^31 - 1. */
 int tsa_kv8_select(const tsa_kv8* cache, const tsa_rows* q, const int32_t* len, const int32_t* n_new, int T, int Hq,
                    int top, int first, int recent, int32_t* blocks, int max_len, void* ws, size_t ws_bytes,
                    void* stream);

@@ -669,7 +669,7 @@ def attn_kv8_fwd(q, cache, len, n_new=None, gate=None, out=None, scale=None, cau
     cache that holds them already: softmax(scale q K^T) V over the keys up to each query's own
     (causal) or all len of them, times sigmoid(gate) if given.  Hq % Hkv == 0.  Rows of padding
     (t >= n_new) are left as they were (0 in an output made here).  max_len: no sequence is longer (a
-    tighter split of the keys; results do not depend on it)."""
+    tighter split of the keys: results for longer ones are right too, their last bits may depend on it)."""
     qp, gp, op, out, Hq, T = _queries(q, cache, gate, out, n_new, stream)
     if max_len is None:
         max_len = cache.max_len
@@ -692,8 +692,8 @@ def _blocks(blocks, cache, T, top):
 def kv8_select(q, cache, len, top, n_new=None, first=1, recent=1, out=None, max_len=None, ws=None, stream=None):
     """The blocks [B, Hkv, T, top] int32 that each query of q [B, Hq, T, D] attends to: the first
     `first`, its own and the `recent` before it, and the best by score, ascending, -1 behind the last.
-    Rows of padding are left as they were (-1 in an output made here).  max_len: no sequence is longer
-    (blocks behind it have no score)."""
+    Rows of padding are left as they were (-1 in an output made here).  max_len: no sequence is longer,
+    nor becomes so in replays of a captured call (blocks behind it have no score and are chosen last)."""
     torch = _torch or _t()
     if q.dim() != 4:
         raise ValueError(f"q: expected [B, Hq, T, D], got {tuple(q.shape)}")
