@@ -211,3 +211,19 @@ def test_tiles_of_medium_row_counts(dev, G, T, blocks):
     o = tsa.attn_kv8_fwd(q.to(dev), c, ints(lens, dev))
     want, tol = expect(q, k, v, lens, [T], True)
     check_out(o.cpu(), want, tol, (G, T, blocks))
+
+
+def test_numbers_beyond_32_bits(dev):
+    """A max_len behind any length is the cache's own; numbers of blocks that no C int holds are refused."""
+    gen = torch.Generator().manual_seed(95)
+    D, L = 64, 64 * 20 + 5
+    k, v = keys(gen, 1, 1, L, D)
+    c = fill(dev, k, v, [L])
+    q, n = rand(gen, 1, 2, 3, D).to(dev), ints([L], dev)
+    for far in (1 << 31, (1 << 32) + 64, 1 << 40):
+        assert tsa.kv8_workspace_bytes(c, 3, 2, far) == tsa.kv8_workspace_bytes(c, 3, 2)
+        assert torch.equal(tsa.attn_kv8_fwd(q, c, n, max_len=far), tsa.attn_kv8_fwd(q, c, n))
+        assert torch.equal(tsa.kv8_select(q, c, n, 5, max_len=far), tsa.kv8_select(q, c, n, 5))
+        for kw in (dict(first=far), dict(recent=far), dict(first=-far - 1)):
+            with pytest.raises(ValueError):
+                tsa.kv8_select(q, c, n, 5, **kw)

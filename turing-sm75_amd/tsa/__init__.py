@@ -628,10 +628,15 @@ def _zeros(shape, cache, stream, dtype=None, value=0):
         return torch.full(shape, value, dtype=dtype or torch.float16, device=cache.device)
 
 
+def _max_len(max_len, cache):
+    """No sequence is longer than the cache, and a C int holds no more."""
+    return cache.max_len if max_len is None or max_len > cache.max_len else max_len
+
+
 def kv8_workspace_bytes(cache, T, Hq, max_len=None, top=0) -> int:
     """Workspace bytes of attn_kv8_fwd (top = 0), or of kv8_select and attn_kv8_blocks_fwd, which may
     share one (top > 0)."""
-    return int(load().tsa_kv8_workspace_bytes(cache._ref, T, Hq, cache.max_len if max_len is None else max_len, top))
+    return int(load().tsa_kv8_workspace_bytes(cache._ref, T, Hq, _max_len(max_len, cache), top))
 
 
 def _queries(q, cache, gate, out, n_new, stream):
@@ -671,8 +676,7 @@ def attn_kv8_fwd(q, cache, len, n_new=None, gate=None, out=None, scale=None, cau
     (t >= n_new) are left as they were (0 in an output made here).  max_len: no sequence is longer (a
     tighter split of the keys: results for longer ones are right too, their last bits may depend on it)."""
     qp, gp, op, out, Hq, T = _queries(q, cache, gate, out, n_new, stream)
-    if max_len is None:
-        max_len = cache.max_len
+    max_len = _max_len(max_len, cache)
     wp, wn, ws = _ws(ws, cache, T, Hq, max_len, 0, stream)
     _kv8_call(load().tsa_attn_kv8_fwd, cache, stream, qp, gp, op, _len(len, cache),
               None if n_new is None else _counts(n_new, "n_new", cache), T, Hq, max_len,
@@ -699,10 +703,11 @@ def kv8_select(q, cache, len, top, n_new=None, first=1, recent=1, out=None, max_
         raise ValueError(f"q: expected [B, Hq, T, D], got {tuple(q.shape)}")
     _, Hq, T, _ = q.shape
     qp = _rows(q, (cache.B, Hq, T, cache.D), "q", cache)
+    if min(top, first, recent) < -1 << 31 or max(top, first, recent) >= 1 << 31:
+        raise ValueError(f"top = {top}, first = {first}, recent = {recent}: at least one is no 32-bit number")
     if out is None:
         out = _zeros((cache.B, cache.Hkv, T, top), cache, stream, torch.int32, -1)
-    if max_len is None:
-        max_len = cache.max_len
+    max_len = _max_len(max_len, cache)
     wp, wn, ws = _ws(ws, cache, T, Hq, max_len, top, stream)
     _kv8_call(load().tsa_kv8_select, cache, stream, qp, _len(len, cache),
               None if n_new is None else _counts(n_new, "n_new", cache), T, Hq, top, first, recent, _blocks(out, cache, T, top),
