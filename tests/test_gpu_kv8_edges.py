@@ -227,3 +227,36 @@ def test_numbers_beyond_32_bits(dev):
         for kw in (dict(first=far), dict(recent=far), dict(first=-far - 1)):
             with pytest.raises(ValueError):
                 tsa.kv8_select(q, c, n, 5, **kw)
+
+
+@pytest.mark.parametrize("D,B,Hkv,G,T,L,cap", [(64, 1, 2, 4, 1, 3000, 3000), (128, 5, 2, 3, 2, 700, 1 << 16), (256, 1, 4, 6, 1, 500, 1 << 15), (64, 70, 1, 2, 1, 200, 1 << 14),
+                                               (64, 2, 1, 8, 9, 900, 900), (64, 1, 1, 8, 70, 2000, 2000), (128, 1, 2, 2, 40, 1500, 1500), (256, 1, 1, 1, 300, 2500, 2500)])
+def test_workspace_of_exactly_its_size(dev, D, B, Hkv, G, T, L, cap):
+    """A call keeps within the bytes that it asks for, with max_len exact, too short and as large as the
+    cache, and gives the same rows whatever the workspace held."""
+    gen = torch.Generator().manual_seed(D + T)
+    c = tsa.Kv8Cache(B, Hkv, D, cap, n_pages=B * (L // 64 + 1), device=dev)
+    c.table[:, :L // 64 + 1] = torch.arange(c.n_pages, dtype=torch.int32, device=dev).view(B, -1)
+    k, v = (rand(gen, B, Hkv, L, D).to(dev) for _ in range(2))
+    n = ints([L - 3 * b for b in range(B)], dev)
+    tsa.kv8_write(c, k, v, n, n)
+    q = rand(gen, B, Hkv * G, T, D).to(dev)
+
+    def guarded(bytes_, fill_):
+        ws = torch.full((bytes_ + 4096,), fill_, dtype=torch.uint8, device=dev)
+        return ws, ws[:bytes_]
+
+    for max_len in (L, 64, None):
+        outs = []
+        for byte in (0xff, 0):
+            whole, ws = guarded(tsa.kv8_workspace_bytes(c, T, Hkv * G, max_len), byte)
+            outs.append(tsa.attn_kv8_fwd(q, c, n, max_len=max_len, ws=ws))
+            assert bool((whole[len(ws):] == byte).all())
+        assert torch.equal(*outs)
+    outs = []
+    for byte in (0xff, 0):
+        whole, ws = guarded(tsa.kv8_workspace_bytes(c, T, Hkv * G, L, 4), byte)
+        blocks = tsa.kv8_select(q, c, n, 4, max_len=L, ws=ws)
+        outs.append((blocks, tsa.attn_kv8_blocks_fwd(q, c, n, blocks, ws=ws)))
+        assert bool((whole[len(ws):] == byte).all())
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
