@@ -335,9 +335,10 @@ size_t tsa_kv8_workspace_bytes(const tsa_kv8* cache, int T, int Hq, int max_len,
 /* Attention of T new tokens per sequence over the cache that holds them already (write first):
  * O = softmax(scale * q K^T) V over the keys j <= the query's position (causal = 1) or j < len,
  * times sigmoid(gate) when gate is not NULL.  q, gate, o [B][Hq][T][D], Hq % Hkv == 0, query head
- * h reads K/V head h / (Hq / Hkv); D in {64, 128, 256}.  A query that sees no key gets 0.  o may
- * be q.  max_len: no sequence is longer; it decides only how the keys are split over workgroups
- * (results for longer ones are right as well; last bits may depend on it). */
+ * h reads K/V head h / (Hq / Hkv); D in {64, 128, 256}.  A query that sees no key, or whose scores
+ * are all minus infinity, gets 0.  o may be q.  max_len: no sequence is longer; it decides only how
+ * the keys are split over workgroups (results for longer ones are right as well; last bits may
+ * depend on it). */
 int tsa_attn_kv8_fwd(const tsa_kv8* cache, const tsa_rows* q, const tsa_rows* gate, const tsa_rows* o,
                      const int32_t* len, const int32_t* n_new, int T, int Hq, int max_len, float scale, int causal,
                      void* ws, size_t ws_bytes, void* stream);

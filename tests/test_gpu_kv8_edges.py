@@ -260,3 +260,23 @@ def test_workspace_of_exactly_its_size(dev, D, B, Hkv, G, T, L, cap):
         outs.append((blocks, tsa.attn_kv8_blocks_fwd(q, c, n, blocks, ws=ws)))
         assert bool((whole[len(ws):] == byte).all())
     assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+
+
+@pytest.mark.parametrize("D,G,T", FORMS)
+def test_scores_of_minus_infinity_alone(dev, D, G, T):
+    """Every key that the first rows see is minus infinity in a channel where q is positive: their
+    scores leave nothing to weigh, and they are 0; the other rows go on without those keys."""
+    gen = torch.Generator().manual_seed(3 * D + T)
+    T = min(T, 60)
+    k, v = keys(gen, 1, 1, T, D)
+    q = rand(gen, 1, G, T, D)
+    q[..., 5] = q[..., 5].abs().clamp_min(0.01)
+    first = (T + 1) // 2
+    k[0, 0, :first, 5] = -math.inf
+    o = tsa.attn_kv8_fwd(q.to(dev), fill(dev, k, v, [T]), ints([T], dev)).cpu()
+    assert not bool(o[:, :, :first].any())
+    K, V = k[0, 0, first:].double(), v[0, 0, first:].double()
+    for g in range(G):
+        for t in range(first, T):
+            want, tol = ko.attend(q[0, g, t], K, V, torch.ones(T - first, dtype=torch.float64), list(range(t - first + 1)), 1 / math.sqrt(D))
+            check_out(o[0, g, t], want, tol, (g, t))
