@@ -364,6 +364,78 @@ int tsa_attn_kv8_blocks_fwd(const tsa_kv8* cache, const tsa_rows* q, const tsa_r
                             const int32_t* len, const int32_t* n_new, int T, int Hq, const int32_t* blocks, int top,
                             float scale, void* ws, size_t ws_bytes, void* stream);
 
+/* ---- Rotary positions of queries and keys, and their gradient.  The attention entry points take
+ * q and k after any rotary embedding; the reference has none.  Pair i of a row at position p, i < rot / 2,
+ * turns by p * f_i radians and is multiplied by amp:
+ *   a' = amp (a cos - b sin), b' = amp (b cos + a sin)
+ * where (a, b) are the elements 2 i and 2 i + 1 (interleaved) or i and i + rot / 2 (halves).  Elements
+ * from rot on pass unchanged.
+ *
+ * tsa_rope_freqs makes the table of frequencies on the host (freq: rot / 2 numbers, host memory),
+ * to be copied to the device once: f_i / 2 pi in units of 2^-64 turns a position, rounded to the
+ * nearest (a table of the caller's own may hold any such numbers).  With it the angle is exact
+ * mod 2 pi to 2^-65 turns times the position.  f_i = base^(-2 i / rot), scaled for longer contexts:
+ *   LINEAR      f_i / factor
+ *   NTK         with base * factor^(rot / (rot - 2)) for base (rot >= 4)
+ *   YARN        f_i (1 - r) + f_i / factor * r, r rising from 0 to 1 between the pairs that turn
+ *               beta_fast and beta_slow times in orig_len positions (their numbers floored and
+ *               ceiled, within 0 .. rot - 1); amp = 0.1 ln(factor) + 1
+ *   WAVELENGTH  f_i for pairs that turn at least `high` times in orig_len positions, f_i / factor up to
+ *               `low` times, and linear in the number of turns between
+ * amp is 1 except for YARN; a caller may change it. ---- */
+enum { TSA_ROPE_PLAIN = 0, TSA_ROPE_LINEAR = 1, TSA_ROPE_NTK = 2, TSA_ROPE_YARN = 3, TSA_ROPE_WAVELENGTH = 4 };
+typedef struct tsa_rope_params {
+    double base, factor, beta_fast, beta_slow, low, high; /* base > 1, factor >= 1, beta_fast > beta_slow > 0, high > low > 0 */
+    int rot, scaling, orig_len;
+} tsa_rope_params;
+int tsa_rope_freqs(const tsa_rope_params* params, uint64_t* freq, float* amp);
+
+typedef struct tsa_rope_plan {
+    const uint64_t* freq; /* on the device */
+    float amp;
+    int rot;         /* even, 2 .. D; multiples of 16 are read 16 bytes at a time, others pair by pair */
+    int interleaved; /* 0 or 1 */
+} tsa_rope_plan;
+
+/* Rotates queries q [B][Hq][T][D] and keys k [B][Hk][T][D] (Hk may be 0: queries alone) of one type
+ * (TSA_TYPE_F16 or TSA_TYPE_F32; the tsa_rows then hold floats) into q_out and k_out, each apart
+ * from its input or the input itself (the same data and strides).  D in {64, 128, 256}.  Row t of
+ * sequence b is at position pos[b * T + t], or without pos at len[b] - n_new[b] + t, or without
+ * len at t; n_new[b] (T each without it) counts the sequence's rows, those behind it being padding
+ * that is neither read nor written.  Positions may be any 32-bit numbers (pos, len and n_new: int32 on the device).  back = 1: the gradient, q and k
+ * being gradients of the rotated rows: the angles with the other sign, times amp. */
+int tsa_rope(const tsa_rope_plan* plan, int type, const tsa_rows* q, const tsa_rows* q_out, int Hq, const tsa_rows* k,
+             const tsa_rows* k_out, int Hk, const int32_t* pos, const int32_t* len, const int32_t* n_new, int B, int T,
+             int D, int back, void* stream);
+
+/* ---- Attention's training pair: the forward that keeps its row statistics, and the backward pass
+ * that makes the probabilities again from them.  tsa_attn_gqa_fwd on rows that lie anywhere, with
+ * lengths: q, gate, o [B][Hq][Tq][D], k, v [B][Hkv][Tk][D], fp16; gate may be NULL.  len_q, len_k
+ * (int32 [B] on the device, or NULL for Tq, Tk each; taken as 0 .. Tq, 0 .. Tk) count each
+ * sequence's rows; the rows behind them are padding that is neither read nor written, in any
+ * tensor.  The queries are the last tokens: under the causal mask query t sees the keys
+ * j <= t + len_k - len_q.  lse [B][Hq][Tq] fp32 gets log(sum_j exp(scale * q.k_j)); a query that sees
+ * no key has o = 0 and lse = -infinity, and its gradients are 0.  A stride_t is at most 2^24
+ * elements, and outputs lie on no input. ---- */
+int tsa_attn_train_fwd(const tsa_rows* q, const tsa_rows* k, const tsa_rows* v, const tsa_rows* gate, const tsa_rows* o,
+                       float* lse, const int32_t* len_q, const int32_t* len_k, int B, int Hq, int Hkv, int Tq, int Tk,
+                       int D, float scale, int causal, void* stream);
+
+/* Workspace bytes of the backward pass (gated: 1 with a gate); 0 for invalid arguments.  A workspace is 16-byte aligned;
+ * calls that share one must be ordered on one stream. */
+size_t tsa_attn_bwd_workspace_bytes(int B, int Hq, int Hkv, int Tq, int Tk, int D, int gated, int causal);
+
+/* The gradients of q, k, v and gate (dgate: NULL without a gate) for the gradient d_out of o, from
+ * the forward's o and lse.  With P = exp(scale q.k - lse), d = sum d_out o (a row's), dO = sigmoid(gate) d_out:
+ *   dv_j = sum_i P_ij dO_i          dq_i = scale sum_j dS_ij k_j        dS_ij = P_ij (dO_i.v_j - d_i)
+ *   dk_j = scale sum_i dS_ij q_i    dgate = d_out o (1 - sigmoid(gate))
+ * Every sum is taken in one order, in 32 bits: the same call gives the same bits.  P and dS are
+ * rounded to fp16 times a power of two that a bound of dS chooses, so d_out may be of any size. */
+int tsa_attn_bwd(const tsa_rows* d_out, const tsa_rows* q, const tsa_rows* k, const tsa_rows* v, const tsa_rows* gate,
+                 const tsa_rows* o, const float* lse, const tsa_rows* dq, const tsa_rows* dk, const tsa_rows* dv,
+                 const tsa_rows* dgate, const int32_t* len_q, const int32_t* len_k, int B, int Hq, int Hkv, int Tq,
+                 int Tk, int D, float scale, int causal, void* ws, size_t ws_bytes, void* stream);
+
 /* The lab's naive GDN check on the device: one thread per state column, fp32, state read
  * and written in global memory, the order of gdn_cpu (src/gdn_sm75.cu:1078-1106) and
  * gdn_serial_kernel (:57-92).  Used by the gdn driver's error check.  Any dk, dv >= 1. */

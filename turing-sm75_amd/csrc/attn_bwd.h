@@ -1,0 +1,916 @@
+// attn_bwd.h -- the backward pass of softmax attention for gfx950 (fp16 MFMA, fp32 sums).
+//
+// With row statistics L (of the forward pass) and d_i = sum dO'_i o'_i:
+//   P_ij = exp(c q_i.k_j - L_i),  dP_ij = dO_i.v_j,  dS_ij = P_ij (dP_ij - d_i)
+//   dV_j = sum_i P_ij dO_i,  dK_j = c sum_i dS_ij q_i,  dQ_i = c sum_j dS_ij k_j
+// and, with a gate, dO = sigma(g) dO', dg = dO' o' (1 - sigma(g)); the gate cancels in d.
+//
+// Three launches: the rows' statistics (attn_bwd_rows_kernel), dK and dV by key tile together with dQ by query
+// tile (attn_bwd_kernel), and, where a key tile's queries were split over workgroups, the sum of
+// their parts (attn_bwd_join_kernel).  S and dP are made twice, once for each kind of tile: 7 products instead of 5, and no
+// T x S memory, no atomics (each sum has one order) and no fp32 dQ to be read and written for
+// every key tile.
+//
+// fp16 range: P and dS are rounded to fp16 as MFMA operands.  Both are multiplied by 2^ref there, one
+// power of two for a workgroup, as large as keeps |dS| 2^ref <= 2^14 and P 2^ref <= 2^15 by the bound
+// |dS_ij| <= |dO_i| |v_j| + |d_i| over its rows and keys, so gradients of any size keep fp16's
+// full precision in dS down to 2^-28 of that bound.  It is folded into the exponential's argument and into the outputs' scale.
+#pragma once
+#include "attn_tiles.h"
+#include "common.h"
+#include "kernels.h"
+
+namespace tsa {
+namespace bwd {
+namespace {
+
+constexpr int kBlk = 32;  // rows and keys of a step
+
+struct BwdArgs {
+    Rows16 q, k, v, g /* dO, gated */, dq, dk, dv;
+    const float* stat;     // [B][Hq][n_qb][64]: L log2(e) of 32 rows (inf: no such row, or it sees no key), then -d
+    const float2* row_max; // [B][Hq][n_qb]: the largest |dO_i| and |d_i| of 32 rows
+    const float* key_max;  // [B][Hkv][n_kb]: the largest |v_j| of 32 keys
+    float* part;           // split key tiles: fp32 sums of each part
+    const int *len_q, *len_k;
+    int B, Hq, Hkv, Tq, Tk, n_qb, n_kb, n_kt, n_part, n_qt, n_kv;  // n_kt, n_qt: tiles; n_kv: workgroups of the key tiles
+    float scale, c2;
+};
+
+// The arguments where the launch left them, read again after each `fresh`: held from the kernel's start for all
+// its branches, they were 80 scalars more than there are, kept in vector registers that the products need.
+typedef const __attribute__((address_space(4))) BwdArgs* args_t;
+__device__ __forceinline__ args_t fresh(args_t a) {
+    asm volatile("" : "+s"(a));
+    return a;
+}
+
+__device__ __forceinline__ int count(const int* len, int b, int most) {
+    return len ? min(max(len[b], 0), most) : most;
+}
+
+// ---------------------------------------------------------------------------------------
+// Row statistics: a workgroup takes 32 rows of dO' and o' (8 lanes a row), or 32 keys' values.
+// ---------------------------------------------------------------------------------------
+struct RowsArgs {
+    Rows16 g, o, gate, v, dgate;
+    half_t* gated;  // dO [B][Hq][Tq][D], with a gate
+    const float* lse;
+    float* stat;
+    float2* row_max;
+    float* key_max;
+    const int *len_q, *len_k;
+    int Hq, Hkv, Tq, Tk, n_qb, n_kb, n_rows;  // n_rows: workgroups of rows, those of keys follow
+};
+
+template <int D>
+__global__ void __launch_bounds__(256) attn_bwd_rows_kernel(RowsArgs a) {
+    __shared__ float2 most[32];
+    const int r = threadIdx.x >> 3, l8 = threadIdx.x & 7;
+    int blk = blockIdx.x;
+    if (blk < a.n_rows) {
+        const int bh = blk / a.n_qb, qb = blk % a.n_qb, b = bh / a.Hq, h = bh % a.Hq;
+        const int n = count(a.len_q, b, a.Tq), t = qb * kBlk + r;
+        float d = 0.f, n2 = 0.f;
+        if (t < n) {
+            const half_t* g = a.g.data + b * a.g.b + h * a.g.h + t * a.g.t;
+            const half_t* o = a.o.data + b * a.o.b + h * a.o.h + t * a.o.t;
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) {
+                const int e0 = 8 * l8 + 64 * i;
+                const half8_t x = *reinterpret_cast<const half8_t*>(g + e0);
+                const half8_t y = *reinterpret_cast<const half8_t*>(o + e0);
+                half8_t z = x;
+                float w[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[j] = (float)x[j];
+                if (a.gated) {
+                    const half8_t gt = *reinterpret_cast<const half8_t*>(a.gate.data + b * a.gate.b + h * a.gate.h + t * a.gate.t + e0);
+                    half8_t dg;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        // 1 / sigma, and 1 - sigma as sigma of the other sign (its own digits where sigma is near 1)
+                        const float inv = 1.f + __expf(-(float)gt[j]), rest = __builtin_amdgcn_rcpf(1.f + __expf((float)gt[j]));
+                        dg[j] = (half_t)(w[j] * (float)y[j] * rest);
+                        z[j] = (half_t)(w[j] * __builtin_amdgcn_rcpf(inv));
+                        // d_i goes with the dO that dP is made of, the rounded one: sum_j dS_ij then stays 0
+                        // and the rounding weighs a fifth less in dQ and dK
+                        if (z[j] != (half_t)0.f) w[j] = (float)z[j] * inv;
+                    }
+                    *reinterpret_cast<half8_t*>(a.gated + ((size_t)bh * a.Tq + t) * D + e0) = z;
+                    *reinterpret_cast<half8_t*>(a.dgate.data + b * a.dgate.b + h * a.dgate.h + t * a.dgate.t + e0) = dg;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    d = fmaf(w[j], (float)y[j], d);
+                    n2 = fmaf((float)z[j], (float)z[j], n2);
+                }
+            }
+        }
+        d = sum8(d);
+        n2 = sum8(n2);
+        if (l8 == 0) {
+            float* st = a.stat + (size_t)blk * 64;
+            const float lse = t < n ? a.lse[(size_t)bh * a.Tq + t] : -INFINITY;
+            st[r] = lse == -INFINITY ? INFINITY : lse * kLog2e;
+            st[32 + r] = -d;
+            most[r] = make_float2(sqrtf(n2), fabsf(d));
+        }
+        __syncthreads();
+        if (threadIdx.x < 64) {  // (NaN rows give NaN results whatever the scale)
+            float2 m = most[threadIdx.x & 31];
+#pragma unroll
+            for (int s = 16; s; s >>= 1) {
+                m.x = fmaxf(m.x, __shfl_xor(m.x, s));
+                m.y = fmaxf(m.y, __shfl_xor(m.y, s));
+            }
+            if (threadIdx.x == 0) a.row_max[blk] = m;
+        }
+    } else {
+        blk -= a.n_rows;
+        const int bh = blk / a.n_kb, kb = blk % a.n_kb, b = bh / a.Hkv, h = bh % a.Hkv;
+        const int t = kb * kBlk + r;
+        float n2 = 0.f;
+        if (t < count(a.len_k, b, a.Tk)) {
+            const half_t* v = a.v.data + b * a.v.b + h * a.v.h + t * a.v.t;
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) {
+                const half8_t x = *reinterpret_cast<const half8_t*>(v + 8 * l8 + 64 * i);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) n2 = fmaf((float)x[j], (float)x[j], n2);
+            }
+        }
+        n2 = sum8(n2);
+        if (l8 == 0) most[r].x = sqrtf(n2);
+        __syncthreads();
+        if (threadIdx.x < 64) {
+            float m = most[threadIdx.x & 31].x;
+#pragma unroll
+            for (int s = 16; s; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
+            if (threadIdx.x == 0) a.key_max[blk] = m;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// What the tiles share
+// ---------------------------------------------------------------------------------------
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) x = fmaxf(x, __shfl_xor(x, s));
+    return x;
+}
+
+// A value as if unknown: what is made from it is made here, not held from an earlier use.
+__device__ __forceinline__ int again(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+// The power of two for a bound of |dS|: 2^ref bound <= 2^14, ref <= 15 (P 2^ref <= 2^15).
+__device__ __forceinline__ float range_ref(float bound) {
+    if (!(bound < 0x1p100f)) bound = 0x1p100f;
+    const int bits = __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, bound));  // (every lane's is the same)
+    const int e = ((bits >> 23) & 255) - 126;                                        // bound < 2^e
+    return (float)min(15, 14 - e);
+}
+
+// One tensor's part of a step's copies: 32 rows of D elements, kW waves, blocks of 1 KiB.  A wave's
+// first block holds rows that its others repeat a multiple of 16 on, so the swizzle is the same and
+// one offset a lane serves all.
+template <int D, int kW>
+struct Copy {
+    static constexpr int kInstr = kBlk * D * 2 / 1024;  // of a tile
+    static constexpr int kStep = kW * 1024 / (2 * D);   // rows from a wave's block to its next
+    static constexpr int kPer = (kInstr + kW - 1) / kW;
+    static_assert(kPer == 1 || kStep % 16 == 0, "a wave's blocks share one swizzle pattern");
+    static_assert(kInstr % kW == 0, "every wave copies");
+};
+// p: the tile's first row; stride in bytes (at most 2^25); last: the last row there is, counted from it.
+template <int D, int kW>
+__device__ __forceinline__ void copy_rows(const char* p, unsigned stride, int last, int lane, int wave, unsigned lds) {
+    using C = Copy<D, kW>;
+    // made again for each copy (held, they take registers that the products need)
+    unsigned l = (unsigned)lane;
+    asm volatile("" : "+v"(l));
+    const unsigned row = (512u / D) * (unsigned)wave + l / (D / 8);
+    const unsigned col = 16u * ((l % (D / 8)) ^ (unsigned)swz<D>((int)row));
+    if (last >= kBlk - 1) {
+        const unsigned off = row * stride + col;
+#pragma unroll
+        for (int j = 0; j < C::kPer; ++j) dma_issue_any(p + (size_t)stride * (C::kStep * j), off, lds + 1024u * (unsigned)(wave + kW * j));
+    } else {
+#pragma unroll
+        for (int j = 0; j < C::kPer; ++j)
+            dma_issue_any(p, (unsigned)min((int)row + C::kStep * j, last) * stride + col, lds + 1024u * (unsigned)(wave + kW * j));
+    }
+}
+
+// A operand of rows: A[row l % 32][16 kk + 8 (l / 32) + s] (addr: row l % 32's chunk l / 32).
+__device__ __forceinline__ half8_t rows_op(unsigned addr, int kk) { return lds_read_b128(addr ^ (32u * kk)); }
+// A operand of columns: A[d = 32 db + l % 32][k slot (l / 32, s)], slot s of k-step ks being row
+// 16 ks + 8 (s / 4) + 4 (l / 32) + s % 4: the order in which a 32 x 32 result holds its rows.
+template <int D>
+__device__ __forceinline__ half8_t cols_op(unsigned a, int ks, int db) {
+    // eight rows on, the swizzle has its bit 1 the other way at D >= 128, and is the same at D = 64
+    constexpr unsigned kUp = D == 64 ? 0u : 32u;
+    const half4_t lo = lds_read_tr16_at((a ^ (64u * db)) + (unsigned)(32 * D * ks));
+    const half4_t up = lds_read_tr16_at((a ^ (64u * db + kUp)) + (unsigned)(32 * D * ks + 16 * D));
+    return half8_t{lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
+}
+
+// kN operands read kPre steps in front of their use, pinned there: left alone, the compiler reads
+// them all at once and spills.
+template <int kN, int kPre, class Read, class Use>
+__device__ __forceinline__ void ahead(const Read& read, const Use& use) {
+    half8_t op[kN];
+#pragma unroll
+    for (int i = 0; i < kPre; ++i) op[i] = read(i);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+        if (i + kPre < kN) op[i + kPre] = read(i + kPre);
+        __builtin_amdgcn_sched_barrier(0);
+        use(i, op[i]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+// The products of a 32-row tile at byte `tile`: its rows with kRB operands a k-step into s, and its
+// columns (from block db0 on) with kRB operands of 16 rows into acc.  Addresses are one XOR next to their read; the empty
+// asm keeps them from being held.
+constexpr int kPreRows = 4, kPreCols = 3;  // over the operands that share a read
+template <int D, int kRB>
+__device__ __forceinline__ void mul_rows(unsigned rows, unsigned tile, const half8_t (&frag)[kRB][D / 16], float16_t (&s)[kRB]) {
+    unsigned a = rows + tile;
+    asm volatile("" : "+v"(a));
+    ahead<D / 16, kPreRows / kRB>([&](int kk) { return rows_op(a, kk); },
+                            [&](int kk, const half8_t& x) {
+#pragma unroll
+                                for (int i = 0; i < kRB; ++i) {
+                                    s[i] = mfma32(x, frag[i][kk], s[i]);
+                                    asm volatile("" : "+v"(s[i]));  // not moved to the result's first use, behind all reads
+                                }
+                            });
+}
+template <int D, int kRB, int kDB>
+__device__ __forceinline__ void mul_cols(unsigned cols, unsigned tile, int db0, const half8_t (&op)[kRB][2], float16_t (&acc)[kRB * kDB]) {
+    unsigned a = (cols + tile) ^ (64u * db0);
+    asm volatile("" : "+v"(a));
+    // a column block's two k-steps one after the other: their addresses are the same but for a constant
+    ahead<2 * kDB, kRB == 2 ? 2 : kPreCols>([&](int i) { return cols_op<D>(a, i & 1, i >> 1); },
+                             [&](int i, const half8_t& x) {
+#pragma unroll
+                                 for (int r = 0; r < kRB; ++r) acc[r * kDB + (i >> 1)] = mfma32(x, op[r][i & 1], acc[r * kDB + (i >> 1)]);
+                             });
+}
+
+typedef float float8_t __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ half8_t pack8(const float16_t& x, int half) {
+    const float8_t y = half ? float8_t{x[8], x[9], x[10], x[11], x[12], x[13], x[14], x[15]}
+                            : float8_t{x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]};
+    return __builtin_convertvector(y, half8_t);
+}
+
+// Half `half` of x times the fp16 values p, rounded to fp16 (a product is v_fma_mixlo_f16: no conversions).
+__device__ __forceinline__ half8_t times(const half8_t& p, const float16_t& x, int half) {
+    half8_t y;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) y[r] = (half_t)fmaf((float)p[r], x[8 * half + r], 0.f);
+    return y;
+}
+
+__device__ __forceinline__ void lds_write_b128(unsigned addr, const half8_t& x) {
+    typedef __attribute__((address_space(3))) half8_t* p_t;
+    *(p_t)(addr) = x;
+}
+__device__ __forceinline__ float4_t lds_read_f4(unsigned addr) {
+    typedef __attribute__((address_space(3))) const float4_t* p_t;
+    return *(p_t)(addr);
+}
+
+// Lane-constant LDS addresses of operand reads in a tile at byte 0.
+template <int D>
+struct OpAddr {
+    unsigned rows, cols;
+    __device__ __forceinline__ OpAddr(int lane, unsigned base) {
+        const int r = lane & 31, hi = lane >> 5;
+        rows = base + (unsigned)r * (2 * D) + 16u * (unsigned)chunk_pos<D>(r, hi);
+        const int i16 = lane & 15, vm = i16 & 3, t = 4 * hi + (i16 >> 2), chunk = 2 * ((lane >> 4) & 1) + (vm >> 1);
+        cols = base + (unsigned)t * (2 * D) + 16u * (unsigned)chunk_pos<D>(t, chunk) + 8u * (vm & 1);
+    }
+};
+
+// ---------------------------------------------------------------------------------------
+// dK and dV of a key tile.  Waves work in pairs that own the same 32 kKB keys: the first (role P)
+// makes S and P and sums dV, the second (role S) makes dP, takes P from LDS, and sums dK.  A wave so
+// holds one operand (K or V) and one result in registers, which is what lets it own 64 keys (32 at
+// D = 256) at two waves a SIMD: every Q and dO operand read from LDS feeds two products, where 32
+// keys a wave would need all of LDS's 128 bytes a cycle to keep the MFMA pipes busy.
+// Results are transposed (lane = key), so P and dS leave the first products in the second's operand
+// layout.  Per step of 32 queries one barrier: P of the step, the tiles of the next one and the end of
+// the last one's reads.
+// ---------------------------------------------------------------------------------------
+template <int D>
+struct KvTile {
+    static constexpr int kKB = D == 256 ? 1 : 2;    // 32-key blocks a pair
+    static constexpr int kPairs = D == 256 ? 4 : 2;
+    static constexpr int kW = 2 * kPairs;
+    static constexpr int kKeys = 32 * kKB * kPairs;
+    static constexpr int kTileB = kBlk * D * 2;     // bytes of a Q or dO tile
+    static constexpr int kStage = 2 * kTileB;
+    static constexpr int kStages = 3;
+    static constexpr int kStatB = 256;
+    static constexpr int kPB = kKB * 2048;          // bytes of a pair's P
+    static constexpr int kStatAt = kStages * kStage, kPAt = kStatAt + kStages * kStatB;
+    static constexpr int kLds = kPAt + 2 * kPairs * kPB;
+    static constexpr int kAcc = kKB * (D / 32);     // 32 x 32 results a wave
+};
+
+// Writes kRB blocks of 32 rows by 32 kDB elements (lane = row, 4 consecutive elements a register group) times f.
+template <int kRB, int kDB>
+__device__ __forceinline__ void store_rows(const float16_t (&acc)[kRB * kDB], half_t* out, long long stride, int row0, int n_rows,
+                                           int lane, float f) {
+#pragma unroll
+    for (int kb = 0; kb < kRB; ++kb) {
+        const int r = row0 + 32 * kb + (lane & 31);
+        if (r >= n_rows) continue;
+        half_t* row = out + r * stride + 4 * (lane >> 5);
+#pragma unroll
+        for (int db = 0; db < kDB; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float16_t& x = acc[kb * kDB + db];
+                *reinterpret_cast<half4_t*>(row + 32 * db + 8 * g) =
+                    half4_t{(half_t)(x[4 * g] * f), (half_t)(x[4 * g + 1] * f), (half_t)(x[4 * g + 2] * f), (half_t)(x[4 * g + 3] * f)};
+            }
+    }
+}
+
+// The steps of a key tile: 32-query blocks first .. n - 1 of each query head of the group.
+struct KvPlan {
+    int n_q, n_k, last0, first, per, steps;
+};
+template <int D, bool kCausal>
+__device__ __forceinline__ KvPlan kv_plan(args_t a, int b, int kt) {
+    KvPlan p;
+    p.n_q = count(a->len_q, b, a->Tq);
+    p.n_k = count(a->len_k, b, a->Tk);
+    p.last0 = p.n_k - p.n_q;  // query i sees keys up to i + last0
+    const int k0 = kt * KvTile<D>::kKeys;
+    p.first = kCausal ? max(0, k0 - p.last0) / kBlk : 0;
+    p.per = max(0, (p.n_q + kBlk - 1) / kBlk - p.first);
+    p.steps = k0 < p.n_k ? p.per * (a->Hq / a->Hkv) : 0;
+    return p;
+}
+
+template <int D, bool kCausal, bool role_p>
+__device__ __forceinline__ void kv_tile(args_t a, half_t* lds, int wg) {
+    using T = KvTile<D>;
+    constexpr int kDB = D / 32, kKK = D / 16;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5;
+    const int pair = wave % T::kPairs;
+    const int n_bh = a->B * a->Hkv;
+    const int bh = wg % n_bh, rest = wg / n_bh, part = rest % a->n_part, kt = rest / a->n_part;
+    const int b = bh / a->Hkv, hk = bh % a->Hkv, G = a->Hq / a->Hkv;
+    const KvPlan pl = kv_plan<D, kCausal>(a, b, kt);
+    const int k0 = kt * T::kKeys + pair * 32 * T::kKB;
+    if (kt * T::kKeys >= pl.n_k) return;
+    const int u0 = (int)((long long)pl.steps * part / a->n_part), u1 = (int)((long long)pl.steps * (part + 1) / a->n_part);
+
+    // K or V of the pair's keys, as B operands: slot s of k-step kk is row[16 kk + 8 hi + s]
+    half8_t frag[T::kKB][kKK];
+    {
+        const auto& src = role_p ? a->k : a->v;
+        const half_t* base = src.data + b * src.b + hk * src.h;
+#pragma unroll
+        for (int kb = 0; kb < T::kKB; ++kb) {
+            const int key = k0 + 32 * kb + (lane & 31);
+#pragma unroll
+            for (int kk = 0; kk < kKK; ++kk)
+                frag[kb][kk] = key < pl.n_k ? *reinterpret_cast<const half8_t*>(base + key * src.t + 16 * kk + 8 * hi) : half8_t{};
+        }
+    }
+    // the scale of P and dS: the workgroup's bound
+    float ref;
+    {
+        float n = 0.f, d = 0.f, v = 0.f;
+        for (int u = u0 + lane; u < u1; u += 64) {
+            const float2 m = a->row_max[(size_t)(b * a->Hq + hk * G + u / pl.per) * a->n_qb + pl.first + u % pl.per];
+            n = fmaxf(n, m.x);
+            d = fmaxf(d, m.y);
+        }
+        const int kb = kt * (T::kKeys / kBlk) + lane;
+        if (lane < T::kKeys / kBlk && kb < a->n_kb) v = a->key_max[(size_t)bh * a->n_kb + kb];
+        ref = range_ref(fmaf(wave_max(n), wave_max(v), wave_max(d)));
+    }
+
+    float16_t acc[T::kAcc];
+#pragma unroll
+    for (int i = 0; i < T::kAcc; ++i) acc[i] = float16_t{};
+
+    const unsigned lds0 = (unsigned)(uintptr_t)(lds_void_t)(void*)lds;
+    const OpAddr<D> op(lane, lds0);
+    const unsigned p_at = lds0 + T::kPAt + (unsigned)pair * T::kPB + 16u * lane;
+
+    // The steps of this part: 32-query blocks of one head after the other's, taken by running pointers
+    // (products of strides held for the loop were more scalars than there are registers).
+    const int n = u1 - u0, end = pl.first + pl.per, last = pl.n_q - 1;
+    const int h0 = hk * G + u0 / max(1, pl.per);
+    int qb = pl.first + u0 % max(1, pl.per), to_copy = qb;  // the current step's block, and the next copies'
+    const unsigned q_row = 2u * (unsigned)a->q.t, g_row = 2u * (unsigned)a->g.t;  // bytes
+    const char* qp = reinterpret_cast<const char*>(a->q.data + b * a->q.b + h0 * a->q.h) + (size_t)q_row * kBlk * qb;
+    const char* gp = reinterpret_cast<const char*>(a->g.data + b * a->g.b + h0 * a->g.h) + (size_t)g_row * kBlk * qb;
+    const float* sp = a->stat + ((size_t)(b * a->Hq + h0) * a->n_qb + qb) * 64;
+    const long long q_jump = 2 * a->q.h - (long long)q_row * kBlk * pl.per, g_jump = 2 * a->g.h - (long long)g_row * kBlk * pl.per;
+    const int s_jump = 64 * (a->n_qb - pl.per);
+    unsigned ring = 0, ring2 = 0;  // stages of the current step and of the next copies
+    auto copy = [&] {  // tiles and statistics of a step
+        const unsigned st = lds0 + ring2 * T::kStage;
+        copy_rows<D, T::kW>(qp, q_row, last - to_copy * kBlk, lane, wave, st);
+        copy_rows<D, T::kW>(gp, g_row, last - to_copy * kBlk, lane, wave, st + T::kTileB);
+        if (wave == 0) dma_issue_any4(sp, 4u * lane, lds0 + T::kStatAt + ring2 * T::kStatB);
+        qp += (size_t)q_row * kBlk, gp += (size_t)g_row * kBlk, sp += 64;
+        if (++to_copy == end) to_copy = pl.first, qp += q_jump, gp += g_jump, sp += s_jump;
+        ring2 = ring2 + 1 == T::kStages ? 0 : ring2 + 1;
+    };
+    // a pair's keys are hidden from a step's queries while the last of those lies in front of the first of them
+    auto hidden = [&](int x) { return kCausal && x * kBlk + kBlk - 1 + pl.last0 < k0; };
+
+    if (n > 0) copy();
+
+    // register r of a result is query 4 hi + 8 (r / 4) + r % 4 of the step: hidden below this
+    auto limit = [&](int x, int kb) { return k0 + 32 * kb + (lane & 31) - pl.last0 - x * kBlk - 4 * hi; };
+    auto partly = [&](int x, int kb) { return kCausal && k0 + 32 * kb + 31 > x * kBlk + pl.last0; };
+    if constexpr (role_p) {
+        half8_t p[T::kKB][2];
+        auto scores = [&](int x, unsigned stage, unsigned at) {  // S of a step, then P, to LDS for the other role
+            const unsigned st = stage * T::kStage, sa = lds0 + T::kStatAt + stage * T::kStatB + 16u * hi;
+            float16_t s[T::kKB];
+#pragma unroll
+            for (int kb = 0; kb < T::kKB; ++kb) s[kb] = float16_t{};
+            mul_rows<D, T::kKB>(op.rows, st, frag, s);
+#pragma unroll
+            for (int kb = 0; kb < T::kKB; ++kb)
+                if (partly(x, kb)) {
+                    const int lim = limit(x, kb);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (8 * (r >> 2) + (r & 3) < lim) s[kb][r] = -INFINITY;
+                }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float4_t l = lds_read_f4(sa + 32u * g);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float m = ref - l[e];
+#pragma unroll
+                    for (int kb = 0; kb < T::kKB; ++kb) s[kb][4 * g + e] = fast_exp2(fmaf(s[kb][4 * g + e], a->c2, m));
+                }
+            }
+#pragma unroll
+            for (int kb = 0; kb < T::kKB; ++kb)
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    p[kb][w] = pack8(s[kb], w);
+                    lds_write_b128(p_at + at + (unsigned)(kb * 2 + w) * 1024u, p[kb][w]);
+                }
+        };
+        // round i: dV of step i - 1, S and P of step i, while step i + 1 is copied
+#pragma clang loop unroll(disable)
+        for (int i = 0, was = 0; i <= n; ++i) {
+            asm volatile("" : "+s"(i));  // (a first round taken out of the loop spills)
+            dma_wait_barrier();
+            if (i + 1 < n) copy();
+            if (i > 0 && !hidden(was)) mul_cols<D, T::kKB, kDB>(op.cols, ring * T::kStage + T::kTileB, 0, p, acc);
+            if (i > 0) ring = ring + 1 == T::kStages ? 0 : ring + 1;
+            if (i < n && !hidden(qb)) {
+                scores(qb, ring, (unsigned)(i & 1) * (T::kPairs * T::kPB));
+            } else {  // no P: what it was is not kept through the other branch
+#pragma unroll
+                for (int x = 0; x < 2 * T::kKB; ++x) asm volatile("" : "=v"(p[x >> 1][x & 1]));
+            }
+            was = qb;
+            qb = qb + 1 == end ? pl.first : qb + 1;
+        }
+    } else {
+        float16_t s[T::kKB];
+        auto products = [&](unsigned stage) {  // dP - d of a step
+            const unsigned st = stage * T::kStage, sa = lds0 + T::kStatAt + stage * T::kStatB + 128u + 16u * hi;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float4_t d = lds_read_f4(sa + 32u * g);
+#pragma unroll
+                for (int kb = 0; kb < T::kKB; ++kb)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[kb][4 * g + e] = d[e];
+            }
+            mul_rows<D, T::kKB>(op.rows, st + T::kTileB, frag, s);
+        };
+        // round i: dS and dK of step i - 1, dP of step i
+#pragma clang loop unroll(disable)
+        for (int i = 0, was = 0; i <= n; ++i) {
+            asm volatile("" : "+s"(i));  // (a first round taken out of the loop spills)
+            dma_wait_barrier();
+            if (i + 1 < n) copy();
+            if (i > 0 && !hidden(was)) {
+                const unsigned at = p_at + (unsigned)((i - 1) & 1) * (T::kPairs * T::kPB);
+                half8_t ds[T::kKB][2];
+                ahead<2 * T::kKB, 1>([&](int x) { return lds_read_b128(at + (unsigned)x * 1024u); },
+                                     [&](int x, const half8_t& y) { ds[x >> 1][x & 1] = times(y, s[x >> 1], x & 1); });
+#pragma unroll
+                for (int kb = 0; kb < T::kKB; ++kb)
+                    if (partly(was, kb)) {  // 0 whatever dP is there
+                        const int lim = limit(was, kb);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            if (8 * (r >> 2) + (r & 3) < lim) ds[kb][r >> 3][r & 7] = (half_t)0.f;
+                    }
+                mul_cols<D, T::kKB, kDB>(op.cols, ring * T::kStage, 0, ds, acc);
+            }
+            if (i > 0) ring = ring + 1 == T::kStages ? 0 : ring + 1;
+            if (i < n && !hidden(qb)) {
+                products(ring);
+            } else {
+#pragma unroll
+                for (int kb = 0; kb < T::kKB; ++kb) asm volatile("" : "=v"(s[kb]));
+            }
+            was = qb;
+            qb = qb + 1 == end ? pl.first : qb + 1;
+        }
+    }
+
+    a = fresh(a);
+    const float f = exp2f(-ref) * (role_p ? 1.f : a->scale);
+    if (a->n_part == 1) {
+        const auto& out = role_p ? a->dv : a->dk;
+        store_rows<T::kKB, kDB>(acc, out.data + b * out.b + hk * out.h, out.t, k0, pl.n_k, again(lane), f);
+    } else {  // [key tile][part][wave][16-byte group][lane]
+        float4_t* w = reinterpret_cast<float4_t*>(a->part) + ((((size_t)bh * a->n_kt + kt) * a->n_part + part) * T::kW + wave) * (T::kAcc * 256) + lane;
+#pragma unroll
+        for (int i = 0; i < T::kAcc; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                w[(4 * i + g) * 64] = float4_t{acc[i][4 * g] * f, acc[i][4 * g + 1] * f, acc[i][4 * g + 2] * f, acc[i][4 * g + 3] * f};
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// dQ of a query tile, D = 64 and 128: a wave owns 32 kMB queries, with Q, dO and dQ in registers, and
+// walks over the keys it sees.  S and dP are transposed (lane = query), so dS leaves them as the B
+// operand of dQ^T += K^T dS^T, and L and d are one register each.
+// ---------------------------------------------------------------------------------------
+template <int D>
+struct QTile {
+    static constexpr bool kRoles = D == 256;  // waves in pairs, as for the key tiles
+    static constexpr int kMB = D == 64 ? 2 : 1;
+    static constexpr int kW = KvTile<D>::kW;
+    static constexpr int kQueries = kRoles ? 32 * kW / 2 : 32 * kMB * kW;
+    static constexpr int kTileB = kBlk * D * 2;
+    static constexpr int kKRing = kRoles ? 4 : 3, kVRing = kRoles ? 2 : 3;
+    static constexpr int kVAt = kKRing * kTileB, kXAt = kVAt + kVRing * kTileB;
+    static constexpr int kLds = kXAt + (kRoles ? 4 * kW / 2 * 2048 : 0);
+};
+
+template <int D>
+__device__ __forceinline__ float q_tile_ref(args_t a, int bh, int bhk, int q0, int q_blocks, int k_blocks, int lane) {
+    float n = 0.f, d = 0.f, v = 0.f;
+    const int qb = q0 / kBlk + lane;
+    if (lane < q_blocks && qb < a->n_qb) {
+        const float2 m = a->row_max[(size_t)bh * a->n_qb + qb];
+        n = m.x;
+        d = m.y;
+    }
+    for (int i = lane; i < k_blocks; i += 64) v = fmaxf(v, a->key_max[(size_t)bhk * a->n_kb + i]);
+    return range_ref(fmaf(wave_max(n), wave_max(v), wave_max(d)));
+}
+
+template <int D, bool kCausal>
+__device__ __forceinline__ void q_tile(args_t a, half_t* lds, int wg) {
+    using T = QTile<D>;
+    constexpr int kDB = D / 32, kKK = D / 16, kMB = T::kMB;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5;
+    const int n_bh = a->B * a->Hq;
+    const int bh = wg % n_bh, qt = kCausal ? a->n_qt - 1 - wg / n_bh : wg / n_bh;
+    const int b = bh / a->Hq, h = bh % a->Hq, hk = h / (a->Hq / a->Hkv), bhk = b * a->Hkv + hk;
+    const int n_q = count(a->len_q, b, a->Tq), n_k = count(a->len_k, b, a->Tk), last0 = n_k - n_q;
+    const int tile0 = qt * T::kQueries;
+    if (tile0 >= n_q) return;
+    const int q0 = tile0 + wave * 32 * kMB;
+    const int k_end = kCausal ? min(n_k, min(tile0 + T::kQueries, n_q) + last0) : n_k;
+    const int n = max(0, (k_end + kBlk - 1) / kBlk);
+    const int my_end = kCausal ? min(n_k, q0 + 32 * kMB + last0) : n_k;  // the wave's own
+
+    half8_t qf[kMB][kKK], gf[kMB][kKK];
+    float l2[kMB], nd[kMB];
+    const float ref = q_tile_ref<D>(a, bh, bhk, tile0, T::kQueries / kBlk, n, lane);
+#pragma unroll
+    for (int m = 0; m < kMB; ++m) {
+        const int q = q0 + 32 * m + (lane & 31);
+        const half_t *qr = a->q.data + b * a->q.b + h * a->q.h + q * a->q.t, *gr = a->g.data + b * a->g.b + h * a->g.h + q * a->g.t;
+        l2[m] = INFINITY;
+        nd[m] = 0.f;
+        if (q < n_q) {
+            const float* st = a->stat + ((size_t)bh * a->n_qb + q / kBlk) * 64 + q % kBlk;
+            l2[m] = st[0] - ref;
+            nd[m] = st[32];
+        }
+#pragma unroll
+        for (int kk = 0; kk < kKK; ++kk) {
+            qf[m][kk] = q < n_q ? *reinterpret_cast<const half8_t*>(qr + 16 * kk + 8 * hi) : half8_t{};
+            gf[m][kk] = q < n_q ? *reinterpret_cast<const half8_t*>(gr + 16 * kk + 8 * hi) : half8_t{};
+        }
+    }
+    float16_t acc[kMB * kDB];
+#pragma unroll
+    for (int i = 0; i < kMB * kDB; ++i) acc[i] = float16_t{};
+
+    const unsigned lds0 = (unsigned)(uintptr_t)(lds_void_t)(void*)lds;
+    const OpAddr<D> op(lane, lds0);
+    const char *kp = reinterpret_cast<const char*>(a->k.data + b * a->k.b + hk * a->k.h), *vp = reinterpret_cast<const char*>(a->v.data + b * a->v.b + hk * a->v.h);
+    const unsigned k_row = 2u * (unsigned)a->k.t, v_row = 2u * (unsigned)a->v.t;
+    unsigned ring = 2, ring2 = 0;  // stages of the current step and of the next copies
+    int left = n_k - 1;            // the last key, counted from the next copies' first
+    auto copy = [&] {
+        const unsigned st = lds0 + ring2 * T::kTileB;
+        copy_rows<D, T::kW>(kp, k_row, left, lane, wave, st);
+        copy_rows<D, T::kW>(vp, v_row, left, lane, wave, st + T::kVAt);
+        kp += (size_t)k_row * kBlk, vp += (size_t)v_row * kBlk, left -= kBlk;
+        ring2 = ring2 == 2 ? 0 : ring2 + 1;
+    };
+    if (n > 0) copy();
+    if (n > 1) copy();
+#pragma clang loop unroll(disable)
+    for (int j = 0; j < n; ++j) {
+        dma_wait_barrier();
+        if (j + 2 < n) copy();
+        ring = ring == 2 ? 0 : ring + 1;
+        if (j * kBlk >= my_end) continue;
+        const unsigned st = ring * T::kTileB;
+        float16_t s[kMB], w[kMB];
+#pragma unroll
+        for (int m = 0; m < kMB; ++m) {
+            s[m] = float16_t{};
+#pragma unroll
+            for (int r = 0; r < 16; ++r) w[m][r] = nd[m];
+        }
+        mul_rows<D, kMB>(op.rows, st, qf, s);
+        mul_rows<D, kMB>(op.rows, T::kVAt + st, gf, w);
+        half8_t ds[kMB][2];
+#pragma unroll
+        for (int m = 0; m < kMB; ++m) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) w[m][r] *= fast_exp2(fmaf(s[m][r], a->c2, -l2[m]));
+            if ((kCausal && j * kBlk + 31 > q0 + 32 * m + last0) || (j + 1) * kBlk > n_k) {
+                // register r is key 32 j + 4 hi + 8 (r / 4) + r % 4
+                const int lim = min(kCausal ? q0 + 32 * m + (lane & 31) + last0 : n_k, n_k - 1) - j * kBlk - 4 * hi;
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (8 * (r >> 2) + (r & 3) > lim) w[m][r] = 0.f;
+            }
+            ds[m][0] = pack8(w[m], 0);
+            ds[m][1] = pack8(w[m], 1);
+        }
+        mul_cols<D, kMB, kDB>(op.cols, st, 0, ds, acc);
+    }
+    a = fresh(a);
+    store_rows<kMB, kDB>(acc, a->dq.data + b * a->dq.b + h * a->dq.h, a->dq.t, q0, n_q, again(lane), exp2f(-ref) * a->scale);
+}
+
+// The same at D = 256, by pairs of waves that own 32 queries: the first makes S and P, the second dP
+// and dS, and each sums half of dQ's columns (the first a step later, when dS has come through LDS).  Q or dO and half of dQ are 128 registers a wave; all of them
+// would not fit in one.
+template <int D, bool kCausal, bool role_p>
+__device__ __forceinline__ void q_tile_roles(args_t a, half_t* lds, int wg) {
+    using T = QTile<D>;
+    constexpr int kDB = D / 64, kKK = D / 16, kPairs = T::kW / 2;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5;
+    const int pair = wave % kPairs;
+    const int n_bh = a->B * a->Hq;
+    const int bh = wg % n_bh, qt = kCausal ? a->n_qt - 1 - wg / n_bh : wg / n_bh;
+    const int b = bh / a->Hq, h = bh % a->Hq, hk = h / (a->Hq / a->Hkv), bhk = b * a->Hkv + hk;
+    const int n_q = count(a->len_q, b, a->Tq), n_k = count(a->len_k, b, a->Tk), last0 = n_k - n_q;
+    const int tile0 = qt * T::kQueries;
+    if (tile0 >= n_q) return;
+    const int q0 = tile0 + pair * 32, my_q = q0 + (lane & 31);
+    const int k_end = kCausal ? min(n_k, min(tile0 + T::kQueries, n_q) + last0) : n_k;
+    const int n = max(0, (k_end + kBlk - 1) / kBlk);
+    const int my_n = max(0, ((kCausal ? min(n_k, q0 + 32 + last0) : n_k) + kBlk - 1) / kBlk);  // steps of the pair's own
+
+    const float ref = q_tile_ref<D>(a, bh, bhk, tile0, T::kQueries / kBlk, n, lane);
+    half8_t frag[1][kKK];
+    float stat = role_p ? INFINITY : 0.f;
+    {
+        const auto& src = role_p ? a->q : a->g;
+        const half_t* row = src.data + b * src.b + h * src.h + my_q * src.t;
+#pragma unroll
+        for (int kk = 0; kk < kKK; ++kk)
+            frag[0][kk] = my_q < n_q ? *reinterpret_cast<const half8_t*>(row + 16 * kk + 8 * hi) : half8_t{};
+        if (my_q < n_q) stat = a->stat[((size_t)bh * a->n_qb + my_q / kBlk) * 64 + my_q % kBlk + (role_p ? 0 : 32)];
+    }
+    float16_t acc[kDB];
+#pragma unroll
+    for (int i = 0; i < kDB; ++i) acc[i] = float16_t{};
+
+    const unsigned lds0 = (unsigned)(uintptr_t)(lds_void_t)(void*)lds;
+    const OpAddr<D> op(lane, lds0);
+    const unsigned p_at = lds0 + T::kXAt + (unsigned)pair * 2048u + 16u * lane, ds_at = p_at + 2 * kPairs * 2048u;
+    const char *kp = reinterpret_cast<const char*>(a->k.data + b * a->k.b + hk * a->k.h), *vp = reinterpret_cast<const char*>(a->v.data + b * a->v.b + hk * a->v.h);
+    const unsigned k_row = 2u * (unsigned)a->k.t, v_row = 2u * (unsigned)a->v.t;
+    int left = n_k - 1;  // the last key, counted from the next copies' first
+    auto copy = [&](int j) {
+        copy_rows<D, T::kW>(kp, k_row, left, lane, wave, lds0 + (unsigned)(j & 3) * T::kTileB);
+        copy_rows<D, T::kW>(vp, v_row, left, lane, wave, lds0 + T::kVAt + (unsigned)(j & 1) * T::kTileB);
+        kp += (size_t)k_row * kBlk, vp += (size_t)v_row * kBlk, left -= kBlk;
+    };
+    const int db0 = role_p ? 0 : kDB;  // dQ^T += K^T dS^T, this role's columns
+    // register r is key 32 j + 4 hi + 8 (r / 4) + r % 4; the last that this lane's query sees
+    auto limit = [&](int j) { return min(kCausal ? my_q + last0 : n_k, n_k - 1) - j * kBlk - 4 * hi; };
+    auto ragged = [&](int j) { return (kCausal && j * kBlk + 31 > q0 + last0) || (j + 1) * kBlk > n_k; };
+    if (n > 0) copy(0);
+    if constexpr (role_p) {
+        auto scores = [&](int j) {
+            const unsigned st = (unsigned)(j & 3) * T::kTileB;
+            float16_t x1[1] = {float16_t{}}, &s = x1[0];
+            mul_rows<D, 1>(op.rows, st, frag, x1);
+            if (ragged(j)) {
+                const int lim = limit(j);
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (8 * (r >> 2) + (r & 3) > lim) s[r] = -INFINITY;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = fast_exp2(fmaf(s[r], a->c2, ref - stat));
+#pragma unroll
+            for (int x = 0; x < 2; ++x) lds_write_b128(p_at + (unsigned)((j & 1) * kPairs * 2048 + x * 1024), pack8(s, x));
+        };
+        auto take = [&](int j) {
+            half8_t ds[1][2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) ds[0][x] = lds_read_b128(ds_at + (unsigned)((j & 1) * kPairs * 2048 + x * 1024));
+            mul_cols<D, 1, kDB>(op.cols, (unsigned)(j & 3) * T::kTileB, db0, ds, acc);
+        };
+        // round j: dQ of step j - 2, S and P of step j, while step j + 1 is copied
+#pragma clang loop unroll(disable)
+        for (int j = 0; j < n + 2; ++j) {
+            asm volatile("" : "+s"(j));
+            dma_wait_barrier();
+            if (j + 1 < n) copy(j + 1);
+            if (j > 1 && j - 2 < my_n) take(j - 2);
+            if (j < my_n) scores(j);
+        }
+    } else {
+        float16_t x1[1], &s = x1[0];
+        auto products = [&](int j) {
+            const unsigned st = (unsigned)(j & 1) * T::kTileB;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = stat;
+            mul_rows<D, 1>(op.rows, T::kVAt + st, frag, x1);
+        };
+        // round j + 1: dS and dQ of step j, dP of step j + 1
+#pragma clang loop unroll(disable)
+        for (int j = -1; j < n + 1; ++j) {
+            asm volatile("" : "+s"(j));
+            dma_wait_barrier();
+            if (j + 2 < n) copy(j + 2);
+            if (j >= 0 && j < my_n) {
+                half8_t ds1[1][2];
+                half8_t(&ds)[2] = ds1[0];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) ds[x] = times(lds_read_b128(p_at + (unsigned)((j & 1) * kPairs * 2048 + x * 1024)), s, x);
+                if (ragged(j)) {
+                    const int lim = limit(j);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (8 * (r >> 2) + (r & 3) > lim) ds[r >> 3][r & 7] = (half_t)0.f;
+                }
+#pragma unroll
+                for (int x = 0; x < 2; ++x) lds_write_b128(ds_at + (unsigned)((j & 1) * kPairs * 2048 + x * 1024), ds[x]);
+                mul_cols<D, 1, kDB>(op.cols, (unsigned)(j & 3) * T::kTileB, db0, ds1, acc);
+            }
+            if (j + 1 < my_n)
+                products(j + 1);
+            else  // no dP: what it was is not kept through the other branch
+                asm volatile("" : "=v"(s));
+        }
+    }
+    a = fresh(a);
+    store_rows<1, kDB>(acc, a->dq.data + b * a->dq.b + h * a->dq.h + (role_p ? 0 : D / 2), a->dq.t, q0, n_q, again(lane), exp2f(-ref) * a->scale);
+}
+
+template <int D, bool kCausal>
+__global__ void __launch_bounds__(64 * KvTile<D>::kW, 2) attn_bwd_kernel(BwdArgs args) {
+    const args_t a = (args_t)__builtin_amdgcn_kernarg_segment_ptr();  // args, the only parameter
+    constexpr int kLds = KvTile<D>::kLds > QTile<D>::kLds ? KvTile<D>::kLds : QTile<D>::kLds;
+    __shared__ __align__(1024) half_t lds[kLds / 2];
+    // the first half of a workgroup's waves makes P, the second dS
+    const bool role_p = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) < KvTile<D>::kPairs;
+    if ((int)blockIdx.x < args.n_kv) {
+        if (role_p)
+            kv_tile<D, kCausal, true>(fresh(a), lds, blockIdx.x);
+        else
+            kv_tile<D, kCausal, false>(fresh(a), lds, blockIdx.x);
+    } else if constexpr (QTile<D>::kRoles) {
+        if (role_p)
+            q_tile_roles<D, kCausal, true>(fresh(a), lds, blockIdx.x - args.n_kv);
+        else
+            q_tile_roles<D, kCausal, false>(fresh(a), lds, blockIdx.x - args.n_kv);
+    } else {
+        q_tile<D, kCausal>(fresh(a), lds, blockIdx.x - args.n_kv);
+    }
+}
+
+// The sum of a split key tile's parts, in their order: one wave for each wave that wrote them.
+template <int D>
+__global__ void __launch_bounds__(64) attn_bwd_join_kernel(BwdArgs a) {
+    using T = KvTile<D>;
+    const int lane = threadIdx.x, n_bh = a.B * a.Hkv;
+    const int wave = blockIdx.x % T::kW, rest = blockIdx.x / T::kW, bh = rest % n_bh, kt = rest / n_bh;
+    const int b = bh / a.Hkv, hk = bh % a.Hkv, n_k = count(a.len_k, b, a.Tk);
+    const int k0 = kt * T::kKeys + wave % T::kPairs * 32 * T::kKB;
+    if (k0 >= n_k) return;
+    const Rows16& out = wave < T::kPairs ? a.dv : a.dk;
+    const float4_t* w = reinterpret_cast<const float4_t*>(a.part) + (((size_t)bh * a.n_kt + kt) * a.n_part * T::kW + wave) * (T::kAcc * 256) + lane;
+    half_t* base = out.data + b * out.b + hk * out.h + 4 * (lane >> 5);
+    const int key = k0 + (lane & 31);
+    for (int i = 0; i < 4 * T::kAcc; ++i) {
+        const int r = key + 32 * (i / (4 * (D / 32))), d = 8 * (i % (4 * (D / 32)));
+        float4_t x = w[(size_t)i * 64];
+        for (int p = 1; p < a.n_part; ++p) x += w[(size_t)p * T::kW * (T::kAcc * 256) + i * 64];
+        if (r < n_k) *reinterpret_cast<half4_t*>(base + r * out.t + d) = half4_t{(half_t)x[0], (half_t)x[1], (half_t)x[2], (half_t)x[3]};
+    }
+}
+
+// Sizes of a call, and where its workspace holds what.
+struct Plan {
+    int n_qb, n_kb, n_kt, n_qt, n_part;
+    size_t stat, row_max, key_max, gated, part, bytes;
+};
+template <int D>
+Plan plan(int B, int Hq, int Hkv, int Tq, int Tk, bool gated, bool causal) {
+    Plan p;
+    auto up = [](long long a, long long b) { return (int)((a + b - 1) / b); };
+    p.n_qb = up(Tq, kBlk), p.n_kb = up(Tk, kBlk);
+    p.n_kt = up(Tk, KvTile<D>::kKeys), p.n_qt = up(Tq, QTile<D>::kQueries);
+    const long long tiles = (long long)B * Hkv * p.n_kt, steps = (long long)(Hq / Hkv) * p.n_qb;
+    const long long want = (768 + tiles - 1) / tiles, most = steps / 8 > 1 ? steps / 8 : 1;
+    p.n_part = tiles >= 512 ? 1 : (int)(want < most ? want : most);
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t was = at;
+        at += (bytes + 255) & ~(size_t)255;
+        return was;
+    };
+    p.stat = take((size_t)B * Hq * p.n_qb * 64 * 4);
+    p.row_max = take((size_t)B * Hq * p.n_qb * 8);
+    p.key_max = take((size_t)B * Hkv * p.n_kb * 4);
+    p.gated = gated ? take((size_t)B * Hq * Tq * D * 2) : 0;
+    p.part = p.n_part > 1 ? take((size_t)tiles * p.n_part * KvTile<D>::kKeys * D * 2 * 4) : 0;
+    p.bytes = at;
+    return p;
+}
+
+template <int D>
+hipError_t backward(const AttnRows& x, const Rows16& d_out, const Rows16& dq, const Rows16& dk, const Rows16& dv, const Rows16& dgate,
+                    int B, int Hq, int Hkv, int Tq, float scale, int causal, void* ws, hipStream_t stream) {
+    const int Tk = x.Sk;
+    const bool gated = x.gate.data != nullptr;
+    const Plan p = plan<D>(B, Hq, Hkv, Tq, Tk, gated, causal != 0);
+    char* w = static_cast<char*>(ws);
+    float* stat = reinterpret_cast<float*>(w + p.stat);
+    float2* row_max = reinterpret_cast<float2*>(w + p.row_max);
+    float* key_max = reinterpret_cast<float*>(w + p.key_max);
+    half_t* g = reinterpret_cast<half_t*>(w + p.gated);
+    RowsArgs r = {d_out, x.o, x.gate, x.v, dgate, gated ? g : nullptr, x.lse, stat, row_max, key_max, x.len_q, x.len_k, Hq, Hkv, Tq, Tk, p.n_qb,
+                  p.n_kb, B * Hq * p.n_qb};
+    hipLaunchKernelGGL(attn_bwd_rows_kernel<D>, dim3(r.n_rows + B * Hkv * p.n_kb), dim3(256), 0, stream, r);
+    const Rows16 dO = gated ? Rows16{g, (long long)Hq * Tq * D, (long long)Tq * D, D} : d_out;
+    BwdArgs a = {x.q, x.k, x.v, dO, dq, dk, dv, stat, row_max, key_max, reinterpret_cast<float*>(w + p.part), x.len_q, x.len_k,
+                 B, Hq, Hkv, Tq, Tk, p.n_qb, p.n_kb, p.n_kt, p.n_part, p.n_qt, B * Hkv * p.n_kt * p.n_part, scale, scale * kLog2e};
+    const dim3 grid(a.n_kv + B * Hq * p.n_qt), block(64 * KvTile<D>::kW);
+    if (causal)
+        hipLaunchKernelGGL((attn_bwd_kernel<D, true>), grid, block, 0, stream, a);
+    else
+        hipLaunchKernelGGL((attn_bwd_kernel<D, false>), grid, block, 0, stream, a);
+    if (p.n_part > 1)
+        hipLaunchKernelGGL(attn_bwd_join_kernel<D>, dim3(B * Hkv * p.n_kt * KvTile<D>::kW), dim3(64), 0, stream, a);
+    return hipGetLastError();
+}
+
+}  // namespace
+}  // namespace bwd
+
+size_t attn_bwd_ws_bytes(int B, int Hq, int Hkv, int Tq, int Tk, int D, bool gated, bool causal) {
+    const bwd::Plan p = D == 256   ? bwd::plan<256>(B, Hq, Hkv, Tq, Tk, gated, causal)
+                   : D == 128 ? bwd::plan<128>(B, Hq, Hkv, Tq, Tk, gated, causal)
+                              : bwd::plan<64>(B, Hq, Hkv, Tq, Tk, gated, causal);
+    return p.bytes;
+}
+
+hipError_t attn_bwd(const AttnRows& x, const Rows16& d_out, const Rows16& dq, const Rows16& dk, const Rows16& dv, const Rows16& dgate,
+                    int B, int Hq, int Hkv, int Tq, int D, float scale, int causal, void* ws, hipStream_t stream) {
+    if (D == 256) return bwd::backward<256>(x, d_out, dq, dk, dv, dgate, B, Hq, Hkv, Tq, scale, causal, ws, stream);
+    if (D == 128) return bwd::backward<128>(x, d_out, dq, dk, dv, dgate, B, Hq, Hkv, Tq, scale, causal, ws, stream);
+    return bwd::backward<64>(x, d_out, dq, dk, dv, dgate, B, Hq, Hkv, Tq, scale, causal, ws, stream);
+}
+
+}  // namespace tsa

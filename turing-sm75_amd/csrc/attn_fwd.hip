@@ -32,6 +32,7 @@
 #include <climits>
 #include <type_traits>
 
+#include "attn_tiles.h"
 #include "common.h"
 #include "kernels.h"
 
@@ -40,19 +41,8 @@ namespace {
 
 constexpr int kKRows = 64;   // keys per LDS tile
 
-// 16-byte chunk swizzle of an LDS tile row: chunk c of row r lives at c ^ swz<D>(r).
-// LDS has 64 banks of 4 bytes; a 256-byte D = 128 row spans all of them, so a chunk's
-// banks depend on its position only.  The K operand reads (ds_read_b128, 16 lanes per
-// cycle) take 16 consecutive rows at one chunk: swz is a permutation of r % 16.  The
-// transposing V reads (ds_read_b64_tr_b16, 32 lanes per cycle) take 4 aligned rows x 4
-// chunks of one aligned chunk block: swz moves the 4 rows to 4 different chunk blocks.
-// At D = 64 two rows share the 64 banks and the other formula keeps both read patterns
-// conflict free.
-template <int D>
-__device__ __forceinline__ int swz(int r) {
-    if (D >= 128) return 4 * (r & 3) + ((r >> 2) & 3);  // D = 256: a row is two bank periods
-    return (2 * (r & 3) + ((r >> 2) & 1)) & 7;
-}
+// The training form's view of its tensors (AttnRows of kernels.h); the others' are dense and take none.
+struct Dense {};
 
 template <int D>
 struct Cfg {
@@ -62,11 +52,6 @@ struct Cfg {
     static constexpr int kDBlocks = D / 32;                      // 32-row blocks of O^T
     static constexpr int kLdsBytes = 2 * 2 * kTile * 2;          // 2 buffers x (K, V)
 };
-
-template <int D>
-__device__ __forceinline__ int chunk_pos(int r, int c) {
-    return c ^ swz<D>(r);
-}
 
 // Map the linear workgroup id to (bh, query tile).  Workgroups are dispatched round
 // robin over the 8 XCDs; when BH is a multiple of 8 the heads are spread over the XCDs so
@@ -96,19 +81,6 @@ __device__ __forceinline__ void map_block(int bid, int BH, int n_qt, bool causal
     qt = causal ? (n_qt - 1 - rank) : rank;
 }
 
-typedef __attribute__((address_space(3))) void* lds_void_t;
-
-// LDS reads at a byte address held as an integer (so that address arithmetic can be an
-// XOR with an immediate plus an offset folded into the instruction).
-__device__ __forceinline__ half8_t lds_read_b128(unsigned addr) {
-    typedef __attribute__((address_space(3))) const half8_t* p_t;
-    return *(p_t)(addr);
-}
-__device__ __forceinline__ half4_t lds_read_tr16_at(unsigned addr) {
-    typedef __attribute__((address_space(3))) fp16x4_t* p_t;
-    return __builtin_bit_cast(half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16((p_t)(addr)));
-}
-
 // K/V tile copy plan.  One LDS-DMA instruction moves 1 KiB (lane l: 16 bytes to M0 + 16*l);
 // a tile of 64 rows x D halfs is kTile instructions, K then V, and wave w of kW issues
 // instructions w + kW j.  LDS chunk position p of row r holds source chunk p ^ swz(r), so
@@ -126,14 +98,6 @@ __device__ __forceinline__ unsigned dma_off(int blk, int lane, int lastrow) {
     const int row = P / Dma<D>::kChunks, cpos = P % Dma<D>::kChunks;
     const int c = cpos ^ swz<D>(row);
     return (unsigned)(min(row, lastrow) * D + c * 8) * 2u;
-}
-// src = base + off (64-bit base in SGPRs, 32-bit VGPR offset).  Inline asm on purpose:
-// the compiler does not track LDS written by DMA per buffer and would wait for every
-// copy in flight before the first LDS read of the other buffer; the kernel orders the
-// copies itself (vmcnt(0) and a barrier at the end of each tile).
-__device__ __forceinline__ void dma_issue(const void* base, unsigned off, unsigned lds_addr) {
-    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(off), "s"(base), "{m0}"(lds_addr)
-                 : "memory");
 }
 // This wave's share of the copies of K/V rows k0..k0+63 into the buffer at lds_buf, in
 // two halves (kPart 0: j < kPerWave/2, kPart 1: the rest) so each can be issued between
@@ -180,19 +144,45 @@ __device__ __forceinline__ void copy_tile(unsigned off0, int wave, const half_t*
     else
         issue_all(std::true_type{});
 }
-__device__ __forceinline__ void dma_wait_barrier() {
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's copies have landed
-    lds_barrier();
+// copy_tile of rows that lie anywhere: K and V have a stride each (bytes, at most 2^25, so a tile's
+// offsets fit 32 bits), and a wave's blocks, whole multiples of 8 rows apart, differ by a scalar
+// offset.  A lane's row and chunk in the wave's first block are made from its number for each half of a
+// tile: held, they cost two registers that D = 256 does not have.
+struct TileRows {
+    const half_t *k, *v;
+    unsigned k_stride, v_stride;
+};
+template <int D, int kPart, int kW, int kRowsT = kKRows>
+__device__ __forceinline__ void copy_tile(const TileRows& src, int lane, int wave, int k0, int S, unsigned lds_buf) {
+    constexpr int kStep = kW * 1024 / (2 * D), kC = D / 8;
+    const int lastrow = S - 1 - k0;
+    asm volatile("" : "+v"(lane));
+    const int row = (64 * wave + lane) / kC;
+    const unsigned col = 16u * (unsigned)((lane % kC) ^ swz<D>(row));
+#pragma unroll
+    for (int j = kPart * Dma<D, kW, kRowsT>::kPerWave / 2; j < (kPart + 1) * Dma<D, kW, kRowsT>::kPerWave / 2; ++j) {
+        constexpr int kT = Dma<D, kW, kRowsT>::kTile;
+        const bool isv = kW * j >= kT;
+        const int dblk = kW * j - (isv ? kT : 0);
+        const int rows = kStep * (dblk / kW);  // rows from the wave's first block to this one
+        const unsigned flip = kStep % 16 == 8 && ((dblk / kW) & 1) ? 32u : 0u;
+        const unsigned stride = isv ? src.v_stride : src.k_stride;
+        // (a full tile's clamp takes no row back)
+        const unsigned o = (unsigned)min(row + rows, lastrow) * stride + (col ^ flip);
+        dma_issue_any(reinterpret_cast<const char*>(isv ? src.v : src.k) + (size_t)k0 * stride, o,
+                  lds_buf + (unsigned)(isv ? kRowsT * D * 2 : 0) + 1024u * (unsigned)(wave + dblk));
+    }
 }
 
 // Epilogue: O = O^T / l (times sigmoid(gate)), 4 consecutive d per store.  O, gate: the head's rows.
 template <int D>
 __device__ __forceinline__ void store_o(const float16_t (&o)[Cfg<D>::kDBlocks], float l, half_t* __restrict__ O,
-                                        const half_t* __restrict__ gate, int my_q, int S, int hi) {
+                                        const half_t* __restrict__ gate, int my_q, int S, int hi, long long o_t = D,
+                                        long long g_t = D) {
     const float inv = l > 0.f ? 1.f / l : 0.f;
     if (my_q < S) {
-        half_t* orow = O + (size_t)my_q * D;
-        const half_t* grow = gate ? gate + (size_t)my_q * D : nullptr;
+        half_t* orow = O + my_q * o_t;
+        const half_t* grow = gate ? gate + my_q * g_t : nullptr;
 #pragma unroll
         for (int db = 0; db < Cfg<D>::kDBlocks; ++db)
 #pragma unroll
@@ -213,16 +203,23 @@ __device__ __forceinline__ void store_o(const float16_t (&o)[Cfg<D>::kDBlocks], 
     }
 }
 
+// A row's statistic: the logarithm of the sum of its exponentials, from the maximum they were taken
+// against (as the exponentials had it) and their sum; minus infinity for a row that sees no key.
+__device__ __forceinline__ float row_lse(float m, float l, float c2) {
+    return l > 0.f ? (m * c2 + __builtin_amdgcn_logf(l)) * 0.69314718056f : (l == 0.f ? -INFINITY : l);
+}
+
 // kW waves per workgroup, 32 query rows each: kW = 4 at D <= 128 (two workgroups per CU,
 // two waves per SIMD), kW = 8 at D = 256 (one workgroup per CU with the 128 KiB of K/V
 // tiles, two waves per SIMD sharing them).
-template <int D, bool kCausal, int kW>
+template <int D, bool kCausal, int kW, class Rows = Dense>
 __global__ void __launch_bounds__(64 * kW, 2)
 attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
                 const half_t* __restrict__ V, const half_t* __restrict__ gate,
                 half_t* __restrict__ O, int S, int BH, int n_qt, int Hq, int group,
-                float c2 /* scale * log2(e) */) {
+                float c2 /* scale * log2(e) */, Rows rows) {
     using C = Cfg<D>;
+    constexpr bool kAny = !std::is_same_v<Rows, Dense>;  // rows anywhere, lengths, row statistics
     // static and 1 KiB aligned: the XOR address forms below need the buffer's low 10 bits zero
     __shared__ __align__(1024) half_t lds[C::kLdsBytes / 2];
 
@@ -234,6 +231,21 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
     const size_t head = (size_t)bh * S * D;  // Q, O, gate: query head bh = b * Hq + h
     const size_t kvhead = (size_t)((bh / Hq) * (Hq / group) + (bh % Hq) / group) * S * D;
     const int q0 = qt * (32 * kW);
+    // Queries and keys of this sequence, and the last key that query 0 sees.
+    const half_t *Qh = Q + head, *Kh = K + kvhead, *Vh = V + kvhead;
+    long long q_t = D, k_t = D, v_t = D, o_t = D, g_t = D;
+    int n_q = S, n_k = S, last0 = 0;
+    if constexpr (kAny) {
+        const int b = bh / Hq, h = bh % Hq, hk = h / group;
+        Qh = Q + b * rows.q.b + h * rows.q.h;
+        Kh = K + b * rows.k.b + hk * rows.k.h;
+        Vh = V + b * rows.v.b + hk * rows.v.h;
+        q_t = rows.q.t, k_t = rows.k.t, v_t = rows.v.t, o_t = rows.o.t, g_t = rows.gate.t;
+        n_q = rows.len_q ? min(max(rows.len_q[b], 0), S) : S;
+        n_k = rows.len_k ? min(max(rows.len_k[b], 0), rows.Sk) : rows.Sk;
+        last0 = n_k - n_q;
+        if (q0 >= n_q) return;
+    }
     const int qw0 = q0 + 32 * wave;
     const int my_q = qw0 + (lane & 31);
 
@@ -242,15 +254,15 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
     half8_t qf[C::kKSteps];
 #pragma unroll
     for (int kk = 0; kk < C::kKSteps; ++kk) {
-        if (my_q < S)
-            qf[kk] = *reinterpret_cast<const half8_t*>(Q + head + (size_t)my_q * D + 16 * kk + 8 * hi);
+        if (my_q < n_q)
+            qf[kk] = *reinterpret_cast<const half8_t*>(Qh + my_q * q_t + 16 * kk + 8 * hi);
         else
             qf[kk] = half8_t{};
     }
 
-    const int kv_end = kCausal ? min(S, q0 + 32 * kW) : S;
+    const int kv_end = kCausal ? min(n_k, q0 + 32 * kW + last0) : n_k;
     const int n_tiles = (kv_end + kKRows - 1) / kKRows;
-    const int wave_kv_end = kCausal ? min(S, qw0 + 32) : S;
+    const int wave_kv_end = kCausal ? min(n_k, qw0 + 32 + last0) : n_k;
 
     float16_t o[C::kDBlocks];
 #pragma unroll
@@ -285,8 +297,20 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
         const int r = 4 * hi + vj + 8 * e;
         va[e] = lds0 + C::kTile * 2 + r * kRowB + 16u * (unsigned)chunk_pos<D>(r, vchunk) + 2u * vsub;
     }
-    copy_tile<D, 0, kW>(off, wave, K + kvhead, V + kvhead, 0, S, lds0);
-    copy_tile<D, 1, kW>(off, wave, K + kvhead, V + kvhead, 0, S, lds0);
+    const TileRows src = {Kh, Vh, 2u * (unsigned)k_t, 2u * (unsigned)v_t};
+    auto copy = [&](auto Part, int k0, unsigned buf) {
+        constexpr int kPart = decltype(Part)::value;
+        if constexpr (kAny)
+            copy_tile<D, kPart, kW>(src, lane, wave, k0, n_k, buf);
+        else
+            copy_tile<D, kPart, kW>(off, wave, Kh, Vh, k0, S, buf);
+    };
+    constexpr std::integral_constant<int, 0> kFirst;
+    constexpr std::integral_constant<int, 1> kSecond;
+    if (!kAny || n_tiles > 0) {
+        copy(kFirst, 0, lds0);
+        copy(kSecond, 0, lds0);
+    }
     dma_wait_barrier();
 
     if constexpr (D <= 128) {
@@ -303,8 +327,8 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
             const unsigned nbuf = lds0 + (unsigned)(u ^ 1) * buf_bytes;
             if (k0 >= wave_kv_end) {  // this wave's queries end before the tile: copies only
                 if (more) {
-                    copy_tile<D, 0, kW>(off, wave, K + kvhead, V + kvhead, k0 + kKRows, S, nbuf);
-                    copy_tile<D, 1, kW>(off, wave, K + kvhead, V + kvhead, k0 + kKRows, S, nbuf);
+                    copy(kFirst, k0 + kKRows, nbuf);
+                    copy(kSecond, k0 + kKRows, nbuf);
                 }
             } else {
                 const unsigned ubase = (unsigned)u * buf_bytes;
@@ -320,7 +344,7 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
                     s[0] = mfma32(lds_read_b128(a), qf[kk], s[0]);
                     s[1] = mfma32(lds_read_b128(a + 32 * kRowB), qf[kk], s[1]);
                     if (kk == C::kKSteps / 2 - 1 && more)
-                        copy_tile<D, 0, kW>(off, wave, K + kvhead, V + kvhead, k0 + kKRows, S, nbuf);
+                        copy(kFirst, k0 + kKRows, nbuf);
                 }
                 // V^T operands of the first key step, read now so that their LDS time runs under
                 // the softmax (V does not depend on P); a wave reads transposed V at ~18 B/clk.
@@ -334,12 +358,12 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
 #pragma unroll
                 for (int db = 0; db < C::kDBlocks; ++db) v0[db] = read_v(0, db);
                 // ---- masks: causal diagonal and keys past S ----
-                if ((kCausal && k0 + kKRows - 1 > qw0) || k0 + kKRows > S) {
+                if ((kCausal && k0 + kKRows - 1 > qw0 + last0) || k0 + kKRows > n_k) {
                     // register r of block kb holds key k0 + 4 hi + c, c = 32 kb + 8 (r / 4) + r % 4:
                     // compare the constant c against per-lane limits
                     const int base = k0 + 4 * hi;
-                    const int lim_q = kCausal ? my_q - base : INT_MAX;  // masked when c > lim_q
-                    const int lim_s = S - base;                         // masked when c >= lim_s
+                    const int lim_q = kCausal ? my_q + last0 - base : INT_MAX;  // masked when c > lim_q
+                    const int lim_s = n_k - base;                         // masked when c >= lim_s
 #pragma unroll
                     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -370,11 +394,14 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        p[2 * kb + (r >> 3)][r & 7] = (half_t)fast_exp2(fmaf(s[kb][r], c2, -mc));
+                    for (int r = 0; r < 16; ++r) {
+                        const float e = fast_exp2(fmaf(s[kb][r], c2, -mc));
+                        if constexpr (kAny) l += e;  // in 32 bits: the sum is an output
+                        p[2 * kb + (r >> 3)][r & 7] = (half_t)e;
+                    }
                 const half2_t one2 = {(half_t)1.f, (half_t)1.f};
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < (kAny ? 0 : 4); ++i)
 #pragma unroll
                     for (int w2 = 0; w2 < 4; ++w2)
                         l = __builtin_amdgcn_fdot2(half2_t{p[i][2 * w2], p[i][2 * w2 + 1]}, one2, l, false);
@@ -383,7 +410,7 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks) {
                     if (ks == 1 && more)
-                        copy_tile<D, 1, kW>(off, wave, K + kvhead, V + kvhead, k0 + kKRows, S, nbuf);
+                        copy(kSecond, k0 + kKRows, nbuf);
 #pragma unroll
                     for (int db = 0; db < C::kDBlocks; ++db)
                         o[db] = mfma32(ks == 0 ? v0[db] : read_v(ks, db), p[ks], o[db]);
@@ -403,18 +430,18 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
             const unsigned nbuf = lds0 + ((t + 1) & 1) * buf_bytes;
             if (k0 >= wave_kv_end) {  // this wave's queries end before the tile: copies only
                 if (more) {
-                    copy_tile<D, 0, kW>(off, wave, K + kvhead, V + kvhead, k0 + kKRows, S, nbuf);
-                    copy_tile<D, 1, kW>(off, wave, K + kvhead, V + kvhead, k0 + kKRows, S, nbuf);
+                    copy(kFirst, k0 + kKRows, nbuf);
+                    copy(kSecond, k0 + kKRows, nbuf);
                 }
             } else {
                 const unsigned ubase = (unsigned)(t & 1) * buf_bytes;
                 // the first half of the next tile's copies goes out at the top
-                if (more) copy_tile<D, 0, kW>(off, wave, K + kvhead, V + kvhead, k0 + kKRows, S, nbuf);
+                if (more) copy(kFirst, k0 + kKRows, nbuf);
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb) {
                     const int kb0 = k0 + 32 * kb;  // first key of this half
                     // a second half wholly past this wave's last query adds nothing
-                    if (kCausal && kb == 1 && kb0 > qw0 + 31) break;
+                    if (kCausal && kb == 1 && kb0 > qw0 + 31 + last0) break;
                     // The XORed addresses are recomputed next to their reads in each half (one
                     // VALU op each) instead of being held: the empty asm hides that they repeat.
                     asm volatile("" : "+v"(ka), "+v"(va[0]), "+v"(va[1]));
@@ -436,12 +463,12 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
                         __builtin_amdgcn_sched_barrier(0);
                     }
                     // ---- masks: causal diagonal and keys past S ----
-                    if ((kCausal && kb0 + 31 > qw0) || kb0 + 32 > S) {
+                    if ((kCausal && kb0 + 31 > qw0 + last0) || kb0 + 32 > n_k) {
                         // register r holds key kb0 + 4 hi + c, c = 8 (r / 4) + r % 4: compare the
                         // constant c against per-lane limits
                         const int base = kb0 + 4 * hi;
-                        const int lim_q = kCausal ? my_q - base : INT_MAX;  // masked when c > lim_q
-                        const int lim_s = S - base;                         // masked when c >= lim_s
+                        const int lim_q = kCausal ? my_q + last0 - base : INT_MAX;  // masked when c > lim_q
+                        const int lim_s = n_k - base;                         // masked when c >= lim_s
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
                             const int c = 8 * (r >> 2) + (r & 3);
@@ -468,12 +495,15 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
                     const float mc = m == -INFINITY ? 0.f : m * c2;
                     half8_t p[2];
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        p[r >> 3][r & 7] = (half_t)fast_exp2(fmaf(sh[r], c2, -mc));
+                    for (int r = 0; r < 16; ++r) {
+                        const float e = fast_exp2(fmaf(sh[r], c2, -mc));
+                        if constexpr (kAny) l += e;
+                        p[r >> 3][r & 7] = (half_t)e;
+                    }
                     // row sum of the fp16 P that multiplies V, on v_dot2_f32_f16
                     const half2_t one2 = {(half_t)1.f, (half_t)1.f};
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
+                    for (int i = 0; i < (kAny ? 0 : 2); ++i)
 #pragma unroll
                         for (int u = 0; u < 4; ++u)
                             l = __builtin_amdgcn_fdot2(half2_t{p[i][2 * u], p[i][2 * u + 1]}, one2, l, false);
@@ -498,7 +528,7 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
                         if (i + kPreV < kSteps)
                             vbuf[i + kPreV] = read_v(2 * kb + (i + kPreV) / C::kDBlocks, (i + kPreV) % C::kDBlocks);
                         if (kb == 0 && i == C::kDBlocks && more)
-                            copy_tile<D, 1, kW>(off, wave, K + kvhead, V + kvhead, k0 + kKRows, S, nbuf);
+                            copy(kSecond, k0 + kKRows, nbuf);
                         o[db] = mfma32(vbuf[i], p[ks], o[db]);
                         __builtin_amdgcn_sched_barrier(0);
                     }
@@ -509,7 +539,15 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
         }
     }
 
-    store_o<D>(o, sum_xor32(l), O + head, gate ? gate + head : nullptr, my_q, S, hi);
+    l = sum_xor32(l);
+    if constexpr (kAny) {
+        const int b = bh / Hq, h = bh % Hq;
+        if (hi == 0 && my_q < n_q) rows.lse[(size_t)bh * S + my_q] = row_lse(m, l, c2);
+        store_o<D>(o, l, O + b * rows.o.b + h * rows.o.h, gate ? gate + b * rows.gate.b + h * rows.gate.h : nullptr, my_q, n_q, hi,
+                   o_t, g_t);
+    } else {
+        store_o<D>(o, l, O + head, gate ? gate + head : nullptr, my_q, S, hi);
+    }
 }
 
 // ---------------------------------------------------------------------------------
@@ -522,13 +560,14 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
 // operand read-ahead and the copies are those of attn_fwd_kernel's D = 256 form.  (kKG = 1: no split, a shorter
 // query tile.)
 // ---------------------------------------------------------------------------------
-template <int D, bool kCausal, int kQG, int kKG, int kKT>
+template <int D, bool kCausal, int kQG, int kKG, int kKT, class Rows = Dense>
 __global__ void __launch_bounds__(64 * kQG * kKG, 2)
 attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
                    const half_t* __restrict__ V, const half_t* __restrict__ gate,
                    half_t* __restrict__ O, int S, int BH, int n_qt, int Hq, int group,
-                   float c2 /* scale * log2(e) */) {
+                   float c2 /* scale * log2(e) */, Rows rows) {
     using C = Cfg<D>;
+    constexpr bool kAny = !std::is_same_v<Rows, Dense>;
     constexpr int kW = kQG * kKG, kRows = kKG * kKT;  // waves; keys per tile
     constexpr int kBuf = 2 * kRows * D;               // halfs per buffer (K, V)
     static_assert(2 * kBuf * 2 >= (kKG - 1) * kQG * 32 * D * 4, "the partial O's fit the tile buffers");
@@ -544,20 +583,35 @@ attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
     const size_t head = (size_t)bh * S * D;
     const size_t kvhead = (size_t)((bh / Hq) * (Hq / group) + (bh % Hq) / group) * S * D;
     const int q0 = qt * (32 * kQG);
+    // Queries and keys of this sequence, and the last key that query 0 sees.
+    const half_t *Qh = Q + head, *Kh = K + kvhead, *Vh = V + kvhead;
+    long long q_t = D, k_t = D, v_t = D, o_t = D, g_t = D;
+    int n_q = S, n_k = S, last0 = 0;
+    if constexpr (kAny) {
+        const int b = bh / Hq, h = bh % Hq, hk = h / group;
+        Qh = Q + b * rows.q.b + h * rows.q.h;
+        Kh = K + b * rows.k.b + hk * rows.k.h;
+        Vh = V + b * rows.v.b + hk * rows.v.h;
+        q_t = rows.q.t, k_t = rows.k.t, v_t = rows.v.t, o_t = rows.o.t, g_t = rows.gate.t;
+        n_q = rows.len_q ? min(max(rows.len_q[b], 0), S) : S;
+        n_k = rows.len_k ? min(max(rows.len_k[b], 0), rows.Sk) : rows.Sk;
+        last0 = n_k - n_q;
+        if (q0 >= n_q) return;
+    }
     const int qw0 = q0 + 32 * qg;
     const int my_q = qw0 + (lane & 31);
 
     half8_t qf[C::kKSteps];
 #pragma unroll
     for (int kk = 0; kk < C::kKSteps; ++kk) {
-        if (my_q < S)
-            qf[kk] = *reinterpret_cast<const half8_t*>(Q + head + (size_t)my_q * D + 16 * kk + 8 * hi);
+        if (my_q < n_q)
+            qf[kk] = *reinterpret_cast<const half8_t*>(Qh + my_q * q_t + 16 * kk + 8 * hi);
         else
             qf[kk] = half8_t{};
     }
-    const int kv_end = kCausal ? min(S, q0 + 32 * kQG) : S;
+    const int kv_end = kCausal ? min(n_k, q0 + 32 * kQG + last0) : n_k;
     const int n_tiles = (kv_end + kRows - 1) / kRows;
-    const int wave_kv_end = kCausal ? min(S, qw0 + 32) : S;
+    const int wave_kv_end = kCausal ? min(n_k, qw0 + 32 + last0) : n_k;
 
     float16_t o[C::kDBlocks];
 #pragma unroll
@@ -580,16 +634,26 @@ attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
         const int r = 4 * hi + vj + 8 * e;
         va[e] = lds0 + goff + kRows * kRowB + r * kRowB + 16u * (unsigned)chunk_pos<D>(r, vchunk) + 2u * vsub;
     }
-    const half_t* Kh = K + kvhead;
-    const half_t* Vh = V + kvhead;
-    copy_tile<D, 0, kW, kRows>(off, wave, Kh, Vh, 0, S, lds0);
-    copy_tile<D, 1, kW, kRows>(off, wave, Kh, Vh, 0, S, lds0);
+    const TileRows src = {Kh, Vh, 2u * (unsigned)k_t, 2u * (unsigned)v_t};
+    auto copy = [&](auto Part, int k0, unsigned buf) {
+        constexpr int kPart = decltype(Part)::value;
+        if constexpr (kAny)
+            copy_tile<D, kPart, kW, kRows>(src, lane, wave, k0, n_k, buf);
+        else
+            copy_tile<D, kPart, kW, kRows>(off, wave, Kh, Vh, k0, S, buf);
+    };
+    constexpr std::integral_constant<int, 0> kFirst;
+    constexpr std::integral_constant<int, 1> kSecond;
+    if (!kAny || n_tiles > 0) {
+        copy(kFirst, 0, lds0);
+        copy(kSecond, 0, lds0);
+    }
     dma_wait_barrier();
 
     for (int t = 0; t < n_tiles; ++t) {
         const unsigned ubase = (unsigned)(t & 1) * kBufB, nbuf = lds0 + (unsigned)((t + 1) & 1) * kBufB;
         const bool more = t + 1 < n_tiles;
-        if (more) copy_tile<D, 0, kW, kRows>(off, wave, Kh, Vh, (t + 1) * kRows, S, nbuf);
+        if (more) copy(kFirst, (t + 1) * kRows, nbuf);
         bool copied = false;
 #pragma unroll
         for (int kb = 0; kb < kKT / 32; ++kb) {
@@ -611,10 +675,10 @@ attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
                 sh = mfma32(kop[kk], qf[kk], sh);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if ((kCausal && kb0 + 31 > qw0) || kb0 + 32 > S) {
+            if ((kCausal && kb0 + 31 > qw0 + last0) || kb0 + 32 > n_k) {
                 const int base = kb0 + 4 * hi;
-                const int lim_q = kCausal ? my_q - base : INT_MAX;
-                const int lim_s = S - base;
+                const int lim_q = kCausal ? my_q + last0 - base : INT_MAX;
+                const int lim_s = n_k - base;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int c = 8 * (r >> 2) + (r & 3);
@@ -638,10 +702,14 @@ attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
             const float mc = m == -INFINITY ? 0.f : m * c2;
             half8_t p[2];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) p[r >> 3][r & 7] = (half_t)fast_exp2(fmaf(sh[r], c2, -mc));
+            for (int r = 0; r < 16; ++r) {
+                const float e = fast_exp2(fmaf(sh[r], c2, -mc));
+                if constexpr (kAny) l += e;
+                p[r >> 3][r & 7] = (half_t)e;
+            }
             const half2_t one2 = {(half_t)1.f, (half_t)1.f};
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < (kAny ? 0 : 2); ++i)
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
                     l = __builtin_amdgcn_fdot2(half2_t{p[i][2 * u], p[i][2 * u + 1]}, one2, l, false);
@@ -663,7 +731,7 @@ attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
                 if (i + kPreV < kSteps)
                     vbuf[i + kPreV] = read_v(2 * kb + (i + kPreV) / C::kDBlocks, (i + kPreV) % C::kDBlocks);
                 if (kb == 0 && i == C::kDBlocks && more) {
-                    copy_tile<D, 1, kW, kRows>(off, wave, Kh, Vh, (t + 1) * kRows, S, nbuf);
+                    copy(kSecond, (t + 1) * kRows, nbuf);
                     copied = true;
                 }
                 o[db] = mfma32(vbuf[i], p[ks], o[db]);
@@ -671,7 +739,7 @@ attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
             }
             __builtin_amdgcn_s_setprio(0);
         }
-        if (more && !copied) copy_tile<D, 1, kW, kRows>(off, wave, Kh, Vh, (t + 1) * kRows, S, nbuf);
+        if (more && !copied) copy(kSecond, (t + 1) * kRows, nbuf);
         dma_wait_barrier();
     }
 
@@ -719,12 +787,19 @@ attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
                 }
         }
     }
-    store_o<D>(o, l, O + head, gate ? gate + head : nullptr, my_q, S, hi);
+    if constexpr (kAny) {
+        const int b = bh / Hq, h = bh % Hq;
+        if (hi == 0 && my_q < n_q) rows.lse[(size_t)bh * S + my_q] = row_lse(m, l, c2);
+        store_o<D>(o, l, O + b * rows.o.b + h * rows.o.h, gate ? gate + b * rows.gate.b + h * rows.gate.h : nullptr, my_q, n_q, hi,
+                   o_t, g_t);
+    } else {
+        store_o<D>(o, l, O + head, gate ? gate + head : nullptr, my_q, S, hi);
+    }
 }
 
-template <int D, bool kCausal>
+template <int D, bool kCausal, class Rows>
 hipError_t launch(const half_t* q, const half_t* k, const half_t* v, const half_t* gate, half_t* o,
-                  int B, int Hq, int Hkv, int S, float scale, hipStream_t stream) {
+                  int B, int Hq, int Hkv, int S, float scale, const Rows& view, hipStream_t stream) {
     constexpr int kW = D == 256 ? 8 : 4;
     const int BH = B * Hq;
     // The split-key forms where whole query tiles leave the device idle or end in a long tail.  The
@@ -734,7 +809,7 @@ hipError_t launch(const half_t* q, const half_t* k, const half_t* v, const half_
     auto split = [&](auto kernel, int rows, int waves) {
         const int n = (S + rows - 1) / rows;
         hipLaunchKernelGGL(kernel, dim3(BH * n), dim3(64 * waves), 0, stream, q, k, v, gate, o, S, BH, n, Hq,
-                           Hq / Hkv, scale * kLog2e);
+                           Hq / Hkv, scale * kLog2e, view);
         return hipGetLastError();
     };
     auto tiles = [&](int rows) { return (long long)BH * ((S + rows - 1) / rows); };
@@ -749,7 +824,7 @@ hipError_t launch(const half_t* q, const half_t* k, const half_t* v, const half_
         const long long whole = tiles(256), half = tiles(128);
         const bool fits = half <= 256 || (kCausal && whole <= (S > 768 ? 192 : S > 448 ? 160 : 0));
         if (S > 128 && whole <= 192 && fits)
-            return split(attn_ksplit_kernel<D, kCausal, 4, 2, 32>, 128, 8);
+            return split(attn_ksplit_kernel<D, kCausal, 4, 2, 32, Rows>, 128, 8);
         // Somewhat more tiles than CUs leave a second round nearly empty: half tiles, two workgroups
         // per CU, 32-key steps and no split there (the same keys in the same order, so the same
         // values).  Causal 216 tiles 119 / 106, 264 137 / 126, 288 157.4 / 159.2; no mask 264 289 / 180,
@@ -759,7 +834,7 @@ hipError_t launch(const half_t* q, const half_t* k, const half_t* v, const half_
         // 255 tiles 59.3 / 65.8; 2048, 256 133.6 / 135.6; 2300, 216 142 / 146).
         const bool ragged = half < 2 * whole && S <= 2048;
         if (whole > 192 && whole <= (kCausal ? 272 : 320) && (kCausal || whole > 256 || S <= 512 || ragged))
-            return split(attn_ksplit_kernel<D, kCausal, 4, 1, 32>, 128, 4);
+            return split(attn_ksplit_kernel<D, kCausal, 4, 1, 32, Rows>, 128, 4);
     } else if (S > 64) {  // (one key tile has nothing to split: 128 heads of S = 64 4.2 / 5.2, D = 128 5.4 / 8.2)
         // 32 rows by four key groups in its first round (D = 128: first workgroup per CU) at lengths
         // that pay the merge: D = 64, causal, 512 tiles of S = 256 7.9 / 6.6 against 6.2 of the next
@@ -767,7 +842,7 @@ hipError_t launch(const half_t* q, const half_t* k, const half_t* v, const half_
         // against 8.6, 512 14.6 / 11.8, 1024 23.0 / 16.9.
         const long long t32 = tiles(32), t64 = tiles(64);
         if (D == 64 ? S >= 192 && t32 <= (S >= 384 ? 512 : 256) : S >= 512 && t32 <= 256)
-            return split(attn_ksplit_kernel<D, kCausal, 1, 4, 32>, 32, 4);
+            return split(attn_ksplit_kernel<D, kCausal, 1, 4, 32, Rows>, 32, 4);
         // 64 rows by two key groups.  Under a mask its first round of 512, and past it the more the
         // longer the tail of whole tiles is: D = 64 512 tiles of S = 256 8.1 / 7.2, 640 8.7 / 10.6, 768 of
         // S = 512 12.1 / 13.7, of S = 1024 18.6 / 17.8, 1024 of S = 1024 20.1 / 20.8, of S = 2048 33.8 / 32.2,
@@ -779,12 +854,25 @@ hipError_t launch(const half_t* q, const half_t* k, const half_t* v, const half_
         const int lim = kCausal   ? min(D == 64 ? 1024 : 896, 512 + max(0, S - 512) / 2)
                         : D == 64 ? (S >= 512 ? 512 : 256)
                                   : (S >= 768 ? 384 : 256);
-        if (t64 <= lim) return split(attn_ksplit_kernel<D, kCausal, 2, 2, D == 64 ? 64 : 32>, 64, 4);
+        if (t64 <= lim) return split(attn_ksplit_kernel<D, kCausal, 2, 2, D == 64 ? 64 : 32, Rows>, 64, 4);
     }
     const int n_qt = (S + 32 * kW - 1) / (32 * kW);
-    hipLaunchKernelGGL((attn_fwd_kernel<D, kCausal, kW>), dim3(BH * n_qt), dim3(64 * kW), 0,
-                       stream, q, k, v, gate, o, S, BH, n_qt, Hq, Hq / Hkv, scale * kLog2e);
+    hipLaunchKernelGGL((attn_fwd_kernel<D, kCausal, kW, Rows>), dim3(BH * n_qt), dim3(64 * kW), 0,
+                       stream, q, k, v, gate, o, S, BH, n_qt, Hq, Hq / Hkv, scale * kLog2e, view);
     return hipGetLastError();
+}
+
+template <class Rows>
+hipError_t launch_any(const half_t* q, const half_t* k, const half_t* v, const half_t* gate, half_t* o, int B, int Hq,
+                      int Hkv, int S, int D, float scale, int causal, const Rows& view, hipStream_t stream) {
+    if (D == 256)
+        return causal ? launch<256, true>(q, k, v, gate, o, B, Hq, Hkv, S, scale, view, stream)
+                      : launch<256, false>(q, k, v, gate, o, B, Hq, Hkv, S, scale, view, stream);
+    if (D == 128)
+        return causal ? launch<128, true>(q, k, v, gate, o, B, Hq, Hkv, S, scale, view, stream)
+                      : launch<128, false>(q, k, v, gate, o, B, Hq, Hkv, S, scale, view, stream);
+    return causal ? launch<64, true>(q, k, v, gate, o, B, Hq, Hkv, S, scale, view, stream)
+                  : launch<64, false>(q, k, v, gate, o, B, Hq, Hkv, S, scale, view, stream);
 }
 
 // ---------------------------------------------------------------------------------
@@ -847,14 +935,14 @@ hipError_t attn_fwd(const void* q, const void* k, const void* v, const void* gat
     auto Vp = static_cast<const half_t*>(v);
     auto G = static_cast<const half_t*>(gate);
     auto Op = static_cast<half_t*>(o);
-    if (D == 256)
-        return causal ? launch<256, true>(Q, K, Vp, G, Op, B, Hq, Hkv, S, scale, stream)
-                      : launch<256, false>(Q, K, Vp, G, Op, B, Hq, Hkv, S, scale, stream);
-    if (D == 128)
-        return causal ? launch<128, true>(Q, K, Vp, G, Op, B, Hq, Hkv, S, scale, stream)
-                      : launch<128, false>(Q, K, Vp, G, Op, B, Hq, Hkv, S, scale, stream);
-    return causal ? launch<64, true>(Q, K, Vp, G, Op, B, Hq, Hkv, S, scale, stream)
-                  : launch<64, false>(Q, K, Vp, G, Op, B, Hq, Hkv, S, scale, stream);
+    return launch_any(Q, K, Vp, G, Op, B, Hq, Hkv, S, D, scale, causal, Dense{}, stream);
+}
+
+hipError_t attn_train_fwd(const Rows16& q, const Rows16& k, const Rows16& v, const Rows16& gate, const Rows16& o, float* lse,
+                          const int* len_q, const int* len_k, int B, int Hq, int Hkv, int Tq, int Tk, int D, float scale,
+                          int causal, hipStream_t stream) {
+    const AttnRows view = {q, k, v, gate, o, lse, len_q, len_k, Tk};
+    return launch_any(q.data, k.data, v.data, gate.data, o.data, B, Hq, Hkv, Tq, D, scale, causal, view, stream);
 }
 
 hipError_t attn_naive(const void* q, const void* k, const void* v, const void* gate, void* o,
@@ -882,6 +970,8 @@ hipError_t attn_naive(const void* q, const void* k, const void* v, const void* g
 
 }  // namespace tsa
 
+// The backward pass of the training form.
+#include "attn_bwd.h"
 // Attention over the 8-bit K/V cache: every block, and blocks that a cheap score selects.
 #include "kv8_attn.h"
 #include "kv8_select.h"

@@ -2,6 +2,7 @@
 //
 // Validation happens here, before any HIP call, so argument errors are reported the same
 // way on machines without a GPU.  The launch functions in kernels.h assume valid input.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -65,7 +66,7 @@ extern "C" const char* tsa_strerror(int code) {
         case TSA_ERR_UNSUPPORTED: return "shape not supported by this library (attention: D in {64,128,256}; GDN: dk = dv = 128, chunk = 64)";
         case TSA_ERR_WORKSPACE: return "workspace is NULL or smaller than the required size";
         case TSA_ERR_LAUNCH: return "the HIP runtime rejected a kernel launch";
-        case TSA_ERR_ARG: return "invalid argument (causal not 0/1, scale not finite / not > 0, eps not finite / not > 0, 8-bit cache: a misaligned buffer, or top < first + recent + 1)";
+        case TSA_ERR_ARG: return "invalid argument (causal not 0/1, scale not finite / not > 0, eps not finite / not > 0, rows or 8-bit cache: a misaligned buffer or stride, top < first + recent + 1, rotary positions: a parameter out of its range)";
         case TSA_ERR_SCRATCH: return "the shapes need more than the 64 MiB device scratch of tsa_gdn_chunked_fwd_noalloc (use tsa_gdn_chunked_fwd with a workspace)";
         default: return "unknown tsa error code";
     }
@@ -472,4 +473,149 @@ extern "C" int tsa_attn_kv8_blocks_fwd(const tsa_kv8* cache, const tsa_rows* q, 
     if ((rc = check_ws(ws, ws_bytes, need))) return rc;
     return from_hip(tsa::kv8_attn_blocks(as_kv8(cache), as_rows(q, B, Hq, T), as_rows(gate, B, Hq, T), as_rows(o, B, Hq, T),
                                          len, n_new, T, Hq, blocks, top, scale, ws, as_stream(stream)));
+}
+
+// ---- rotary positions ----
+extern "C" int tsa_rope_freqs(const tsa_rope_params* p, uint64_t* freq, float* amp) {
+    if (!p || !freq || !amp) return TSA_ERR_NULL;
+    if (p->rot < 2 || p->rot % 2 != 0) return TSA_ERR_SHAPE;
+    if (!(p->base > 1.0) || !std::isfinite(p->base)) return TSA_ERR_ARG;
+    const int kind = p->scaling;
+    if (kind < TSA_ROPE_PLAIN || kind > TSA_ROPE_WAVELENGTH) return TSA_ERR_ARG;
+    if (kind != TSA_ROPE_PLAIN && (!(p->factor >= 1.0) || !std::isfinite(p->factor))) return TSA_ERR_ARG;
+    if (kind == TSA_ROPE_NTK && p->rot < 4) return TSA_ERR_ARG;
+    if ((kind == TSA_ROPE_YARN || kind == TSA_ROPE_WAVELENGTH) && p->orig_len < 1) return TSA_ERR_ARG;
+    if (kind == TSA_ROPE_YARN && !(p->beta_slow > 0.0 && p->beta_fast > p->beta_slow && std::isfinite(p->beta_fast))) return TSA_ERR_ARG;
+    if (kind == TSA_ROPE_WAVELENGTH && !(p->low > 0.0 && p->high > p->low && std::isfinite(p->high))) return TSA_ERR_ARG;
+    // in the host's widest floats (64 bits of mantissa): the result has as many
+    const long double pi = 3.14159265358979323846264338327950288L;
+    const long double R = p->rot, s = p->factor, n = p->orig_len;
+    const long double base = kind == TSA_ROPE_NTK ? p->base * std::pow(s, R / (R - 2)) : (long double)p->base;
+    long double lo = 0, hi = 0;
+    if (kind == TSA_ROPE_YARN) {
+        auto pair_that_turns = [&](long double times) { return R * std::log(n / (times * 2 * pi)) / (2 * std::log(base)); };
+        lo = std::max(std::floor(pair_that_turns(p->beta_fast)), 0.0L);
+        hi = std::min(std::ceil(pair_that_turns(p->beta_slow)), R - 1);
+    }
+    for (int i = 0; i < p->rot / 2; ++i) {
+        long double f = std::pow(base, -2.0L * i / R);
+        if (kind == TSA_ROPE_LINEAR) f /= s;
+        if (kind == TSA_ROPE_YARN) {
+            const long double ramp = std::min(std::max((i - lo) / std::max(hi - lo, 0.001L), 0.0L), 1.0L);
+            f = f * (1 - ramp) + f / s * ramp;
+        }
+        if (kind == TSA_ROPE_WAVELENGTH) {
+            const long double turns = n * f / (2 * pi);
+            const long double keep = std::min(std::max((turns - p->low) / ((long double)p->high - p->low), 0.0L), 1.0L);
+            f = f * keep + f / s * (1 - keep);
+        }
+        freq[i] = (uint64_t)std::floor(f / (2 * pi) * 18446744073709551616.0L + 0.5L);  // f <= 1 radian: below 2^62
+    }
+    *amp = kind == TSA_ROPE_YARN ? (float)(0.1L * std::log(s) + 1) : 1.f;
+    return TSA_OK;
+}
+
+namespace {
+
+tsa::RopeRows as_rope(const tsa_rows* r, int B, int H, int T) {
+    const tsa::Rows16 x = as_rows(r, B, H, T);
+    return {x.data, x.b, x.h, x.t};
+}
+
+// An input and its output: apart, or the same rows.
+int check_rope(const tsa_rows* x, const tsa_rows* y, int B, int H, int T) {
+    int rc = check_rows(x, B, H, T, false);
+    if (rc || (rc = check_rows(y, B, H, T, true))) return rc;
+    if (x->data != y->data) return TSA_OK;
+    const tsa::RopeRows a = as_rope(x, B, H, T), b = as_rope(y, B, H, T);
+    return a.b == b.b && a.h == b.h && a.t == b.t ? TSA_OK : TSA_ERR_ARG;
+}
+
+}  // namespace
+
+extern "C" int tsa_rope(const tsa_rope_plan* plan, int type, const tsa_rows* q, const tsa_rows* q_out, int Hq, const tsa_rows* k,
+                        const tsa_rows* k_out, int Hk, const int32_t* pos, const int32_t* len, const int32_t* n_new, int B, int T,
+                        int D, int back, void* stream) {
+    if (!plan || !plan->freq) return TSA_ERR_NULL;
+    if (B < 1 || T < 1 || Hq < 1 || Hk < 0 || D < 1) return TSA_ERR_SHAPE;
+    if (D != 64 && D != 128 && D != 256) return TSA_ERR_UNSUPPORTED;
+    if (plan->rot < 2 || plan->rot % 2 != 0 || plan->rot > D) return TSA_ERR_SHAPE;
+    if (plan->interleaved != 0 && plan->interleaved != 1) return TSA_ERR_ARG;
+    if (!std::isfinite(plan->amp) || (type != TSA_TYPE_F16 && type != TSA_TYPE_F32) || (back != 0 && back != 1)) return TSA_ERR_ARG;
+    // threads of a head group, and groups of heads
+    if (!fits_int(B, T, D) || (long long)Hq + Hk > 65535) return TSA_ERR_SHAPE;
+    int rc = check_rope(q, q_out, B, Hq, T);
+    if (rc) return rc;
+    if (Hk > 0 && (rc = check_rope(k, k_out, B, Hk, T))) return rc;
+    const tsa::RopeRows none = {nullptr, 0, 0, 0};
+    static_assert(sizeof(unsigned long long) == sizeof(uint64_t), "the table's type");
+    return from_hip(tsa::rope(reinterpret_cast<const unsigned long long*>(plan->freq), plan->amp, plan->rot, plan->interleaved,
+                              type == TSA_TYPE_F32, as_rope(q, B, Hq, T), as_rope(q_out, B, Hq, T), Hq,
+                              Hk ? as_rope(k, B, Hk, T) : none, Hk ? as_rope(k_out, B, Hk, T) : none, Hk, pos, len, n_new, B, T, D,
+                              back, as_stream(stream)));
+}
+
+// ---- attention's training pair ----
+namespace {
+
+int check_train_sizes(int B, int Hq, int Hkv, int Tq, int Tk, int D) {
+    if (B < 1 || Hq < 1 || Hkv < 1 || Tq < 1 || Tk < 1 || D < 1 || Hq % Hkv != 0) return TSA_ERR_SHAPE;
+    if (D != 64 && D != 128 && D != 256) return TSA_ERR_UNSUPPORTED;
+    // rows of all heads, and positions, in ints
+    return fits_int(B, Hq, Tq) && fits_int(B, Hkv, Tk) && (long long)Tq + Tk <= INT_MAX - 1024 ? TSA_OK : TSA_ERR_SHAPE;
+}
+
+// Rows whose tiles are copied: offsets within a tile of 64 rows fit 32 bits.
+int check_tile_rows(const tsa_rows* r, int B, int H, int T, bool out) {
+    const int rc = check_rows(r, B, H, T, out);
+    if (rc) return rc;
+    return T > 1 && r->stride_t > 1 << 24 ? TSA_ERR_SHAPE : TSA_OK;
+}
+
+int check_train(const tsa_rows* q, const tsa_rows* k, const tsa_rows* v, const tsa_rows* gate, const tsa_rows* o, const float* lse,
+                int B, int Hq, int Hkv, int Tq, int Tk, int D, float scale, int causal, bool fwd) {
+    int rc = check_train_sizes(B, Hq, Hkv, Tq, Tk, D);
+    if (rc) return rc;
+    if (!lse) return TSA_ERR_NULL;
+    if ((rc = check_tile_rows(q, B, Hq, Tq, false)) || (rc = check_tile_rows(k, B, Hkv, Tk, false)) ||
+        (rc = check_tile_rows(v, B, Hkv, Tk, false)) || (rc = check_tile_rows(o, B, Hq, Tq, fwd)))
+        return rc;
+    if (gate && (rc = check_tile_rows(gate, B, Hq, Tq, false))) return rc;
+    if ((causal != 0 && causal != 1) || !(scale > 0.f) || !std::isfinite(scale)) return TSA_ERR_ARG;
+    return TSA_OK;
+}
+
+}  // namespace
+
+extern "C" int tsa_attn_train_fwd(const tsa_rows* q, const tsa_rows* k, const tsa_rows* v, const tsa_rows* gate, const tsa_rows* o,
+                                  float* lse, const int32_t* len_q, const int32_t* len_k, int B, int Hq, int Hkv, int Tq, int Tk,
+                                  int D, float scale, int causal, void* stream) {
+    const int rc = check_train(q, k, v, gate, o, lse, B, Hq, Hkv, Tq, Tk, D, scale, causal, true);
+    if (rc) return rc;
+    return from_hip(tsa::attn_train_fwd(as_rows(q, B, Hq, Tq), as_rows(k, B, Hkv, Tk), as_rows(v, B, Hkv, Tk), as_rows(gate, B, Hq, Tq),
+                                        as_rows(o, B, Hq, Tq), lse, len_q, len_k, B, Hq, Hkv, Tq, Tk, D, scale, causal,
+                                        as_stream(stream)));
+}
+
+extern "C" size_t tsa_attn_bwd_workspace_bytes(int B, int Hq, int Hkv, int Tq, int Tk, int D, int gated, int causal) {
+    if (check_train_sizes(B, Hq, Hkv, Tq, Tk, D) || (gated != 0 && gated != 1) || (causal != 0 && causal != 1)) return 0;
+    return tsa::attn_bwd_ws_bytes(B, Hq, Hkv, Tq, Tk, D, gated != 0, causal != 0);
+}
+
+extern "C" int tsa_attn_bwd(const tsa_rows* d_out, const tsa_rows* q, const tsa_rows* k, const tsa_rows* v, const tsa_rows* gate,
+                            const tsa_rows* o, const float* lse, const tsa_rows* dq, const tsa_rows* dk, const tsa_rows* dv,
+                            const tsa_rows* dgate, const int32_t* len_q, const int32_t* len_k, int B, int Hq, int Hkv, int Tq,
+                            int Tk, int D, float scale, int causal, void* ws, size_t ws_bytes, void* stream) {
+    int rc = check_train(q, k, v, gate, o, lse, B, Hq, Hkv, Tq, Tk, D, scale, causal, false);
+    if (rc) return rc;
+    if ((rc = check_tile_rows(d_out, B, Hq, Tq, false)) || (rc = check_tile_rows(dq, B, Hq, Tq, true)) ||
+        (rc = check_tile_rows(dk, B, Hkv, Tk, true)) || (rc = check_tile_rows(dv, B, Hkv, Tk, true)))
+        return rc;
+    if (gate && (rc = check_tile_rows(dgate, B, Hq, Tq, true))) return rc;
+    if ((rc = check_ws(ws, ws_bytes, tsa::attn_bwd_ws_bytes(B, Hq, Hkv, Tq, Tk, D, gate != nullptr, causal != 0)))) return rc;
+    const tsa::AttnRows x = {as_rows(q, B, Hq, Tq), as_rows(k, B, Hkv, Tk), as_rows(v, B, Hkv, Tk), as_rows(gate, B, Hq, Tq),
+                             as_rows(o, B, Hq, Tq), const_cast<float*>(lse), len_q, len_k, Tk};
+    return from_hip(tsa::attn_bwd(x, as_rows(d_out, B, Hq, Tq), as_rows(dq, B, Hq, Tq), as_rows(dk, B, Hkv, Tk), as_rows(dv, B, Hkv, Tk),
+                                  gate ? as_rows(dgate, B, Hq, Tq) : tsa::Rows16{nullptr, 0, 0, 0}, B, Hq, Hkv, Tq, D, scale, causal,
+                                  ws, as_stream(stream)));
 }

@@ -16,6 +16,39 @@ hipError_t attn_naive(const void* q, const void* k, const void* v, const void* g
 hipError_t attn_valu(const void* q, const void* k, const void* v, void* o, int B, int H, int S,
                      int D, float scale, int causal, hipStream_t stream);
 
+// fp16 rows of D elements that lie anywhere (tsa_rows of include/tsa.h): element strides between
+// sequences, heads and tokens.
+struct Rows16 {
+    _Float16* data;
+    long long b, h, t;
+};
+
+// The training pair.  len_q, len_k: device arrays [B] (null: Tq, Tk each); queries are the last of
+// the keys (query t sees keys up to t + len_k - len_q under the causal mask).  lse: [B][Hq][Tq].
+struct AttnRows {
+    Rows16 q, k, v, gate, o;
+    float* lse;
+    const int *len_q, *len_k;
+    int Sk;
+};
+hipError_t attn_train_fwd(const Rows16& q, const Rows16& k, const Rows16& v, const Rows16& gate, const Rows16& o, float* lse,
+                          const int* len_q, const int* len_k, int B, int Hq, int Hkv, int Tq, int Tk, int D, float scale,
+                          int causal, hipStream_t stream);
+
+// x: the forward's tensors; o and gate are read.  ws: attn_bwd_ws_bytes bytes.
+size_t attn_bwd_ws_bytes(int B, int Hq, int Hkv, int Tq, int Tk, int D, bool gated, bool causal);
+hipError_t attn_bwd(const AttnRows& x, const Rows16& d_out, const Rows16& dq, const Rows16& dk, const Rows16& dv, const Rows16& dgate,
+                    int B, int Hq, int Hkv, int Tq, int D, float scale, int causal, void* ws, hipStream_t stream);
+
+// Rotary positions (tsa_rope): rows of fp16 or fp32; k may have 0 heads; back: the gradient.
+struct RopeRows {
+    void* data;
+    long long b, h, t;
+};
+hipError_t rope(const unsigned long long* freq, float amp, int rot, int interleaved, int f32, const RopeRows& q,
+                const RopeRows& q_out, int Hq, const RopeRows& k, const RopeRows& k_out, int Hk, const int* pos,
+                const int* len, const int* n_new, int B, int T, int D, int back, hipStream_t stream);
+
 // Raw inputs of the fused pre-ops (the target model's layer): a, b [B][T][Hv]; dt_bias, A
 // [Hv] (A = -exp(A_log)); eps of the q / k l2 norms.  g_log = softplus(a + dt_bias) * A,
 // beta = sigmoid(b), q and k normalised per head row.
@@ -99,8 +132,7 @@ hipError_t gdn_naive(const void* q, const void* k, const void* v, const float* g
                      const float* beta, float* state, void* out, int B, int T, int Hq, int Hv,
                      int dk, int dv, float scale, bool f32, hipStream_t stream);
 
-// The 8-bit K/V cache (tsa_kv8 of include/tsa.h, with typed pointers) and fp16 rows of D
-// elements that lie anywhere (tsa_rows).  len, n_new: device arrays [B]; n_new may be null.
+// The 8-bit K/V cache (tsa_kv8 of include/tsa.h, with typed pointers).  len, n_new: device arrays [B]; n_new may be null.
 struct Kv8 {
     unsigned char *k, *v;
     float *k_scale, *v_scale;
@@ -109,10 +141,6 @@ struct Kv8 {
     _Float16 *k_open, *v_open;
     const int* table;
     int B, Hkv, D, n_pages, max_blocks;
-};
-struct Rows16 {
-    _Float16* data;
-    long long b, h, t;
 };
 hipError_t kv8_write(const Kv8& c, const Rows16& k, const Rows16& v, const int* len, const int* n_new, int T,
                      hipStream_t stream);

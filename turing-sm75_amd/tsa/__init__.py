@@ -56,6 +56,17 @@ class TsaRows(ctypes.Structure):
                 ("stride_t", ctypes.c_int64)]
 
 
+class TsaRopeParams(ctypes.Structure):
+    """The tsa_rope_params of include/tsa.h."""
+    _fields_ = [(n, ctypes.c_double) for n in ("base", "factor", "beta_fast", "beta_slow", "low", "high")] + \
+               [(n, ctypes.c_int) for n in ("rot", "scaling", "orig_len")]
+
+
+class TsaRopePlan(ctypes.Structure):
+    """The tsa_rope_plan of include/tsa.h."""
+    _fields_ = [("freq", ctypes.c_void_p), ("amp", ctypes.c_float), ("rot", ctypes.c_int), ("interleaved", ctypes.c_int)]
+
+
 _tp = ctypes.POINTER(TsaTensor)
 
 
@@ -93,6 +104,11 @@ _SIGNATURES = {
     "tsa_kv8_workspace_bytes": (_sz, [_vp] + [_i] * 4),
     "tsa_attn_kv8_fwd": (_i, [_vp] * 6 + [_i] * 3 + [_f, _i, _vp, _sz, _vp]),
     "tsa_kv8_select": (_i, [_vp] * 4 + [_i] * 5 + [_vp, _i, _vp, _sz, _vp]),
+    "tsa_rope_freqs": (_i, [_vp] * 3),
+    "tsa_rope": (_i, [_vp, _i, _vp, _vp, _i, _vp, _vp, _i] + [_vp] * 3 + [_i] * 4 + [_vp]),
+    "tsa_attn_train_fwd": (_i, [_vp] * 8 + [_i] * 6 + [_f, _i, _vp]),
+    "tsa_attn_bwd_workspace_bytes": (_sz, [_i] * 8),
+    "tsa_attn_bwd": (_i, [_vp] * 13 + [_i] * 6 + [_f, _i, _vp, _sz, _vp]),
     "tsa_attn_kv8_blocks_fwd": (_i, [_vp] * 6 + [_i] * 2 + [_vp, _i, _f, _vp, _sz, _vp]),
 }
 
@@ -726,3 +742,211 @@ def attn_kv8_blocks_fwd(q, cache, len, blocks, n_new=None, gate=None, out=None, 
               None if n_new is None else _counts(n_new, "n_new", cache), T, Hq, _blocks(blocks, cache, T, top), top,
               1.0 / math.sqrt(cache.D) if scale is None else float(scale), wp, wn)
     return out
+
+
+# ---------------------------------------------------------------------------------------
+# rotary positions, and attention's training pair
+# ---------------------------------------------------------------------------------------
+ROPE_SCALINGS = (None, "linear", "ntk", "yarn", "wavelength")
+
+
+class Rope:
+    """Rotary positions of heads of D elements (include/tsa.h, tsa_rope): pairs of the first `rot`
+    elements (default all) turn by position * base^(-2 i / rot), scaled by one of ROPE_SCALINGS.
+    interleaved: pairs (2 i, 2 i + 1), otherwise (i, i + rot / 2).  Holds the table of frequencies on
+    `device`."""
+
+    def __init__(self, D, rot=None, base=10000.0, interleaved=False, scaling=None, factor=1.0, orig_len=0, beta_fast=32.0,
+                 beta_slow=1.0, low=1.0, high=4.0, amp=None, device="cuda"):
+        torch = _torch or _t()
+        rot = D if rot is None else rot
+        if D not in (64, 128, 256):
+            raise ValueError(f"D must be 64, 128 or 256, got {D}")
+        if rot < 2 or rot % 2 or rot > D:
+            raise ValueError(f"rot must be even, 2 .. {D}, got {rot}")
+        if scaling not in ROPE_SCALINGS:
+            raise ValueError(f"scaling must be one of {ROPE_SCALINGS}, got {scaling!r}")
+        if not 0 <= orig_len < 1 << 31:
+            raise ValueError(f"orig_len is no 32-bit count: {orig_len}")
+        params = TsaRopeParams(base, factor, beta_fast, beta_slow, low, high, rot, ROPE_SCALINGS.index(scaling), orig_len)
+        table, found = (ctypes.c_uint64 * (rot // 2))(), ctypes.c_float()
+        _check(load().tsa_rope_freqs(ctypes.addressof(params), ctypes.addressof(table), ctypes.addressof(found)))
+        self.D, self.rot, self.interleaved = D, rot, bool(interleaved)
+        self.amp = found.value if amp is None else float(amp)
+        self.turns = [f * 2.0 ** -64 for f in table]
+        # torch has few operations on uint64: the same bits as int64
+        self.freq = torch.tensor([f - (1 << 64) if f >> 63 else f for f in table], dtype=torch.int64).to(device)
+        if self.freq.device.type != "cuda":
+            raise ValueError(f"a table of frequencies lies on a GPU, not on {device}")
+        self.index = self.freq.get_device()
+        self.view = TsaRopePlan(_ptr(self.freq), self.amp, rot, int(self.interleaved))
+        self._ref = ctypes.byref(self.view)
+
+
+def _rows_on(t, shape, name, index, dtype):
+    """A [B, H, T, D] tensor on GPU `index` as a tsa_rows: rows of consecutive elements, any other strides."""
+    torch = _torch or _t()
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype is dtype and t.is_cuda and t.get_device() == index and t.shape == shape:
+        b, h, r, d = t.stride()
+        if d == 1:
+            return _ROWS.pack(t.data_ptr(), b, h, r)
+    raise ValueError(f"{name}: expected {dtype} {tuple(shape)} on GPU {index} with consecutive row elements, got "
+                     f"{tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}")
+
+
+def _ints_on(t, shape, name, index):
+    """A contiguous int32 tensor on GPU `index`, or None."""
+    if t is None:
+        return None
+    torch = _torch or _t()
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype is not torch.int32 or not t.is_cuda or t.get_device() != index or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous int32 tensor of {tuple(shape)} on GPU {index}, got {tuple(t.shape)} "
+                         f"{t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
+def _call_on(fn, index, stream, *args):
+    """The entry point on GPU `index`, made the current one for the call where it is another."""
+    torch = _torch or _t()
+    if torch._C._cuda_getDevice() == index:
+        _check(fn(*args, torch._C._cuda_getCurrentRawStream(index) if stream is None else stream.cuda_stream))
+    else:
+        with torch.cuda.device(index):
+            _check(fn(*args, _stream(stream)))
+
+
+def _new_like(x, padded, stream):
+    """An output shaped and laid out like x, 0 where padding is left as it was, made on the stream that writes it."""
+    torch = _torch or _t()
+    make = torch.zeros_like if padded else torch.empty_like
+    fmt = torch.preserve_format
+    # an expanded input (stride 0) has no layout for an output
+    if any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
+        fmt = torch.contiguous_format
+    if stream is None and torch._C._cuda_getDevice() == x.get_device():
+        return make(x, memory_format=fmt)
+    with torch.cuda.stream(torch.cuda.current_stream(x.device) if stream is None else stream):
+        return make(x, memory_format=fmt)
+
+
+def _four(t, name):
+    if not isinstance(t, (_torch or _t()).Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dim() != 4 or not t.is_cuda:
+        raise ValueError(f"{name}: expected a 4-d tensor on a GPU, got {tuple(t.shape)} on {t.device}")
+    return t.shape
+
+
+def _rope(rope, q, k, pos, len, n_new, q_out, k_out, back, stream):
+    torch = _torch or _t()
+    B, Hq, T, D = _four(q, "q")
+    if q.dtype is not torch.float16 and q.dtype is not torch.float32:
+        raise ValueError(f"q: expected fp16 or fp32, got {q.dtype}")
+    if D != rope.D:
+        raise ValueError(f"q has heads of {D} elements, the rotation {rope.D}")
+    i, dtype = rope.index, q.dtype
+    q_in = _rows_on(q, q.shape, "q", i, dtype)
+    if k is None:
+        if k_out is not None:
+            raise ValueError("k_out without k")
+        Hk, k_in = 0, None
+    else:
+        Hk = _four(k, "k")[1]
+        k_in = _rows_on(k, (B, Hk, T, D), "k", i, dtype)
+    at = _ints_on(pos, (B, T), "pos", i), _ints_on(len, (B,), "len", i), _ints_on(n_new, (B,), "n_new", i)
+    q_out = _new_like(q, n_new is not None, stream) if q_out is None else q_out
+    if k is not None and k_out is None:
+        k_out = _new_like(k, n_new is not None, stream)
+    _call_on(load().tsa_rope, i, stream, rope._ref, TSA_TYPE_F32 if dtype is torch.float32 else TSA_TYPE_F16, q_in,
+             _rows_on(q_out, q.shape, "q_out", i, dtype), Hq, k_in, None if k is None else _rows_on(k_out, k.shape, "k_out", i, dtype),
+             Hk, *at, B, T, D, back)
+    return q_out, k_out
+
+
+def rope_fwd(rope, q, k=None, pos=None, len=None, n_new=None, q_out=None, k_out=None, stream=None):
+    """Rotates q [B, Hq, T, D] and k [B, Hk, T, D] (fp16 or fp32, rows of consecutive elements, any other
+    strides) and returns (q_out, k_out); q_out may be q, k_out may be k.  Row t is at pos[b, t] (int32
+    [B, T]), or at len[b] - n_new[b] + t (int32 [B]; the cache's len and n_new), or at t.  Rows behind
+    n_new (default T) are left as they were (0 in outputs made here)."""
+    return _rope(rope, q, k, pos, len, n_new, q_out, k_out, 0, stream)
+
+
+def rope_bwd(rope, dq, dk=None, pos=None, len=None, n_new=None, q_out=None, k_out=None, stream=None):
+    """The gradients of rope_fwd's q and k from those of its outputs, with the same positions."""
+    return _rope(rope, dq, dk, pos, len, n_new, q_out, k_out, 1, stream)
+
+
+def _train_shapes(q, k, v, gate, len_q, len_k):
+    torch = _torch or _t()
+    B, Hq, Tq, D = _four(q, "q")
+    _, Hkv, Tk, _ = _four(k, "k")
+    i, half = q.get_device(), torch.float16
+    views = (_rows_on(q, q.shape, "q", i, half), _rows_on(k, (B, Hkv, Tk, D), "k", i, half), _rows_on(v, (B, Hkv, Tk, D), "v", i, half),
+             None if gate is None else _rows_on(gate, q.shape, "gate", i, half))
+    return views, (_ints_on(len_q, (B,), "len_q", i), _ints_on(len_k, (B,), "len_k", i)), (B, Hq, Hkv, Tq, Tk, D)
+
+
+def _stat(lse, shape, name, index):
+    torch = _torch or _t()
+    if not isinstance(lse, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if lse.dtype is not torch.float32 or not lse.is_cuda or lse.get_device() != index or lse.shape != shape or not lse.is_contiguous():
+        raise ValueError(f"{name}: expected contiguous fp32 {tuple(shape)} on GPU {index}, got {tuple(lse.shape)} {lse.dtype} on {lse.device}")
+    return lse.data_ptr()
+
+
+def attn_train_fwd(q, k, v, gate=None, len_q=None, len_k=None, out=None, lse=None, scale=None, causal=True, stream=None):
+    """The forward pass that attn_bwd goes back from: returns (o, lse) for q, gate [B, Hq, Tq, D] and k, v
+    [B, Hkv, Tk, D] fp16 (rows of consecutive elements, any other strides), o = softmax(scale q K^T) V, times
+    sigmoid(gate) if given, lse [B, Hq, Tq] fp32 the logarithms of the softmax sums.  len_q, len_k (int32
+    [B], default Tq, Tk) count each sequence's rows; under the causal mask query t sees keys up to
+    t + len_k - len_q.  Rows of padding are left as they were (0 in outputs made here)."""
+    torch = _torch or _t()
+    views, lens, (B, Hq, Hkv, Tq, Tk, D) = _train_shapes(q, k, v, gate, len_q, len_k)
+    i = q.get_device()
+    if out is None:
+        out = _new_like(q, len_q is not None, stream)
+    op = _rows_on(out, q.shape, "out", i, torch.float16)
+    if lse is None:
+        with torch.cuda.stream(torch.cuda.current_stream(q.device) if stream is None else stream):
+            lse = torch.zeros(B, Hq, Tq, dtype=torch.float32, device=q.device)
+    _call_on(load().tsa_attn_train_fwd, i, stream, *views, op, _stat(lse, (B, Hq, Tq), "lse", i), *lens, B, Hq, Hkv, Tq, Tk, D,
+             1.0 / math.sqrt(D) if scale is None else float(scale), 1 if causal else 0)
+    return out, lse
+
+
+def attn_bwd_workspace_bytes(B, Hq, Hkv, Tq, Tk, D, gated=False, causal=True) -> int:
+    """Workspace bytes of one attn_bwd call."""
+    return int(load().tsa_attn_bwd_workspace_bytes(B, Hq, Hkv, Tq, Tk, D, 1 if gated else 0, 1 if causal else 0))
+
+
+def attn_bwd(d_out, q, k, v, out, lse, gate=None, len_q=None, len_k=None, dq=None, dk=None, dv=None, dgate=None, scale=None,
+             causal=True, ws=None, stream=None):
+    """The gradients (dq, dk, dv, dgate; dgate None without a gate) for the gradient d_out of attn_train_fwd's
+    o, from its o and lse and the arguments it had.  Shared key and value heads get the sum over their
+    query heads.  Rows of padding are left as they were (0 in outputs made here).  Outputs lie on no input."""
+    torch = _torch or _t()
+    views, lens, (B, Hq, Hkv, Tq, Tk, D) = _train_shapes(q, k, v, gate, len_q, len_k)
+    i, half = q.get_device(), torch.float16
+    if gate is None and dgate is not None:
+        raise ValueError("dgate without gate")
+    gp, op = _rows_on(d_out, q.shape, "d_out", i, half), _rows_on(out, q.shape, "out", i, half)
+    lp = _stat(lse, (B, Hq, Tq), "lse", i)
+    dq = _new_like(q, len_q is not None, stream) if dq is None else dq
+    dk = _new_like(k, len_k is not None, stream) if dk is None else dk
+    dv = _new_like(v, len_k is not None, stream) if dv is None else dv
+    if gate is not None and dgate is None:
+        dgate = _new_like(gate, len_q is not None, stream)
+    grads = (_rows_on(dq, q.shape, "dq", i, half), _rows_on(dk, k.shape, "dk", i, half), _rows_on(dv, v.shape, "dv", i, half),
+             None if gate is None else _rows_on(dgate, q.shape, "dgate", i, half))
+    if ws is None:
+        ws = _scratch(attn_bwd_workspace_bytes(B, Hq, Hkv, Tq, Tk, D, gate is not None, causal), q.device, stream)
+    elif not ws.is_cuda or ws.get_device() != i or not ws.is_contiguous():
+        raise ValueError(f"ws: expected a contiguous tensor on GPU {i}, got one on {ws.device}")
+    _call_on(load().tsa_attn_bwd, i, stream, gp, *views, op, lp, *grads, *lens, B, Hq, Hkv, Tq, Tk, D,
+             1.0 / math.sqrt(D) if scale is None else float(scale), 1 if causal else 0, _ptr(ws), ws.numel() * ws.element_size())
+    return dq, dk, dv, dgate
