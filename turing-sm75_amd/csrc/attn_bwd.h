@@ -16,6 +16,9 @@
 // |dS_ij| <= |dO_i| |v_j| + |d_i| over its rows and keys, so gradients of any size keep fp16's
 // full precision in dS down to 2^-28 of that bound.  It is folded into the exponential's argument and into the outputs' scale.
 #pragma once
+#include <algorithm>
+#include <cmath>
+
 #include "attn_tiles.h"
 #include "common.h"
 #include "kernels.h"
@@ -156,8 +159,18 @@ __global__ void __launch_bounds__(256) attn_bwd_rows_kernel(RowsArgs a) {
 // What the tiles share
 // ---------------------------------------------------------------------------------------
 __device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) x = fmaxf(x, __shfl_xor(x, s));
+    x = fmaxf(x, dpp_mov<kDppXor1>(x));
+    x = fmaxf(x, dpp_mov<kDppXor2>(x));
+    x = fmaxf(x, dpp_mov<kDppHalfMirror>(x));
+    x = fmaxf(x, dpp_mov<kDppRowMirror>(x));
+    return max_xor32(max_xor16(x));
+}
+// 2^-ref
+__device__ __forceinline__ float scale_back(float ref) { return __builtin_ldexpf(1.f, -(int)ref); }
+
+// A value that is made here, not at its first use.
+__device__ __forceinline__ float pinned(float x) {
+    asm volatile("" : "+v"(x));
     return x;
 }
 
@@ -175,36 +188,51 @@ __device__ __forceinline__ float range_ref(float bound) {
     return (float)min(15, 14 - e);
 }
 
-// One tensor's part of a step's copies: 32 rows of D elements, kW waves, blocks of 1 KiB.  A wave's
-// first block holds rows that its others repeat a multiple of 16 on, so the swizzle is the same and
-// one offset a lane serves all.
-template <int D, int kW>
+// Copies of tiles of 32 rows of D elements by kN waves, 1 KiB an instruction.  The swizzle of a
+// block's rows repeats every kPeriod blocks; a wave takes kPat neighbouring blocks and those a multiple of kPeriod
+// on, so one offset a lane and tensor serves all of them, with a difference in the odd ones.
+template <int D, int kN>
 struct Copy {
-    static constexpr int kInstr = kBlk * D * 2 / 1024;  // of a tile
-    static constexpr int kStep = kW * 1024 / (2 * D);   // rows from a wave's block to its next
-    static constexpr int kPer = (kInstr + kW - 1) / kW;
-    static_assert(kPer == 1 || kStep % 16 == 0, "a wave's blocks share one swizzle pattern");
-    static_assert(kInstr % kW == 0, "every wave copies");
-};
-// p: the tile's first row; stride in bytes (at most 2^25); last: the last row there is, counted from it.
-template <int D, int kW>
-__device__ __forceinline__ void copy_rows(const char* p, unsigned stride, int last, int lane, int wave, unsigned lds) {
-    using C = Copy<D, kW>;
-    // made again for each copy (held, they take registers that the products need)
-    unsigned l = (unsigned)lane;
-    asm volatile("" : "+v"(l));
-    const unsigned row = (512u / D) * (unsigned)wave + l / (D / 8);
-    const unsigned col = 16u * ((l % (D / 8)) ^ (unsigned)swz<D>((int)row));
-    if (last >= kBlk - 1) {
-        const unsigned off = row * stride + col;
+    static constexpr int kBlocks = kBlk * D * 2 / 1024, kRows = 512 / D;  // of a tile; rows a block
+    static constexpr int kPeriod = D == 64 ? 1 : 16 / kRows;
+    static constexpr int kPat = kPeriod > kN ? kPeriod / kN : 1;
+    static constexpr int kNext = kPeriod > kN ? kPeriod : kN;  // blocks from one of a wave's groups to its next
+    static constexpr int kPer = kBlocks / (kN * kPat);         // groups a wave
+    static constexpr unsigned kFlip = D == 128 ? 16 : 128;     // bytes by which a chunk moves from a block to the next, by XOR
+    static_assert(kPat <= 2 && kPer * kN * kPat == kBlocks && kNext * kRows % (D == 64 ? 8 : 16) == 0, "one offset serves all groups");
+    int w;  // which of the kN waves
+
+    __device__ __forceinline__ int row(int lane) const { return kRows * kPat * w + lane / (D / 8); }
+    __device__ __forceinline__ unsigned col(int lane) const { return 16u * (unsigned)((lane % (D / 8)) ^ swz<D>(row(lane))); }
+    // This lane's offset from a tile's first row; stride in bytes, at most 2^25.
+    __device__ __forceinline__ unsigned offset(int lane, unsigned stride) const { return (unsigned)row(lane) * stride + col(lane); }
+    // p: the tile's first row; last: the last row there is, counted from it.
+    __device__ __forceinline__ void operator()(const char* p, unsigned stride, unsigned off, int last, int lane, unsigned lds) const {
+        lds += 1024u * (unsigned)(kPat * w);
+        int l = lane;  // (what is made of it is not held from copy to copy)
+        asm volatile("" : "+v"(l));
+        if (last >= kBlk - 1) {
+            const unsigned delta = (col(l) ^ kFlip) - col(l);
 #pragma unroll
-        for (int j = 0; j < C::kPer; ++j) dma_issue_any(p + (size_t)stride * (C::kStep * j), off, lds + 1024u * (unsigned)(wave + kW * j));
-    } else {
+            for (int j = 0; j < kPer; ++j)
 #pragma unroll
-        for (int j = 0; j < C::kPer; ++j)
-            dma_issue_any(p, (unsigned)min((int)row + C::kStep * j, last) * stride + col, lds + 1024u * (unsigned)(wave + kW * j));
+                for (int i = 0; i < kPat; ++i) {
+                    const int blk = kNext * j + i;
+                    dma_issue_any(p + (size_t)stride * (unsigned)(kRows * blk), off + (i ? delta : 0), lds + 1024u * (unsigned)blk);
+                }
+        } else {  // rows past the last are that one again
+            const int r = row(l);
+            const unsigned c = col(l);
+#pragma unroll
+            for (int j = 0; j < kPer; ++j)
+#pragma unroll
+                for (int i = 0; i < kPat; ++i) {
+                    const int blk = kNext * j + i;
+                    dma_issue_any(p, (unsigned)min(r + kRows * blk, last) * stride + (i ? c ^ kFlip : c), lds + 1024u * (unsigned)blk);
+                }
+        }
     }
-}
+};
 
 // A operand of rows: A[row l % 32][16 kk + 8 (l / 32) + s] (addr: row l % 32's chunk l / 32).
 __device__ __forceinline__ half8_t rows_op(unsigned addr, int kk) { return lds_read_b128(addr ^ (32u * kk)); }
@@ -262,6 +290,39 @@ __device__ __forceinline__ void mul_cols(unsigned cols, unsigned tile, int db0, 
 #pragma unroll
                                  for (int r = 0; r < kRB; ++r) acc[r * kDB + (i >> 1)] = mfma32(x, op[r][i & 1], acc[r * kDB + (i >> 1)]);
                              });
+}
+
+// The same with other work, a share of it behind each operand's products: while the matrix pipe has
+// them, the wave goes on.  op(ks): the kRB operands of 16 rows; work(i): share i of 2 kDB.
+template <int D, int kRB, int kDB, class Op, class Work>
+__device__ __forceinline__ void mul_cols_beside(unsigned cols, unsigned tile, int db0, const Op& op, float16_t (&acc)[kRB * kDB], const Work& work) {
+    const unsigned base = (cols + tile) ^ (64u * db0);
+    constexpr int kPre = kRB == 2 ? 1 : kPreCols;
+    half8_t x[2 * kDB], y[2][kRB];
+    unsigned a = base;
+    asm volatile("" : "+v"(a));
+    op(0, y[0]);
+#pragma unroll
+    for (int i = 0; i < kPre; ++i) x[i] = cols_op<D>(a, i / kDB, i % kDB);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 2 * kDB; ++i) {
+        const int n = i + kPre;
+        if (n == kDB) {  // the second k-step's addresses are made again
+            a = base;
+            asm volatile("" : "+v"(a));
+        }
+        if (n < 2 * kDB) x[n] = cols_op<D>(a, n / kDB, n % kDB);
+        if (i == kDB - 1) op(1, y[1]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int r = 0; r < kRB; ++r) {
+            acc[r * kDB + i % kDB] = mfma32(x[i], y[i / kDB][r], acc[r * kDB + i % kDB]);
+            asm volatile("" : "+v"(acc[r * kDB + i % kDB]));
+        }
+        work(i);
+        __builtin_amdgcn_sched_barrier(0);
+    }
 }
 
 typedef float float8_t __attribute__((ext_vector_type(8)));
@@ -326,23 +387,31 @@ struct KvTile {
     static constexpr int kAcc = kKB * (D / 32);     // 32 x 32 results a wave
 };
 
-// Writes kRB blocks of 32 rows by 32 kDB elements (lane = row, 4 consecutive elements a register group) times f.
+// Writes kRB blocks of 32 rows by 32 kDB elements (lane = row, 4 consecutive elements a register group)
+// times f.  They go through LDS (the wave's own at `lds`, 64 kRB 32 kDB bytes; no wave reads tiles any more): from the
+// registers, an instruction's 64 lanes would write 16 bytes of each of 32 rows, and the address unit was
+// 3.5 us of a short call.
 template <int kRB, int kDB>
 __device__ __forceinline__ void store_rows(const float16_t (&acc)[kRB * kDB], half_t* out, long long stride, int row0, int n_rows,
-                                           int lane, float f) {
+                                           int lane, float f, unsigned lds) {
+    typedef __attribute__((address_space(3))) half4_t* p4_t;
+    constexpr int kC = 4 * kDB;  // 16-byte chunks a row, chunk c of row r at c ^ (r % kC)
+    const int r = lane & 31;
 #pragma unroll
-    for (int kb = 0; kb < kRB; ++kb) {
-        const int r = row0 + 32 * kb + (lane & 31);
-        if (r >= n_rows) continue;
-        half_t* row = out + r * stride + 4 * (lane >> 5);
+    for (int kb = 0; kb < kRB; ++kb)
 #pragma unroll
         for (int db = 0; db < kDB; ++db)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const float16_t& x = acc[kb * kDB + db];
-                *reinterpret_cast<half4_t*>(row + 32 * db + 8 * g) =
+                *(p4_t)(lds + 16u * (unsigned)((32 * kb + r) * kC + ((4 * db + g) ^ (r % kC))) + 8u * (unsigned)(lane >> 5)) =
                     half4_t{(half_t)(x[4 * g] * f), (half_t)(x[4 * g + 1] * f), (half_t)(x[4 * g + 2] * f), (half_t)(x[4 * g + 3] * f)};
             }
+#pragma unroll
+    for (int i = 0; i < kRB * 32 * kC / 64; ++i) {
+        const int u = 64 * i + lane, row = u / kC, c = (u % kC) ^ (row % kC);
+        const half8_t x = lds_read_b128(lds + 16u * (unsigned)u);
+        if (row0 + row < n_rows) *reinterpret_cast<half8_t*>(out + (row0 + row) * stride + 8 * c) = x;
     }
 }
 
@@ -377,33 +446,6 @@ __device__ __forceinline__ void kv_tile(args_t a, half_t* lds, int wg) {
     if (kt * T::kKeys >= pl.n_k) return;
     const int u0 = (int)((long long)pl.steps * part / a->n_part), u1 = (int)((long long)pl.steps * (part + 1) / a->n_part);
 
-    // K or V of the pair's keys, as B operands: slot s of k-step kk is row[16 kk + 8 hi + s]
-    half8_t frag[T::kKB][kKK];
-    {
-        const auto& src = role_p ? a->k : a->v;
-        const half_t* base = src.data + b * src.b + hk * src.h;
-#pragma unroll
-        for (int kb = 0; kb < T::kKB; ++kb) {
-            const int key = k0 + 32 * kb + (lane & 31);
-#pragma unroll
-            for (int kk = 0; kk < kKK; ++kk)
-                frag[kb][kk] = key < pl.n_k ? *reinterpret_cast<const half8_t*>(base + key * src.t + 16 * kk + 8 * hi) : half8_t{};
-        }
-    }
-    // the scale of P and dS: the workgroup's bound
-    float ref;
-    {
-        float n = 0.f, d = 0.f, v = 0.f;
-        for (int u = u0 + lane; u < u1; u += 64) {
-            const float2 m = a->row_max[(size_t)(b * a->Hq + hk * G + u / pl.per) * a->n_qb + pl.first + u % pl.per];
-            n = fmaxf(n, m.x);
-            d = fmaxf(d, m.y);
-        }
-        const int kb = kt * (T::kKeys / kBlk) + lane;
-        if (lane < T::kKeys / kBlk && kb < a->n_kb) v = a->key_max[(size_t)bh * a->n_kb + kb];
-        ref = range_ref(fmaf(wave_max(n), wave_max(v), wave_max(d)));
-    }
-
     float16_t acc[T::kAcc];
 #pragma unroll
     for (int i = 0; i < T::kAcc; ++i) acc[i] = float16_t{};
@@ -424,11 +466,14 @@ __device__ __forceinline__ void kv_tile(args_t a, half_t* lds, int wg) {
     const long long q_jump = 2 * a->q.h - (long long)q_row * kBlk * pl.per, g_jump = 2 * a->g.h - (long long)g_row * kBlk * pl.per;
     const int s_jump = 64 * (a->n_qb - pl.per);
     unsigned ring = 0, ring2 = 0;  // stages of the current step and of the next copies
+    // (by the second role: the first has the exponentials to do)
+    const Copy<D, T::kPairs> copier = {pair};
+    const unsigned q_off = copier.offset(lane, q_row), g_off = copier.offset(lane, g_row);
     auto copy = [&] {  // tiles and statistics of a step
         const unsigned st = lds0 + ring2 * T::kStage;
-        copy_rows<D, T::kW>(qp, q_row, last - to_copy * kBlk, lane, wave, st);
-        copy_rows<D, T::kW>(gp, g_row, last - to_copy * kBlk, lane, wave, st + T::kTileB);
-        if (wave == 0) dma_issue_any4(sp, 4u * lane, lds0 + T::kStatAt + ring2 * T::kStatB);
+        copier(qp, q_row, q_off, last - to_copy * kBlk, lane, st);
+        copier(gp, g_row, g_off, last - to_copy * kBlk, lane, st + T::kTileB);
+        if (pair == 0) dma_issue_any4(sp, 4u * lane, lds0 + T::kStatAt + ring2 * T::kStatB);
         qp += (size_t)q_row * kBlk, gp += (size_t)g_row * kBlk, sp += 64;
         if (++to_copy == end) to_copy = pl.first, qp += q_jump, gp += g_jump, sp += s_jump;
         ring2 = ring2 + 1 == T::kStages ? 0 : ring2 + 1;
@@ -436,58 +481,92 @@ __device__ __forceinline__ void kv_tile(args_t a, half_t* lds, int wg) {
     // a pair's keys are hidden from a step's queries while the last of those lies in front of the first of them
     auto hidden = [&](int x) { return kCausal && x * kBlk + kBlk - 1 + pl.last0 < k0; };
 
-    if (n > 0) copy();
+    if (!role_p && n > 0) copy();
+    // K or V of the pair's keys, as B operands: slot s of k-step kk is row[16 kk + 8 hi + s]
+    half8_t frag[T::kKB][kKK];
+    {
+        const auto& src = role_p ? a->k : a->v;
+        const half_t* base = src.data + b * src.b + hk * src.h;
+#pragma unroll
+        for (int kb = 0; kb < T::kKB; ++kb) {
+            // (past the last key its row again: what comes of it stays in lanes that store nothing)
+            const half_t* row = base + min(k0 + 32 * kb + (lane & 31), pl.n_k - 1) * src.t + 8 * hi;
+#pragma unroll
+            for (int kk = 0; kk < kKK; ++kk) frag[kb][kk] = *reinterpret_cast<const half8_t*>(row + 16 * kk);
+        }
+    }
+    // the scale of P and dS: the workgroup's bound
+    float ref;
+    {
+        float n = 0.f, d = 0.f, v = 0.f;
+        for (int u = u0 + lane; u < u1; u += 64) {
+            const float2 m = a->row_max[(size_t)(b * a->Hq + hk * G + u / pl.per) * a->n_qb + pl.first + u % pl.per];
+            n = fmaxf(n, m.x);
+            d = fmaxf(d, m.y);
+        }
+        const int kb = kt * (T::kKeys / kBlk) + lane;
+        if (lane < T::kKeys / kBlk && kb < a->n_kb) v = a->key_max[(size_t)bh * a->n_kb + kb];
+        ref = range_ref(fmaf(wave_max(n), wave_max(v), wave_max(d)));
+    }
+
 
     // register r of a result is query 4 hi + 8 (r / 4) + r % 4 of the step: hidden below this
     auto limit = [&](int x, int kb) { return k0 + 32 * kb + (lane & 31) - pl.last0 - x * kBlk - 4 * hi; };
     auto partly = [&](int x, int kb) { return kCausal && k0 + 32 * kb + 31 > x * kBlk + pl.last0; };
     if constexpr (role_p) {
-        half8_t p[T::kKB][2];
-        auto scores = [&](int x, unsigned stage, unsigned at) {  // S of a step, then P, to LDS for the other role
-            const unsigned st = stage * T::kStage, sa = lds0 + T::kStatAt + stage * T::kStatB + 16u * hi;
-            float16_t s[T::kKB];
-#pragma unroll
-            for (int kb = 0; kb < T::kKB; ++kb) s[kb] = float16_t{};
-            mul_rows<D, T::kKB>(op.rows, st, frag, s);
-#pragma unroll
-            for (int kb = 0; kb < T::kKB; ++kb)
-                if (partly(x, kb)) {
-                    const int lim = limit(x, kb);
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (8 * (r >> 2) + (r & 3) < lim) s[kb][r] = -INFINITY;
-                }
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const float4_t l = lds_read_f4(sa + 32u * g);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float m = ref - l[e];
-#pragma unroll
-                    for (int kb = 0; kb < T::kKB; ++kb) s[kb][4 * g + e] = fast_exp2(fmaf(s[kb][4 * g + e], a->c2, m));
-                }
-            }
-#pragma unroll
-            for (int kb = 0; kb < T::kKB; ++kb)
-#pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    p[kb][w] = pack8(s[kb], w);
-                    lds_write_b128(p_at + at + (unsigned)(kb * 2 + w) * 1024u, p[kb][w]);
-                }
+        // round i: S of step i, then its P beside dV of step i - 1, while step i + 1 is copied.  P goes to LDS, for the
+        // other role and for this one's next round
+        float16_t s[T::kKB];
+        float4_t l;
+        unsigned sa = 0, p_new = 0, p_old = 0;
+        auto soft = [&](int x) {  // value x of S to P, 16 a key block
+            const int kb = x >> 4, r = x & 15;
+            if (x == 0) l = lds_read_f4(sa);
+            s[kb][r] = pinned(fast_exp2(fmaf(s[kb][r], a->c2, ref - l[r & 3])));
+            if ((r & 3) == 3 && x + 1 < 16 * T::kKB) l = lds_read_f4(sa + 32u * (((r >> 2) + 1) & 3));
+            if ((r & 7) == 7) lds_write_b128(p_new + (unsigned)(kb * 2 + (r >> 3)) * 1024u, pack8(s[kb], r >> 3));
         };
-        // round i: dV of step i - 1, S and P of step i, while step i + 1 is copied
+        auto p_op = [&](int ks, half8_t (&y)[T::kKB]) {
+#pragma unroll
+            for (int kb = 0; kb < T::kKB; ++kb) y[kb] = lds_read_b128(p_old + (unsigned)(kb * 2 + ks) * 1024u);
+        };
+        constexpr int kShare = 16 * T::kKB / (2 * kDB);
 #pragma clang loop unroll(disable)
         for (int i = 0, was = 0; i <= n; ++i) {
             asm volatile("" : "+s"(i));  // (a first round taken out of the loop spills)
             dma_wait_barrier();
-            if (i + 1 < n) copy();
-            if (i > 0 && !hidden(was)) mul_cols<D, T::kKB, kDB>(op.cols, ring * T::kStage + T::kTileB, 0, p, acc);
+            const unsigned done = ring;  // step i - 1's stage
             if (i > 0) ring = ring + 1 == T::kStages ? 0 : ring + 1;
-            if (i < n && !hidden(qb)) {
-                scores(qb, ring, (unsigned)(i & 1) * (T::kPairs * T::kPB));
-            } else {  // no P: what it was is not kept through the other branch
+            const bool sums = i > 0 && !hidden(was), scores = i < n && !hidden(qb);
+            p_new = p_at + (unsigned)(i & 1) * (T::kPairs * T::kPB);
+            p_old = p_at + (unsigned)(~i & 1) * (T::kPairs * T::kPB);
+            sa = lds0 + T::kStatAt + ring * T::kStatB + 16u * hi;
+            if (scores) {
 #pragma unroll
-                for (int x = 0; x < 2 * T::kKB; ++x) asm volatile("" : "=v"(p[x >> 1][x & 1]));
+                for (int kb = 0; kb < T::kKB; ++kb) s[kb] = float16_t{};
+                mul_rows<D, T::kKB>(op.rows, ring * T::kStage, frag, s);
+#pragma unroll
+                for (int kb = 0; kb < T::kKB; ++kb)
+                    if (partly(qb, kb)) {
+                        const int lim = limit(qb, kb);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            if (8 * (r >> 2) + (r & 3) < lim) s[kb][r] = -INFINITY;
+                    }
+            } else {  // (what S was is not kept through this branch)
+#pragma unroll
+                for (int kb = 0; kb < T::kKB; ++kb) asm volatile("" : "=v"(s[kb]));
+            }
+            // one place that adds to dV (with more, the compiler moves the sums between registers): where there is no step i
+            // its P is made of anything, and read by no one
+            if (sums) {
+                mul_cols_beside<D, T::kKB, kDB>(op.cols, done * T::kStage + T::kTileB, 0, p_op, acc, [&](int x) {
+#pragma unroll
+                    for (int j = 0; j < kShare; ++j) soft(x * kShare + j);
+                });
+            } else if (scores) {
+#pragma unroll
+                for (int x = 0; x < 16 * T::kKB; ++x) soft(x);
             }
             was = qb;
             qb = qb + 1 == end ? pl.first : qb + 1;
@@ -539,11 +618,13 @@ __device__ __forceinline__ void kv_tile(args_t a, half_t* lds, int wg) {
         }
     }
 
+    lds_barrier();  // the tiles' LDS becomes the outputs'
     a = fresh(a);
-    const float f = exp2f(-ref) * (role_p ? 1.f : a->scale);
+    const float f = scale_back(ref) * (role_p ? 1.f : a->scale);
     if (a->n_part == 1) {
         const auto& out = role_p ? a->dv : a->dk;
-        store_rows<T::kKB, kDB>(acc, out.data + b * out.b + hk * out.h, out.t, k0, pl.n_k, again(lane), f);
+        store_rows<T::kKB, kDB>(acc, out.data + b * out.b + hk * out.h, out.t, k0, pl.n_k, again(lane), f,
+                                lds0 + (unsigned)wave * (64u * T::kKB * 32 * kDB));
     } else {  // [key tile][part][wave][16-byte group][lane]
         float4_t* w = reinterpret_cast<float4_t*>(a->part) + ((((size_t)bh * a->n_kt + kt) * a->n_part + part) * T::kW + wave) * (T::kAcc * 256) + lane;
 #pragma unroll
@@ -602,22 +683,18 @@ __device__ __forceinline__ void q_tile(args_t a, half_t* lds, int wg) {
 
     half8_t qf[kMB][kKK], gf[kMB][kKK];
     float l2[kMB], nd[kMB];
-    const float ref = q_tile_ref<D>(a, bh, bhk, tile0, T::kQueries / kBlk, n, lane);
 #pragma unroll
     for (int m = 0; m < kMB; ++m) {
-        const int q = q0 + 32 * m + (lane & 31);
-        const half_t *qr = a->q.data + b * a->q.b + h * a->q.h + q * a->q.t, *gr = a->g.data + b * a->g.b + h * a->g.h + q * a->g.t;
-        l2[m] = INFINITY;
-        nd[m] = 0.f;
-        if (q < n_q) {
-            const float* st = a->stat + ((size_t)bh * a->n_qb + q / kBlk) * 64 + q % kBlk;
-            l2[m] = st[0] - ref;
-            nd[m] = st[32];
-        }
+        const int q = min(q0 + 32 * m + (lane & 31), n_q - 1);  // (past the last query its row again, as for the keys)
+        const half_t* qr = a->q.data + b * a->q.b + h * a->q.h + q * a->q.t + 8 * hi;
+        const half_t* gr = a->g.data + b * a->g.b + h * a->g.h + q * a->g.t + 8 * hi;
+        const float* st = a->stat + ((size_t)bh * a->n_qb + q / kBlk) * 64 + q % kBlk;
+        l2[m] = st[0];
+        nd[m] = st[32];
 #pragma unroll
         for (int kk = 0; kk < kKK; ++kk) {
-            qf[m][kk] = q < n_q ? *reinterpret_cast<const half8_t*>(qr + 16 * kk + 8 * hi) : half8_t{};
-            gf[m][kk] = q < n_q ? *reinterpret_cast<const half8_t*>(gr + 16 * kk + 8 * hi) : half8_t{};
+            qf[m][kk] = *reinterpret_cast<const half8_t*>(qr + 16 * kk);
+            gf[m][kk] = *reinterpret_cast<const half8_t*>(gr + 16 * kk);
         }
     }
     float16_t acc[kMB * kDB];
@@ -630,15 +707,20 @@ __device__ __forceinline__ void q_tile(args_t a, half_t* lds, int wg) {
     const unsigned k_row = 2u * (unsigned)a->k.t, v_row = 2u * (unsigned)a->v.t;
     unsigned ring = 2, ring2 = 0;  // stages of the current step and of the next copies
     int left = n_k - 1;            // the last key, counted from the next copies' first
+    const Copy<D, T::kW> copier = {wave};
+    const unsigned k_off = copier.offset(lane, k_row), v_off = copier.offset(lane, v_row);
     auto copy = [&] {
         const unsigned st = lds0 + ring2 * T::kTileB;
-        copy_rows<D, T::kW>(kp, k_row, left, lane, wave, st);
-        copy_rows<D, T::kW>(vp, v_row, left, lane, wave, st + T::kVAt);
+        copier(kp, k_row, k_off, left, lane, st);
+        copier(vp, v_row, v_off, left, lane, st + T::kVAt);
         kp += (size_t)k_row * kBlk, vp += (size_t)v_row * kBlk, left -= kBlk;
         ring2 = ring2 == 2 ? 0 : ring2 + 1;
     };
     if (n > 0) copy();
     if (n > 1) copy();
+    const float ref = q_tile_ref<D>(a, bh, bhk, tile0, T::kQueries / kBlk, n, lane);
+#pragma unroll
+    for (int m = 0; m < kMB; ++m) l2[m] -= ref;
 #pragma clang loop unroll(disable)
     for (int j = 0; j < n; ++j) {
         dma_wait_barrier();
@@ -672,8 +754,10 @@ __device__ __forceinline__ void q_tile(args_t a, half_t* lds, int wg) {
         }
         mul_cols<D, kMB, kDB>(op.cols, st, 0, ds, acc);
     }
+    lds_barrier();  // the tiles' LDS becomes the outputs'
     a = fresh(a);
-    store_rows<kMB, kDB>(acc, a->dq.data + b * a->dq.b + h * a->dq.h, a->dq.t, q0, n_q, again(lane), exp2f(-ref) * a->scale);
+    store_rows<kMB, kDB>(acc, a->dq.data + b * a->dq.b + h * a->dq.h, a->dq.t, q0, n_q, again(lane), scale_back(ref) * a->scale,
+                         lds0 + (unsigned)wave * (64u * kMB * 32 * kDB));
 }
 
 // The same at D = 256, by pairs of waves that own 32 queries: the first makes S and P, the second dP
@@ -696,16 +780,15 @@ __device__ __forceinline__ void q_tile_roles(args_t a, half_t* lds, int wg) {
     const int n = max(0, (k_end + kBlk - 1) / kBlk);
     const int my_n = max(0, ((kCausal ? min(n_k, q0 + 32 + last0) : n_k) + kBlk - 1) / kBlk);  // steps of the pair's own
 
-    const float ref = q_tile_ref<D>(a, bh, bhk, tile0, T::kQueries / kBlk, n, lane);
     half8_t frag[1][kKK];
-    float stat = role_p ? INFINITY : 0.f;
+    float stat;
     {
         const auto& src = role_p ? a->q : a->g;
-        const half_t* row = src.data + b * src.b + h * src.h + my_q * src.t;
+        const int q = min(my_q, n_q - 1);
+        const half_t* row = src.data + b * src.b + h * src.h + q * src.t + 8 * hi;
 #pragma unroll
-        for (int kk = 0; kk < kKK; ++kk)
-            frag[0][kk] = my_q < n_q ? *reinterpret_cast<const half8_t*>(row + 16 * kk + 8 * hi) : half8_t{};
-        if (my_q < n_q) stat = a->stat[((size_t)bh * a->n_qb + my_q / kBlk) * 64 + my_q % kBlk + (role_p ? 0 : 32)];
+        for (int kk = 0; kk < kKK; ++kk) frag[0][kk] = *reinterpret_cast<const half8_t*>(row + 16 * kk);
+        stat = a->stat[((size_t)bh * a->n_qb + q / kBlk) * 64 + q % kBlk + (role_p ? 0 : 32)];
     }
     float16_t acc[kDB];
 #pragma unroll
@@ -717,46 +800,58 @@ __device__ __forceinline__ void q_tile_roles(args_t a, half_t* lds, int wg) {
     const char *kp = reinterpret_cast<const char*>(a->k.data + b * a->k.b + hk * a->k.h), *vp = reinterpret_cast<const char*>(a->v.data + b * a->v.b + hk * a->v.h);
     const unsigned k_row = 2u * (unsigned)a->k.t, v_row = 2u * (unsigned)a->v.t;
     int left = n_k - 1;  // the last key, counted from the next copies' first
+    const Copy<D, kPairs> copier = {pair};  // (by the second role: the first has the exponentials to do)
+    const unsigned k_off = copier.offset(lane, k_row), v_off = copier.offset(lane, v_row);
     auto copy = [&](int j) {
-        copy_rows<D, T::kW>(kp, k_row, left, lane, wave, lds0 + (unsigned)(j & 3) * T::kTileB);
-        copy_rows<D, T::kW>(vp, v_row, left, lane, wave, lds0 + T::kVAt + (unsigned)(j & 1) * T::kTileB);
+        copier(kp, k_row, k_off, left, lane, lds0 + (unsigned)(j & 3) * T::kTileB);
+        copier(vp, v_row, v_off, left, lane, lds0 + T::kVAt + (unsigned)(j & 1) * T::kTileB);
         kp += (size_t)k_row * kBlk, vp += (size_t)v_row * kBlk, left -= kBlk;
     };
     const int db0 = role_p ? 0 : kDB;  // dQ^T += K^T dS^T, this role's columns
     // register r is key 32 j + 4 hi + 8 (r / 4) + r % 4; the last that this lane's query sees
     auto limit = [&](int j) { return min(kCausal ? my_q + last0 : n_k, n_k - 1) - j * kBlk - 4 * hi; };
     auto ragged = [&](int j) { return (kCausal && j * kBlk + 31 > q0 + last0) || (j + 1) * kBlk > n_k; };
-    if (n > 0) copy(0);
+    if (!role_p && n > 0) copy(0);
+    const float ref = q_tile_ref<D>(a, bh, bhk, tile0, T::kQueries / kBlk, n, lane);
     if constexpr (role_p) {
-        auto scores = [&](int j) {
-            const unsigned st = (unsigned)(j & 3) * T::kTileB;
-            float16_t x1[1] = {float16_t{}}, &s = x1[0];
-            mul_rows<D, 1>(op.rows, st, frag, x1);
-            if (ragged(j)) {
-                const int lim = limit(j);
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (8 * (r >> 2) + (r & 3) > lim) s[r] = -INFINITY;
-            }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = fast_exp2(fmaf(s[r], a->c2, ref - stat));
-#pragma unroll
-            for (int x = 0; x < 2; ++x) lds_write_b128(p_at + (unsigned)((j & 1) * kPairs * 2048 + x * 1024), pack8(s, x));
+        // round j: S of step j, then its P beside dQ of step j - 2
+        float16_t x1[1], &s = x1[0];
+        const float l = ref - stat;
+        unsigned p_new = 0, ds_old = 0;
+        auto soft = [&](int x) {
+            s[x] = pinned(fast_exp2(fmaf(s[x], a->c2, l)));
+            if ((x & 7) == 7) lds_write_b128(p_new + (unsigned)(x >> 3) * 1024u, pack8(s, x >> 3));
         };
-        auto take = [&](int j) {
-            half8_t ds[1][2];
-#pragma unroll
-            for (int x = 0; x < 2; ++x) ds[0][x] = lds_read_b128(ds_at + (unsigned)((j & 1) * kPairs * 2048 + x * 1024));
-            mul_cols<D, 1, kDB>(op.cols, (unsigned)(j & 3) * T::kTileB, db0, ds, acc);
-        };
-        // round j: dQ of step j - 2, S and P of step j, while step j + 1 is copied
+        auto ds_op = [&](int ks, half8_t (&y)[1]) { y[0] = lds_read_b128(ds_old + (unsigned)ks * 1024u); };
 #pragma clang loop unroll(disable)
         for (int j = 0; j < n + 2; ++j) {
             asm volatile("" : "+s"(j));
             dma_wait_barrier();
-            if (j + 1 < n) copy(j + 1);
-            if (j > 1 && j - 2 < my_n) take(j - 2);
-            if (j < my_n) scores(j);
+            const bool sums = j > 1 && j - 2 < my_n, scores = j < my_n;
+            p_new = p_at + (unsigned)((j & 1) * kPairs * 2048);
+            ds_old = ds_at + (unsigned)((j & 1) * kPairs * 2048);
+            const unsigned done = (unsigned)((j - 2) & 3) * T::kTileB;
+            if (scores) {
+                s = float16_t{};
+                mul_rows<D, 1>(op.rows, (unsigned)(j & 3) * T::kTileB, frag, x1);
+                if (ragged(j)) {
+                    const int lim = limit(j);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (8 * (r >> 2) + (r & 3) > lim) s[r] = -INFINITY;
+                }
+            } else {
+                asm volatile("" : "=v"(s));
+            }
+            if (sums) {  // (as for the key tiles)
+                mul_cols_beside<D, 1, kDB>(op.cols, done, db0, ds_op, acc, [&](int x) {
+#pragma unroll
+                    for (int i = 0; i < 8 / kDB; ++i) soft(x * (8 / kDB) + i);
+                });
+            } else if (scores) {
+#pragma unroll
+                for (int x = 0; x < 16; ++x) soft(x);
+            }
         }
     } else {
         float16_t x1[1], &s = x1[0];
@@ -793,8 +888,10 @@ __device__ __forceinline__ void q_tile_roles(args_t a, half_t* lds, int wg) {
                 asm volatile("" : "=v"(s));
         }
     }
+    lds_barrier();  // the tiles' LDS becomes the outputs'
     a = fresh(a);
-    store_rows<1, kDB>(acc, a->dq.data + b * a->dq.b + h * a->dq.h + (role_p ? 0 : D / 2), a->dq.t, q0, n_q, again(lane), exp2f(-ref) * a->scale);
+    store_rows<1, kDB>(acc, a->dq.data + b * a->dq.b + h * a->dq.h + (role_p ? 0 : D / 2), a->dq.t, q0, n_q, again(lane), scale_back(ref) * a->scale,
+                       lds0 + (unsigned)wave * (64u * 32 * kDB));
 }
 
 template <int D, bool kCausal>
@@ -819,25 +916,30 @@ __global__ void __launch_bounds__(64 * KvTile<D>::kW, 2) attn_bwd_kernel(BwdArgs
     }
 }
 
-// The sum of a split key tile's parts, in their order: one wave for each wave that wrote them.
+// The sum of a split key tile's parts, in their order: a thread for each 16-byte group that a lane wrote,
+// all parts' loads on their way at once.
 template <int D>
-__global__ void __launch_bounds__(64) attn_bwd_join_kernel(BwdArgs a) {
+__global__ void __launch_bounds__(256) attn_bwd_join_kernel(BwdArgs a) {
     using T = KvTile<D>;
-    const int lane = threadIdx.x, n_bh = a.B * a.Hkv;
-    const int wave = blockIdx.x % T::kW, rest = blockIdx.x / T::kW, bh = rest % n_bh, kt = rest / n_bh;
+    constexpr int kWgs = T::kAcc;  // workgroups that a wave's 4 kAcc groups take
+    const int lane = threadIdx.x & 63, n_bh = a.B * a.Hkv;
+    const int i = blockIdx.x % kWgs * 4 + (threadIdx.x >> 6);
+    const int wave = blockIdx.x / kWgs % T::kW, rest = blockIdx.x / (kWgs * T::kW), bh = rest % n_bh, kt = rest / n_bh;
     const int b = bh / a.Hkv, hk = bh % a.Hkv, n_k = count(a.len_k, b, a.Tk);
-    const int k0 = kt * T::kKeys + wave % T::kPairs * 32 * T::kKB;
-    if (k0 >= n_k) return;
-    const Rows16& out = wave < T::kPairs ? a.dv : a.dk;
-    const float4_t* w = reinterpret_cast<const float4_t*>(a.part) + (((size_t)bh * a.n_kt + kt) * a.n_part * T::kW + wave) * (T::kAcc * 256) + lane;
-    half_t* base = out.data + b * out.b + hk * out.h + 4 * (lane >> 5);
-    const int key = k0 + (lane & 31);
-    for (int i = 0; i < 4 * T::kAcc; ++i) {
-        const int r = key + 32 * (i / (4 * (D / 32))), d = 8 * (i % (4 * (D / 32)));
-        float4_t x = w[(size_t)i * 64];
-        for (int p = 1; p < a.n_part; ++p) x += w[(size_t)p * T::kW * (T::kAcc * 256) + i * 64];
-        if (r < n_k) *reinterpret_cast<half4_t*>(base + r * out.t + d) = half4_t{(half_t)x[0], (half_t)x[1], (half_t)x[2], (half_t)x[3]};
+    const int key = kt * T::kKeys + wave % T::kPairs * 32 * T::kKB + 32 * (i / (D / 8)) + (lane & 31);
+    if (key >= n_k) return;
+    const float4_t* w = reinterpret_cast<const float4_t*>(a.part) + (((size_t)bh * a.n_kt + kt) * a.n_part * T::kW + wave) * (T::kAcc * 256) + i * 64 + lane;
+    constexpr size_t kPart = (size_t)T::kW * (T::kAcc * 256);
+    float4_t x = w[0];
+    int p = 1;
+    for (; p + 4 <= a.n_part; p += 4) {
+        const float4_t y0 = w[p * kPart], y1 = w[(p + 1) * kPart], y2 = w[(p + 2) * kPart], y3 = w[(p + 3) * kPart];
+        x = x + y0 + y1 + y2 + y3;
     }
+    for (; p < a.n_part; ++p) x += w[p * kPart];
+    const Rows16& out = wave < T::kPairs ? a.dv : a.dk;
+    *reinterpret_cast<half4_t*>(out.data + b * out.b + hk * out.h + key * out.t + 4 * (lane >> 5) + 8 * (i % (D / 8))) =
+        half4_t{(half_t)x[0], (half_t)x[1], (half_t)x[2], (half_t)x[3]};
 }
 
 // Sizes of a call, and where its workspace holds what.
@@ -851,9 +953,19 @@ Plan plan(int B, int Hq, int Hkv, int Tq, int Tk, bool gated, bool causal) {
     auto up = [](long long a, long long b) { return (int)((a + b - 1) / b); };
     p.n_qb = up(Tq, kBlk), p.n_kb = up(Tk, kBlk);
     p.n_kt = up(Tk, KvTile<D>::kKeys), p.n_qt = up(Tq, QTile<D>::kQueries);
+    // A key tile's queries are split over workgroups where the longest tile would outlast the rest of the
+    // device's work: in products of a step, against what a workgroup slot has to do on average (of
+    // what a causal mask leaves).  A part costs its fp32 sums' way to memory and back (256 KiB at D = 256)
+    // and the join, so it has 16 steps at least.  us per call by parts: 128 tiles of 768 steps
+    // (24/4 heads x 4096, D = 256) 1236 / 842 / 841 / 832 / 841 (1, 2, 3, 4, 6); 96 of 66 steps (3 x 701 over 1999)
+    // 119 / 113 / 128 / 140; 512 of 256 steps (4 x 2048, 32/8 heads, D = 128; a longest tile of 1.1 averages)
+    // 608 / 598 / 606 / 627; 64 of 16 steps (2 x 512, D = 64) 51.5 / 55.9.
     const long long tiles = (long long)B * Hkv * p.n_kt, steps = (long long)(Hq / Hkv) * p.n_qb;
-    const long long want = (768 + tiles - 1) / tiles, most = steps / 8 > 1 ? steps / 8 : 1;
-    p.n_part = tiles >= 512 ? 1 : (int)(want < most ? want : most);
+    const long long slots = D == 256 ? 256 : 512;
+    const double seen = causal ? 1 - 0.5 * std::min(1.0, (double)Tq / Tk) : 1;
+    const double longest = 4.0 * steps, average = seen * (4.0 * tiles * steps + 3.0 * B * Hq * p.n_qt * p.n_kb) / slots;
+    const double want = longest > 1.3 * average ? std::ceil(longest / (0.9 * average)) : 1;
+    p.n_part = (int)std::max(1.0, std::min(want, (double)(steps / 16)));
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t was = at;
@@ -892,7 +1004,7 @@ hipError_t backward(const AttnRows& x, const Rows16& d_out, const Rows16& dq, co
     else
         hipLaunchKernelGGL((attn_bwd_kernel<D, false>), grid, block, 0, stream, a);
     if (p.n_part > 1)
-        hipLaunchKernelGGL(attn_bwd_join_kernel<D>, dim3(B * Hkv * p.n_kt * KvTile<D>::kW), dim3(64), 0, stream, a);
+        hipLaunchKernelGGL(attn_bwd_join_kernel<D>, dim3(B * Hkv * p.n_kt * KvTile<D>::kW * KvTile<D>::kAcc), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 

@@ -53,8 +53,25 @@ struct RopeArgs {
     int Hq, H, B, T, rot, units, per, flip;  // H: heads of q and k; units a row; heads a thread; flip: turn back
 };
 
+// kVec pairs: interleaved in x then y, or their first elements in x and their second in y.
+template <typename T, bool kInter, int kVec>
+__device__ __forceinline__ void rotate(T (&x)[kVec], T (&y)[kVec], const float (&s)[kVec], const float (&c)[kVec]) {
+    T e[2 * kVec];
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) e[kInter ? i : 2 * i] = x[i], e[kInter ? kVec + i : 2 * i + 1] = y[i];
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+        const float p = (float)e[2 * i], q = (float)e[2 * i + 1];
+        e[2 * i] = (T)fmaf(p, c[i], -(q * s[i]));
+        e[2 * i + 1] = (T)fmaf(q, c[i], p * s[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) x[i] = e[kInter ? i : 2 * i], y[i] = e[kInter ? kVec + i : 2 * i + 1];
+}
+
 // Unit u of a row: pairs u kVec .. + kVec - 1 while those are below rot / 2, then the elements behind
 // the rotated ones, 2 kVec at a time (only where they have to be copied: out of place).
+constexpr int kAtOnce = 4;
 template <typename T, bool kInter, int kVec>
 __global__ void __launch_bounds__(256) rope_kernel(RopeArgs a) {
     const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -79,38 +96,32 @@ __global__ void __launch_bounds__(256) rope_kernel(RopeArgs a) {
     const int up = kInter || !turn ? lo + kVec : lo + a.rot / 2;
     const int h0 = blockIdx.y * a.per, h1 = min(h0 + a.per, a.H);
     using P = Pack<T, kVec>;
-    for (int h = h0; h < h1; ++h) {
+    auto rows = [&](int h, const T*& src, T*& dst) {
         const bool is_q = h < a.Hq;
         const RopeTensor& x = is_q ? a.q : a.k;
         const int hh = is_q ? h : h - a.Hq;
-        const T* src = static_cast<const T*>(x.in) + b * x.in_b + hh * x.in_h + t * x.in_t;
-        T* dst = static_cast<T*>(x.out) + b * x.out_b + hh * x.out_h + t * x.out_t;
-        P v0 = *reinterpret_cast<const P*>(src + lo), v1 = *reinterpret_cast<const P*>(src + up);
-        if (turn) {
-            if constexpr (kInter) {
-                T* e = v0.x;
-                T f[2 * kVec];
+        src = static_cast<const T*>(x.in) + b * x.in_b + hh * x.in_h + t * x.in_t;
+        dst = static_cast<T*>(x.out) + b * x.out_b + hh * x.out_h + t * x.out_t;
+    };
+    // kAtOnce heads' loads on their way together
+    for (int h = h0; h < h1; h += kAtOnce) {
+        P v[kAtOnce][2];
+        T* dst[kAtOnce];
 #pragma unroll
-                for (int i = 0; i < kVec; ++i) f[i] = v0.x[i], f[kVec + i] = v1.x[i];
-#pragma unroll
-                for (int i = 0; i < kVec; ++i) {
-                    const float p = (float)f[2 * i], q = (float)f[2 * i + 1];
-                    f[2 * i] = (T)fmaf(p, c[i], -(q * s[i]));
-                    f[2 * i + 1] = (T)fmaf(q, c[i], p * s[i]);
-                }
-#pragma unroll
-                for (int i = 0; i < kVec; ++i) e[i] = f[i], v1.x[i] = f[kVec + i];
-            } else {
-#pragma unroll
-                for (int i = 0; i < kVec; ++i) {
-                    const float p = (float)v0.x[i], q = (float)v1.x[i];
-                    v0.x[i] = (T)fmaf(p, c[i], -(q * s[i]));
-                    v1.x[i] = (T)fmaf(q, c[i], p * s[i]);
-                }
+        for (int i = 0; i < kAtOnce; ++i)
+            if (h + i < h1) {
+                const T* src;
+                rows(h + i, src, dst[i]);
+                v[i][0] = *reinterpret_cast<const P*>(src + lo);
+                v[i][1] = *reinterpret_cast<const P*>(src + up);
             }
-        }
-        *reinterpret_cast<P*>(dst + lo) = v0;
-        *reinterpret_cast<P*>(dst + up) = v1;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+            if (h + i < h1) {
+                if (turn) rotate<T, kInter, kVec>(v[i][0].x, v[i][1].x, s, c);
+                *reinterpret_cast<P*>(dst[i] + lo) = v[i][0];
+                *reinterpret_cast<P*>(dst[i] + up) = v[i][1];
+            }
     }
 }
 
@@ -138,8 +149,10 @@ hipError_t rope(const unsigned long long* freq, float amp, int rot, int interlea
     const bool copy = rot < D && (q.data != q_out.data || (Hk && k.data != k_out.data));
     const int H = Hq + Hk, units = (copy ? D : rot) / (wide ? 16 : 2);
     const long long threads = (long long)B * T * units;
-    int per = 8;
-    const dim3 grid((unsigned)((threads + 255) / 256), (unsigned)((H + per - 1) / per));
+    // heads a thread: one where that does not fill the device, else 8 to share the sines
+    const long long groups = (threads + 255) / 256;
+    const int per = groups * H <= 2048 ? 1 : groups * H <= 8192 ? 4 : 8;
+    const dim3 grid((unsigned)groups, (unsigned)((H + per - 1) / per));
     RopeArgs a = {tensor(q, q_out), tensor(k, k_out), freq, pos, len, n_new, amp, Hq, H, B, T, rot, units, per, back};
     if (f32)
         return interleaved ? launch_rope<float, true>(a, grid, wide, stream) : launch_rope<float, false>(a, grid, wide, stream);

@@ -785,10 +785,9 @@ class Rope:
 
 def _rows_on(t, shape, name, index, dtype):
     """A [B, H, T, D] tensor on GPU `index` as a tsa_rows: rows of consecutive elements, any other strides."""
-    torch = _torch or _t()
-    if not isinstance(t, torch.Tensor):
+    if not isinstance(t, (_torch or _t()).Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if t.dtype is dtype and t.is_cuda and t.get_device() == index and t.shape == shape:
+    if t.dtype is dtype and t.get_device() == index and t.shape == shape:  # (index is a GPU's: not -1)
         b, h, r, d = t.stride()
         if d == 1:
             return _ROWS.pack(t.data_ptr(), b, h, r)
