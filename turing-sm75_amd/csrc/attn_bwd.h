@@ -320,6 +320,7 @@ __device__ __forceinline__ void mul_cols_beside(unsigned cols, unsigned tile, in
             acc[r * kDB + i % kDB] = mfma32(x[i], y[i / kDB][r], acc[r * kDB + i % kDB]);
             asm volatile("" : "+v"(acc[r * kDB + i % kDB]));
         }
+        __builtin_amdgcn_sched_barrier(0);
         work(i);
         __builtin_amdgcn_sched_barrier(0);
     }
@@ -439,6 +440,10 @@ __device__ __forceinline__ void kv_tile(args_t a, half_t* lds, int wg) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5;
     const int pair = wave % T::kPairs;
     const int n_bh = a->B * a->Hkv;
+    // Workgroups go round the 256 CUs (an XCD after the other); each round begins one CU further on, so that
+    // a long sequence's tiles, a power of two apart in a padded batch, do not share CUs (lengths 2048, 273, 546, 819 of
+    // 32/8 heads, D = 128: 322 -> 215 us with the split in two).
+    if (wg / 256 < a->n_kv / 256) wg = wg / 256 * 256 + (wg + wg / 256 * 8) % 256;
     const int bh = wg % n_bh, rest = wg / n_bh, part = rest % a->n_part, kt = rest / a->n_part;
     const int b = bh / a->Hkv, hk = bh % a->Hkv, G = a->Hq / a->Hkv;
     const KvPlan pl = kv_plan<D, kCausal>(a, b, kt);
@@ -482,6 +487,18 @@ __device__ __forceinline__ void kv_tile(args_t a, half_t* lds, int wg) {
     auto hidden = [&](int x) { return kCausal && x * kBlk + kBlk - 1 + pl.last0 < k0; };
 
     if (!role_p && n > 0) copy();
+    // the scale of P and dS is the workgroup's bound; its first loads, and K's or V's, on their way together
+    float most_g = 0.f, most_d = 0.f, most_v = 0.f;
+    auto row_most = [&](int u) {
+        const float2 m = a->row_max[(size_t)(b * a->Hq + hk * G + u / pl.per) * a->n_qb + pl.first + u % pl.per];
+        most_g = fmaxf(most_g, m.x);
+        most_d = fmaxf(most_d, m.y);
+    };
+    if (u0 + lane < u1) row_most(u0 + lane);
+    {
+        const int kb = kt * (T::kKeys / kBlk) + lane;
+        if (lane < T::kKeys / kBlk && kb < a->n_kb) most_v = a->key_max[(size_t)bh * a->n_kb + kb];
+    }
     // K or V of the pair's keys, as B operands: slot s of k-step kk is row[16 kk + 8 hi + s]
     half8_t frag[T::kKB][kKK];
     {
@@ -495,20 +512,8 @@ __device__ __forceinline__ void kv_tile(args_t a, half_t* lds, int wg) {
             for (int kk = 0; kk < kKK; ++kk) frag[kb][kk] = *reinterpret_cast<const half8_t*>(row + 16 * kk);
         }
     }
-    // the scale of P and dS: the workgroup's bound
-    float ref;
-    {
-        float n = 0.f, d = 0.f, v = 0.f;
-        for (int u = u0 + lane; u < u1; u += 64) {
-            const float2 m = a->row_max[(size_t)(b * a->Hq + hk * G + u / pl.per) * a->n_qb + pl.first + u % pl.per];
-            n = fmaxf(n, m.x);
-            d = fmaxf(d, m.y);
-        }
-        const int kb = kt * (T::kKeys / kBlk) + lane;
-        if (lane < T::kKeys / kBlk && kb < a->n_kb) v = a->key_max[(size_t)bh * a->n_kb + kb];
-        ref = range_ref(fmaf(wave_max(n), wave_max(v), wave_max(d)));
-    }
-
+    for (int u = u0 + 64 + lane; u < u1; u += 64) row_most(u);
+    const float ref = range_ref(fmaf(wave_max(most_g), wave_max(most_v), wave_max(most_d)));
 
     // register r of a result is query 4 hi + 8 (r / 4) + r % 4 of the step: hidden below this
     auto limit = [&](int x, int kb) { return k0 + 32 * kb + (lane & 31) - pl.last0 - x * kBlk - 4 * hi; };
@@ -516,13 +521,13 @@ __device__ __forceinline__ void kv_tile(args_t a, half_t* lds, int wg) {
     if constexpr (role_p) {
         // round i: S of step i, then its P beside dV of step i - 1, while step i + 1 is copied.  P goes to LDS, for the
         // other role and for this one's next round
+        const float c2 = a->c2;
         float16_t s[T::kKB];
         float4_t l;
         unsigned sa = 0, p_new = 0, p_old = 0;
         auto soft = [&](int x) {  // value x of S to P, 16 a key block
             const int kb = x >> 4, r = x & 15;
-            if (x == 0) l = lds_read_f4(sa);
-            s[kb][r] = pinned(fast_exp2(fmaf(s[kb][r], a->c2, ref - l[r & 3])));
+            s[kb][r] = pinned(fast_exp2(fmaf(s[kb][r], c2, ref - l[r & 3])));
             if ((r & 3) == 3 && x + 1 < 16 * T::kKB) l = lds_read_f4(sa + 32u * (((r >> 2) + 1) & 3));
             if ((r & 7) == 7) lds_write_b128(p_new + (unsigned)(kb * 2 + (r >> 3)) * 1024u, pack8(s[kb], r >> 3));
         };
@@ -541,6 +546,7 @@ __device__ __forceinline__ void kv_tile(args_t a, half_t* lds, int wg) {
             p_new = p_at + (unsigned)(i & 1) * (T::kPairs * T::kPB);
             p_old = p_at + (unsigned)(~i & 1) * (T::kPairs * T::kPB);
             sa = lds0 + T::kStatAt + ring * T::kStatB + 16u * hi;
+            l = lds_read_f4(sa);
             if (scores) {
 #pragma unroll
                 for (int kb = 0; kb < T::kKB; ++kb) s[kb] = float16_t{};
@@ -705,6 +711,7 @@ __device__ __forceinline__ void q_tile(args_t a, half_t* lds, int wg) {
     const OpAddr<D> op(lane, lds0);
     const char *kp = reinterpret_cast<const char*>(a->k.data + b * a->k.b + hk * a->k.h), *vp = reinterpret_cast<const char*>(a->v.data + b * a->v.b + hk * a->v.h);
     const unsigned k_row = 2u * (unsigned)a->k.t, v_row = 2u * (unsigned)a->v.t;
+    const float c2 = a->c2;
     unsigned ring = 2, ring2 = 0;  // stages of the current step and of the next copies
     int left = n_k - 1;            // the last key, counted from the next copies' first
     const Copy<D, T::kW> copier = {wave};
@@ -741,7 +748,7 @@ __device__ __forceinline__ void q_tile(args_t a, half_t* lds, int wg) {
 #pragma unroll
         for (int m = 0; m < kMB; ++m) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) w[m][r] *= fast_exp2(fmaf(s[m][r], a->c2, -l2[m]));
+            for (int r = 0; r < 16; ++r) w[m][r] *= fast_exp2(fmaf(s[m][r], c2, -l2[m]));
             if ((kCausal && j * kBlk + 31 > q0 + 32 * m + last0) || (j + 1) * kBlk > n_k) {
                 // register r is key 32 j + 4 hi + 8 (r / 4) + r % 4
                 const int lim = min(kCausal ? q0 + 32 * m + (lane & 31) + last0 : n_k, n_k - 1) - j * kBlk - 4 * hi;
@@ -816,10 +823,10 @@ __device__ __forceinline__ void q_tile_roles(args_t a, half_t* lds, int wg) {
     if constexpr (role_p) {
         // round j: S of step j, then its P beside dQ of step j - 2
         float16_t x1[1], &s = x1[0];
-        const float l = ref - stat;
+        const float l = ref - stat, c2 = a->c2;
         unsigned p_new = 0, ds_old = 0;
         auto soft = [&](int x) {
-            s[x] = pinned(fast_exp2(fmaf(s[x], a->c2, l)));
+            s[x] = pinned(fast_exp2(fmaf(s[x], c2, l)));
             if ((x & 7) == 7) lds_write_b128(p_new + (unsigned)(x >> 3) * 1024u, pack8(s, x >> 3));
         };
         auto ds_op = [&](int ks, half8_t (&y)[1]) { y[0] = lds_read_b128(ds_old + (unsigned)ks * 1024u); };
@@ -948,24 +955,22 @@ struct Plan {
     size_t stat, row_max, key_max, gated, part, bytes;
 };
 template <int D>
-Plan plan(int B, int Hq, int Hkv, int Tq, int Tk, bool gated, bool causal) {
+Plan plan(int B, int Hq, int Hkv, int Tq, int Tk, bool gated, bool causal, bool ragged) {
     Plan p;
     auto up = [](long long a, long long b) { return (int)((a + b - 1) / b); };
     p.n_qb = up(Tq, kBlk), p.n_kb = up(Tk, kBlk);
     p.n_kt = up(Tk, KvTile<D>::kKeys), p.n_qt = up(Tq, QTile<D>::kQueries);
     // A key tile's queries are split over workgroups where the longest tile would outlast the rest of the
-    // device's work: in products of a step, against what a workgroup slot has to do on average (of
-    // what a causal mask leaves).  A part costs its fp32 sums' way to memory and back (256 KiB at D = 256)
-    // and the join, so it has 16 steps at least.  us per call by parts: 128 tiles of 768 steps
-    // (24/4 heads x 4096, D = 256) 1236 / 842 / 841 / 832 / 841 (1, 2, 3, 4, 6); 96 of 66 steps (3 x 701 over 1999)
-    // 119 / 113 / 128 / 140; 512 of 256 steps (4 x 2048, 32/8 heads, D = 128; a longest tile of 1.1 averages)
-    // 608 / 598 / 606 / 627; 64 of 16 steps (2 x 512, D = 64) 51.5 / 55.9.
+    // device's work: in products of a step, against 1.3 times what a workgroup slot has to do on average
+    // (of what a causal mask leaves, and of 0.7 of that where sequences have lengths, which only the device knows).  A part
+    // costs its fp32 sums' way to memory and back (256 KiB at D = 256) and the join, so it has 16 steps at least.  us per
+    // call by parts (1, 2, 3, 4, 6): 128 tiles of 768 steps (24/4 heads x 4096, D = 256) 1175 / 809 / 807 / 804 / 817;
+    // 96 of 66 steps (3 x 701 over 1999, D = 256, ragged) 108 / 103 / 118 / 129 / 142; 64 of 16 steps (2 x 512, D = 64) 51.5 / 55.9.
     const long long tiles = (long long)B * Hkv * p.n_kt, steps = (long long)(Hq / Hkv) * p.n_qb;
     const long long slots = D == 256 ? 256 : 512;
-    const double seen = causal ? 1 - 0.5 * std::min(1.0, (double)Tq / Tk) : 1;
+    const double seen = (causal ? 1 - 0.5 * std::min(1.0, (double)Tq / Tk) : 1) * (ragged ? 0.7 : 1);
     const double longest = 4.0 * steps, average = seen * (4.0 * tiles * steps + 3.0 * B * Hq * p.n_qt * p.n_kb) / slots;
-    const double want = longest > 1.3 * average ? std::ceil(longest / (0.9 * average)) : 1;
-    p.n_part = (int)std::max(1.0, std::min(want, (double)(steps / 16)));
+    p.n_part = (int)std::max(1.0, std::min(std::ceil(longest / (1.3 * average)), (double)(steps / 16)));
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t was = at;
@@ -986,7 +991,7 @@ hipError_t backward(const AttnRows& x, const Rows16& d_out, const Rows16& dq, co
                     int B, int Hq, int Hkv, int Tq, float scale, int causal, void* ws, hipStream_t stream) {
     const int Tk = x.Sk;
     const bool gated = x.gate.data != nullptr;
-    const Plan p = plan<D>(B, Hq, Hkv, Tq, Tk, gated, causal != 0);
+    const Plan p = plan<D>(B, Hq, Hkv, Tq, Tk, gated, causal != 0, x.len_q || x.len_k);
     char* w = static_cast<char*>(ws);
     float* stat = reinterpret_cast<float*>(w + p.stat);
     float2* row_max = reinterpret_cast<float2*>(w + p.row_max);
@@ -1012,10 +1017,14 @@ hipError_t backward(const AttnRows& x, const Rows16& d_out, const Rows16& dq, co
 }  // namespace bwd
 
 size_t attn_bwd_ws_bytes(int B, int Hq, int Hkv, int Tq, int Tk, int D, bool gated, bool causal) {
-    const bwd::Plan p = D == 256   ? bwd::plan<256>(B, Hq, Hkv, Tq, Tk, gated, causal)
-                   : D == 128 ? bwd::plan<128>(B, Hq, Hkv, Tq, Tk, gated, causal)
-                              : bwd::plan<64>(B, Hq, Hkv, Tq, Tk, gated, causal);
-    return p.bytes;
+    size_t most = 0;  // with lengths or without
+    for (const bool ragged : {false, true}) {
+        const bwd::Plan p = D == 256   ? bwd::plan<256>(B, Hq, Hkv, Tq, Tk, gated, causal, ragged)
+                            : D == 128 ? bwd::plan<128>(B, Hq, Hkv, Tq, Tk, gated, causal, ragged)
+                                       : bwd::plan<64>(B, Hq, Hkv, Tq, Tk, gated, causal, ragged);
+        most = std::max(most, p.bytes);
+    }
+    return most;
 }
 
 hipError_t attn_bwd(const AttnRows& x, const Rows16& d_out, const Rows16& dq, const Rows16& dk, const Rows16& dv, const Rows16& dgate,
