@@ -393,7 +393,7 @@ int tsa_rope_freqs(const tsa_rope_params* params, uint64_t* freq, float* amp);
 typedef struct tsa_rope_plan {
     const uint64_t* freq; /* on the device */
     float amp;
-    int rot;         /* even, 2 .. D; multiples of 16 are read 16 bytes at a time, others pair by pair */
+    int rot;         /* even, 2 .. D; loads are as wide as rot allows, 16 bytes of fp16 at multiples of 16 */
     int interleaved; /* 0 or 1 */
 } tsa_rope_plan;
 

@@ -7,10 +7,13 @@
 // distance from the nearest quarter turn, at most an eighth, then becomes a float, and sine and
 // cosine are their power series to x^9 and x^10 (rest below 2.5e-9 at pi / 4).
 //
-// Bound by memory: every element is read and written once.  A thread keeps the sines and cosines of
-// kVec pairs of one token and walks over some of its heads, so they cost a fraction of a head's
-// loads and stores (kVec = 8: two 16-byte loads of fp16).
+// Bound by memory: every element is read and written once.  A workgroup takes some tokens of all heads (or a
+// share of them): it makes the sines and cosines of their pairs once, one a thread, and leaves them in
+// LDS; then a thread turns kVec pairs of a head at a time (kVec = 8: two 16-byte loads of fp16).  Neighbouring
+// threads go over a row, then over what lies next to it in memory, tokens or heads.
 #pragma once
+#include <algorithm>
+
 #include "common.h"
 #include "kernels.h"
 
@@ -50,7 +53,9 @@ struct RopeArgs {
     const unsigned long long* freq;
     const int *pos, *len, *n_new;
     float amp;
-    int Hq, H, B, T, rot, units, per, flip;  // H: heads of q and k; units a row; heads a thread; flip: turn back
+    // H: heads of q and k; units a row; tokens, and items (units of all their rows), a workgroup column;
+    // share: items a workgroup; flip: turn back; heads_next: a token's heads lie side by side
+    int Hq, H, B, T, rot, units, tokens, items, share, flip, heads_next;
 };
 
 // kVec pairs: interleaved in x then y, or their first elements in x and their second in y.
@@ -69,68 +74,93 @@ __device__ __forceinline__ void rotate(T (&x)[kVec], T (&y)[kVec], const float (
     for (int i = 0; i < kVec; ++i) x[i] = e[kInter ? i : 2 * i], y[i] = e[kInter ? kVec + i : 2 * i + 1];
 }
 
+constexpr int kThreads = 256, kAtOnce = 4, kAngles = 512;  // angles a workgroup makes at most: tokens rot / 2
+
 // Unit u of a row: pairs u kVec .. + kVec - 1 while those are below rot / 2, then the elements behind
 // the rotated ones, 2 kVec at a time (only where they have to be copied: out of place).
-constexpr int kAtOnce = 4;
 template <typename T, bool kInter, int kVec>
-__global__ void __launch_bounds__(256) rope_kernel(RopeArgs a) {
-    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
-    const int u = (int)(at % a.units);
-    const long long row = at / a.units;  // (sequence, token)
-    if (row >= (long long)a.B * a.T) return;
-    const int b = (int)(row / a.T), t = (int)(row % a.T);
-    const int n = a.n_new ? min(max(a.n_new[b], 0), a.T) : a.T;
-    if (t >= n) return;
-    const bool turn = u * 2 * kVec < a.rot;
-    float s[kVec], c[kVec];
-    if (turn) {
-        const long long p = a.pos ? (long long)a.pos[row] : (a.len ? (long long)a.len[b] - n : 0) + t;
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-            sincos_turns((unsigned long long)p * a.freq[u * kVec + i], s[i], c[i]);
-            s[i] *= a.flip ? -a.amp : a.amp;
-            c[i] *= a.amp;
+__global__ void __launch_bounds__(kThreads) rope_kernel(RopeArgs a) {
+    __shared__ __align__(16) float sines[kAngles], cosines[kAngles];
+    const int tid = threadIdx.x, half = a.rot / 2;
+    const long long row0 = (long long)blockIdx.x * a.tokens, rows = (long long)a.B * a.T;
+    // Row r of the column, if it is a token (not padding, nor past the last).
+    auto token = [&](int r, int& b, int& t, int& n) {
+        const long long row = row0 + r;
+        if (row >= rows) return false;
+        b = (int)((unsigned)row / (unsigned)a.T);  // (rows of all sequences fit an int)
+        t = (int)((unsigned)row % (unsigned)a.T);
+        n = a.n_new ? min(max(a.n_new[b], 0), a.T) : a.T;
+        return t < n;
+    };
+    for (int i = tid; i < a.tokens * half; i += kThreads) {
+        const int r = (int)((unsigned)i / (unsigned)half), pair = i - r * half;
+        int b, t, n;
+        if (token(r, b, t, n)) {
+            const long long p = a.pos ? (long long)a.pos[row0 + r] : (a.len ? (long long)a.len[b] - n : 0) + t;
+            float s, c;
+            sincos_turns((unsigned long long)p * a.freq[pair], s, c);
+            sines[i] = s * (a.flip ? -a.amp : a.amp);
+            cosines[i] = c * a.amp;
         }
     }
-    const int lo = kInter || !turn ? u * 2 * kVec : u * kVec;  // the unit's elements: kVec at lo, kVec at up
-    const int up = kInter || !turn ? lo + kVec : lo + a.rot / 2;
-    const int h0 = blockIdx.y * a.per, h1 = min(h0 + a.per, a.H);
+    __syncthreads();
     using P = Pack<T, kVec>;
-    auto rows = [&](int h, const T*& src, T*& dst) {
-        const bool is_q = h < a.Hq;
-        const RopeTensor& x = is_q ? a.q : a.k;
-        const int hh = is_q ? h : h - a.Hq;
-        src = static_cast<const T*>(x.in) + b * x.in_b + hh * x.in_h + t * x.in_t;
-        dst = static_cast<T*>(x.out) + b * x.out_b + hh * x.out_h + t * x.out_t;
-    };
-    // kAtOnce heads' loads on their way together
-    for (int h = h0; h < h1; h += kAtOnce) {
+    const int end = min(a.items, (int)(blockIdx.y + 1) * a.share);
+    // kAtOnce units' loads on their way together
+    for (int i0 = blockIdx.y * a.share + tid; i0 < end; i0 += kThreads * kAtOnce) {
         P v[kAtOnce][2];
-        T* dst[kAtOnce];
+        T *lo[kAtOnce], *up[kAtOnce];
+        int angle[kAtOnce];  // of the unit's first pair; -1: copied, -2: nothing there
 #pragma unroll
-        for (int i = 0; i < kAtOnce; ++i)
-            if (h + i < h1) {
-                const T* src;
-                rows(h + i, src, dst[i]);
-                v[i][0] = *reinterpret_cast<const P*>(src + lo);
-                v[i][1] = *reinterpret_cast<const P*>(src + up);
-            }
+        for (int j = 0; j < kAtOnce; ++j) {
+            const int i = i0 + j * kThreads;
+            angle[j] = -2;
+            if (i >= end) continue;
+            const int x = (int)((unsigned)i / (unsigned)a.units), u = i - x * a.units;
+            int h, r;
+            if (a.heads_next)
+                r = (int)((unsigned)x / (unsigned)a.H), h = x - r * a.H;
+            else
+                h = (int)((unsigned)x / (unsigned)a.tokens), r = x - h * a.tokens;
+            int b, t, n;
+            if (!token(r, b, t, n)) continue;
+            const bool turn = u * 2 * kVec < a.rot, is_q = h < a.Hq;
+            const RopeTensor& y = is_q ? a.q : a.k;
+            const int hh = is_q ? h : h - a.Hq;
+            // the unit's elements: kVec at e0, kVec at e1
+            const int e0 = kInter || !turn ? u * 2 * kVec : u * kVec, e1 = kInter || !turn ? e0 + kVec : e0 + half;
+            const T* src = static_cast<const T*>(y.in) + b * y.in_b + hh * y.in_h + t * y.in_t;
+            T* dst = static_cast<T*>(y.out) + b * y.out_b + hh * y.out_h + t * y.out_t;
+            v[j][0] = *reinterpret_cast<const P*>(src + e0);
+            v[j][1] = *reinterpret_cast<const P*>(src + e1);
+            lo[j] = dst + e0, up[j] = dst + e1;
+            angle[j] = turn ? r * half + u * kVec : -1;
+        }
 #pragma unroll
-        for (int i = 0; i < kAtOnce; ++i)
-            if (h + i < h1) {
-                if (turn) rotate<T, kInter, kVec>(v[i][0].x, v[i][1].x, s, c);
-                *reinterpret_cast<P*>(dst[i] + lo) = v[i][0];
-                *reinterpret_cast<P*>(dst[i] + up) = v[i][1];
+        for (int j = 0; j < kAtOnce; ++j) {
+            if (angle[j] == -2) continue;
+            if (angle[j] >= 0) {
+                float s[kVec], c[kVec];
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) s[e] = sines[angle[j] + e], c[e] = cosines[angle[j] + e];
+                rotate<T, kInter, kVec>(v[j][0].x, v[j][1].x, s, c);
             }
+            *reinterpret_cast<P*>(lo[j]) = v[j][0];
+            *reinterpret_cast<P*>(up[j]) = v[j][1];
+        }
     }
 }
 
 template <typename T, bool kInter>
-hipError_t launch_rope(RopeArgs& a, const dim3& grid, bool wide, hipStream_t stream) {
-    if (wide)
-        hipLaunchKernelGGL((rope_kernel<T, kInter, 8>), grid, dim3(256), 0, stream, a);
+hipError_t launch_rope(const RopeArgs& a, const dim3& grid, int vec, hipStream_t stream) {
+    if (vec == 8)
+        hipLaunchKernelGGL((rope_kernel<T, kInter, 8>), grid, dim3(kThreads), 0, stream, a);
+    else if (vec == 4)
+        hipLaunchKernelGGL((rope_kernel<T, kInter, 4>), grid, dim3(kThreads), 0, stream, a);
+    else if (vec == 2)
+        hipLaunchKernelGGL((rope_kernel<T, kInter, 2>), grid, dim3(kThreads), 0, stream, a);
     else
-        hipLaunchKernelGGL((rope_kernel<T, kInter, 1>), grid, dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((rope_kernel<T, kInter, 1>), grid, dim3(kThreads), 0, stream, a);
     return hipGetLastError();
 }
 
@@ -143,20 +173,25 @@ RopeTensor tensor(const RopeRows& in, const RopeRows& out) {
 hipError_t rope(const unsigned long long* freq, float amp, int rot, int interleaved, int f32, const RopeRows& q,
                 const RopeRows& q_out, int Hq, const RopeRows& k, const RopeRows& k_out, int Hk, const int* pos,
                 const int* len, const int* n_new, int B, int T, int D, int back, hipStream_t stream) {
-    // 16-byte loads need rows whose pairs come in eights
-    const bool wide = rot % 16 == 0;
+    // the widest loads that the rotated part's halves allow (16 bytes of fp16 where rot is a multiple of 16)
+    const int vec = rot % 16 == 0 ? 8 : rot % 8 == 0 ? 4 : rot % 4 == 0 ? 2 : 1;
     // elements that do not turn are copied unless every tensor is rotated in place
     const bool copy = rot < D && (q.data != q_out.data || (Hk && k.data != k_out.data));
-    const int H = Hq + Hk, units = (copy ? D : rot) / (wide ? 16 : 2);
-    const long long threads = (long long)B * T * units;
-    // heads a thread: one where that does not fill the device, else 8 to share the sines
-    const long long groups = (threads + 255) / 256;
-    const int per = groups * H <= 2048 ? 1 : groups * H <= 8192 ? 4 : 8;
-    const dim3 grid((unsigned)groups, (unsigned)((H + per - 1) / per));
-    RopeArgs a = {tensor(q, q_out), tensor(k, k_out), freq, pos, len, n_new, amp, Hq, H, B, T, rot, units, per, back};
+    RopeArgs a = {tensor(q, q_out), tensor(k, k_out), freq, pos, len, n_new, amp, Hq, Hq + Hk, B, T, rot, (copy ? D : rot) / (2 * vec)};
+    const long long rows = (long long)B * T;
+    // tokens of a workgroup: two units a thread, at most 256 angles, and 512 workgroups where there are the rows
+    a.tokens = (int)std::max<long long>(1, std::min<long long>({512 / (a.H * a.units), 512 / rot, rows / 512}));
+    a.items = a.tokens * a.H * a.units;
+    a.flip = back;
+    a.heads_next = q.h < q.t && T > 1;
+    // one workgroup a column of tokens where there are enough of them; else its items are dealt out, a unit a thread at least
+    const long long columns = (rows + a.tokens - 1) / a.tokens, most = (a.items + kThreads - 1) / kThreads;
+    const long long deal = std::max(1LL, std::min({most, 1024 / columns, 65535LL}));
+    a.share = (int)((most + deal - 1) / deal) * kThreads;
+    const dim3 grid((unsigned)columns, (unsigned)((a.items + a.share - 1) / a.share));
     if (f32)
-        return interleaved ? launch_rope<float, true>(a, grid, wide, stream) : launch_rope<float, false>(a, grid, wide, stream);
-    return interleaved ? launch_rope<half_t, true>(a, grid, wide, stream) : launch_rope<half_t, false>(a, grid, wide, stream);
+        return interleaved ? launch_rope<float, true>(a, grid, vec, stream) : launch_rope<float, false>(a, grid, vec, stream);
+    return interleaved ? launch_rope<half_t, true>(a, grid, vec, stream) : launch_rope<half_t, false>(a, grid, vec, stream);
 }
 
 }  // namespace tsa

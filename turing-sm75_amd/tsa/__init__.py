@@ -783,22 +783,24 @@ class Rope:
         self._ref = ctypes.byref(self.view)
 
 
+_pack_rows = _ROWS.pack
+_tensor = None  # torch.Tensor, once torch is there
+
+
 def _rows_on(t, shape, name, index, dtype):
     """A [B, H, T, D] tensor on GPU `index` as a tsa_rows: rows of consecutive elements, any other strides."""
-    if not isinstance(t, (_torch or _t()).Tensor):
+    if t.__class__ is not _tensor and not isinstance(t, (_torch or _t()).Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if t.dtype is dtype and t.get_device() == index and t.shape == shape:  # (index is a GPU's: not -1)
+    if t.dtype is dtype and t.shape == shape and t.get_device() == index:  # (index is a GPU's: not -1)
         b, h, r, d = t.stride()
         if d == 1:
-            return _ROWS.pack(t.data_ptr(), b, h, r)
+            return _pack_rows(t.data_ptr(), b, h, r)
     raise ValueError(f"{name}: expected {dtype} {tuple(shape)} on GPU {index} with consecutive row elements, got "
                      f"{tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}")
 
 
 def _ints_on(t, shape, name, index):
-    """A contiguous int32 tensor on GPU `index`, or None."""
-    if t is None:
-        return None
+    """A contiguous int32 tensor on GPU `index`."""
     torch = _torch or _t()
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
@@ -833,36 +835,42 @@ def _new_like(x, padded, stream):
 
 
 def _four(t, name):
-    if not isinstance(t, (_torch or _t()).Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor")
-    if t.dim() != 4 or not t.is_cuda:
-        raise ValueError(f"{name}: expected a 4-d tensor on a GPU, got {tuple(t.shape)} on {t.device}")
-    return t.shape
+    global _tensor
+    if t.__class__ is not _tensor:
+        _tensor = (_torch or _t()).Tensor
+        if not isinstance(t, _tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+    shape = t.shape
+    if shape.__len__() != 4 or not t.is_cuda:
+        raise ValueError(f"{name}: expected a 4-d tensor on a GPU, got {tuple(shape)} on {t.device}")
+    return shape
 
 
 def _rope(rope, q, k, pos, len, n_new, q_out, k_out, back, stream):
     torch = _torch or _t()
-    B, Hq, T, D = _four(q, "q")
-    if q.dtype is not torch.float16 and q.dtype is not torch.float32:
-        raise ValueError(f"q: expected fp16 or fp32, got {q.dtype}")
+    q_shape = B, Hq, T, D = _four(q, "q")
+    i, dtype = rope.index, q.dtype
+    if dtype is not torch.float16 and dtype is not torch.float32:
+        raise ValueError(f"q: expected fp16 or fp32, got {dtype}")
     if D != rope.D:
         raise ValueError(f"q has heads of {D} elements, the rotation {rope.D}")
-    i, dtype = rope.index, q.dtype
-    q_in = _rows_on(q, q.shape, "q", i, dtype)
+    q_in = _rows_on(q, q_shape, "q", i, dtype)
     if k is None:
         if k_out is not None:
             raise ValueError("k_out without k")
         Hk, k_in = 0, None
     else:
         Hk = _four(k, "k")[1]
-        k_in = _rows_on(k, (B, Hk, T, D), "k", i, dtype)
-    at = _ints_on(pos, (B, T), "pos", i), _ints_on(len, (B,), "len", i), _ints_on(n_new, (B,), "n_new", i)
-    q_out = _new_like(q, n_new is not None, stream) if q_out is None else q_out
-    if k is not None and k_out is None:
-        k_out = _new_like(k, n_new is not None, stream)
-    _call_on(load().tsa_rope, i, stream, rope._ref, TSA_TYPE_F32 if dtype is torch.float32 else TSA_TYPE_F16, q_in,
-             _rows_on(q_out, q.shape, "q_out", i, dtype), Hq, k_in, None if k is None else _rows_on(k_out, k.shape, "k_out", i, dtype),
-             Hk, *at, B, T, D, back)
+        k_shape = (B, Hk, T, D)
+        k_in = _rows_on(k, k_shape, "k", i, dtype)
+        if k_out is None:
+            k_out = _new_like(k, n_new is not None, stream)
+    if q_out is None:
+        q_out = _new_like(q, n_new is not None, stream)
+    _call_on((_lib or load()).tsa_rope, i, stream, rope._ref, TSA_TYPE_F32 if dtype is torch.float32 else TSA_TYPE_F16, q_in,
+             _rows_on(q_out, q_shape, "q_out", i, dtype), Hq, k_in, None if k is None else _rows_on(k_out, k_shape, "k_out", i, dtype),
+             Hk, None if pos is None else _ints_on(pos, (B, T), "pos", i), None if len is None else _ints_on(len, (B,), "len", i),
+             None if n_new is None else _ints_on(n_new, (B,), "n_new", i), B, T, D, back)
     return q_out, k_out
 
 
@@ -886,7 +894,8 @@ def _train_shapes(q, k, v, gate, len_q, len_k):
     i, half = q.get_device(), torch.float16
     views = (_rows_on(q, q.shape, "q", i, half), _rows_on(k, (B, Hkv, Tk, D), "k", i, half), _rows_on(v, (B, Hkv, Tk, D), "v", i, half),
              None if gate is None else _rows_on(gate, q.shape, "gate", i, half))
-    return views, (_ints_on(len_q, (B,), "len_q", i), _ints_on(len_k, (B,), "len_k", i)), (B, Hq, Hkv, Tq, Tk, D)
+    lens = (None if len_q is None else _ints_on(len_q, (B,), "len_q", i), None if len_k is None else _ints_on(len_k, (B,), "len_k", i))
+    return views, lens, (B, Hq, Hkv, Tq, Tk, D)
 
 
 def _stat(lse, shape, name, index):
@@ -913,7 +922,7 @@ def attn_train_fwd(q, k, v, gate=None, len_q=None, len_k=None, out=None, lse=Non
     if lse is None:
         with torch.cuda.stream(torch.cuda.current_stream(q.device) if stream is None else stream):
             lse = torch.zeros(B, Hq, Tq, dtype=torch.float32, device=q.device)
-    _call_on(load().tsa_attn_train_fwd, i, stream, *views, op, _stat(lse, (B, Hq, Tq), "lse", i), *lens, B, Hq, Hkv, Tq, Tk, D,
+    _call_on((_lib or load()).tsa_attn_train_fwd, i, stream, *views, op, _stat(lse, (B, Hq, Tq), "lse", i), *lens, B, Hq, Hkv, Tq, Tk, D,
              1.0 / math.sqrt(D) if scale is None else float(scale), 1 if causal else 0)
     return out, lse
 
@@ -946,6 +955,6 @@ def attn_bwd(d_out, q, k, v, out, lse, gate=None, len_q=None, len_k=None, dq=Non
         ws = _scratch(attn_bwd_workspace_bytes(B, Hq, Hkv, Tq, Tk, D, gate is not None, causal), q.device, stream)
     elif not ws.is_cuda or ws.get_device() != i or not ws.is_contiguous():
         raise ValueError(f"ws: expected a contiguous tensor on GPU {i}, got one on {ws.device}")
-    _call_on(load().tsa_attn_bwd, i, stream, gp, *views, op, lp, *grads, *lens, B, Hq, Hkv, Tq, Tk, D,
+    _call_on((_lib or load()).tsa_attn_bwd, i, stream, gp, *views, op, lp, *grads, *lens, B, Hq, Hkv, Tq, Tk, D,
              1.0 / math.sqrt(D) if scale is None else float(scale), 1 if causal else 0, _ptr(ws), ws.numel() * ws.element_size())
     return dq, dk, dv, dgate
