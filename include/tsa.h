@@ -415,8 +415,10 @@ int tsa_rope(const tsa_rope_plan* plan, int type, const tsa_rows* q, const tsa_r
  * sequence's rows; the rows behind them are padding that is neither read nor written, in any
  * tensor.  The queries are the last tokens: under the causal mask query t sees the keys
  * j <= t + len_k - len_q.  lse [B][Hq][Tq] fp32 gets log(sum_j exp(scale * q.k_j)); a query that sees
- * no key has o = 0 and lse = -infinity, and its gradients are 0.  A stride_t is at most 2^24
- * elements, and outputs lie on no input. ---- */
+ * no key has o = 0 and lse = -infinity, and its gradients are 0.  An infinity or NaN of a token reaches
+ * what sees it (a key's the queries behind it, a query's the keys in front of it; there it may make
+ * NaN of whole rows) and nothing that the mask or the lengths hide it from.  A stride_t is at most
+ * 2^24 elements, and outputs lie on no input. ---- */
 int tsa_attn_train_fwd(const tsa_rows* q, const tsa_rows* k, const tsa_rows* v, const tsa_rows* gate, const tsa_rows* o,
                        float* lse, const int32_t* len_q, const int32_t* len_k, int B, int Hq, int Hkv, int Tq, int Tk,
                        int D, float scale, int causal, void* stream);

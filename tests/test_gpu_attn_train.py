@@ -288,3 +288,66 @@ def test_whole_layer(dev):
     for got, x in ((xq, dq), (xk, dk)):
         y = orc.rotate(x, pos, f, amp, False, back=True)
         within("rotated back", got, y, orc.rotate_bound(x, y, pos, f, amp, False) + 2.0 ** -25, n)
+
+
+NO_NUMBERS = [math.nan, math.inf, -math.inf]
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("Tq,Tk,at", [(200, 200, 100), (150, 187, 186), (70, 70, 33), (513, 513, 480), (90, 40, 20), (1100, 1100, 1000)])
+@pytest.mark.parametrize("where", ["k", "v"])
+def test_no_numbers_in_a_hidden_key(dev, D, Tq, Tk, at, where):
+    """A token's infinity or NaN reaches the queries that see it, and no others: not o, lse or dq of queries
+    in front of it, which the mask hides it from."""
+    q, k, v, gate, do = make(dev, 14, 1, 2, 1, Tq, Tk, D, True)
+    want_o, want_l, bo, bl = orc.forward(q, k, v, gate)
+    clean = tsa.attn_train_fwd(q, k, v, gate)
+    want, bound = orc.backward(do, q, k, v, *clean, gate)
+    x = {"k": k, "v": v}[where]
+    for i, bad in enumerate(NO_NUMBERS):
+        kept = x[:, :, at].clone()
+        x[:, :, at, (5 + 7 * i) % D] = bad
+        o, lse = tsa.attn_train_fwd(q, k, v, gate)
+        dq = tsa.attn_bwd(do, q, k, v, o, lse, gate)[0]
+        x[:, :, at] = kept
+        before = max(0, at - (Tk - Tq))  # queries in front of the token
+        rows = slice(0, before)
+        assert ((o.double() - want_o).abs() <= bo)[:, :, rows].all()
+        seen = torch.isfinite(want_l[:, :, rows])
+        assert ((lse.double() - want_l).abs()[:, :, rows] <= (bl + 2.0 ** -22 * want_l.abs())[:, :, rows])[seen].all()
+        # (o of these rows may differ in its last bit from the clean call's, and d with it: twice the bound, and that of d)
+        slack = 2.0 ** -10 * (do.double() * clean[0].double()).abs().sum(-1, keepdim=True) * k.double().abs().amax() / math.sqrt(D)
+        assert ((dq.double() - want["dq"]).abs() <= 2 * bound["dq"] + slack)[:, :, rows].all()
+        # what sees it: an infinite key's score is minus infinity where the query has the other sign there, a
+        # weight of 0, so only the others' rows hold no number
+        hit = torch.ones(1, 2, Tq, dtype=torch.bool, device=dev)
+        if where == "k" and not math.isnan(bad):
+            hit = q[..., (5 + 7 * i) % D].double() * bad > 0
+        hit[:, :, rows] = False
+        assert (~torch.isfinite(o)).any(-1)[hit].all()
+        assert (~torch.isfinite(dq)).any(-1)[hit].all()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("Tq,Tk,at", [(200, 200, 100), (150, 187, 3), (70, 70, 33), (513, 513, 500), (90, 40, 70), (1100, 1100, 40)])
+@pytest.mark.parametrize("where", ["q", "do"])
+def test_no_numbers_in_a_query(dev, D, Tq, Tk, at, where):
+    """A query's (or its gradient's) infinity or NaN reaches the keys that it sees, and no others."""
+    q, k, v, gate, do = make(dev, 15, 1, 2, 1, Tq, Tk, D, False)
+    clean = tsa.attn_train_fwd(q, k, v)
+    want, bound = orc.backward(do, q, k, v, *clean)
+    # without the row at all: what keys in front of it get from the others is not looked at
+    x = {"q": q, "do": do}[where]
+    for i, bad in enumerate(NO_NUMBERS):
+        kept = x[:, :, at].clone()
+        x[:, :, at, (3 + 11 * i) % D] = bad
+        o, lse = tsa.attn_train_fwd(q, k, v)
+        dq, dk, dv, _ = tsa.attn_bwd(do, q, k, v, o, lse)
+        x[:, :, at] = kept
+        first = max(0, at + (Tk - Tq) + 1)  # the first key that the query does not see
+        for name, got in (("dk", dk), ("dv", dv)):
+            assert ((got.double() - want[name]).abs() <= bound[name])[:, :, first:].all(), name
+            assert first == 0 or (~torch.isfinite(got[:, :, :first])).any(-1).all(), name
+        others = torch.arange(Tq, device=dev) != at
+        assert ((dq.double() - want["dq"]).abs() <= bound["dq"])[:, :, others].all()
+        assert (~torch.isfinite(dq[:, :, at])).any() or first == 0

@@ -32,8 +32,8 @@ constexpr int kBlk = 32;  // rows and keys of a step
 struct BwdArgs {
     Rows16 q, k, v, g /* dO, gated */, dq, dk, dv;
     const float* stat;     // [B][Hq][n_qb][64]: L log2(e) of 32 rows (inf: no such row, or it sees no key), then -d
-    const float2* row_max; // [B][Hq][n_qb]: the largest |dO_i| and |d_i| of 32 rows
-    const float* key_max;  // [B][Hkv][n_kb]: the largest |v_j| of 32 keys
+    const float2* row_max; // [B][Hq][n_qb]: the largest |dO_i| and |d_i| of 32 rows; the second below 0: one is bad
+    const float* key_max;  // [B][Hkv][n_kb]: the largest |v_j| of 32 keys; below 0: a bad k_j among them
     float* part;           // split key tiles: fp32 sums of each part
     const int *len_q, *len_k;
     int B, Hq, Hkv, Tq, Tk, n_qb, n_kb, n_kt, n_part, n_qt, n_kv;  // n_kt, n_qt: tiles; n_kv: workgroups of the key tiles
@@ -52,11 +52,19 @@ __device__ __forceinline__ int count(const int* len, int b, int most) {
     return len ? min(max(len[b], 0), most) : most;
 }
 
+// Infinities and NaN reach what sees them and nothing else.  In the products themselves a pair that the
+// mask hides has a weight of 0, but 0 times an infinity is NaN.  So a causal call's workgroups that
+// meet a bad row (one whose dO or statistic is none, or, for dQ, whose key is none) copy their tiles through registers and
+// put 0 for what is no number there; what sees the row gets its NaN from P, whose statistic is NaN
+// (a bad key's queries have such statistics from the forward pass).
+constexpr float kBad = 1e-30f;  // added below 0, so that a bound of 0 shows the mark too
+__device__ __forceinline__ bool finite16(half_t x) { return __builtin_fabsf((float)x) < INFINITY; }
+
 // ---------------------------------------------------------------------------------------
 // Row statistics: a workgroup takes 32 rows of dO' and o' (8 lanes a row), or 32 keys' values.
 // ---------------------------------------------------------------------------------------
 struct RowsArgs {
-    Rows16 g, o, gate, v, dgate;
+    Rows16 g, o, gate, k, v, dgate;  // k: null without a mask
     half_t* gated;  // dO [B][Hq][Tq][D], with a gate
     const float* lse;
     float* stat;
@@ -115,42 +123,54 @@ __global__ void __launch_bounds__(256) attn_bwd_rows_kernel(RowsArgs a) {
         if (l8 == 0) {
             float* st = a.stat + (size_t)blk * 64;
             const float lse = t < n ? a.lse[(size_t)bh * a.Tq + t] : -INFINITY;
-            st[r] = lse == -INFINITY ? INFINITY : lse * kLog2e;
+            const bool bad = !(n2 < INFINITY) || !(lse < INFINITY);
+            st[r] = bad ? NAN : lse == -INFINITY ? INFINITY : lse * kLog2e;
             st[32 + r] = -d;
-            most[r] = make_float2(sqrtf(n2), fabsf(d));
+            // (a bad row, or one with no d, is left out of the bound: its results are NaN at any scale)
+            most[r] = bad ? make_float2(0.f, -kBad) : make_float2(sqrtf(n2), fabsf(d) < INFINITY ? fabsf(d) : 0.f);
         }
         __syncthreads();
-        if (threadIdx.x < 64) {  // (NaN rows give NaN results whatever the scale)
+        if (threadIdx.x < 64) {
             float2 m = most[threadIdx.x & 31];
+            const bool bad = __builtin_amdgcn_ballot_w64(m.y < 0.f) != 0;
 #pragma unroll
             for (int s = 16; s; s >>= 1) {
                 m.x = fmaxf(m.x, __shfl_xor(m.x, s));
                 m.y = fmaxf(m.y, __shfl_xor(m.y, s));
             }
-            if (threadIdx.x == 0) a.row_max[blk] = m;
+            if (threadIdx.x == 0) a.row_max[blk] = make_float2(m.x, bad ? -fmaxf(m.y, 0.f) - kBad : m.y);
         }
     } else {
         blk -= a.n_rows;
         const int bh = blk / a.n_kb, kb = blk % a.n_kb, b = bh / a.Hkv, h = bh % a.Hkv;
         const int t = kb * kBlk + r;
-        float n2 = 0.f;
+        float n2 = 0.f, k2 = 0.f;
         if (t < count(a.len_k, b, a.Tk)) {
             const half_t* v = a.v.data + b * a.v.b + h * a.v.h + t * a.v.t;
+            const half_t* k = a.k.data ? a.k.data + b * a.k.b + h * a.k.h + t * a.k.t : nullptr;
 #pragma unroll
             for (int i = 0; i < D / 64; ++i) {
                 const half8_t x = *reinterpret_cast<const half8_t*>(v + 8 * l8 + 64 * i);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) n2 = fmaf((float)x[j], (float)x[j], n2);
+                if (k) {
+                    const half8_t y = *reinterpret_cast<const half8_t*>(k + 8 * l8 + 64 * i);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) k2 = fmaf((float)y[j], (float)y[j], k2);
+                }
             }
         }
         n2 = sum8(n2);
-        if (l8 == 0) most[r].x = sqrtf(n2);
+        k2 = sum8(k2);
+        // (a value that is none is left out of the bound; its queries' d is none either)
+        if (l8 == 0) most[r] = make_float2(n2 < INFINITY ? sqrtf(n2) : 0.f, k2 < INFINITY ? 0.f : -1.f);
         __syncthreads();
         if (threadIdx.x < 64) {
-            float m = most[threadIdx.x & 31].x;
+            float2 m = most[threadIdx.x & 31];
+            const bool bad = __builtin_amdgcn_ballot_w64(m.y < 0.f) != 0;
 #pragma unroll
-            for (int s = 16; s; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
-            if (threadIdx.x == 0) a.key_max[blk] = m;
+            for (int s = 16; s; s >>= 1) m.x = fmaxf(m.x, __shfl_xor(m.x, s));
+            if (threadIdx.x == 0) a.key_max[blk] = bad ? -m.x - kBad : m.x;
         }
     }
 }
@@ -188,6 +208,15 @@ __device__ __forceinline__ float range_ref(float bound) {
     return (float)min(15, 14 - e);
 }
 
+__device__ __forceinline__ void lds_write_b128(unsigned addr, const half8_t& x) {
+    typedef __attribute__((address_space(3))) half8_t* p_t;
+    *(p_t)(addr) = x;
+}
+__device__ __forceinline__ float4_t lds_read_f4(unsigned addr) {
+    typedef __attribute__((address_space(3))) const float4_t* p_t;
+    return *(p_t)(addr);
+}
+
 // Copies of tiles of 32 rows of D elements by kN waves, 1 KiB an instruction.  The swizzle of a
 // block's rows repeats every kPeriod blocks; a wave takes kPat neighbouring blocks and those a multiple of kPeriod
 // on, so one offset a lane and tensor serves all of them, with a difference in the odd ones.
@@ -207,11 +236,23 @@ struct Copy {
     // This lane's offset from a tile's first row; stride in bytes, at most 2^25.
     __device__ __forceinline__ unsigned offset(int lane, unsigned stride) const { return (unsigned)row(lane) * stride + col(lane); }
     // p: the tile's first row; last: the last row there is, counted from it.
-    __device__ __forceinline__ void operator()(const char* p, unsigned stride, unsigned off, int last, int lane, unsigned lds) const {
+    __device__ __forceinline__ void operator()(const char* p, unsigned stride, unsigned off, int last, int lane, unsigned lds,
+                                               bool clean = false) const {
         lds += 1024u * (unsigned)(kPat * w);
         int l = lane;  // (what is made of it is not held from copy to copy)
         asm volatile("" : "+v"(l));
-        if (last >= kBlk - 1) {
+        if (clean) {  // through registers, with 0 for what is no number
+            const int r = row(l);
+            const unsigned c = col(l);
+#pragma unroll 1
+            for (int k = 0; k < kPer * kPat; ++k) {
+                const int blk = kNext * (k / kPat) + k % kPat;
+                half8_t x = *reinterpret_cast<const half8_t*>(p + (size_t)stride * (unsigned)min(r + kRows * blk, last) + (k % kPat ? c ^ kFlip : c));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = finite16(x[e]) ? x[e] : (half_t)0.f;
+                lds_write_b128(lds + 1024u * (unsigned)blk + 16u * (unsigned)l, x);
+            }
+        } else if (last >= kBlk - 1) {
             const unsigned delta = (col(l) ^ kFlip) - col(l);
 #pragma unroll
             for (int j = 0; j < kPer; ++j)
@@ -341,15 +382,6 @@ __device__ __forceinline__ half8_t times(const half8_t& p, const float16_t& x, i
     return y;
 }
 
-__device__ __forceinline__ void lds_write_b128(unsigned addr, const half8_t& x) {
-    typedef __attribute__((address_space(3))) half8_t* p_t;
-    *(p_t)(addr) = x;
-}
-__device__ __forceinline__ float4_t lds_read_f4(unsigned addr) {
-    typedef __attribute__((address_space(3))) const float4_t* p_t;
-    return *(p_t)(addr);
-}
-
 // Lane-constant LDS addresses of operand reads in a tile at byte 0.
 template <int D>
 struct OpAddr {
@@ -471,13 +503,28 @@ __device__ __forceinline__ void kv_tile(args_t a, half_t* lds, int wg) {
     const long long q_jump = 2 * a->q.h - (long long)q_row * kBlk * pl.per, g_jump = 2 * a->g.h - (long long)g_row * kBlk * pl.per;
     const int s_jump = 64 * (a->n_qb - pl.per);
     unsigned ring = 0, ring2 = 0;  // stages of the current step and of the next copies
+    // the scale of P and dS is the workgroup's bound
+    float most_g = 0.f, most_d = 0.f, most_v = 0.f;
+    bool some_bad = false;
+    auto row_most = [&](int u) {
+        const float2 m = a->row_max[(size_t)(b * a->Hq + hk * G + u / pl.per) * a->n_qb + pl.first + u % pl.per];
+        most_g = fmaxf(most_g, m.x);
+        most_d = fmaxf(most_d, fabsf(m.y));
+        if (m.y < 0.f) some_bad = true;
+    };
+    for (int u = u0 + lane; u < u1; u += 64) row_most(u);
+    {
+        const int kb = kt * (T::kKeys / kBlk) + lane;
+        if (lane < T::kKeys / kBlk && kb < a->n_kb) most_v = fabsf(a->key_max[(size_t)bh * a->n_kb + kb]);
+    }
+    const bool bad = kCausal && __builtin_amdgcn_ballot_w64(some_bad) != 0;
     // (by the second role: the first has the exponentials to do)
     const Copy<D, T::kPairs> copier = {pair};
     const unsigned q_off = copier.offset(lane, q_row), g_off = copier.offset(lane, g_row);
     auto copy = [&] {  // tiles and statistics of a step
         const unsigned st = lds0 + ring2 * T::kStage;
-        copier(qp, q_row, q_off, last - to_copy * kBlk, lane, st);
-        copier(gp, g_row, g_off, last - to_copy * kBlk, lane, st + T::kTileB);
+        copier(qp, q_row, q_off, last - to_copy * kBlk, lane, st, kCausal && bad);
+        copier(gp, g_row, g_off, last - to_copy * kBlk, lane, st + T::kTileB, kCausal && bad);
         if (pair == 0) dma_issue_any4(sp, 4u * lane, lds0 + T::kStatAt + ring2 * T::kStatB);
         qp += (size_t)q_row * kBlk, gp += (size_t)g_row * kBlk, sp += 64;
         if (++to_copy == end) to_copy = pl.first, qp += q_jump, gp += g_jump, sp += s_jump;
@@ -487,18 +534,6 @@ __device__ __forceinline__ void kv_tile(args_t a, half_t* lds, int wg) {
     auto hidden = [&](int x) { return kCausal && x * kBlk + kBlk - 1 + pl.last0 < k0; };
 
     if (!role_p && n > 0) copy();
-    // the scale of P and dS is the workgroup's bound; its first loads, and K's or V's, on their way together
-    float most_g = 0.f, most_d = 0.f, most_v = 0.f;
-    auto row_most = [&](int u) {
-        const float2 m = a->row_max[(size_t)(b * a->Hq + hk * G + u / pl.per) * a->n_qb + pl.first + u % pl.per];
-        most_g = fmaxf(most_g, m.x);
-        most_d = fmaxf(most_d, m.y);
-    };
-    if (u0 + lane < u1) row_most(u0 + lane);
-    {
-        const int kb = kt * (T::kKeys / kBlk) + lane;
-        if (lane < T::kKeys / kBlk && kb < a->n_kb) most_v = a->key_max[(size_t)bh * a->n_kb + kb];
-    }
     // K or V of the pair's keys, as B operands: slot s of k-step kk is row[16 kk + 8 hi + s]
     half8_t frag[T::kKB][kKK];
     {
@@ -512,11 +547,13 @@ __device__ __forceinline__ void kv_tile(args_t a, half_t* lds, int wg) {
             for (int kk = 0; kk < kKK; ++kk) frag[kb][kk] = *reinterpret_cast<const half8_t*>(row + 16 * kk);
         }
     }
-    for (int u = u0 + 64 + lane; u < u1; u += 64) row_most(u);
     const float ref = range_ref(fmaf(wave_max(most_g), wave_max(most_v), wave_max(most_d)));
 
     // register r of a result is query 4 hi + 8 (r / 4) + r % 4 of the step: hidden below this
-    auto limit = [&](int x, int kb) { return k0 + 32 * kb + (lane & 31) - pl.last0 - x * kBlk - 4 * hi; };
+    auto limit = [&](int x, int kb) {
+        const int l = again(lane);
+        return k0 + 32 * kb + (l & 31) - pl.last0 - x * kBlk - 4 * (l >> 5);
+    };
     auto partly = [&](int x, int kb) { return kCausal && k0 + 32 * kb + 31 > x * kBlk + pl.last0; };
     if constexpr (role_p) {
         // round i: S of step i, then its P beside dV of step i - 1, while step i + 1 is copied.  P goes to LDS, for the
@@ -574,6 +611,17 @@ __device__ __forceinline__ void kv_tile(args_t a, half_t* lds, int wg) {
 #pragma unroll
                 for (int x = 0; x < 16 * T::kKB; ++x) soft(x);
             }
+            if (kCausal && bad && scores)  // a bad row's P is NaN where it is hidden too
+#pragma unroll 1
+                for (int x = 0; x < 2 * T::kKB; ++x)
+                    if (partly(qb, x >> 1)) {
+                        const int lim = limit(qb, x >> 1) - 16 * (x & 1);
+                        half8_t y = lds_read_b128(p_new + (unsigned)x * 1024u);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (8 * (e >> 2) + (e & 3) < lim) y[e] = (half_t)0.f;
+                        lds_write_b128(p_new + (unsigned)x * 1024u, y);
+                    }
             was = qb;
             qb = qb + 1 == end ? pl.first : qb + 1;
         }
@@ -659,16 +707,27 @@ struct QTile {
 };
 
 template <int D>
-__device__ __forceinline__ float q_tile_ref(args_t a, int bh, int bhk, int q0, int q_blocks, int k_blocks, int lane) {
-    float n = 0.f, d = 0.f, v = 0.f;
+__device__ __forceinline__ float q_tile_ref(args_t a, int bh, int q0, int q_blocks, float most_v, int lane) {
+    float n = 0.f, d = 0.f;
     const int qb = q0 / kBlk + lane;
     if (lane < q_blocks && qb < a->n_qb) {
         const float2 m = a->row_max[(size_t)bh * a->n_qb + qb];
         n = m.x;
-        d = m.y;
+        d = fabsf(m.y);
     }
-    for (int i = lane; i < k_blocks; i += 64) v = fmaxf(v, a->key_max[(size_t)bhk * a->n_kb + i]);
-    return range_ref(fmaf(wave_max(n), wave_max(v), wave_max(d)));
+    return range_ref(fmaf(wave_max(n), wave_max(most_v), wave_max(d)));
+}
+// The largest |v_j| of the key blocks of this lane, and whether some lane's holds a bad key.
+__device__ __forceinline__ float key_most(args_t a, int bhk, int k_blocks, int lane, bool& bad) {
+    float v = 0.f;
+    bool some = false;
+    for (int i = lane; i < k_blocks; i += 64) {
+        const float x = a->key_max[(size_t)bhk * a->n_kb + i];
+        v = fmaxf(v, fabsf(x));
+        if (x < 0.f) some = true;
+    }
+    bad = __builtin_amdgcn_ballot_w64(some) != 0;
+    return v;
 }
 
 template <int D, bool kCausal>
@@ -713,19 +772,21 @@ __device__ __forceinline__ void q_tile(args_t a, half_t* lds, int wg) {
     const unsigned k_row = 2u * (unsigned)a->k.t, v_row = 2u * (unsigned)a->v.t;
     const float c2 = a->c2;
     unsigned ring = 2, ring2 = 0;  // stages of the current step and of the next copies
+    bool bad;
+    const float most_v = key_most(a, bhk, n, lane, bad);
     int left = n_k - 1;            // the last key, counted from the next copies' first
     const Copy<D, T::kW> copier = {wave};
     const unsigned k_off = copier.offset(lane, k_row), v_off = copier.offset(lane, v_row);
     auto copy = [&] {
         const unsigned st = lds0 + ring2 * T::kTileB;
-        copier(kp, k_row, k_off, left, lane, st);
+        copier(kp, k_row, k_off, left, lane, st, kCausal && bad);
         copier(vp, v_row, v_off, left, lane, st + T::kVAt);
         kp += (size_t)k_row * kBlk, vp += (size_t)v_row * kBlk, left -= kBlk;
         ring2 = ring2 == 2 ? 0 : ring2 + 1;
     };
     if (n > 0) copy();
     if (n > 1) copy();
-    const float ref = q_tile_ref<D>(a, bh, bhk, tile0, T::kQueries / kBlk, n, lane);
+    const float ref = q_tile_ref<D>(a, bh, tile0, T::kQueries / kBlk, most_v, lane);
 #pragma unroll
     for (int m = 0; m < kMB; ++m) l2[m] -= ref;
 #pragma clang loop unroll(disable)
@@ -806,11 +867,13 @@ __device__ __forceinline__ void q_tile_roles(args_t a, half_t* lds, int wg) {
     const unsigned p_at = lds0 + T::kXAt + (unsigned)pair * 2048u + 16u * lane, ds_at = p_at + 2 * kPairs * 2048u;
     const char *kp = reinterpret_cast<const char*>(a->k.data + b * a->k.b + hk * a->k.h), *vp = reinterpret_cast<const char*>(a->v.data + b * a->v.b + hk * a->v.h);
     const unsigned k_row = 2u * (unsigned)a->k.t, v_row = 2u * (unsigned)a->v.t;
+    bool bad;
+    const float most_v = key_most(a, bhk, n, lane, bad);
     int left = n_k - 1;  // the last key, counted from the next copies' first
     const Copy<D, kPairs> copier = {pair};  // (by the second role: the first has the exponentials to do)
     const unsigned k_off = copier.offset(lane, k_row), v_off = copier.offset(lane, v_row);
     auto copy = [&](int j) {
-        copier(kp, k_row, k_off, left, lane, lds0 + (unsigned)(j & 3) * T::kTileB);
+        copier(kp, k_row, k_off, left, lane, lds0 + (unsigned)(j & 3) * T::kTileB, kCausal && bad);
         copier(vp, v_row, v_off, left, lane, lds0 + T::kVAt + (unsigned)(j & 1) * T::kTileB);
         kp += (size_t)k_row * kBlk, vp += (size_t)v_row * kBlk, left -= kBlk;
     };
@@ -819,7 +882,7 @@ __device__ __forceinline__ void q_tile_roles(args_t a, half_t* lds, int wg) {
     auto limit = [&](int j) { return min(kCausal ? my_q + last0 : n_k, n_k - 1) - j * kBlk - 4 * hi; };
     auto ragged = [&](int j) { return (kCausal && j * kBlk + 31 > q0 + last0) || (j + 1) * kBlk > n_k; };
     if (!role_p && n > 0) copy(0);
-    const float ref = q_tile_ref<D>(a, bh, bhk, tile0, T::kQueries / kBlk, n, lane);
+    const float ref = q_tile_ref<D>(a, bh, tile0, T::kQueries / kBlk, most_v, lane);
     if constexpr (role_p) {
         // round j: S of step j, then its P beside dQ of step j - 2
         float16_t x1[1], &s = x1[0];
@@ -997,7 +1060,7 @@ hipError_t backward(const AttnRows& x, const Rows16& d_out, const Rows16& dq, co
     float2* row_max = reinterpret_cast<float2*>(w + p.row_max);
     float* key_max = reinterpret_cast<float*>(w + p.key_max);
     half_t* g = reinterpret_cast<half_t*>(w + p.gated);
-    RowsArgs r = {d_out, x.o, x.gate, x.v, dgate, gated ? g : nullptr, x.lse, stat, row_max, key_max, x.len_q, x.len_k, Hq, Hkv, Tq, Tk, p.n_qb,
+    RowsArgs r = {d_out, x.o, x.gate, causal ? x.k : Rows16{nullptr, 0, 0, 0}, x.v, dgate, gated ? g : nullptr, x.lse, stat, row_max, key_max, x.len_q, x.len_k, Hq, Hkv, Tq, Tk, p.n_qb,
                   p.n_kb, B * Hq * p.n_qb};
     hipLaunchKernelGGL(attn_bwd_rows_kernel<D>, dim3(r.n_rows + B * Hkv * p.n_kb), dim3(256), 0, stream, r);
     const Rows16 dO = gated ? Rows16{g, (long long)Hq * Tq * D, (long long)Tq * D, D} : d_out;

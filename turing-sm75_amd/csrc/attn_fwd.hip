@@ -214,6 +214,65 @@ __device__ __forceinline__ int xcd_group(const Rows& rows, int group) {
         return rows.len_q || rows.len_k ? 1 : group;
 }
 
+// Infinities and NaN of a value reach the queries that see its key and no others.  A hidden key's weight
+// is 0, but 0 times an infinity is NaN: in a block of 32 keys that the mask cuts (two a wave at most, its last)
+// the training form looks for such values, and where there are any leaves the block out of the products
+// and adds it at the end, key by key.  Blocks that are hidden whole are left out as well.
+template <int D>
+__device__ __forceinline__ bool bad_block(unsigned rows, int lane) {  // rows: 32 rows in LDS
+    typedef unsigned uint4_t __attribute__((ext_vector_type(4)));
+    unsigned most = 0;
+    const unsigned at = rows + (unsigned)(lane & 31) * (2 * D) + (unsigned)(lane >> 5) * D;
+#pragma unroll 4
+    for (int i = 0; i < D / 16; ++i) {
+        const uint4_t x = __builtin_bit_cast(uint4_t, lds_read_b128(at + 16u * i));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) most = max(most, max(x[e] & 0x7fffu, (x[e] >> 16) & 0x7fffu));
+    }
+    return __builtin_amdgcn_ballot_w64(most >= 0x7c00u) != 0;
+}
+// Adds the 32 keys from kb0 on to O^T, one after the other (m: the final maximum; l has them already).
+template <int D>
+__device__ __forceinline__ void add_block(float16_t (&o)[Cfg<D>::kDBlocks], const half_t* q, const half_t* K, const half_t* V,
+                                          long long k_t, long long v_t, int kb0, int n_k, int last, int hi, float m, float c2) {
+#pragma unroll 1
+    for (int j = 0; j < 32 && kb0 + j < n_k; ++j) {
+        const half_t *k = K + (kb0 + j) * k_t + 8 * hi, *v = V + (kb0 + j) * v_t + 4 * hi;
+        float s = 0.f;
+#pragma unroll 1
+        for (int kk = 0; kk < Cfg<D>::kKSteps; ++kk) {
+            const half8_t x = *reinterpret_cast<const half8_t*>(k + 16 * kk), y = *reinterpret_cast<const half8_t*>(q + 16 * kk + 8 * hi);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s = fmaf((float)x[e], (float)y[e], s);
+        }
+        s = sum_xor32(s);
+        const bool sees = kb0 + j <= last;  // (no branch: the sums would be moved between registers)
+        const float p = sees ? (float)(half_t)fast_exp2(fmaf(s, c2, -(m * c2))) : 0.f;
+#pragma unroll
+        for (int db = 0; db < Cfg<D>::kDBlocks; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const half4_t x = *reinterpret_cast<const half4_t*>(v + 32 * db + 8 * g);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[db][4 * g + e] = fmaf(p, sees ? (float)x[e] : 0.f, o[db][4 * g + e]);
+                asm volatile("" ::: "memory");
+            }
+    }
+}
+// The blocks of 32 keys that a wave leaves out.
+struct Left {
+    int first = -1, second = -1;
+    // Whether the block at kb0 is left out; qw0: the wave's first query, as a key; rows: its values in LDS.
+    template <int D>
+    __device__ __forceinline__ bool out(int kb0, int qw0, unsigned rows, int lane) {
+        if (kb0 > qw0 + 31) return true;
+        if (kb0 + 31 <= qw0 || !bad_block<D>(rows, lane)) return false;
+        second = first;
+        first = kb0;
+        return true;
+    }
+};
+
 // A row's statistic: the logarithm of the sum of its exponentials, from the maximum they were taken
 // against (as the exponentials had it) and their sum; minus infinity for a row that sees no key.
 __device__ __forceinline__ float row_lse(float m, float l, float c2) {
@@ -278,6 +337,7 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
     float16_t o[C::kDBlocks];
 #pragma unroll
     for (int i = 0; i < C::kDBlocks; ++i) o[i] = float16_t{};
+    [[maybe_unused]] Left left;
     float m = -INFINITY;  // max of raw scores (q . k) the exponentials are taken against
     float l = 0.f;        // running sum of this lane's half of the keys
 
@@ -383,6 +443,13 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
                             if (c > lim_q || c >= lim_s) s[kb][r] = -INFINITY;
                         }
                 }
+                bool out[2] = {false, false};
+                if constexpr (kAny && kCausal) {
+                    if (k0 + kKRows - 1 > qw0 + last0)
+#pragma unroll
+                        for (int kb = 0; kb < 2; ++kb)
+                            out[kb] = left.out<D>(k0 + 32 * kb, qw0 + last0, lds0 + C::kTile * 2 + ubase + 32u * kb * kRowB, lane);
+                }
                 // ---- online softmax (exp2 domain), as in the loop below ----
                 float mx = -INFINITY;
 #pragma unroll
@@ -422,6 +489,7 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
                 for (int ks = 0; ks < 4; ++ks) {
                     if (ks == 1 && more)
                         copy(kSecond, k0 + kKRows, nbuf);
+                    if (kAny && kCausal && out[ks >> 1]) continue;
 #pragma unroll
                     for (int db = 0; db < C::kDBlocks; ++db)
                         o[db] = mfma32(ks == 0 ? v0[db] : read_v(ks, db), p[ks], o[db]);
@@ -527,6 +595,11 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
                         const half4_t up = lds_read_tr16_at((va[1] ^ (64u * db)) + o);
                         return half8_t{lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
                     };
+                    bool out = false;
+                    if constexpr (kAny && kCausal)
+                        if (kb0 + 31 > qw0 + last0) out = left.out<D>(kb0, qw0 + last0, lds0 + C::kTile * 2 + ubase + 32u * kb * kRowB, lane);
+                    if (kAny && kb == 0 && more) copy(kSecond, k0 + kKRows, nbuf);
+                    if (!(kAny && kCausal && out)) {
                     __builtin_amdgcn_sched_barrier(0);
                     __builtin_amdgcn_s_setprio(1);
                     constexpr int kSteps = 2 * C::kDBlocks, kPreV = 2;
@@ -538,23 +611,33 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
                         const int ks = i / C::kDBlocks, db = i % C::kDBlocks;
                         if (i + kPreV < kSteps)
                             vbuf[i + kPreV] = read_v(2 * kb + (i + kPreV) / C::kDBlocks, (i + kPreV) % C::kDBlocks);
-                        if (kb == 0 && i == C::kDBlocks && more)
+                        if (!kAny && kb == 0 && i == C::kDBlocks && more)
                             copy(kSecond, k0 + kKRows, nbuf);
                         o[db] = mfma32(vbuf[i], p[ks], o[db]);
                         __builtin_amdgcn_sched_barrier(0);
                     }
                     __builtin_amdgcn_s_setprio(0);
+                    }
                 }
             }
             dma_wait_barrier();
         }
     }
 
+    // (made again from the lane's number: held through the loop, they spill at D = 256)
+    int end_lane = lane;
+    if constexpr (kAny) asm volatile("" : "+v"(end_lane));
+    [[maybe_unused]] const int end_q = qw0 + (end_lane & 31), end_hi = end_lane >> 5;
+    if constexpr (kAny && kCausal) {
+#pragma unroll 1
+        for (; left.first >= 0; left.first = left.second, left.second = -1)
+            add_block<D>(o, Qh + min(end_q, n_q - 1) * q_t, Kh, Vh, k_t, v_t, left.first, n_k, end_q + last0, end_hi, m, c2);
+    }
     l = sum_xor32(l);
     if constexpr (kAny) {
         const int b = bh / Hq, h = bh % Hq;
-        if (hi == 0 && my_q < n_q) rows.lse[(size_t)bh * S + my_q] = row_lse(m, l, c2);
-        store_o<D>(o, l, O + b * rows.o.b + h * rows.o.h, gate ? gate + b * rows.gate.b + h * rows.gate.h : nullptr, my_q, n_q, hi,
+        if (end_hi == 0 && end_q < n_q) rows.lse[(size_t)bh * S + end_q] = row_lse(m, l, c2);
+        store_o<D>(o, l, O + b * rows.o.b + h * rows.o.h, gate ? gate + b * rows.gate.b + h * rows.gate.h : nullptr, end_q, n_q, end_hi,
                    o_t, g_t);
     } else {
         store_o<D>(o, l, O + head, gate ? gate + head : nullptr, my_q, S, hi);
@@ -627,6 +710,7 @@ attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
     float16_t o[C::kDBlocks];
 #pragma unroll
     for (int i = 0; i < C::kDBlocks; ++i) o[i] = float16_t{};
+    [[maybe_unused]] Left left;
     float m = -INFINITY, l = 0.f;
 
     const int krow = lane & 31, ksw = swz<D>(krow);
@@ -730,6 +814,11 @@ attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
                 const half4_t up = lds_read_tr16_at((va[1] ^ (64u * db)) + a);
                 return half8_t{lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
             };
+            if constexpr (kAny && kCausal) {
+                if (kb0 + 31 > qw0 + last0 &&
+                    left.out<D>(kb0, qw0 + last0, lds0 + goff + kRows * kRowB + ubase + 32u * kb * kRowB, lane))
+                    continue;
+            }
             __builtin_amdgcn_sched_barrier(0);
             __builtin_amdgcn_s_setprio(1);
             constexpr int kSteps = 2 * C::kDBlocks, kPreV = 2;
@@ -754,6 +843,11 @@ attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
         dma_wait_barrier();
     }
 
+    if constexpr (kAny && kCausal) {
+#pragma unroll 1
+        for (; left.first >= 0; left.first = left.second, left.second = -1)
+            add_block<D>(o, Qh + min(my_q, n_q - 1) * q_t, Kh, Vh, k_t, v_t, left.first, n_k, my_q + last0, hi, m, c2);
+    }
     // ---- merge: the partial O's of the key groups past the first, lane for lane, through the tile
     // buffers (every wave is past its last read of them) ----
     l = sum_xor32(l);
