@@ -156,22 +156,31 @@ template <int D, int kPart, int kW, int kRowsT = kKRows>
 __device__ __forceinline__ void copy_tile(const TileRows& src, int lane, int wave, int k0, int S, unsigned lds_buf) {
     constexpr int kStep = kW * 1024 / (2 * D), kC = D / 8;
     const int lastrow = S - 1 - k0;
-    asm volatile("" : "+v"(lane));
-    const int row = (64 * wave + lane) / kC;
-    const unsigned col = 16u * (unsigned)((lane % kC) ^ swz<D>(row));
+    auto issue_all = [&](auto Ragged) {
+        int l = lane;
+        asm volatile("" : "+v"(l));
+        const int row = (64 * wave + l) / kC;
+        const unsigned col = 16u * (unsigned)((l % kC) ^ swz<D>(row));
 #pragma unroll
-    for (int j = kPart * Dma<D, kW, kRowsT>::kPerWave / 2; j < (kPart + 1) * Dma<D, kW, kRowsT>::kPerWave / 2; ++j) {
-        constexpr int kT = Dma<D, kW, kRowsT>::kTile;
-        const bool isv = kW * j >= kT;
-        const int dblk = kW * j - (isv ? kT : 0);
-        const int rows = kStep * (dblk / kW);  // rows from the wave's first block to this one
-        const unsigned flip = kStep % 16 == 8 && ((dblk / kW) & 1) ? 32u : 0u;
-        const unsigned stride = isv ? src.v_stride : src.k_stride;
-        // (a full tile's clamp takes no row back)
-        const unsigned o = (unsigned)min(row + rows, lastrow) * stride + (col ^ flip);
-        dma_issue_any(reinterpret_cast<const char*>(isv ? src.v : src.k) + (size_t)k0 * stride, o,
-                  lds_buf + (unsigned)(isv ? kRowsT * D * 2 : 0) + 1024u * (unsigned)(wave + dblk));
-    }
+        for (int j = kPart * Dma<D, kW, kRowsT>::kPerWave / 2; j < (kPart + 1) * Dma<D, kW, kRowsT>::kPerWave / 2; ++j) {
+            constexpr int kT = Dma<D, kW, kRowsT>::kTile;
+            const bool isv = kW * j >= kT;
+            const int dblk = kW * j - (isv ? kT : 0);
+            const int rows = kStep * (dblk / kW);  // rows from the wave's first block to this one
+            const unsigned c = col ^ (kStep % 16 == 8 && ((dblk / kW) & 1) ? 32u : 0u);
+            const unsigned stride = isv ? src.v_stride : src.k_stride;
+            const char* p = reinterpret_cast<const char*>(isv ? src.v : src.k) + (size_t)k0 * stride;
+            const unsigned lds = lds_buf + (unsigned)(isv ? kRowsT * D * 2 : 0) + 1024u * (unsigned)(wave + dblk);
+            if constexpr (decltype(Ragged)::value)
+                dma_issue_any(p, (unsigned)min(row + rows, lastrow) * stride + c, lds);
+            else
+                dma_issue_any(p + (size_t)stride * (unsigned)rows, (unsigned)row * stride + c, lds);
+        }
+    };
+    if (lastrow >= kRowsT - 1)
+        issue_all(std::false_type{});
+    else  // rows past the last are that one again
+        issue_all(std::true_type{});
 }
 
 // Epilogue: O = O^T / l (times sigmoid(gate)), 4 consecutive d per store.  O, gate: the head's rows.
@@ -220,16 +229,18 @@ __device__ __forceinline__ int xcd_group(const Rows& rows, int group) {
 // and adds it at the end, key by key.  Blocks that are hidden whole are left out as well.
 template <int D>
 __device__ __forceinline__ bool bad_block(unsigned rows, int lane) {  // rows: 32 rows in LDS
-    typedef unsigned uint4_t __attribute__((ext_vector_type(4)));
-    unsigned most = 0;
+    typedef unsigned short ushort8_t __attribute__((ext_vector_type(8)));
+    ushort8_t most = {};
     const unsigned at = rows + (unsigned)(lane & 31) * (2 * D) + (unsigned)(lane >> 5) * D;
-#pragma unroll 4
+#pragma unroll 2
     for (int i = 0; i < D / 16; ++i) {
-        const uint4_t x = __builtin_bit_cast(uint4_t, lds_read_b128(at + 16u * i));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) most = max(most, max(x[e] & 0x7fffu, (x[e] >> 16) & 0x7fffu));
+        const ushort8_t x = __builtin_bit_cast(ushort8_t, lds_read_b128(at + 16u * i));
+        most = __builtin_elementwise_max(most, x & (unsigned short)0x7fff);
     }
-    return __builtin_amdgcn_ballot_w64(most >= 0x7c00u) != 0;
+    unsigned short one = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) one = max(one, most[e]);
+    return __builtin_amdgcn_ballot_w64(one >= 0x7c00) != 0;
 }
 // Adds the 32 keys from kb0 on to O^T, one after the other (m: the final maximum; l has them already).
 template <int D>
@@ -260,13 +271,14 @@ __device__ __forceinline__ void add_block(float16_t (&o)[Cfg<D>::kDBlocks], cons
     }
 }
 // The blocks of 32 keys that a wave leaves out.
+template <int D>
 struct Left {
     int first = -1, second = -1;
     // Whether the block at kb0 is left out; qw0: the wave's first query, as a key; rows: its values in LDS.
-    template <int D>
     __device__ __forceinline__ bool out(int kb0, int qw0, unsigned rows, int lane) {
-        if (kb0 > qw0 + 31) return true;
-        if (kb0 + 31 <= qw0 || !bad_block<D>(rows, lane)) return false;
+        if (kb0 + 31 <= qw0) return false;
+        if (kb0 > qw0 + 31) return true;  // (hidden whole)
+        if (!bad_block<D>(rows, lane)) return false;
         second = first;
         first = kb0;
         return true;
@@ -306,7 +318,8 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
     long long q_t = D, k_t = D, v_t = D, o_t = D, g_t = D;
     int n_q = S, n_k = S, last0 = 0;
     if constexpr (kAny) {
-        const int b = bh / Hq, h = bh % Hq, hk = h / group;
+        const int b = __builtin_amdgcn_readfirstlane(bh / Hq), h = __builtin_amdgcn_readfirstlane(bh % Hq);
+        const int hk = __builtin_amdgcn_readfirstlane(h / group);
         Qh = Q + b * rows.q.b + h * rows.q.h;
         Kh = K + b * rows.k.b + hk * rows.k.h;
         Vh = V + b * rows.v.b + hk * rows.v.h;
@@ -337,7 +350,7 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
     float16_t o[C::kDBlocks];
 #pragma unroll
     for (int i = 0; i < C::kDBlocks; ++i) o[i] = float16_t{};
-    [[maybe_unused]] Left left;
+    [[maybe_unused]] Left<D> left;
     float m = -INFINITY;  // max of raw scores (q . k) the exponentials are taken against
     float l = 0.f;        // running sum of this lane's half of the keys
 
@@ -448,7 +461,7 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
                     if (k0 + kKRows - 1 > qw0 + last0)
 #pragma unroll
                         for (int kb = 0; kb < 2; ++kb)
-                            out[kb] = left.out<D>(k0 + 32 * kb, qw0 + last0, lds0 + C::kTile * 2 + ubase + 32u * kb * kRowB, lane);
+                            out[kb] = left.out(k0 + 32 * kb, qw0 + last0, lds0 + C::kTile * 2 + ubase + 32u * kb * kRowB, lane);
                 }
                 // ---- online softmax (exp2 domain), as in the loop below ----
                 float mx = -INFINITY;
@@ -597,7 +610,7 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
                     };
                     bool out = false;
                     if constexpr (kAny && kCausal)
-                        if (kb0 + 31 > qw0 + last0) out = left.out<D>(kb0, qw0 + last0, lds0 + C::kTile * 2 + ubase + 32u * kb * kRowB, lane);
+                        if (kb0 + 31 > qw0 + last0) out = left.out(kb0, qw0 + last0, lds0 + C::kTile * 2 + ubase + 32u * kb * kRowB, lane);
                     if (kAny && kb == 0 && more) copy(kSecond, k0 + kKRows, nbuf);
                     if (!(kAny && kCausal && out)) {
                     __builtin_amdgcn_sched_barrier(0);
@@ -635,7 +648,7 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
     }
     l = sum_xor32(l);
     if constexpr (kAny) {
-        const int b = bh / Hq, h = bh % Hq;
+        const int b = __builtin_amdgcn_readfirstlane(bh / Hq), h = __builtin_amdgcn_readfirstlane(bh % Hq);
         if (end_hi == 0 && end_q < n_q) rows.lse[(size_t)bh * S + end_q] = row_lse(m, l, c2);
         store_o<D>(o, l, O + b * rows.o.b + h * rows.o.h, gate ? gate + b * rows.gate.b + h * rows.gate.h : nullptr, end_q, n_q, end_hi,
                    o_t, g_t);
@@ -682,7 +695,8 @@ attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
     long long q_t = D, k_t = D, v_t = D, o_t = D, g_t = D;
     int n_q = S, n_k = S, last0 = 0;
     if constexpr (kAny) {
-        const int b = bh / Hq, h = bh % Hq, hk = h / group;
+        const int b = __builtin_amdgcn_readfirstlane(bh / Hq), h = __builtin_amdgcn_readfirstlane(bh % Hq);
+        const int hk = __builtin_amdgcn_readfirstlane(h / group);
         Qh = Q + b * rows.q.b + h * rows.q.h;
         Kh = K + b * rows.k.b + hk * rows.k.h;
         Vh = V + b * rows.v.b + hk * rows.v.h;
@@ -710,7 +724,7 @@ attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
     float16_t o[C::kDBlocks];
 #pragma unroll
     for (int i = 0; i < C::kDBlocks; ++i) o[i] = float16_t{};
-    [[maybe_unused]] Left left;
+    [[maybe_unused]] Left<D> left;
     float m = -INFINITY, l = 0.f;
 
     const int krow = lane & 31, ksw = swz<D>(krow);
@@ -816,7 +830,7 @@ attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
             };
             if constexpr (kAny && kCausal) {
                 if (kb0 + 31 > qw0 + last0 &&
-                    left.out<D>(kb0, qw0 + last0, lds0 + goff + kRows * kRowB + ubase + 32u * kb * kRowB, lane))
+                    left.out(kb0, qw0 + last0, lds0 + goff + kRows * kRowB + ubase + 32u * kb * kRowB, lane))
                     continue;
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -843,10 +857,13 @@ attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
         dma_wait_barrier();
     }
 
+    int end_lane = lane;
+    if constexpr (kAny) asm volatile("" : "+v"(end_lane));
+    [[maybe_unused]] const int end_q = qw0 + (end_lane & 31), end_hi = end_lane >> 5;
     if constexpr (kAny && kCausal) {
 #pragma unroll 1
         for (; left.first >= 0; left.first = left.second, left.second = -1)
-            add_block<D>(o, Qh + min(my_q, n_q - 1) * q_t, Kh, Vh, k_t, v_t, left.first, n_k, my_q + last0, hi, m, c2);
+            add_block<D>(o, Qh + min(end_q, n_q - 1) * q_t, Kh, Vh, k_t, v_t, left.first, n_k, end_q + last0, end_hi, m, c2);
     }
     // ---- merge: the partial O's of the key groups past the first, lane for lane, through the tile
     // buffers (every wave is past its last read of them) ----
@@ -893,9 +910,9 @@ attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
         }
     }
     if constexpr (kAny) {
-        const int b = bh / Hq, h = bh % Hq;
-        if (hi == 0 && my_q < n_q) rows.lse[(size_t)bh * S + my_q] = row_lse(m, l, c2);
-        store_o<D>(o, l, O + b * rows.o.b + h * rows.o.h, gate ? gate + b * rows.gate.b + h * rows.gate.h : nullptr, my_q, n_q, hi,
+        const int b = __builtin_amdgcn_readfirstlane(bh / Hq), h = __builtin_amdgcn_readfirstlane(bh % Hq);
+        if (end_hi == 0 && end_q < n_q) rows.lse[(size_t)bh * S + end_q] = row_lse(m, l, c2);
+        store_o<D>(o, l, O + b * rows.o.b + h * rows.o.h, gate ? gate + b * rows.gate.b + h * rows.gate.h : nullptr, end_q, n_q, end_hi,
                    o_t, g_t);
     } else {
         store_o<D>(o, l, O + head, gate ? gate + head : nullptr, my_q, S, hi);
