@@ -224,28 +224,53 @@ __device__ __forceinline__ int xcd_group(const Rows& rows, int group) {
 }
 
 // Infinities and NaN of a value reach the queries that see its key and no others.  A hidden key's weight
-// is 0, but 0 times an infinity is NaN: in a block of 32 keys that the mask cuts (two a wave at most, its last)
-// the training form looks for such values, and where there are any leaves the block out of the products
-// and adds it at the end, key by key.  Blocks that are hidden whole are left out as well.
+// is 0, but 0 times an infinity is NaN: the training form looks at its sums when the keys are through, and
+// a wave that finds such a number there, and one among the values of the last keys (from the first that
+// some query of it does not see on), has its workgroup take the keys once more.  The wave then ends before those
+// keys and adds them one by one.  (Looking at the values of each cut block as it came took 8192 tokens from
+// 840 to 862 us at D = 256 and from 576 to 583 at D = 128, and 1000 tokens from 22.5 to 24.5 at D = 64.)
 template <int D>
-__device__ __forceinline__ bool bad_block(unsigned rows, int lane) {  // rows: 32 rows in LDS
-    typedef unsigned short ushort8_t __attribute__((ext_vector_type(8)));
-    ushort8_t most = {};
-    const unsigned at = rows + (unsigned)(lane & 31) * (2 * D) + (unsigned)(lane >> 5) * D;
-#pragma unroll 2
-    for (int i = 0; i < D / 16; ++i) {
-        const ushort8_t x = __builtin_bit_cast(ushort8_t, lds_read_b128(at + 16u * i));
-        most = __builtin_elementwise_max(most, x & (unsigned short)0x7fff);
-    }
-    unsigned short one = 0;
+__device__ __forceinline__ bool not_finite(const float16_t (&o)[Cfg<D>::kDBlocks]) {
+    float t = 0.f;  // NaN if one is infinite or NaN
 #pragma unroll
-    for (int e = 0; e < 8; ++e) one = max(one, most[e]);
-    return __builtin_amdgcn_ballot_w64(one >= 0x7c00) != 0;
+    for (int db = 0; db < Cfg<D>::kDBlocks; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) t = fmaf(o[db][r], 0.f, t);
+    return __builtin_amdgcn_ballot_w64(t != 0.f) != 0;
 }
-// Adds the 32 keys from kb0 on to O^T, one after the other (m: the final maximum; l has them already).
+template <int D>
+__device__ __forceinline__ bool bad_rows(const half_t* V, long long v_t, int from, int to, int lane) {
+    bool bad = false;
+#pragma unroll 1
+    for (int j = from + lane; j < to; j += 64)
+#pragma unroll 1
+        for (int i = 0; i < D; i += 8) {
+            const half8_t x = *reinterpret_cast<const half8_t*>(V + j * v_t + i);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) bad |= !(__builtin_fabsf((float)x[e]) < INFINITY);
+        }
+    return __builtin_amdgcn_ballot_w64(bad) != 0;
+}
+// The lane's number, made anew: held through the loop it spills at D = 256, and so does what is made of it.
+__device__ __forceinline__ int lane_now() {
+    unsigned all = ~0u;
+    asm volatile("" : "+s"(all));
+    return __builtin_amdgcn_mbcnt_hi(all, __builtin_amdgcn_mbcnt_lo(all, 0u));
+}
+// Whether a wave of the workgroup says so.
+template <int kW>
+__device__ __forceinline__ bool any_wave(int* flags, int wave, int lane, bool mine) {
+    if (lane == 0) flags[wave] = mine;
+    lds_barrier();
+    int any = 0;
+#pragma unroll
+    for (int w = 0; w < kW; ++w) any |= flags[w];
+    return __builtin_amdgcn_readfirstlane(any) != 0;
+}
+// Adds the 32 keys from kb0 on to O^T, one after the other (m: the final maximum).
 template <int D>
 __device__ __forceinline__ void add_block(float16_t (&o)[Cfg<D>::kDBlocks], const half_t* q, const half_t* K, const half_t* V,
-                                          long long k_t, long long v_t, int kb0, int n_k, int last, int hi, float m, float c2) {
+                                          long long k_t, long long v_t, int kb0, int n_k, int last, int hi, float m, float& l, float c2) {
 #pragma unroll 1
     for (int j = 0; j < 32 && kb0 + j < n_k; ++j) {
         const half_t *k = K + (kb0 + j) * k_t + 8 * hi, *v = V + (kb0 + j) * v_t + 4 * hi;
@@ -258,7 +283,8 @@ __device__ __forceinline__ void add_block(float16_t (&o)[Cfg<D>::kDBlocks], cons
         }
         s = sum_xor32(s);
         const bool sees = kb0 + j <= last;  // (no branch: the sums would be moved between registers)
-        const float p = sees ? (float)(half_t)fast_exp2(fmaf(s, c2, -(m * c2))) : 0.f;
+        const float e = sees ? fast_exp2(fmaf(s, c2, -(m * c2))) : 0.f, p = (float)(half_t)e;
+        l += hi ? 0.f : e;
 #pragma unroll
         for (int db = 0; db < Cfg<D>::kDBlocks; ++db)
 #pragma unroll
@@ -270,21 +296,6 @@ __device__ __forceinline__ void add_block(float16_t (&o)[Cfg<D>::kDBlocks], cons
             }
     }
 }
-// The blocks of 32 keys that a wave leaves out.
-template <int D>
-struct Left {
-    int first = -1, second = -1;
-    // Whether the block at kb0 is left out; qw0: the wave's first query, as a key; rows: its values in LDS.
-    __device__ __forceinline__ bool out(int kb0, int qw0, unsigned rows, int lane) {
-        if (kb0 + 31 <= qw0) return false;
-        if (kb0 > qw0 + 31) return true;  // (hidden whole)
-        if (!bad_block<D>(rows, lane)) return false;
-        second = first;
-        first = kb0;
-        return true;
-    }
-};
-
 // A row's statistic: the logarithm of the sum of its exponentials, from the maximum they were taken
 // against (as the exponentials had it) and their sum; minus infinity for a row that sees no key.
 __device__ __forceinline__ float row_lse(float m, float l, float c2) {
@@ -305,9 +316,7 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
     // static and 1 KiB aligned: the XOR address forms below need the buffer's low 10 bits zero
     __shared__ __align__(1024) half_t lds[C::kLdsBytes / 2];
 
-    const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int hi = lane >> 5;  // which half of the wave
     int bh, qt;
     map_block(blockIdx.x, BH, n_qt, kCausal, xcd_group<Rows>(rows, group), bh, qt, D <= 128);
     const size_t head = (size_t)bh * S * D;  // Q, O, gate: query head bh = b * Hq + h
@@ -330,8 +339,20 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
         if (q0 >= n_q) return;
     }
     const int qw0 = q0 + 32 * wave;
-    const int my_q = qw0 + (lane & 31);
 
+    const int kv_end = kCausal ? min(n_k, q0 + 32 * kW + last0) : n_k;
+    int n_tiles = (kv_end + kKRows - 1) / kKRows;
+    const int wave_kv_end = kCausal ? min(n_k, qw0 + 32 + last0) : n_k;
+    int end = wave_kv_end;  // of the keys that this wave takes in the loop
+    float m = -INFINITY;    // max of raw scores (q . k) the exponentials are taken against
+    float l;                // running sum of this lane's half of the keys
+
+[[maybe_unused]] keys:
+    if constexpr (kAny) asm volatile("" : "+s"(n_tiles));
+    const int lane = kAny ? lane_now() : threadIdx.x & 63;
+    const int hi = lane >> 5;  // which half of the wave
+    const int my_q = qw0 + (lane & 31);
+    l = 0.f;
     // This wave's 32 query rows as the B operand of S^T = K Q^T: slot s of k-step kk is
     // Q[my_q][16*kk + 8*hi + s].
     half8_t qf[C::kKSteps];
@@ -343,16 +364,9 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
             qf[kk] = half8_t{};
     }
 
-    const int kv_end = kCausal ? min(n_k, q0 + 32 * kW + last0) : n_k;
-    const int n_tiles = (kv_end + kKRows - 1) / kKRows;
-    const int wave_kv_end = kCausal ? min(n_k, qw0 + 32 + last0) : n_k;
-
     float16_t o[C::kDBlocks];
 #pragma unroll
     for (int i = 0; i < C::kDBlocks; ++i) o[i] = float16_t{};
-    [[maybe_unused]] Left<D> left;
-    float m = -INFINITY;  // max of raw scores (q . k) the exponentials are taken against
-    float l = 0.f;        // running sum of this lane's half of the keys
 
     // Lane-constant parts of the LDS addresses.
     const int krow = lane & 31;            // K operand row within a 32-key block
@@ -409,7 +423,7 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
             const int k0 = t * kKRows;
             const bool more = t + 1 < n_tiles;
             const unsigned nbuf = lds0 + (unsigned)(u ^ 1) * buf_bytes;
-            if (k0 >= wave_kv_end) {  // this wave's queries end before the tile: copies only
+            if (k0 >= end) {  // this wave's queries end before the tile: copies only
                 if (more) {
                     copy(kFirst, k0 + kKRows, nbuf);
                     copy(kSecond, k0 + kKRows, nbuf);
@@ -456,13 +470,6 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
                             if (c > lim_q || c >= lim_s) s[kb][r] = -INFINITY;
                         }
                 }
-                bool out[2] = {false, false};
-                if constexpr (kAny && kCausal) {
-                    if (k0 + kKRows - 1 > qw0 + last0)
-#pragma unroll
-                        for (int kb = 0; kb < 2; ++kb)
-                            out[kb] = left.out(k0 + 32 * kb, qw0 + last0, lds0 + C::kTile * 2 + ubase + 32u * kb * kRowB, lane);
-                }
                 // ---- online softmax (exp2 domain), as in the loop below ----
                 float mx = -INFINITY;
 #pragma unroll
@@ -502,7 +509,6 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
                 for (int ks = 0; ks < 4; ++ks) {
                     if (ks == 1 && more)
                         copy(kSecond, k0 + kKRows, nbuf);
-                    if (kAny && kCausal && out[ks >> 1]) continue;
 #pragma unroll
                     for (int db = 0; db < C::kDBlocks; ++db)
                         o[db] = mfma32(ks == 0 ? v0[db] : read_v(ks, db), p[ks], o[db]);
@@ -520,7 +526,7 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
             const int k0 = t * kKRows;
             const bool more = t + 1 < n_tiles;
             const unsigned nbuf = lds0 + ((t + 1) & 1) * buf_bytes;
-            if (k0 >= wave_kv_end) {  // this wave's queries end before the tile: copies only
+            if (k0 >= end) {  // this wave's queries end before the tile: copies only
                 if (more) {
                     copy(kFirst, k0 + kKRows, nbuf);
                     copy(kSecond, k0 + kKRows, nbuf);
@@ -608,11 +614,7 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
                         const half4_t up = lds_read_tr16_at((va[1] ^ (64u * db)) + o);
                         return half8_t{lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
                     };
-                    bool out = false;
-                    if constexpr (kAny && kCausal)
-                        if (kb0 + 31 > qw0 + last0) out = left.out(kb0, qw0 + last0, lds0 + C::kTile * 2 + ubase + 32u * kb * kRowB, lane);
                     if (kAny && kb == 0 && more) copy(kSecond, k0 + kKRows, nbuf);
-                    if (!(kAny && kCausal && out)) {
                     __builtin_amdgcn_sched_barrier(0);
                     __builtin_amdgcn_s_setprio(1);
                     constexpr int kSteps = 2 * C::kDBlocks, kPreV = 2;
@@ -630,21 +632,27 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
                         __builtin_amdgcn_sched_barrier(0);
                     }
                     __builtin_amdgcn_s_setprio(0);
-                    }
                 }
             }
             dma_wait_barrier();
         }
     }
 
-    // (made again from the lane's number: held through the loop, they spill at D = 256)
-    int end_lane = lane;
-    if constexpr (kAny) asm volatile("" : "+v"(end_lane));
+    [[maybe_unused]] const int end_lane = kAny ? lane_now() : 0;
     [[maybe_unused]] const int end_q = qw0 + (end_lane & 31), end_hi = end_lane >> 5;
-    if constexpr (kAny && kCausal) {
+    if constexpr (kAny) {
+        const int cut = max(kCausal ? min(n_k, qw0 + last0 + 1) : n_k, 0) / kKRows * kKRows;
+        const bool bad = cut < end && not_finite<D>(o) && bad_rows<D>(Vh, v_t, cut, min(n_k, (end + kKRows - 1) / kKRows * kKRows), end_lane);
+        if (any_wave<kW>(reinterpret_cast<int*>(lds), wave, end_lane, bad)) {
+            if (bad) end = cut;
+            lds_barrier();  // (the flags are where the tiles go)
+            goto keys;
+        }
+        if (end < wave_kv_end) {
 #pragma unroll 1
-        for (; left.first >= 0; left.first = left.second, left.second = -1)
-            add_block<D>(o, Qh + min(end_q, n_q - 1) * q_t, Kh, Vh, k_t, v_t, left.first, n_k, end_q + last0, end_hi, m, c2);
+            for (int k0 = end; k0 < wave_kv_end; k0 += 32)
+                add_block<D>(o, Qh + min(end_q, n_q - 1) * q_t, Kh, Vh, k_t, v_t, k0, n_k, kCausal ? end_q + last0 : n_k, end_hi, m, l, c2);
+        }
     }
     l = sum_xor32(l);
     if constexpr (kAny) {
@@ -679,12 +687,11 @@ attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
     constexpr int kBuf = 2 * kRows * D;               // halfs per buffer (K, V)
     static_assert(2 * kBuf * 2 >= (kKG - 1) * kQG * 32 * D * 4, "the partial O's fit the tile buffers");
     __shared__ __align__(1024) half_t lds[2 * kBuf];
+    __shared__ int flags[kAny ? kW : 1];
     __shared__ float2 ml[kKG][kKG > 1 ? kQG : 1][kKG > 1 ? 64 : 1];
 
-    const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int qg = kKG == 1 ? wave : wave % kQG, kg = kKG == 1 ? 0 : wave / kQG;
-    const int hi = lane >> 5;
     int bh, qt;
     map_block(blockIdx.x, BH, n_qt, kCausal, xcd_group<Rows>(rows, group), bh, qt, kKG == 1);
     const size_t head = (size_t)bh * S * D;
@@ -707,8 +714,19 @@ attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
         if (q0 >= n_q) return;
     }
     const int qw0 = q0 + 32 * qg;
-    const int my_q = qw0 + (lane & 31);
 
+    const int kv_end = kCausal ? min(n_k, q0 + 32 * kQG + last0) : n_k;
+    int n_tiles = (kv_end + kRows - 1) / kRows;
+    const int wave_kv_end = kCausal ? min(n_k, qw0 + 32 + last0) : n_k;
+    int end = wave_kv_end;
+    float m = -INFINITY, l;
+
+[[maybe_unused]] keys:
+    if constexpr (kAny) asm volatile("" : "+s"(n_tiles));
+    const int lane = kAny ? lane_now() : threadIdx.x & 63;
+    const int hi = lane >> 5;  // which half of the wave
+    const int my_q = qw0 + (lane & 31);
+    l = 0.f;
     half8_t qf[C::kKSteps];
 #pragma unroll
     for (int kk = 0; kk < C::kKSteps; ++kk) {
@@ -717,15 +735,9 @@ attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
         else
             qf[kk] = half8_t{};
     }
-    const int kv_end = kCausal ? min(n_k, q0 + 32 * kQG + last0) : n_k;
-    const int n_tiles = (kv_end + kRows - 1) / kRows;
-    const int wave_kv_end = kCausal ? min(n_k, qw0 + 32 + last0) : n_k;
-
     float16_t o[C::kDBlocks];
 #pragma unroll
     for (int i = 0; i < C::kDBlocks; ++i) o[i] = float16_t{};
-    [[maybe_unused]] Left<D> left;
-    float m = -INFINITY, l = 0.f;
 
     const int krow = lane & 31, ksw = swz<D>(krow);
     const int g16 = lane >> 4, i16 = lane & 15;
@@ -767,7 +779,7 @@ attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
 #pragma unroll
         for (int kb = 0; kb < kKT / 32; ++kb) {
             const int kb0 = t * kRows + kKT * kg + 32 * kb;  // first key of this half
-            if (kb0 >= wave_kv_end) break;
+            if (kb0 >= end) break;
             asm volatile("" : "+v"(ka), "+v"(va[0]), "+v"(va[1]));
             constexpr int kPreK = 3;
             float16_t sh = float16_t{};
@@ -828,11 +840,6 @@ attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
                 const half4_t up = lds_read_tr16_at((va[1] ^ (64u * db)) + a);
                 return half8_t{lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
             };
-            if constexpr (kAny && kCausal) {
-                if (kb0 + 31 > qw0 + last0 &&
-                    left.out(kb0, qw0 + last0, lds0 + goff + kRows * kRowB + ubase + 32u * kb * kRowB, lane))
-                    continue;
-            }
             __builtin_amdgcn_sched_barrier(0);
             __builtin_amdgcn_s_setprio(1);
             constexpr int kSteps = 2 * C::kDBlocks, kPreV = 2;
@@ -857,13 +864,21 @@ attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
         dma_wait_barrier();
     }
 
-    int end_lane = lane;
-    if constexpr (kAny) asm volatile("" : "+v"(end_lane));
+    [[maybe_unused]] const int end_lane = kAny ? lane_now() : 0;
     [[maybe_unused]] const int end_q = qw0 + (end_lane & 31), end_hi = end_lane >> 5;
-    if constexpr (kAny && kCausal) {
+    if constexpr (kAny) {
+        const int cut = max(kCausal ? min(n_k, qw0 + last0 + 1) : n_k, 0) / 32 * 32;
+        const bool bad = cut < end && not_finite<D>(o) && bad_rows<D>(Vh, v_t, cut, min(n_k, (end + 32 - 1) / 32 * 32), end_lane);
+        if (any_wave<kW>(flags, wave, end_lane, bad)) {
+            if (bad) end = cut;
+            goto keys;
+        }
+        if (end < wave_kv_end) {
 #pragma unroll 1
-        for (; left.first >= 0; left.first = left.second, left.second = -1)
-            add_block<D>(o, Qh + min(end_q, n_q - 1) * q_t, Kh, Vh, k_t, v_t, left.first, n_k, end_q + last0, end_hi, m, c2);
+            for (int k0 = end; k0 < wave_kv_end; k0 += 32)
+                if (k0 / kKT % kKG == kg)
+                    add_block<D>(o, Qh + min(end_q, n_q - 1) * q_t, Kh, Vh, k_t, v_t, k0, n_k, kCausal ? end_q + last0 : n_k, end_hi, m, l, c2);
+        }
     }
     // ---- merge: the partial O's of the key groups past the first, lane for lane, through the tile
     // buffers (every wave is past its last read of them) ----
