@@ -418,7 +418,8 @@ int tsa_rope(const tsa_rope_plan* plan, int type, const tsa_rows* q, const tsa_r
  * no key has o = 0 and lse = -infinity, and its gradients are 0.  An infinity or NaN of a token reaches
  * what sees it (a key's the queries behind it, a query's the keys in front of it; there it may make
  * NaN of whole rows) and nothing that the mask or the lengths hide it from.  A stride_t is at most
- * 2^24 elements, and outputs lie on no input. ---- */
+ * 2^24 elements, all sequences' and heads' blocks of 32 rows (queries' and keys') are fewer than 2^23, and outputs
+ * lie on no input. ---- */
 int tsa_attn_train_fwd(const tsa_rows* q, const tsa_rows* k, const tsa_rows* v, const tsa_rows* gate, const tsa_rows* o,
                        float* lse, const int32_t* len_q, const int32_t* len_k, int B, int Hq, int Hkv, int Tq, int Tk,
                        int D, float scale, int causal, void* stream);

@@ -134,3 +134,12 @@ def test_backward_workspace():
     for bad in ((0, 4, 2, 3, 5, 64, 0, 1), (2, 3, 2, 3, 5, 64, 0, 1), (2, 4, 2, 3, 5, 96, 0, 1), (2, 4, 2, 3, 5, 64, 2, 1), (2, 4, 2, 3, 5, 64, 0, 2),
                 (2, 4, 2, 1 << 30, 5, 64, 0, 1)):
         assert lib.tsa_attn_bwd_workspace_bytes(*bad) == 0, bad
+
+
+@pytest.mark.parametrize("call", [fwd, bwd], ids=lambda f: f.__name__)
+def test_pair_of_too_many_rows(call):
+    """More blocks of 32 rows than a launch has threads for."""
+    assert call(B=1 << 22, Hq=1, Hkv=1, Tq=1, Tk=1) == tsa.TSA_ERR_SHAPE
+    assert call(B=1, Hq=1, Hkv=1, Tq=1 << 27, Tk=1 << 27) == tsa.TSA_ERR_SHAPE
+    assert tsa.load().tsa_attn_bwd_workspace_bytes(1 << 22, 1, 1, 1, 1, 64, 0, 1) == 0
+    assert tsa.load().tsa_attn_bwd_workspace_bytes((1 << 22) - 1, 1, 1, 1, 1, 64, 0, 1) > 0

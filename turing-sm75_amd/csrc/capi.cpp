@@ -561,8 +561,9 @@ namespace {
 int check_train_sizes(int B, int Hq, int Hkv, int Tq, int Tk, int D) {
     if (B < 1 || Hq < 1 || Hkv < 1 || Tq < 1 || Tk < 1 || D < 1 || Hq % Hkv != 0) return TSA_ERR_SHAPE;
     if (D != 64 && D != 128 && D != 256) return TSA_ERR_UNSUPPORTED;
-    // rows of all heads, and positions, in ints
-    return fits_int(B, Hq, Tq) && fits_int(B, Hkv, Tk) && (long long)Tq + Tk <= INT_MAX - 1024 ? TSA_OK : TSA_ERR_SHAPE;
+    // rows of all heads, and positions, in ints; a launch's threads, up to 512 for 32 rows, below 2^32
+    if (!fits_int(B, Hq, Tq) || !fits_int(B, Hkv, Tk) || (long long)Tq + Tk > INT_MAX - 1024) return TSA_ERR_SHAPE;
+    return (long long)B * ((long long)Hq * ((Tq + 31) / 32) + (long long)Hkv * ((Tk + 31) / 32)) < 1 << 23 ? TSA_OK : TSA_ERR_SHAPE;
 }
 
 // Rows whose tiles are copied: offsets within a tile of 64 rows fit 32 bits.
