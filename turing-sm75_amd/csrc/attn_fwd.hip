@@ -63,14 +63,15 @@ struct Cfg {
 // tiles first.
 // With two workgroups per CU (two) and no more workgroups than that, a CU's second one starts
 // with its first and the sum of the two decides: the later workgroups then go lightest first
-// (32 heads, S = 2001, D = 128: 52.5 -> 51.0 us).
+// (32 heads, S = 2001, D = 128: 52.5 -> 51.0 us).  turn: how many CUs further on each round of an XCD's CUs begins.
 __device__ __forceinline__ void map_block(int bid, int BH, int n_qt, bool causal, int group,
-                                          int& bh, int& qt, bool two = false) {
+                                          int& bh, int& qt, bool two = false, int turn = 0) {
     int rank;
     if ((BH & 7) == 0) {
         constexpr int kCus = 32;  // per XCD
         const int xcd = bid & 7, hpx = BH >> 3, slots = hpx * n_qt;
         int slot = bid >> 3;
+        if (slot / kCus < slots / kCus) slot = slot / kCus * kCus + (slot + slot / kCus * turn) % kCus;
         if (two && causal && slot >= kCus && slots <= 2 * kCus) slot = slots - 1 - (slot - kCus);
         bh = group > 1 ? xcd * hpx + slot % hpx : (slot % hpx) * 8 + xcd;
         rank = slot / hpx;
@@ -223,6 +224,17 @@ __device__ __forceinline__ int xcd_group(const Rows& rows, int group) {
         return rows.len_q || rows.len_k ? 1 : group;
 }
 
+// In a padded batch of a power of two of sequences, a long one's tiles of several lengths would meet on the same CUs, round
+// after round; each round so begins further on, by the heads of a sequence that an XCD has (lengths as above, D = 64:
+// 60 -> 47 us).  With four workgroups a CU only: at D = 128, two, nothing changed, and at D = 256, one, 24/4 heads took 163 for 147.
+template <int D, class Rows>
+__device__ __forceinline__ int cu_turn(const Rows& rows, int Hq) {
+    if constexpr (std::is_same_v<Rows, Dense> || D > 64)
+        return 0;
+    else
+        return rows.len_q || rows.len_k ? max(Hq / 8, 1) : 0;
+}
+
 // Infinities and NaN of a value reach the queries that see its key and no others.  A hidden key's weight
 // is 0, but 0 times an infinity is NaN: the training form looks at its sums when the keys are through, and
 // a wave that finds such a number there, and one among the values of the last keys (from the first that
@@ -318,7 +330,7 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int bh, qt;
-    map_block(blockIdx.x, BH, n_qt, kCausal, xcd_group<Rows>(rows, group), bh, qt, D <= 128);
+    map_block(blockIdx.x, BH, n_qt, kCausal, xcd_group<Rows>(rows, group), bh, qt, D <= 128, cu_turn<D>(rows, Hq));
     const size_t head = (size_t)bh * S * D;  // Q, O, gate: query head bh = b * Hq + h
     const size_t kvhead = (size_t)((bh / Hq) * (Hq / group) + (bh % Hq) / group) * S * D;
     const int q0 = qt * (32 * kW);
