@@ -184,8 +184,20 @@ __device__ __forceinline__ void copy_tile(const TileRows& src, int lane, int wav
         issue_all(std::true_type{});
 }
 
+// sigmoid(x) to 2.4 2^-24 of it (0.6 on average, 1.5 without): the exponent's argument in two floats, the reciprocal with one Newton
+// step.  For the training form: where a query sees one key, dS is nothing but o's rounding to fp16, and an o on the other
+// side of a rounding is twice that in one element.  No call got slower by it.
+__device__ __forceinline__ float sigmoid_close(float x) {
+    const float g = x;
+    x = fminf(fmaxf(x, -80.f), 80.f);  // (further out it is 0 beside fp16's least value, or 1)
+    constexpr float kHi = 1.44269504f, kLo = 1.92596299e-8f;  // log2(e) = kHi + kLo
+    const float y = -x * kHi, rest = fmaf(-x, kHi, -y) - x * kLo;
+    const float e = __builtin_amdgcn_exp2f(y), d = fmaf(e, rest * 0.69314718f, e) + 1.f, r = __builtin_amdgcn_rcpf(d);
+    return g == g ? fmaf(fmaf(-d, r, 1.f), r, r) : g;
+}
+
 // Epilogue: O = O^T / l (times sigmoid(gate)), 4 consecutive d per store.  O, gate: the head's rows.
-template <int D>
+template <int D, bool kClose = false>
 __device__ __forceinline__ void store_o(const float16_t (&o)[Cfg<D>::kDBlocks], float l, half_t* __restrict__ O,
                                         const half_t* __restrict__ gate, int my_q, int S, int hi, long long o_t = D,
                                         long long g_t = D) {
@@ -204,7 +216,8 @@ __device__ __forceinline__ void store_o(const float16_t (&o)[Cfg<D>::kDBlocks], 
                     // sigmoid by the hardware reciprocal (1 ulp): an IEEE division per element
                     // was ~10 VALU ops, 128 of them per lane at D = 256 in every workgroup's tail
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) f[e] = inv * __builtin_amdgcn_rcpf(1.f + __expf(-(float)g4[e]));
+                    for (int e = 0; e < 4; ++e)
+                        f[e] = inv * (kClose ? sigmoid_close((float)g4[e]) : __builtin_amdgcn_rcpf(1.f + __expf(-(float)g4[e])));
                 }
                 const half4_t v4 = {(half_t)(o[db][4 * rg] * f[0]), (half_t)(o[db][4 * rg + 1] * f[1]),
                                     (half_t)(o[db][4 * rg + 2] * f[2]), (half_t)(o[db][4 * rg + 3] * f[3])};
@@ -670,7 +683,7 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
     if constexpr (kAny) {
         const int b = __builtin_amdgcn_readfirstlane(bh / Hq), h = __builtin_amdgcn_readfirstlane(bh % Hq);
         if (end_hi == 0 && end_q < n_q) rows.lse[(size_t)bh * S + end_q] = row_lse(m, l, c2);
-        store_o<D>(o, l, O + b * rows.o.b + h * rows.o.h, gate ? gate + b * rows.gate.b + h * rows.gate.h : nullptr, end_q, n_q, end_hi,
+        store_o<D, true>(o, l, O + b * rows.o.b + h * rows.o.h, gate ? gate + b * rows.gate.b + h * rows.gate.h : nullptr, end_q, n_q, end_hi,
                    o_t, g_t);
     } else {
         store_o<D>(o, l, O + head, gate ? gate + head : nullptr, my_q, S, hi);
@@ -939,7 +952,7 @@ attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
     if constexpr (kAny) {
         const int b = __builtin_amdgcn_readfirstlane(bh / Hq), h = __builtin_amdgcn_readfirstlane(bh % Hq);
         if (end_hi == 0 && end_q < n_q) rows.lse[(size_t)bh * S + end_q] = row_lse(m, l, c2);
-        store_o<D>(o, l, O + b * rows.o.b + h * rows.o.h, gate ? gate + b * rows.gate.b + h * rows.gate.h : nullptr, end_q, n_q, end_hi,
+        store_o<D, true>(o, l, O + b * rows.o.b + h * rows.o.h, gate ? gate + b * rows.gate.b + h * rows.gate.h : nullptr, end_q, n_q, end_hi,
                    o_t, g_t);
     } else {
         store_o<D>(o, l, O + head, gate ? gate + head : nullptr, my_q, S, hi);
@@ -961,7 +974,13 @@ hipError_t launch(const half_t* q, const half_t* k, const half_t* v, const half_
                            Hq / Hkv, scale * kLog2e, view);
         return hipGetLastError();
     };
-    auto tiles = [&](int rows) { return (long long)BH * ((S + rows - 1) / rows); };
+    // A padded batch's tiles count as 0.7 of them at D <= 128: the lengths, on the device, leave some empty.  Lengths
+    // that leave 0.6 of the queries: D = 64 5 x 777, 12 heads 18.5 / 15.8, 4 x 1024, 16 heads 21.6 / 20.2; D = 128 34.1 /
+    // 28.4, 3 x 1500, 16 heads 46.6 / 36; lengths that leave all: 19.5 / 21, 23.2 / 26, 37.5 / 39.4, 50.4 / 57.  At D = 256,
+    // 24 heads, 3 x 1000 61.4 / 54.4, but 5 x 500 35.6 / 39.9: not there.
+    int tenths = 10;
+    if constexpr (!std::is_same_v<Rows, Dense> && D <= 128) tenths = view.len_q ? 7 : 10;
+    auto tiles = [&](int rows) { return (long long)BH * ((S + rows - 1) / rows) * tenths / 10; };
     if constexpr (D == 256) {
         // 128 rows by two key groups.  Without a mask while its workgroups fit the CUs (96 tiles of
         // S = 2048 100 / 68, 144 of S = 1500 81 / 107): it moves K and V for half the queries, 10 TB/s from
