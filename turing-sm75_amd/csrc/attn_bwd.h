@@ -111,7 +111,11 @@ __global__ void __launch_bounds__(256) attn_bwd_rows_kernel(RowsArgs a) {
                         // 1 / sigma, and 1 - sigma as sigma of the other sign (its own digits where sigma is near 1)
                         const float inv = 1.f + __expf(-(float)gt[j]), rest = __builtin_amdgcn_rcpf(1.f + __expf((float)gt[j]));
                         dg[j] = (half_t)(w[j] * (float)y[j] * rest);
-                        z[j] = (half_t)(w[j] * __builtin_amdgcn_rcpf(inv));
+                        // (the product as a float, unseen: else one use of z gets it rounded at once and another twice, and
+                        // where these differ d and dP come from different values)
+                        float g32 = w[j] * __builtin_amdgcn_rcpf(inv);
+                        asm volatile("" : "+v"(g32));
+                        z[j] = (half_t)g32;
                         // d_i goes with the dO that dP is made of, the rounded one: sum_j dS_ij then stays 0
                         // and the rounding weighs a fifth less in dQ and dK
                         if (z[j] != (half_t)0.f) w[j] = (float)z[j] * inv;
