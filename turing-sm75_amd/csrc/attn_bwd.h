@@ -11,10 +11,12 @@
 // T x S memory, no atomics (each sum has one order) and no fp32 dQ to be read and written for
 // every key tile.
 //
-// fp16 range: P and dS are rounded to fp16 as MFMA operands.  Both are multiplied by 2^ref there, one
-// power of two for a workgroup, as large as keeps |dS| 2^ref <= 2^14 and P 2^ref <= 2^15 by the bound
-// |dS_ij| <= |dO_i| |v_j| + |d_i| over its rows and keys, so gradients of any size keep fp16's
-// full precision in dS down to 2^-28 of that bound.  It is folded into the exponential's argument and into the outputs' scale.
+// fp16 range: P and dS are rounded to fp16 as MFMA operands.  P is multiplied by 2^15 there, whatever the gradients
+// are, and keeps fp16's full precision down to 2^-29.  dS has a power of two for a workgroup, 2^ref, as large as keeps
+// |dS| 2^ref <= 2^14 by the bound |dS_ij| <= |dO_i| |v_j| + |d_i| over its rows and keys, so gradients of any size keep
+// full precision in dS down to 2^-28 of that bound.  Where dS is made of the rounded P, the difference of the two powers
+// goes into dP - d in 32 bits (one power for both, in the exponential's argument alone, would save that product, 0.2 to 0.9 %
+// of the long calls, and leave P no bits where dO is large: 1.7 % of dV at 8192 keys and dO of 8192).
 // Both roundings (half a step, 2^-11 of a value at most) are what the matrix instructions at this rate take; with
 // them, and that of dO where there is a gate, a gradient's relative error is 3.3e-4 to 5.6e-4 against 64 bits,
 // of which rounding it to fp16 is 2.1e-4.
@@ -212,12 +214,14 @@ __device__ __forceinline__ int again(int x) {
     return x;
 }
 
-// The power of two for a bound of |dS|: 2^ref bound <= 2^14, ref <= 15 (P 2^ref <= 2^15).
+// P's power of two, whatever the gradients are.
+constexpr float kRefP = 15.f;
+// dS's for a bound of |dS|: 2^ref bound <= 2^14 (from 2^-60 down it stays: gradients of that size are 0 in fp16).
 __device__ __forceinline__ float range_ref(float bound) {
     if (!(bound < 0x1p100f)) bound = 0x1p100f;
     const int bits = __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, bound));  // (every lane's is the same)
     const int e = ((bits >> 23) & 255) - 126;                                        // bound < 2^e
-    return (float)min(15, 14 - e);
+    return (float)min(60, 14 - e);
 }
 
 __device__ __forceinline__ void lds_write_b128(unsigned addr, const half8_t& x) {
@@ -386,11 +390,11 @@ __device__ __forceinline__ half8_t pack8(const float16_t& x, int half) {
     return __builtin_convertvector(y, half8_t);
 }
 
-// Half `half` of x times the fp16 values p, rounded to fp16 (a product is v_fma_mixlo_f16: no conversions).
-__device__ __forceinline__ half8_t times(const half8_t& p, const float16_t& x, int half) {
+// Half `half` of x up times the fp16 values p, rounded to fp16 (a product is v_fma_mixlo_f16: no conversions).
+__device__ __forceinline__ half8_t times(const half8_t& p, const float16_t& x, int half, float up) {
     half8_t y;
 #pragma unroll
-    for (int r = 0; r < 8; ++r) y[r] = (half_t)fmaf((float)p[r], x[8 * half + r], 0.f);
+    for (int r = 0; r < 8; ++r) y[r] = (half_t)fmaf((float)p[r], x[8 * half + r] * up, 0.f);
     return y;
 }
 
@@ -515,7 +519,7 @@ __device__ __forceinline__ void kv_tile(args_t a, half_t* lds, int wg) {
     const long long q_jump = 2 * a->q.h - (long long)q_row * kBlk * pl.per, g_jump = 2 * a->g.h - (long long)g_row * kBlk * pl.per;
     const int s_jump = 64 * (a->n_qb - pl.per);
     unsigned ring = 0, ring2 = 0;  // stages of the current step and of the next copies
-    // the scale of P and dS is the workgroup's bound
+    // the scale of dS is the workgroup's bound
     float most_g = 0.f, most_d = 0.f, most_v = 0.f;
     bool some_bad = false;
     auto row_most = [&](int u) {
@@ -559,7 +563,7 @@ __device__ __forceinline__ void kv_tile(args_t a, half_t* lds, int wg) {
             for (int kk = 0; kk < kKK; ++kk) frag[kb][kk] = *reinterpret_cast<const half8_t*>(row + 16 * kk);
         }
     }
-    const float ref = range_ref(fmaf(wave_max(most_g), wave_max(most_v), wave_max(most_d)));
+    const float ref = range_ref(fmaf(wave_max(most_g), wave_max(most_v), wave_max(most_d))), up = scale_back(kRefP - ref);
 
     // register r of a result is query 4 hi + 8 (r / 4) + r % 4 of the step: hidden below this
     auto limit = [&](int x, int kb) {
@@ -576,7 +580,7 @@ __device__ __forceinline__ void kv_tile(args_t a, half_t* lds, int wg) {
         unsigned sa = 0, p_new = 0, p_old = 0;
         auto soft = [&](int x) {  // value x of S to P, 16 a key block
             const int kb = x >> 4, r = x & 15;
-            s[kb][r] = pinned(fast_exp2(fmaf(s[kb][r], c2, ref - l[r & 3])));
+            s[kb][r] = pinned(fast_exp2(fmaf(s[kb][r], c2, kRefP - l[r & 3])));
             if ((r & 3) == 3 && x + 1 < 16 * T::kKB) l = lds_read_f4(sa + 32u * (((r >> 2) + 1) & 3));
             if ((r & 7) == 7) lds_write_b128(p_new + (unsigned)(kb * 2 + (r >> 3)) * 1024u, pack8(s[kb], r >> 3));
         };
@@ -661,7 +665,7 @@ __device__ __forceinline__ void kv_tile(args_t a, half_t* lds, int wg) {
                 const unsigned at = p_at + (unsigned)((i - 1) & 1) * (T::kPairs * T::kPB);
                 half8_t ds[T::kKB][2];
                 ahead<2 * T::kKB, 1>([&](int x) { return lds_read_b128(at + (unsigned)x * 1024u); },
-                                     [&](int x, const half8_t& y) { ds[x >> 1][x & 1] = times(y, s[x >> 1], x & 1); });
+                                     [&](int x, const half8_t& y) { ds[x >> 1][x & 1] = times(y, s[x >> 1], x & 1, up); });
 #pragma unroll
                 for (int kb = 0; kb < T::kKB; ++kb)
                     if (partly(was, kb)) {  // 0 whatever dP is there
@@ -686,7 +690,7 @@ __device__ __forceinline__ void kv_tile(args_t a, half_t* lds, int wg) {
 
     lds_barrier();  // the tiles' LDS becomes the outputs'
     a = fresh(a);
-    const float f = scale_back(ref) * (role_p ? 1.f : a->scale);
+    const float f = role_p ? scale_back(kRefP) : scale_back(ref) * a->scale;
     if (a->n_part == 1) {
         const auto& out = role_p ? a->dv : a->dk;
         store_rows<T::kKB, kDB>(acc, out.data + b * out.b + hk * out.h, out.t, k0, pl.n_k, again(lane), f,
@@ -898,7 +902,7 @@ __device__ __forceinline__ void q_tile_roles(args_t a, half_t* lds, int wg) {
     if constexpr (role_p) {
         // round j: S of step j, then its P beside dQ of step j - 2
         float16_t x1[1], &s = x1[0];
-        const float l = ref - stat, c2 = a->c2;
+        const float l = kRefP - stat, c2 = a->c2;
         unsigned p_new = 0, ds_old = 0;
         auto soft = [&](int x) {
             s[x] = pinned(fast_exp2(fmaf(s[x], c2, l)));
@@ -937,6 +941,7 @@ __device__ __forceinline__ void q_tile_roles(args_t a, half_t* lds, int wg) {
         }
     } else {
         float16_t x1[1], &s = x1[0];
+        const float up = scale_back(kRefP - ref);
         auto products = [&](int j) {
             const unsigned st = (unsigned)(j & 1) * T::kTileB;
 #pragma unroll
@@ -953,7 +958,7 @@ __device__ __forceinline__ void q_tile_roles(args_t a, half_t* lds, int wg) {
                 half8_t ds1[1][2];
                 half8_t(&ds)[2] = ds1[0];
 #pragma unroll
-                for (int x = 0; x < 2; ++x) ds[x] = times(lds_read_b128(p_at + (unsigned)((j & 1) * kPairs * 2048 + x * 1024)), s, x);
+                for (int x = 0; x < 2; ++x) ds[x] = times(lds_read_b128(p_at + (unsigned)((j & 1) * kPairs * 2048 + x * 1024)), s, x, up);
                 if (ragged(j)) {
                     const int lim = limit(j);
 #pragma unroll
