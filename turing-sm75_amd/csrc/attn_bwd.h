@@ -11,7 +11,8 @@
 // T x S memory, no atomics (each sum has one order) and no fp32 dQ to be read and written for
 // every key tile.
 //
-// fp16 range: P and dS are rounded to fp16 as MFMA operands.  P is multiplied by 2^15 there, whatever the gradients
+// fp16 range: P and dS are rounded to fp16 as MFMA operands, and with a gate dO, each small row times a power of two of
+// its own (a small gradient behind a closed gate would have few of fp16's bits, or none).  P is multiplied by 2^15 there, whatever the gradients
 // are, and keeps fp16's full precision down to 2^-29.  dS has a power of two for a workgroup, 2^ref, as large as keeps
 // |dS| 2^ref <= 2^14 by the bound |dS_ij| <= |dO_i| |v_j| + |d_i| over its rows and keys, so gradients of any size keep
 // full precision in dS down to 2^-28 of that bound.  Where dS is made of the rounded P, the difference of the two powers
@@ -41,12 +42,12 @@ constexpr int kBlk = 32;  // rows and keys of a step
 
 struct BwdArgs {
     Rows16 q, k, v, g /* dO, gated */, dq, dk, dv;
-    const float* stat;     // [B][Hq][n_qb][64]: L log2(e) of 32 rows (inf: no such row, or it sees no key), then -d
+    const float* stat;     // [B][Hq][n_qb][64]: L log2(e) + power of 32 rows (inf: no such row, or it sees no key), then -d 2^power
     const float2* row_max; // [B][Hq][n_qb]: the largest |dO_i| and |d_i| of 32 rows; the second below 0: one is bad
     const float* key_max;  // [B][Hkv][n_kb]: the largest |v_j| of 32 keys; below 0: a bad k_j among them
     float* part;           // split key tiles: fp32 sums of each part
     const int *len_q, *len_k;
-    int B, Hq, Hkv, Tq, Tk, n_qb, n_kb, n_kt, n_part, n_qt, n_kv;  // n_kt, n_qt: tiles; n_kv: workgroups of the key tiles
+    int B, Hq, Hkv, Tq, Tk, n_qb, n_kb, n_kt, n_part, n_qt, n_kv, gated;  // n_kt, n_qt: tiles; n_kv: workgroups of the key tiles; gated: rows of g have powers
     float scale, c2;
 };
 
@@ -70,12 +71,20 @@ __device__ __forceinline__ int count(const int* len, int b, int most) {
 constexpr float kBad = 1e-30f;  // added below 0, so that a bound of 0 shows the mark too
 __device__ __forceinline__ bool finite16(half_t x) { return __builtin_fabsf((float)x) < INFINITY; }
 
+// The power of two with which a row of this norm is kept where a gate makes its dO: 2^power norm is at least
+// 2^7 (its largest element 2^3, and what is 2^17 below that has fp16's full precision), larger rows stay.  Below 2^-41
+// it stays too: such gradients are 0 in fp16.
+__device__ __forceinline__ int row_power(float norm) {
+    const int e = (int)(__builtin_bit_cast(unsigned, norm) >> 23 & 255) - 126;  // norm < 2^e
+    return min(max(8 - e, 0), 48);
+}
+
 // ---------------------------------------------------------------------------------------
 // Row statistics: a workgroup takes 32 rows of dO' and o' (8 lanes a row), or 32 keys' values.
 // ---------------------------------------------------------------------------------------
 struct RowsArgs {
     Rows16 g, o, gate, k, v, dgate;  // k: null without a mask
-    half_t* gated;  // dO [B][Hq][Tq][D], with a gate
+    half_t* gated;  // with a gate: dO [B][Hq][Tq][D], each row times 2^power
     const float* lse;
     float* stat;
     float2* row_max;
@@ -85,7 +94,7 @@ struct RowsArgs {
 };
 
 template <int D>
-__global__ void __launch_bounds__(256) attn_bwd_rows_kernel(RowsArgs a) {
+__global__ void __launch_bounds__(256, 3) attn_bwd_rows_kernel(RowsArgs a) {
     __shared__ float2 most[32];
     const int r = threadIdx.x >> 3, l8 = threadIdx.x & 7;
     int blk = blockIdx.x;
@@ -93,55 +102,71 @@ __global__ void __launch_bounds__(256) attn_bwd_rows_kernel(RowsArgs a) {
         const int bh = blk / a.n_qb, qb = blk % a.n_qb, b = bh / a.Hq, h = bh % a.Hq;
         const int n = count(a.len_q, b, a.Tq), t = qb * kBlk + r;
         float d = 0.f, n2 = 0.f;
+        half8_t x[D / 64], y[D / 64];
+        float z[D / 8], u[D / 8];  // with a gate: dO, and o' / sigma
         if (t < n) {
-            const half_t* g = a.g.data + b * a.g.b + h * a.g.h + t * a.g.t;
-            const half_t* o = a.o.data + b * a.o.b + h * a.o.h + t * a.o.t;
+            const half_t* g = a.g.data + b * a.g.b + h * a.g.h + t * a.g.t + 8 * l8;
+            const half_t* o = a.o.data + b * a.o.b + h * a.o.h + t * a.o.t + 8 * l8;
 #pragma unroll
             for (int i = 0; i < D / 64; ++i) {
-                const int e0 = 8 * l8 + 64 * i;
-                const half8_t x = *reinterpret_cast<const half8_t*>(g + e0);
-                const half8_t y = *reinterpret_cast<const half8_t*>(o + e0);
-                half8_t z = x;
-                float w[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) w[j] = (float)x[j];
-                if (a.gated) {
-                    const half8_t gt = *reinterpret_cast<const half8_t*>(a.gate.data + b * a.gate.b + h * a.gate.h + t * a.gate.t + e0);
-                    half8_t dg;
+                x[i] = *reinterpret_cast<const half8_t*>(g + 64 * i);
+                y[i] = *reinterpret_cast<const half8_t*>(o + 64 * i);
+                if (!a.gated) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        // 1 / sigma, and 1 - sigma as sigma of the other sign (its own digits where sigma is near 1)
-                        const float inv = 1.f + __expf(-(float)gt[j]), rest = __builtin_amdgcn_rcpf(1.f + __expf((float)gt[j]));
-                        dg[j] = (half_t)(w[j] * (float)y[j] * rest);
-                        // (the product as a float, unseen: else one use of z gets it rounded at once and another twice, and
-                        // where these differ d and dP come from different values)
-                        float g32 = w[j] * __builtin_amdgcn_rcpf(inv);
-                        asm volatile("" : "+v"(g32));
-                        z[j] = (half_t)g32;
-                        // d_i goes with the dO that dP is made of, the rounded one: sum_j dS_ij then stays 0
-                        // and the rounding weighs a fifth less in dQ and dK
-                        if (z[j] != (half_t)0.f) w[j] = (float)z[j] * inv;
+                        d = fmaf((float)x[i][j], (float)y[i][j], d);
+                        n2 = fmaf((float)x[i][j], (float)x[i][j], n2);
                     }
-                    *reinterpret_cast<half8_t*>(a.gated + ((size_t)bh * a.Tq + t) * D + e0) = z;
-                    *reinterpret_cast<half8_t*>(a.dgate.data + b * a.dgate.b + h * a.dgate.h + t * a.dgate.t + e0) = dg;
+                    continue;
                 }
+                const half8_t gt = *reinterpret_cast<const half8_t*>(a.gate.data + b * a.gate.b + h * a.gate.h + t * a.gate.t + 8 * l8 + 64 * i);
+                half8_t dg;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    d = fmaf(w[j], (float)y[j], d);
-                    n2 = fmaf((float)z[j], (float)z[j], n2);
+                    // 1 / sigma, and 1 - sigma as sigma of the other sign (its own digits where sigma is near 1)
+                    const float inv = 1.f + __expf(-(float)gt[j]), rest = __builtin_amdgcn_rcpf(1.f + __expf((float)gt[j]));
+                    const float w = (float)x[i][j], o1 = (float)y[i][j];
+                    dg[j] = (half_t)(w * o1 * rest);
+                    z[8 * i + j] = w * __builtin_amdgcn_rcpf(inv);
+                    u[8 * i + j] = o1 * inv;
+                    n2 = fmaf(z[8 * i + j], z[8 * i + j], n2);
                 }
+                *reinterpret_cast<half8_t*>(a.dgate.data + b * a.dgate.b + h * a.dgate.h + t * a.dgate.t + 8 * l8 + 64 * i) = dg;
+            }
+        }
+        n2 = sum8(n2);
+        const float norm = sqrtf(n2);
+        const int power = a.gated ? row_power(norm) : 0;
+        if (a.gated && t < n) {
+            const float up = __builtin_ldexpf(1.f, power);
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) {
+                half8_t z16;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    // (the product as a float, unseen: else one use of it gets it rounded at once and another twice, and
+                    // where these differ d and dP come from different values)
+                    float g32 = z[8 * i + j] * up;
+                    asm volatile("" : "+v"(g32));
+                    z16[j] = (half_t)g32;
+                    // d_i goes with the dO that dP is made of, the rounded one: sum_j dS_ij then stays 0
+                    // and the rounding weighs a fifth less in dQ and dK
+                    const float r = (float)z16[j];
+                    d = r != 0.f ? fmaf(r, u[8 * i + j], d) : d;  // (o' / sigma may be 0 times infinity)
+                }
+                *reinterpret_cast<half8_t*>(a.gated + ((size_t)bh * a.Tq + t) * D + 8 * l8 + 64 * i) = z16;
             }
         }
         d = sum8(d);
-        n2 = sum8(n2);
         if (l8 == 0) {
             float* st = a.stat + (size_t)blk * 64;
             const float lse = t < n ? a.lse[(size_t)bh * a.Tq + t] : -INFINITY;
             const bool bad = !(n2 < INFINITY) || !(lse < INFINITY);
-            st[r] = bad ? NAN : lse == -INFINITY ? INFINITY : lse * kLog2e;
+            st[r] = bad ? NAN : lse == -INFINITY ? INFINITY : fmaf(lse, kLog2e, (float)power);
             st[32 + r] = -d;
+            const float d1 = fabsf(__builtin_ldexpf(d, -power));
             // (a bad row, or one with no d, is left out of the bound: its results are NaN at any scale)
-            most[r] = bad ? make_float2(0.f, -kBad) : make_float2(sqrtf(n2), fabsf(d) < INFINITY ? fabsf(d) : 0.f);
+            most[r] = bad ? make_float2(0.f, -kBad) : make_float2(norm, d1 < INFINITY ? d1 : 0.f);
         }
         __syncthreads();
         if (threadIdx.x < 64) {
@@ -214,14 +239,24 @@ __device__ __forceinline__ int again(int x) {
     return x;
 }
 
-// P's power of two, whatever the gradients are.
-constexpr float kRefP = 15.f;
-// dS's for a bound of |dS|: 2^ref bound <= 2^14 (from 2^-60 down it stays: gradients of that size are 0 in fp16).
+// dS's power of two for a bound of |dS|: 2^ref bound <= 2^14 (from 2^-60 down it stays: gradients of that size are 0 in fp16).
 __device__ __forceinline__ float range_ref(float bound) {
     if (!(bound < 0x1p100f)) bound = 0x1p100f;
     const int bits = __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, bound));  // (every lane's is the same)
     const int e = ((bits >> 23) & 255) - 126;                                        // bound < 2^e
     return (float)min(60, 14 - e);
+}
+// A workgroup's powers of two from the largest |dO_i|, |v_j| and |d_i| (every lane's are the same).  P's is 15 above the
+// least of its rows', that of the largest |dO_i|: what a row's own power is above that, the statistic takes off its P.
+struct Powers {
+    float p, ds, up;  // up: 2^ds / 2^p, for dP - d
+};
+__device__ __forceinline__ Powers powers(args_t a, float most_g, float most_v, float most_d) {
+    Powers x;
+    x.p = 15.f + (a->gated ? (float)row_power(__builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, most_g)))) : 0.f);
+    x.ds = range_ref(fmaf(most_g, most_v, most_d));
+    x.up = scale_back(x.p - x.ds);
+    return x;
 }
 
 __device__ __forceinline__ void lds_write_b128(unsigned addr, const half8_t& x) {
@@ -563,7 +598,7 @@ __device__ __forceinline__ void kv_tile(args_t a, half_t* lds, int wg) {
             for (int kk = 0; kk < kKK; ++kk) frag[kb][kk] = *reinterpret_cast<const half8_t*>(row + 16 * kk);
         }
     }
-    const float ref = range_ref(fmaf(wave_max(most_g), wave_max(most_v), wave_max(most_d))), up = scale_back(kRefP - ref);
+    const Powers pw = powers(a, wave_max(most_g), wave_max(most_v), wave_max(most_d));
 
     // register r of a result is query 4 hi + 8 (r / 4) + r % 4 of the step: hidden below this
     auto limit = [&](int x, int kb) {
@@ -580,7 +615,7 @@ __device__ __forceinline__ void kv_tile(args_t a, half_t* lds, int wg) {
         unsigned sa = 0, p_new = 0, p_old = 0;
         auto soft = [&](int x) {  // value x of S to P, 16 a key block
             const int kb = x >> 4, r = x & 15;
-            s[kb][r] = pinned(fast_exp2(fmaf(s[kb][r], c2, kRefP - l[r & 3])));
+            s[kb][r] = pinned(fast_exp2(fmaf(s[kb][r], c2, pw.p - l[r & 3])));
             if ((r & 3) == 3 && x + 1 < 16 * T::kKB) l = lds_read_f4(sa + 32u * (((r >> 2) + 1) & 3));
             if ((r & 7) == 7) lds_write_b128(p_new + (unsigned)(kb * 2 + (r >> 3)) * 1024u, pack8(s[kb], r >> 3));
         };
@@ -665,7 +700,7 @@ __device__ __forceinline__ void kv_tile(args_t a, half_t* lds, int wg) {
                 const unsigned at = p_at + (unsigned)((i - 1) & 1) * (T::kPairs * T::kPB);
                 half8_t ds[T::kKB][2];
                 ahead<2 * T::kKB, 1>([&](int x) { return lds_read_b128(at + (unsigned)x * 1024u); },
-                                     [&](int x, const half8_t& y) { ds[x >> 1][x & 1] = times(y, s[x >> 1], x & 1, up); });
+                                     [&](int x, const half8_t& y) { ds[x >> 1][x & 1] = times(y, s[x >> 1], x & 1, pw.up); });
 #pragma unroll
                 for (int kb = 0; kb < T::kKB; ++kb)
                     if (partly(was, kb)) {  // 0 whatever dP is there
@@ -690,7 +725,7 @@ __device__ __forceinline__ void kv_tile(args_t a, half_t* lds, int wg) {
 
     lds_barrier();  // the tiles' LDS becomes the outputs'
     a = fresh(a);
-    const float f = role_p ? scale_back(kRefP) : scale_back(ref) * a->scale;
+    const float f = role_p ? scale_back(pw.p) : scale_back(pw.ds) * a->scale;
     if (a->n_part == 1) {
         const auto& out = role_p ? a->dv : a->dk;
         store_rows<T::kKB, kDB>(acc, out.data + b * out.b + hk * out.h, out.t, k0, pl.n_k, again(lane), f,
@@ -723,7 +758,7 @@ struct QTile {
 };
 
 template <int D>
-__device__ __forceinline__ float q_tile_ref(args_t a, int bh, int q0, int q_blocks, float most_v, int lane) {
+__device__ __forceinline__ Powers q_tile_powers(args_t a, int bh, int q0, int q_blocks, float most_v, int lane) {
     float n = 0.f, d = 0.f;
     const int qb = q0 / kBlk + lane;
     if (lane < q_blocks && qb < a->n_qb) {
@@ -731,7 +766,7 @@ __device__ __forceinline__ float q_tile_ref(args_t a, int bh, int q0, int q_bloc
         n = m.x;
         d = fabsf(m.y);
     }
-    return range_ref(fmaf(wave_max(n), wave_max(most_v), wave_max(d)));
+    return powers(a, wave_max(n), wave_max(most_v), wave_max(d));
 }
 // The largest |v_j| of the key blocks of this lane, and whether some lane's holds a bad key.
 __device__ __forceinline__ float key_most(args_t a, int bhk, int k_blocks, int lane, bool& bad) {
@@ -802,9 +837,9 @@ __device__ __forceinline__ void q_tile(args_t a, half_t* lds, int wg) {
     };
     if (n > 0) copy();
     if (n > 1) copy();
-    const float ref = q_tile_ref<D>(a, bh, tile0, T::kQueries / kBlk, most_v, lane);
+    const Powers pw = q_tile_powers<D>(a, bh, tile0, T::kQueries / kBlk, most_v, lane);
 #pragma unroll
-    for (int m = 0; m < kMB; ++m) l2[m] -= ref;
+    for (int m = 0; m < kMB; ++m) l2[m] -= pw.ds;
 #pragma clang loop unroll(disable)
     for (int j = 0; j < n; ++j) {
         dma_wait_barrier();
@@ -840,7 +875,7 @@ __device__ __forceinline__ void q_tile(args_t a, half_t* lds, int wg) {
     }
     lds_barrier();  // the tiles' LDS becomes the outputs'
     a = fresh(a);
-    store_rows<kMB, kDB>(acc, a->dq.data + b * a->dq.b + h * a->dq.h, a->dq.t, q0, n_q, again(lane), scale_back(ref) * a->scale,
+    store_rows<kMB, kDB>(acc, a->dq.data + b * a->dq.b + h * a->dq.h, a->dq.t, q0, n_q, again(lane), scale_back(pw.ds) * a->scale,
                          lds0 + (unsigned)wave * (64u * kMB * 32 * kDB));
 }
 
@@ -898,11 +933,11 @@ __device__ __forceinline__ void q_tile_roles(args_t a, half_t* lds, int wg) {
     auto limit = [&](int j) { return min(kCausal ? my_q + last0 : n_k, n_k - 1) - j * kBlk - 4 * hi; };
     auto ragged = [&](int j) { return (kCausal && j * kBlk + 31 > q0 + last0) || (j + 1) * kBlk > n_k; };
     if (!role_p && n > 0) copy(0);
-    const float ref = q_tile_ref<D>(a, bh, tile0, T::kQueries / kBlk, most_v, lane);
+    const Powers pw = q_tile_powers<D>(a, bh, tile0, T::kQueries / kBlk, most_v, lane);
     if constexpr (role_p) {
         // round j: S of step j, then its P beside dQ of step j - 2
         float16_t x1[1], &s = x1[0];
-        const float l = kRefP - stat, c2 = a->c2;
+        const float l = pw.p - stat, c2 = a->c2;
         unsigned p_new = 0, ds_old = 0;
         auto soft = [&](int x) {
             s[x] = pinned(fast_exp2(fmaf(s[x], c2, l)));
@@ -941,7 +976,6 @@ __device__ __forceinline__ void q_tile_roles(args_t a, half_t* lds, int wg) {
         }
     } else {
         float16_t x1[1], &s = x1[0];
-        const float up = scale_back(kRefP - ref);
         auto products = [&](int j) {
             const unsigned st = (unsigned)(j & 1) * T::kTileB;
 #pragma unroll
@@ -958,7 +992,7 @@ __device__ __forceinline__ void q_tile_roles(args_t a, half_t* lds, int wg) {
                 half8_t ds1[1][2];
                 half8_t(&ds)[2] = ds1[0];
 #pragma unroll
-                for (int x = 0; x < 2; ++x) ds[x] = times(lds_read_b128(p_at + (unsigned)((j & 1) * kPairs * 2048 + x * 1024)), s, x, up);
+                for (int x = 0; x < 2; ++x) ds[x] = times(lds_read_b128(p_at + (unsigned)((j & 1) * kPairs * 2048 + x * 1024)), s, x, pw.up);
                 if (ragged(j)) {
                     const int lim = limit(j);
 #pragma unroll
@@ -977,7 +1011,7 @@ __device__ __forceinline__ void q_tile_roles(args_t a, half_t* lds, int wg) {
     }
     lds_barrier();  // the tiles' LDS becomes the outputs'
     a = fresh(a);
-    store_rows<1, kDB>(acc, a->dq.data + b * a->dq.b + h * a->dq.h + (role_p ? 0 : D / 2), a->dq.t, q0, n_q, again(lane), scale_back(ref) * a->scale,
+    store_rows<1, kDB>(acc, a->dq.data + b * a->dq.b + h * a->dq.h + (role_p ? 0 : D / 2), a->dq.t, q0, n_q, again(lane), scale_back(pw.ds) * a->scale,
                        lds0 + (unsigned)wave * (64u * 32 * kDB));
 }
 
@@ -1082,7 +1116,7 @@ hipError_t backward(const AttnRows& x, const Rows16& d_out, const Rows16& dq, co
     hipLaunchKernelGGL(attn_bwd_rows_kernel<D>, dim3(r.n_rows + B * Hkv * p.n_kb), dim3(256), 0, stream, r);
     const Rows16 dO = gated ? Rows16{g, (long long)Hq * Tq * D, (long long)Tq * D, D} : d_out;
     BwdArgs a = {x.q, x.k, x.v, dO, dq, dk, dv, stat, row_max, key_max, reinterpret_cast<float*>(w + p.part), x.len_q, x.len_k,
-                 B, Hq, Hkv, Tq, Tk, p.n_qb, p.n_kb, p.n_kt, p.n_part, p.n_qt, B * Hkv * p.n_kt * p.n_part, scale, scale * kLog2e};
+                 B, Hq, Hkv, Tq, Tk, p.n_qb, p.n_kb, p.n_kt, p.n_part, p.n_qt, B * Hkv * p.n_kt * p.n_part, gated, scale, scale * kLog2e};
     const dim3 grid(a.n_kv + B * Hq * p.n_qt), block(64 * KvTile<D>::kW);
     if (causal)
         hipLaunchKernelGGL((attn_bwd_kernel<D, true>), grid, block, 0, stream, a);
