@@ -542,7 +542,7 @@ extern "C" int tsa_rope(const tsa_rope_plan* plan, int type, const tsa_rows* q, 
     if (plan->rot < 2 || plan->rot % 2 != 0 || plan->rot > D) return TSA_ERR_SHAPE;
     if (plan->interleaved != 0 && plan->interleaved != 1) return TSA_ERR_ARG;
     if (!std::isfinite(plan->amp) || (type != TSA_TYPE_F16 && type != TSA_TYPE_F32) || (back != 0 && back != 1)) return TSA_ERR_ARG;
-    // threads of a head group, and groups of heads
+    // rows of all sequences, and a workgroup's units of all heads, in ints
     if (!fits_int(B, T, D) || (long long)Hq + Hk > 65535) return TSA_ERR_SHAPE;
     int rc = check_rope(q, q_out, B, Hq, T);
     if (rc) return rc;

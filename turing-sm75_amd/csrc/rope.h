@@ -78,6 +78,7 @@ __device__ __forceinline__ void rotate(T (&x)[kVec], T (&y)[kVec], const float (
 }
 
 constexpr int kThreads = 256, kAtOnce = 4, kAngles = 256;  // angles a workgroup makes at most: tokens rot / 2
+constexpr int kColumns = 1 << 23;  // columns of tokens in a grid's x (whose threads are fewer than 2^32); the next ones are in its z
 
 // Unit u of a row: pairs u kVec .. + kVec - 1 while those are below rot / 2, then the elements behind
 // the rotated ones, 2 kVec at a time (only where they have to be copied: out of place).
@@ -85,7 +86,7 @@ template <typename T, bool kInter, int kVec>
 __global__ void __launch_bounds__(kThreads) rope_kernel(RopeArgs a) {
     __shared__ __align__(16) float sines[kAngles], cosines[kAngles];
     const int tid = threadIdx.x, half = a.rot / 2;
-    const long long row0 = (long long)blockIdx.x * a.tokens, rows = (long long)a.B * a.T;
+    const long long row0 = ((long long)blockIdx.z * kColumns + blockIdx.x) * a.tokens, rows = (long long)a.B * a.T;
     // Row r of the column, if it is a token (not padding, nor past the last).
     auto token = [&](int r, int& b, int& t, int& n) {
         const long long row = row0 + r;
@@ -209,7 +210,8 @@ hipError_t rope(const unsigned long long* freq, float amp, int rot, int interlea
     const long long columns = (rows + a.tokens - 1) / a.tokens, most = (a.items + kThreads - 1) / kThreads;
     const long long deal = std::max(1LL, std::min({most, 1024 / columns, 65535LL}));
     a.share = (int)((most + deal - 1) / deal) * kThreads;
-    const dim3 grid((unsigned)columns, (unsigned)((a.items + a.share - 1) / a.share));
+    const dim3 grid((unsigned)std::min<long long>(columns, kColumns), (unsigned)((a.items + a.share - 1) / a.share),
+                    (unsigned)((columns + kColumns - 1) / kColumns));
     if (f32)
         return interleaved ? launch_rope<float, true>(a, grid, vec, stream) : launch_rope<float, false>(a, grid, vec, stream);
     return interleaved ? launch_rope<half_t, true>(a, grid, vec, stream) : launch_rope<half_t, false>(a, grid, vec, stream);
