@@ -292,6 +292,18 @@ __device__ __forceinline__ bool any_wave(int* flags, int wave, int lane, bool mi
     for (int w = 0; w < kW; ++w) any |= flags[w];
     return __builtin_amdgcn_readfirstlane(any) != 0;
 }
+// What is taken off the scaled scores in front of their exponential.  The training form's exponentials (and their sum) are 2^7
+// times their value against the maximum, so that weights down to 2^-21 of that have fp16's full precision as operands: one key far
+// above the others would leave these few bits, or none.  They are 2^8 above it at most (the maximum follows only then),
+// and fp16 holds 2^15.  (A product with 2^7 behind the exponential took 8192 tokens, D = 256, from 864 to 882 us.)
+constexpr float kPUp = 7.f;
+template <bool kAny>
+__device__ __forceinline__ float exp_base(float m, float c2) {
+    if constexpr (kAny)
+        return m == -INFINITY ? -kPUp : fmaf(m, c2, -kPUp);
+    else
+        return m == -INFINITY ? 0.f : m * c2;
+}
 // Adds the 32 keys from kb0 on to O^T, one after the other (m: the final maximum).
 template <int D>
 __device__ __forceinline__ void add_block(float16_t (&o)[Cfg<D>::kDBlocks], const half_t* q, const half_t* K, const half_t* V,
@@ -308,7 +320,7 @@ __device__ __forceinline__ void add_block(float16_t (&o)[Cfg<D>::kDBlocks], cons
         }
         s = sum_xor32(s);
         const bool sees = kb0 + j <= last;  // (no branch: the sums would be moved between registers)
-        const float e = sees ? fast_exp2(fmaf(s, c2, -(m * c2))) : 0.f, p = (float)(half_t)e;
+        const float e = sees ? fast_exp2(fmaf(s, c2, -exp_base<true>(m, c2))) : 0.f, p = (float)(half_t)e;
         l += hi ? 0.f : e;
 #pragma unroll
         for (int db = 0; db < Cfg<D>::kDBlocks; ++db)
@@ -321,10 +333,19 @@ __device__ __forceinline__ void add_block(float16_t (&o)[Cfg<D>::kDBlocks], cons
             }
     }
 }
+// The sum of a row's exponentials as they would be without exp_base's own rounding (2^-22 of them at scores below 8, which
+// a row of one key, whose weight is 1 and rounds to it, would show as o's last bits).  Past scores of some hundreds the
+// weights' roundings do not take that out any more, and the sum stays as they have it.
+__device__ __forceinline__ float true_sum(float m, float l, float c2) {
+    float p = m * c2;
+    asm volatile("" : "+v"(p));  // (not one operation with the difference)
+    const float s = p - kPUp, t = s - p, off = ((s - exp_base<true>(m, c2)) + ((p - (s - t)) - (kPUp + t))) + fmaf(m, c2, -p);
+    return fabsf(off) < 0x1p-16f ? fmaf(l, off * -0.69314718056f, l) : l;
+}
 // A row's statistic: the logarithm of the sum of its exponentials, from the maximum they were taken
-// against (as the exponentials had it) and their sum; minus infinity for a row that sees no key.
+// against and their sum; minus infinity for a row that sees no key.
 __device__ __forceinline__ float row_lse(float m, float l, float c2) {
-    return l > 0.f ? (m * c2 + __builtin_amdgcn_logf(l)) * 0.69314718056f : (l == 0.f ? -INFINITY : l);
+    return l > 0.f ? fmaf(m, c2, __builtin_amdgcn_logf(l) - kPUp) * 0.69314718056f : (l == 0.f ? -INFINITY : l);
 }
 
 // kW waves per workgroup, 32 query rows each: kW = 4 at D <= 128 (two workgroups per CU,
@@ -512,7 +533,7 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
 #pragma unroll
                         for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
                 }
-                const float mc = m == -INFINITY ? 0.f : m * c2;
+                const float mc = exp_base<kAny>(m, c2);
                 half8_t p[4];
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
@@ -615,7 +636,7 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
 #pragma unroll
                             for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
                     }
-                    const float mc = m == -INFINITY ? 0.f : m * c2;
+                    const float mc = exp_base<kAny>(m, c2);
                     half8_t p[2];
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
@@ -679,6 +700,7 @@ attn_fwd_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
                 add_block<D>(o, Qh + min(end_q, n_q - 1) * q_t, Kh, Vh, k_t, v_t, k0, n_k, kCausal ? end_q + last0 : n_k, end_hi, m, l, c2);
         }
     }
+    if constexpr (kAny) l = true_sum(m, l, c2);
     l = sum_xor32(l);
     if constexpr (kAny) {
         const int b = __builtin_amdgcn_readfirstlane(bh / Hq), h = __builtin_amdgcn_readfirstlane(bh % Hq);
@@ -845,7 +867,7 @@ attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
 #pragma unroll
                     for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
             }
-            const float mc = m == -INFINITY ? 0.f : m * c2;
+            const float mc = exp_base<kAny>(m, c2);
             half8_t p[2];
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
@@ -907,6 +929,7 @@ attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
     }
     // ---- merge: the partial O's of the key groups past the first, lane for lane, through the tile
     // buffers (every wave is past its last read of them) ----
+    if constexpr (kAny) l = true_sum(m, l, c2);
     l = sum_xor32(l);
     float4* part = reinterpret_cast<float4*>(lds);
     constexpr int kPart4 = C::kDBlocks * 4 * 64;  // float4s per wave's O
