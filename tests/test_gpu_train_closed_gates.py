@@ -32,10 +32,10 @@ def bounds(do, q, k, v, o, lse, gate, causal):
     norm = g.norm(dim=-1, keepdim=True)
     eg = (orc.U + 2.0 ** -18) * g.abs() + torch.where(norm < 2.0 ** 7, 2.0 ** -32 * norm, 2.0 ** -25)
     rel = torch.expm1(2 * ((D + 4) * 2.0 ** -23 * c * (q.abs() @ k.abs().transpose(2, 3)) + 2.0 ** -22 * (lse.abs() + 64)))
-    floor_p = 2.0 ** -40 * (2 * norm.amax() / norm).clamp_min(1)
+    floor_p = 2.0 ** -40 * torch.where(norm > 0, (2 * norm.amax() / norm).clamp_min(1), 1.0)
     ep = torch.where(see, p * (orc.U + rel) + floor_p, 0.0)
     # (d is made of the rounded dO: the row's sum of dS stays 0, and the rounding of dO is that of dP - d)
-    edp = eg @ v.abs().transpose(2, 3) + (eg * (o / sig).abs()).sum(-1, keepdim=True) + \
+    edp = eg @ v.abs().transpose(2, 3) + torch.where(sig > 0, eg * (o / sig).abs(), 0.0).sum(-1, keepdim=True) + \
         (D + 8) * 2.0 ** -23 * (g.abs() @ v.abs().transpose(2, 3) + (do * o).abs().sum(-1, keepdim=True))
     most = float(norm.amax() * v.norm(dim=-1).amax() + d.abs().amax())
     eds = torch.where(see, ds.abs() * (2 * orc.U + rel) + (p + ep) * edp + floor_p * (dp - d).abs() + most * 2.0 ** -38, 0.0)
@@ -104,3 +104,21 @@ def test_a_single_key_behind_a_closed_gate(dev, D):
     want = c * ds * k.double()
     assert ((dq.double() - want).abs() <= 1.01 * c * off * k.double().abs() + 2.0 ** -11 * want.abs() + 2.0 ** -25).all()
     assert want.abs().mean() > 2.0 ** -22  # (what is looked at is there)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_gates_at_the_ends(dev, D):
+    """Gates that close or open fully, and whole rows of them: sigmoid is 0 or 1, and nothing becomes NaN."""
+    q, k, v, gate, do = make(dev, 95, 1, 2, 1, 70, 70, D, True)
+    ends = [-65504.0, -300.0, -88.7, -80.0, -30.0, 30.0, 80.0, 88.7, 65504.0, float("inf"), -float("inf")]
+    gate[..., :len(ends)] = torch.tensor(ends, device=dev).half()
+    for i, x in enumerate(ends):
+        gate[:, :, 3 * i] = x
+    o, lse = tsa.attn_train_fwd(q, k, v, gate)
+    grads = tsa.attn_bwd(do, q, k, v, o, lse, gate)
+    for (name, want, bound), got in zip(bounds(do, q, k, v, o, lse, gate.double().clamp(-1e3, 1e3), True), grads):
+        within(name, got, want, bound)
+    want = do.double() * o.double() * (1 - torch.sigmoid(gate.double()))
+    assert ((grads[3].double() - want).abs() <= 1.01 * orc.U * want.abs() + 2.0 ** -20 * want.abs() + 2.0 ** -25).all()
+    shut = torch.isin(torch.arange(70, device=dev), torch.tensor([3 * i for i, x in enumerate(ends) if x <= -300], device=dev))
+    assert not grads[0][:, :, shut].any()
