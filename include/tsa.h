@@ -398,8 +398,9 @@ typedef struct tsa_rope_plan {
 } tsa_rope_plan;
 
 /* Rotates queries q [B][Hq][T][D] and keys k [B][Hk][T][D] (Hk may be 0: queries alone) of one type
- * (TSA_TYPE_F16 or TSA_TYPE_F32; the tsa_rows then hold floats) into q_out and k_out, each apart
- * from its input or the input itself (the same data and strides).  D in {64, 128, 256}.  Row t of
+ * (TSA_TYPE_F16 or TSA_TYPE_F32; the tsa_rows then hold floats) into q_out and k_out, each its own
+ * input (the same data and strides) or apart from every other tensor.  D in {64, 128, 256}; B * T * D is at most
+ * 2^31 - 1, Hq + Hk at most 65535.  Row t of
  * sequence b is at position pos[b * T + t], or without pos at len[b] - n_new[b] + t, or without
  * len at t; n_new[b] (T each without it) counts the sequence's rows, those behind it being padding
  * that is neither read nor written.  Positions may be any 32-bit numbers (pos, len and n_new: int32 on the device).  back = 1: the gradient, q and k

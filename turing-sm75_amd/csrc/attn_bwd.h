@@ -19,13 +19,13 @@
 // goes into dP - d in 32 bits (one power for both, in the exponential's argument alone, would save that product, 0.2 to 0.9 %
 // of the long calls, and leave P no bits where dO is large: 1.7 % of dV at 8192 keys and dO of 8192).
 // Both roundings (half a step, 2^-11 of a value at most) are what the matrix instructions at this rate take; with
-// them, and that of dO where there is a gate, a gradient's relative error is 3.3e-4 to 5.6e-4 against 64 bits,
+// them, and that of dO where there is a gate, a gradient's relative error is 3.6e-4 to 6.1e-4 against 64 bits,
 // of which rounding it to fp16 is 2.1e-4.
 //
-// Bound by the matrix pipes: 8192 tokens of 32 heads, D = 128, causal, take 1770 us, which is 1.08 PFLOP/s by the
-// seven products, nine tenths of what a large fp16 product of a library reaches on the same card (1.2, where
-// its power ends it); 4096 tokens of 24 heads over 4, D = 256, with a gate 780 us, of which the products are 720
-// (0.99 PFLOP/s), the rows 55 and the join 16.
+// Bound by the matrix pipes: 8192 tokens of 32 heads, D = 128, causal, take 1750 to 1800 us from box to box, which is
+// 1.07 to 1.10 PFLOP/s by the seven products, nine tenths of what a large fp16 product of a library reaches on the same
+// card (1.2, where its power ends it); 4096 tokens of 24 heads over 4, D = 256, with a gate 782 to 805 us, of which the
+// products are 715 to 735 (0.98 to 1.01 PFLOP/s), the rows 53 and the join 15.
 #pragma once
 #include <algorithm>
 #include <cmath>
@@ -1079,7 +1079,10 @@ Plan plan(int B, int Hq, int Hkv, int Tq, int Tk, bool gated, bool causal, bool 
     // (of what a causal mask leaves, and of 0.7 of that where sequences have lengths, which only the device knows).  A part
     // costs its fp32 sums' way to memory and back (256 KiB at D = 256) and the join, so it has 16 steps at least.  us per
     // call by parts (1, 2, 3, 4, 6): 128 tiles of 768 steps (24/4 heads x 4096, D = 256) 1175 / 809 / 807 / 804 / 817;
-    // 96 of 66 steps (3 x 701 over 1999, D = 256, ragged) 108 / 103 / 118 / 129 / 142; 64 of 16 steps (2 x 512, D = 64) 51.5 / 55.9.
+    // 96 of 66 steps (3 x 701 over 1999, D = 256, ragged) 108 / 103 / 118 / 129 / 142 (there the query tiles, which are
+    // not split, walk 63 steps of 3 products: those are the longest); 64 of 16 steps (2 x 512, D = 64) 51.5 / 55.9.  The 0.7 is
+    // of batches with one full sequence and far shorter others; where lengths are passed that leave all rows, 4 x 2048 of 32/8 heads, D =
+    // 128, take 571 for 524 without them, of 24/4 heads, D = 256, 856 for 809.
     const long long tiles = (long long)B * Hkv * p.n_kt, steps = (long long)(Hq / Hkv) * p.n_qb;
     const long long slots = D == 256 ? 256 : 512;
     const double seen = (causal ? 1 - 0.5 * std::min(1.0, (double)Tq / Tk) : 1) * (ragged ? 0.7 : 1);

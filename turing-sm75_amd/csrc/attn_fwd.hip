@@ -228,7 +228,8 @@ __device__ __forceinline__ void store_o(const float16_t (&o)[Cfg<D>::kDBlocks], 
 
 // The heads that map_block keeps on one XCD.  With lengths every head goes its own way: a sequence's heads
 // side by side would leave the long ones of a padded batch to few XCDs (lengths 2048, 273, 546, 819 of
-// 32 heads, D = 128: 193 -> 80 us).
+// 32 heads, D = 128: 193 -> 80 us).  Lengths that leave all rows pay for it with what an XCD's grouped heads would share of K and V:
+// 4 x 2048 of 32/8 heads, D = 128, 175 us for 172 without lengths, of 24/4 heads, D = 256, 241 for 234, D = 64 the same.
 template <class Rows>
 __device__ __forceinline__ int xcd_group(const Rows& rows, int group) {
     if constexpr (std::is_same_v<Rows, Dense>)
@@ -945,8 +946,8 @@ attn_ksplit_kernel(const half_t* __restrict__ Q, const half_t* __restrict__ K,
         }
         lds_barrier();
         if (kg > 0) return;
-        // (a group without keys for the row has m = -inf and factor 0; group 0 holds key 0, which every
-        // row sees)
+        // (a group without keys for the row has m = -inf and factor 0; group 0 holds key 0, which every row sees but for
+        // the training form's rows that see no key: all factors 0, and so l and O)
 #pragma unroll 1
         for (int i = 1; i < kKG; ++i) {
             const float2 x = ml[i][qg][lane];
@@ -1026,7 +1027,9 @@ hipError_t launch(const half_t* q, const half_t* k, const half_t* v, const half_
         const bool ragged = half < 2 * whole && S <= 2048;
         if (whole > 192 && whole <= (kCausal ? 272 : 320) && (kCausal || whole > 256 || S <= 512 || ragged))
             return split(attn_ksplit_kernel<D, kCausal, 4, 1, 32, Rows>, 128, 4);
-    } else if (S > 64) {  // (one key tile has nothing to split: 128 heads of S = 64 4.2 / 5.2, D = 128 5.4 / 8.2)
+    } else if (S > 64) {
+        // (one key tile has nothing to split: 128 heads of S = 64 4.2 / 5.2, D = 128 5.4 / 8.2.  The training form chooses by its
+        // queries too, so few queries over many keys, which could be split, are not.)
         // 32 rows by four key groups in its first round (D = 128: first workgroup per CU) at lengths
         // that pay the merge: D = 64, causal, 512 tiles of S = 256 7.9 / 6.6 against 6.2 of the next
         // form, 384 9.4 / 7.0 against 7.3, 1024 17.6 / 10.7; D = 128 256 tiles of S = 256 10.3 / 9.5
