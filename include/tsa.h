@@ -435,7 +435,8 @@ size_t tsa_attn_bwd_workspace_bytes(int B, int Hq, int Hkv, int Tq, int Tk, int 
  *   dk_j = scale sum_i dS_ij q_i    dgate = d_out o (1 - sigmoid(gate))
  * Every sum is taken in one order, in 32 bits: the same call gives the same bits.  P is rounded
  * to fp16 times 2^15, dS times a power of two that a bound of it chooses, and dO, with a gate, times one that
- * its row chooses, so d_out may be of any size. */
+ * its row chooses, so d_out may be of any size.  P is as good as lse's 32 bits: off by 2^-23 |lse|, 1e-3 at scores of
+ * 10^4, and by its whole size where scores reach 10^7. */
 int tsa_attn_bwd(const tsa_rows* d_out, const tsa_rows* q, const tsa_rows* k, const tsa_rows* v, const tsa_rows* gate,
                  const tsa_rows* o, const float* lse, const tsa_rows* dq, const tsa_rows* dk, const tsa_rows* dv,
                  const tsa_rows* dgate, const int32_t* len_q, const int32_t* len_k, int B, int Hq, int Hkv, int Tq,

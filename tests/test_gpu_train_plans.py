@@ -113,3 +113,41 @@ def test_whole_tiles_of_a_padded_batch(dev, D, causal, Hq, Hkv):
         within("o", o[b:b + 1], want, bo, n[b:b + 1])
         m = int(n[b])
         assert ((lse[b:b + 1].double() - want_l).abs() <= bl + 2.0 ** -22 * want_l.abs())[:, :, :m].all() and not lse[b, :, m:].any()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_captured_step_of_a_padded_batch(dev, D):
+    """Rotary positions, forward, backward and back in one graph, with split key tiles, replayed with other lengths."""
+    B, Hq, Hkv, T = 3, 8, 2, 600
+    assert splits(B, Hq, Hkv, T, T, D, True)
+    x = make(dev, 130, B, Hq, Hkv, T, T, D, True, "bshd")
+    q, k, v, gate, do = x
+    n = lens(dev, [600, 1, 333])
+    rope = tsa.Rope(D, rot=32)
+    ws = torch.empty(tsa.attn_bwd_workspace_bytes(B, Hq, Hkv, T, T, D, gated=True), dtype=torch.uint8, device=dev)
+    new = lambda: [torch.zeros_like(q), torch.zeros_like(k), *outputs(x)]  # noqa: E731
+
+    def run(y, ws):
+        qr, kr, o, lse, dq, dk, dv, dg = y
+        tsa.rope_fwd(rope, q, k, n_new=n, q_out=qr, k_out=kr)
+        tsa.attn_train_fwd(qr, kr, v, gate, len_q=n, len_k=n, out=o, lse=lse)
+        tsa.attn_bwd(do, qr, kr, v, o, lse, gate, len_q=n, len_k=n, dq=dq, dk=dk, dv=dv, dgate=dg, ws=ws)
+        tsa.rope_bwd(rope, dq, dk, n_new=n, q_out=dq, k_out=dk)
+
+    got = new()
+    run(got, ws)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        run(got, ws)
+    for i, length in enumerate(([600, 1, 333], [0, 600, 599], [77, 600, 600], [600, 0, 64])):
+        n.copy_(lens(dev, length))
+        for a, b in zip(x, make(dev, 131 + i, B, Hq, Hkv, T, T, D, True, "bshd")):
+            a.copy_(b)
+        for a in got:
+            a.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        want = new()
+        run(want, None)
+        assert same(got, want) and any(a.any() for a in got)

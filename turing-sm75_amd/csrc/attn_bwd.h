@@ -12,8 +12,8 @@
 // every key tile.
 //
 // fp16 range: P and dS are rounded to fp16 as MFMA operands, and with a gate dO, each small row times a power of two of
-// its own (a small gradient behind a closed gate would have few of fp16's bits, or none).  P is multiplied by 2^15 there, whatever the gradients
-// are, and keeps fp16's full precision down to 2^-29.  dS has a power of two for a workgroup, 2^ref, as large as keeps
+// its own (a small gradient behind a closed gate would have few of fp16's bits, or none), which is taken off its P again.
+// P is multiplied by 2^15 there, whatever the gradients are, and keeps fp16's full precision down to 2^-29.  dS has a power of two for a workgroup, 2^ref, as large as keeps
 // |dS| 2^ref <= 2^14 by the bound |dS_ij| <= |dO_i| |v_j| + |d_i| over its rows and keys, so gradients of any size keep
 // full precision in dS down to 2^-28 of that bound.  Where dS is made of the rounded P, the difference of the two powers
 // goes into dP - d in 32 bits (one power for both, in the exponential's argument alone, would save that product, 0.2 to 0.9 %
@@ -72,8 +72,8 @@ constexpr float kBad = 1e-30f;  // added below 0, so that a bound of 0 shows the
 __device__ __forceinline__ bool finite16(half_t x) { return __builtin_fabsf((float)x) < INFINITY; }
 
 // The power of two with which a row of this norm is kept where a gate makes its dO: 2^power norm is at least
-// 2^7 (its largest element 2^3, and what is 2^17 below that has fp16's full precision), larger rows stay.  Below 2^-41
-// it stays too: such gradients are 0 in fp16.
+// 2^7 (its largest element 2^3, and what is 2^17 below that has fp16's full precision), larger rows stay as they are.  It
+// ends at 48, for norms of 2^-41: smaller gradients are 0 in fp16.
 __device__ __forceinline__ int row_power(float norm) {
     const int e = (int)(__builtin_bit_cast(unsigned, norm) >> 23 & 255) - 126;  // norm < 2^e
     return min(max(8 - e, 0), 48);
@@ -239,7 +239,7 @@ __device__ __forceinline__ int again(int x) {
     return x;
 }
 
-// dS's power of two for a bound of |dS|: 2^ref bound <= 2^14 (from 2^-60 down it stays: gradients of that size are 0 in fp16).
+// dS's power of two for a bound of |dS|: 2^ref bound <= 2^14 (up to 2^60: smaller gradients are 0 in fp16).
 __device__ __forceinline__ float range_ref(float bound) {
     if (!(bound < 0x1p100f)) bound = 0x1p100f;
     const int bits = __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, bound));  // (every lane's is the same)
